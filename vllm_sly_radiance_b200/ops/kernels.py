@@ -355,6 +355,48 @@ def moe_grouped_mlp(q, s, counts, w_gate_up, w_down, I: int, H: int) -> torch.Te
 
 
 # ---------------------------------------------------------------------------------------------
+# adapters
+# ---------------------------------------------------------------------------------------------
+def lora_add(y: torch.Tensor, x, bank, plan, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """y [T, N] bf16 (the shared projection's output) plus the low-rank delta of each row's adapter:
+    out[t] = y[t] + scale * B (A x[t]) for the rows of ``plan`` (models/lora.AdapterPlan) that have
+    an adapter in ``bank`` (models/lora.AdapterBank), y[t] for the others.  x: bf16 [T, K] or the
+    (e4m3, scale) pair the linear itself takes.  out may be y (in place); a new tensor by default."""
+    xq, xs = x if isinstance(x, tuple) else (x, None)
+    T = y.shape[0]
+    if y.dim() != 2 or xq.dim() != 2 or xq.shape[0] != T or plan.num_rows != T:
+        raise ValueError(f"lora_add: y {tuple(y.shape)}, x {tuple(xq.shape)} and a plan of "
+                         f"{plan.num_rows} rows")
+    if xq.shape[1] != bank.K or y.shape[1] != bank.N or plan.num_slots > bank.L:
+        raise ValueError(f"lora_add: {xq.shape[1]} -> {y.shape[1]} features and {plan.num_slots} "
+                         f"slots, adapters of {bank.K} -> {bank.N} and {bank.L}")
+    if y.dtype != torch.bfloat16 or xq.dtype != (torch.bfloat16 if xs is None
+                                                 else torch.float8_e4m3fn):
+        raise ValueError("lora_add: y bf16, x bf16 or (e4m3, scale)")
+    if xs is not None and (xs.dtype != torch.float32 or xs.shape != (T,) or not xs.is_contiguous()):
+        raise ValueError("lora_add: x scales fp32 [T]")
+    if y.device != bank.device or xq.device != y.device or plan.buf.device != y.device or \
+            (xs is not None and xs.device != y.device):
+        raise ValueError("lora_add: operands on one device")
+    if out is None:
+        out = torch.empty(T, bank.N, dtype=torch.bfloat16, device=y.device)
+    elif out.shape != y.shape or out.dtype != y.dtype or out.device != y.device:
+        raise ValueError("lora_add: out as y")
+    if T == 0:
+        return out
+    if xq.stride(1) != 1 or y.stride(1) != 1 or out.stride(1) != 1:
+        raise ValueError("lora_add: rows must be contiguous")
+    if not y.is_cuda:
+        out.copy_(ref.lora_add(y, x, bank, plan.slots))
+        return out
+    dev = y.device
+    ext().lora_add(y, xq, xs if xs is not None else _empty(dev), bank.a, bank.b, bank.scale,
+                   bank.ranks, bank.slices, plan.buf, plan.max_tiles, plan.tile_rows, out,
+                   status_word(dev))
+    return out
+
+
+# ---------------------------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------------------------
 def qkv_prologue(qkv, positions, q_norm_w, k_norm_w, cos_sin, k_cache, v_cache, slot_mapping, *,

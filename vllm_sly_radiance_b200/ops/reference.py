@@ -314,3 +314,21 @@ def apply_top_k_top_p(logits: torch.Tensor, top_k: torch.Tensor, top_p: torch.Te
     masked = srt.masked_fill(~keep, float("-inf"))
     out.scatter_(1, idx, masked)
     return out
+
+
+# ---------------------------------------------------------------------------------------------
+# adapters
+# ---------------------------------------------------------------------------------------------
+def lora_add(y, x, bank, slots) -> torch.Tensor:
+    """Per adapter in use: y rows + scale * (x A^T) B^T of each slice, in fp32, rounded once."""
+    xf = x[0].float() * x[1].float()[:, None] if isinstance(x, tuple) else x.float()
+    slots = torch.as_tensor(slots)
+    out = y.float().clone()
+    for l in sorted(set(slots.tolist()) - {-1}):
+        rows = (slots == l).nonzero()[:, 0]
+        r = int(bank.ranks[l])
+        for s in range(bank.S):
+            n0, n1 = bank.slices[s], bank.slices[s + 1]
+            v = xf[rows] @ bank.a[l, s, :r].float().t()
+            out[rows, n0:n1] += float(bank.scale[l]) * (v @ bank.b[l, n0:n1, :r].float().t())
+    return out.to(torch.bfloat16)
