@@ -20,15 +20,14 @@ def test_plan_covers_every_row_once(T, tile_rows):
     slots = np.random.default_rng(T).integers(-1, 7, T)
     w, mt, tr = AdapterPlan.pack(slots, 7, tile_rows=tile_rows)
     n = w[0]
-    assert w.size == AdapterPlan.words(T, mt) and n <= mt
-    perm = w[4 + 4 * mt:]
-    assert sorted(perm) == list(range(T))
-    seen = 0
-    for s, first, rows, _ in w[4:4 + 4 * n].reshape(n, 4):
-        assert first == seen and 0 < rows <= tr
-        assert (slots[perm[first:first + rows]] == s).all()
-        seen += rows
-    assert seen == T
+    assert w.size == AdapterPlan.words(mt, tr) and n <= mt
+    seen = []
+    for i, (s, rows, _, _) in enumerate(w[4:4 + 4 * n].reshape(n, 4)):
+        assert 0 < rows <= tr
+        r = w[4 + 4 * mt + i * tr:][:rows]
+        assert (slots[r] == s).all()
+        seen += r.tolist()
+    assert sorted(seen) == list(range(T))
 
 
 def test_plan_refusals():

@@ -204,8 +204,8 @@ def test_lora_bad_plan_is_reported():
     """A plan buffer that names rows or slots that do not exist is refused on the device, with the status word set."""
     y, x, a, b, sc, rk, sl = make(4, 128, [64], 8, 2, False)
     bank = AdapterBank(a.to(DEV), b.to(DEV), sc.to(DEV), rk.to(DEV), sl)
-    for at, val in ((4, 2), (5, 3), (6, 99), (4 + 4 * 2, 4), (4 + 4 * 2, -1)):
-        w, mt, tr = AdapterPlan.pack(np.array([0, 0, 1, 1]), 2)
+    for tile_rows, at, val in [(tr, *q) for tr in (16, 128) for q in ((0, 3), (4, 2), (5, 129), (5, -1), (12, 4), (12, -1))]:
+        w, mt, tr = AdapterPlan.pack(np.array([0, 0, 1, 1]), 2, tile_rows=tile_rows)
         assert mt == 2
         w[at] = val
         plan = AdapterPlan(torch.from_numpy(w).to(DEV), 4, mt, tr, 2)
@@ -213,3 +213,25 @@ def test_lora_bad_plan_is_reported():
         with pytest.raises(K.KernelFaultError):
             K.check_status(torch.device(DEV, 0))
     K.check_status(torch.device(DEV, 0))
+
+
+def test_lora_refusals():
+    y, x, a, b, sc, rk, sl = make(4, 32, [16, 8], 8, 3, False)
+    bank = AdapterBank(a.to(DEV), b.to(DEV), sc.to(DEV), rk.to(DEV), sl)
+    y, x = y.to(DEV), x.to(DEV)
+    plan = AdapterPlan.build([0, 1, 2, -1], 3, DEV)
+    q = torch.zeros(4, 32, device=DEV).to(torch.float8_e4m3fn)
+    buf = torch.zeros(8 * 24, dtype=torch.bfloat16, device=DEV)
+    yv = buf[:96].view(4, 24)
+    for args in ((y[:, :23], x, plan), (y.float(), x, plan), (y, x[:, :31], plan), (y, x[:3], plan), (y, x.half(), plan),
+                 (y, torch.zeros(32, 4, dtype=torch.bfloat16, device=DEV).t(), plan), (y, (q, torch.ones(4, 1, device=DEV)), plan),
+                 (y, (q, torch.ones(4)), plan), (y, (x, torch.ones(4, device=DEV)), plan), (y, q, plan),
+                 (y, x, AdapterPlan.build([0, 1, 2], 3, DEV)), (y, x, AdapterPlan.build([0, 1, 2, 0], 4, DEV)),
+                 (y, x, AdapterPlan.build([0, 1, 2, 0], 3, "cpu")), (y, x, plan, y.float()), (y, x, plan, y[:3]),
+                 (yv, x, plan, buf[24:120].view(4, 24)),                      # overlaps y but is not y
+                 (y, x, plan, x[:, :24]),                                     # overlaps x
+                 (y, x, plan, y[:1].expand(4, 24))):                          # rows on top of one another
+        with pytest.raises(ValueError):
+            K.lora_add(args[0], args[1], bank, args[2], out=args[3] if len(args) > 3 else None)
+    assert K.lora_add(y[:0], x[:0], bank, AdapterPlan.build([], 3, DEV)).shape == (0, 24)
+    K.check_status(y.device)

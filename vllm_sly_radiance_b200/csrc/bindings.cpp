@@ -144,10 +144,7 @@ void allreduce_oneshot(std::vector<int64_t> peers, int64_t rank, torch::Tensor i
                        int64_t slot_bytes, torch::Tensor out, torch::Tensor residual,
                        torch::Tensor weight, double eps, torch::Tensor res_out, torch::Tensor q,
                        torch::Tensor scale, int64_t num_blocks, torch::Tensor status);
-void lora_add(torch::Tensor y, torch::Tensor x, torch::Tensor xs, torch::Tensor a, torch::Tensor b,
-              torch::Tensor scale, torch::Tensor ranks, std::vector<int64_t> slices,
-              torch::Tensor plan, int64_t max_tiles, int64_t tile_rows, torch::Tensor out,
-              torch::Tensor status);
+void lora_bind(pybind11::module_& m);
 void cache_move(torch::Tensor table, torch::Tensor pieces, torch::Tensor status, int64_t num_items,
                 torch::Tensor groups, torch::Tensor dst);
 }  // namespace rad
@@ -211,7 +208,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "decode W4A8 GEMM with its producer fused in (1: add + RMSNorm + e4m3, 2: SiLU*mul + e4m3)");
   m.def("push_allreduce_recv", &rad::push_allreduce_recv,
         "receiving half of the GEMM-fused all-reduce (+ add / RMSNorm / e4m3 quant)");
-  m.def("lora_add", &rad::lora_add, "projection output + the low-rank deltas of each row's adapter");
+  rad::lora_bind(m);
   m.def("cache_move", &rad::cache_move, "cache items (pages, states) -> other items of the same caches");
   m.def("ipc_handle", &rad::ipc_handle, "CUDA IPC handle of a device buffer");
   m.def("ipc_open", &rad::ipc_open, "open a peer's IPC handle -> device pointer");

@@ -1,13 +1,22 @@
 // Low-rank adapters of many requests beside a shared projection.
 //
-//   v[t, s, j] = x[t, :] . A[l, s, j, :]                                  j < rank[l]
-//   out[t, n]  = y[t, n] + scale[l] * sum_j v[t, s(n), j] * B[l, n, j]    l = slot of row t, or y[t, n] for none
+//   v[t, s, j] = scale[l] * x[t, :] . A[l, s, j, :]                  j < rank[l], l = slot of row t
+//   out[t, n]  = y[t, n] + sum_j v[t, s(n), j] * B[l, n, j]          or y[t, n] for a row without an adapter
 //
 // x: bf16 rows, or e4m3 rows with one fp32 scale each (the pair a W4A8 linear takes).  A [L, S, R, K], B [L, N, R]
 // bf16; s(n) is the part of a merged projection that output feature n belongs to.  The rows come sorted by adapter in
-// tiles of one adapter each (the plan); a tile of rows without an adapter only carries y over when out is not y.
+// tiles of one adapter each (the plan): 16 rows a tile for decode batches, 128 for prompts.
 //
-// plan (int32): [0] tiles in use, [4 ...] (slot, first position, rows, 0) per tile, then the row of each position.
+// plan (int32): [0] tiles in use; from word 4 (slot, rows, 0, 0) per tile; then tile_rows row numbers per tile.
+//
+// Three forms:
+//   decode_kernel           16-row tiles, all CTAs at once on the SMs: one launch, latency bound
+//   shrink16 + expand16     more 16-row tiles: two launches that overlap, bound by the adapters' bytes
+//   shrink128 + expand128   128-row tiles: tcgen05, bound by x, y and out
+//
+// Rounding: products of bf16 (or e4m3) numbers are exact in the MMA and summed in 32 bits.  v enters the second product
+// as the sum of two bf16 numbers, so that its error is 2^-16 and not 2^-8: the second half doubles MMAs that wait on
+// memory anyway.  The result is rounded once.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -32,31 +41,47 @@ struct Args {
   __nv_bfloat16* out;
   int64_t out_ld;
   const int* plan;
-  float* v;                 // [splits, T, S, Rp], by position
+  float* v;                 // 16-row tiles: fp32 [splits, tile rows, S, Rp]; 128: bf16 [tile rows, S, 2, Rp]
   int* status;
-  int T, K, N, L, S, R, max_tiles;
+  int T, K, N, L, S, R, max_tiles, tile_rows;
   int Rp;                   // R rounded up to 16: row of v
-  int splits;               // shares of K, one partial v each
+  int splits;               // shares of K
+  int steps;                // feature steps of a CTA
   int off[MAX_S + 1];       // slice s = output features [off[s], off[s + 1])
 };
 
-struct Tile { int slot, first, rows, rank; };
+struct Tile { int slot, rows, rank; };
 
+// Tile i < max_tiles.  False: not in use, or a plan of other rows or adapters (refused, status word).  The count and
+// the record are read together.
 DEVI bool load_tile(const Args& p, int i, Tile& t) {
-  const int4 q = reinterpret_cast<const int4*>(p.plan + 4)[i];
-  t.slot = q.x; t.first = q.y; t.rows = q.z; t.rank = 0;
-  if (q.x >= p.L || q.y < 0 || q.z < 0 || q.y > p.T - q.z) {      // a plan of other rows or adapters: refused
+  const int n = p.plan[0];
+  const int2 q = *reinterpret_cast<const int2*>(p.plan + 4 + 4 * (int64_t)i);
+  t.slot = q.x; t.rows = q.y; t.rank = 0;
+  if (i >= n) return false;
+  if (q.x >= p.L || q.y < 0 || q.y > p.tile_rows || n > p.max_tiles) {
     if (threadIdx.x == 0) atomicExch(p.status, (int)kErrBounds);
     return false;
   }
   if (q.x >= 0) t.rank = min(max(p.rank[q.x], 0), p.R);
   return true;
 }
-DEVI const int* perm(const Args& p) { return p.plan + 4 + 4 * p.max_tiles; }
-DEVI int row_of(const Args& p, int pos) {
-  const int r = perm(p)[pos];
-  if (r < 0 || r >= p.T) { atomicExch(p.status, (int)kErrBounds); return -1; }
-  return r;
+// row number of row r of tile i (-1: beyond the tile, or refused)
+DEVI int row_of(const Args& p, int i, int r, int rows) {
+  const int v = p.plan[4 + 4 * (int64_t)p.max_tiles + (int64_t)i * p.tile_rows + r];
+  if (r >= rows) return -1;
+  if (v < 0 || v >= p.T) {
+    atomicExch(p.status, (int)kErrBounds);
+    return -1;
+  }
+  return v;
+}
+// slice of the CTA's `span` output features: -> first feature, end of the slice
+DEVI int slice_of(const Args& p, int ch, int span, int& s, int& ne) {
+  s = 0;
+  while (ch >= (p.off[s + 1] - p.off[s] + span - 1) / span) ch -= (p.off[s + 1] - p.off[s] + span - 1) / span, ++s;
+  ne = p.off[s + 1];
+  return p.off[s] + ch * span;
 }
 
 // D[16 x 8] += A[16 x 16] B[16 x 8], bf16 with 32-bit sums
@@ -107,73 +132,6 @@ DEVI uint4 load8(const void* row, int k, int K) {
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
 
-// v, small tiles.  One CTA per (16 rank rows of a slice, share of K) and 16 rows at a time; its warps split the share.
-// The adapter's rank rows are the 16-row operand of the MMA and the tokens its 8 columns.  Both operands go from global
-// memory straight to registers: the sum over k has no order, so the four threads that share a rank row or a token each
-// take 8 neighbouring k of a 32-block (16 bytes) and hand them to two MMAs in the same, permuted, order on both sides.
-// The shares of K leave one partial v each; the expanding kernel adds them up in their order.
-template <bool FP8, bool VEC>
-__global__ void __launch_bounds__(256) shrink_kernel(const __grid_constant__ Args p) {
-  __shared__ float red[8][16][20];                       // [warp][token][rank]
-  pdl_wait();
-  pdl_trigger();
-  const int nt = min(p.plan[0], p.max_tiles), warp = threadIdx.x / 32, lane = threadIdx.x & 31;
-  const int groups = p.Rp / 16, s = blockIdx.y / groups, j0 = blockIdx.y % groups * 16;
-  const int g = lane >> 2, k8 = (lane & 3) * 8;
-  const int per = ((p.K + 31) / 32 + gridDim.z * 8 - 1) / (gridDim.z * 8) * 32;
-  const int kb = (blockIdx.z * 8 + warp) * per, ke = min(kb + per, p.K);
-  for (int i = blockIdx.x; i < nt; i += gridDim.x) {
-    Tile t;
-    if (!load_tile(p, i, t) || j0 >= t.rank) continue;   // uniform over the CTA
-    const __nv_bfloat16* a = p.a + ((int64_t)(t.slot * p.S + s) * p.R + j0) * p.K;
-    const bool u0 = j0 + g < t.rank, u1 = j0 + g + 8 < t.rank;
-    for (int m0 = 0; m0 < t.rows; m0 += 16) {
-      const uint8_t* x[2] = {nullptr, nullptr};
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        if (m0 + 8 * h + g < t.rows) {
-          const int r = row_of(p, t.first + m0 + 8 * h + g);
-          if (r >= 0) x[h] = static_cast<const uint8_t*>(p.x) + r * p.x_ld * (FP8 ? 1 : 2);
-        }
-      const bool two = m0 + 8 < t.rows;
-      float c[2][4] = {};
-#pragma unroll 4
-      for (int k = kb; k < ke; k += 32) {
-        const uint4 z = make_uint4(0, 0, 0, 0);
-        const uint4 a0 = u0 ? load8<false, VEC>(a + (int64_t)g * p.K, k + k8, p.K) : z;
-        const uint4 a1 = u1 ? load8<false, VEC>(a + (int64_t)(g + 8) * p.K, k + k8, p.K) : z;
-        const uint4 x0 = x[0] ? load8<FP8, VEC>(x[0], k + k8, p.K) : z;
-        mma_16816(c[0], a0.x, a1.x, a0.y, a1.y, x0.x, x0.y);
-        mma_16816(c[0], a0.z, a1.z, a0.w, a1.w, x0.z, x0.w);
-        if (two) {
-          const uint4 x1 = x[1] ? load8<FP8, VEC>(x[1], k + k8, p.K) : z;
-          mma_16816(c[1], a0.x, a1.x, a0.y, a1.y, x1.x, x1.y);
-          mma_16816(c[1], a0.z, a1.z, a0.w, a1.w, x1.z, x1.w);
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) red[warp][8 * h + 2 * (lane & 3) + (e & 1)][g + 8 * (e >> 1)] = c[h][e];
-      __syncthreads();
-      const int m = threadIdx.x / 16, j = threadIdx.x % 16;
-      if (m0 + m < t.rows) {
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < 8; ++w) v += red[w][m][j];
-        const int pos = t.first + m0 + m;
-        float f = p.scale[t.slot];
-        if (FP8) {
-          const int r = row_of(p, pos);
-          f *= r >= 0 ? p.xs[r] : 0.f;
-        }
-        p.v[(((int64_t)blockIdx.z * p.T + pos) * p.S + s) * p.Rp + j0 + j] = v * f;
-      }
-      __syncthreads();
-    }
-  }
-}
-
 // 8 neighbouring features of a row from `at` on, those below ne
 template <bool VEC>
 DEVI uint4 load_y(const __nv_bfloat16* row, int at, int ne) {
@@ -185,189 +143,852 @@ DEVI uint4 load_y(const __nv_bfloat16* row, int at, int ne) {
   return v;
 }
 
-// out = y + v B.  A warp takes 16 rows and steps over the features by 64.  The 8 columns of MMA m of a 32-feature block
-// are the features 8 (c / 2) + 2 m + c % 2, so that each thread ends with 8 neighbouring features of two rows: y and out
-// move in 16-byte vectors and nothing is staged; y of the next step is on its way during the MMAs of this one.  v is
-// held as the sum of two bf16 numbers (its error is then 2^-16, not 2^-8), which doubles MMAs that wait on memory
-// anyway.  MB: 16-row blocks of a tile, one per warp; with MB = 1 the warps take neighbouring features instead.  KBC:
-// rank blocks of 16 whose v stays in registers; NS: steps of a warp.
-template <int KBC, int MB, bool VEC>
-__global__ void __launch_bounds__(256, 2) expand_kernel(const __grid_constant__ Args p) {
-  constexpr int WN = 8 / MB, NS = MB == 1 ? 1 : 4, CH = 64 * NS * WN;      // CH: features of a CTA
+// four 32-bit values of v as two bf16 numbers each: the second holds what the first rounds off (error 2^-16)
+DEVI void split_v(float4 f, bool use, uint32_t& h0, uint32_t& h1, uint32_t& l0, uint32_t& l1) {
+  const float u[4] = {use ? f.x : 0.f, use ? f.y : 0.f, use ? f.z : 0.f, use ? f.w : 0.f};
+  float d[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    d[e] = u[e] - bf16_round(u[e]);
+    if (!(fabsf(d[e]) <= 3.4e38f)) d[e] = 0.f;             // infinities and NaN stay in the first number
+  }
+  h0 = pack2(u[0], u[1]); h1 = pack2(u[2], u[3]);
+  l0 = pack2(d[0], d[1]); l1 = pack2(d[2], d[3]);
+}
+
+// out = y + c for the 16 rows x 32 NB features of second_product (add: false, out = y)
+template <int NB, bool VEC>
+DEVI void store_step(__nv_bfloat16* const (&to)[2], const __nv_bfloat16* const (&yr)[2], const uint4 (&y)[NB][2],
+                     const float (&c)[NB][4][4], int n0, int ne, bool add) {
+  const int q4 = threadIdx.x & 3;
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int at = n0 + 32 * n + 8 * q4;
+      if (yr[h] == nullptr || at >= ne) continue;
+      uint4 o = y[n][h];
+      if (add) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+          const __nv_bfloat162 f = *reinterpret_cast<const __nv_bfloat162*>(&w[m]);
+          w[m] = pack2(__low2float(f) + c[n][m][2 * h], __high2float(f) + c[n][m][2 * h + 1]);
+        }
+      }
+      if (VEC && at + 8 <= ne) *reinterpret_cast<uint4*>(to[h] + at) = o;
+      else
+        for (int e = 0; e < 8; ++e)
+          if (at + e < ne) to[h][at + e] = reinterpret_cast<const __nv_bfloat16*>(&o)[e];
+    }
+}
+
+// ---------------------------------------------------------------------------------------------
+// 16-row tiles
+// ---------------------------------------------------------------------------------------------
+// First product of one warp's share of k: the adapter's rank rows are the 16-row operand of the MMA and the tokens its 8
+// columns.  Both operands go from global memory straight to registers: the sum over k has no order, so the four threads
+// that share a rank row or a token each take 8 neighbouring k of a 32-block (16 bytes) and hand them to two MMAs in the
+// same, permuted, order on both sides.  The warp's sums go to red[warp][token][rank].  JG: 16-row rank groups.
+template <int JG> constexpr int RS = 16 * JG + 4;          // row of red: the fragment writes meet no bank twice
+
+template <int JG, bool FP8, bool VEC>
+DEVI void first_product(const Args& p, const __nv_bfloat16* a, const uint8_t* const (&x)[2], bool two, int ranks, int kb,
+                        int ke, float* red) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
-  int s = 0, ch = blockIdx.x;
-  while (ch >= (p.off[s + 1] - p.off[s] + CH - 1) / CH) ch -= (p.off[s + 1] - p.off[s] + CH - 1) / CH, ++s;
-  const int nb = p.off[s] + ch * CH + warp % WN * 64 * NS, ne = p.off[s + 1];
-  const int nt = min(p.plan[0], p.max_tiles), mb = warp / WN * 16;
-  bool first = true;
-  for (int i = blockIdx.y; i < nt; i += gridDim.y) {
-    Tile t;
-    const bool ok = load_tile(p, i, t) && !(t.slot < 0 && p.out == p.y);
-    for (int m0 = mb; ok && m0 < t.rows && nb < ne; m0 += 16 * MB) {
-      const __nv_bfloat16* yr[2];
-      __nv_bfloat16* to[2];
-      uint4 y[2][2];
+  float c[JG][2][4] = {};
+#pragma unroll 2
+  for (int k = kb; k < ke; k += 32) {
+    const uint4 z = make_uint4(0, 0, 0, 0);
+    uint4 xa[2], aa[JG][2];
+    xa[0] = x[0] ? load8<FP8, VEC>(x[0], k + 8 * q4, p.K) : z;
+    xa[1] = two && x[1] ? load8<FP8, VEC>(x[1], k + 8 * q4, p.K) : z;
+#pragma unroll
+    for (int j = 0; j < JG; ++j)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int r = m0 + 8 * h + g < t.rows ? row_of(p, t.first + m0 + 8 * h + g) : -1;
-        yr[h] = r >= 0 ? p.y + r * p.y_ld : nullptr;
-        to[h] = p.out + r * p.out_ld;
-        // y was complete before the shrinking kernel started: it is read ahead of the wait for that kernel
-#pragma unroll
-        for (int n = 0; n < 2; ++n) y[n][h] = load_y<VEC>(yr[h], nb + 32 * n + 8 * q4, ne);
+        const int jr = 16 * j + 8 * h + g;
+        aa[j][h] = jr < ranks ? load8<false, VEC>(a + (int64_t)jr * p.K, k + 8 * q4, p.K) : z;
       }
-      if (first) pdl_wait();
-      first = false;
-      uint32_t vh[KBC][4], vl[KBC][4];
-#pragma unroll 1
-      for (int st = 0; st < NS; ++st) {
-        const int n0 = nb + 64 * st;
-        if (n0 >= ne) break;
-        uint4 yn[2][2];
-        if (NS > 1 && st + 1 < NS) {
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+    for (int j = 0; j < JG; ++j)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) yn[n][h] = load_y<VEC>(yr[h], n0 + 64 + 32 * n + 8 * q4, ne);
+      for (int h = 0; h < 2; ++h)
+        if (h == 0 || two) {
+          mma_16816(c[j][h], aa[j][0].x, aa[j][1].x, aa[j][0].y, aa[j][1].y, xa[h].x, xa[h].y);
+          mma_16816(c[j][h], aa[j][0].z, aa[j][1].z, aa[j][0].w, aa[j][1].w, xa[h].z, xa[h].w);
         }
-        float c[2][4][4] = {};
+  }
+#pragma unroll
+  for (int j = 0; j < JG; ++j)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        red[(warp * 16 + 8 * h + 2 * q4 + (e & 1)) * RS<JG> + 16 * j + g + 8 * (e >> 1)] = c[j][h][e];
+}
+template <int JG>
+DEVI float red_sum(const float* red, int o) {
+  float f = 0.f;
+#pragma unroll
+  for (int w = 0; w < 8; ++w) f += red[(w * 16 + o / (16 * JG)) * RS<JG> + o % (16 * JG)];
+  return f;
+}
+
+// B of NB 32-feature blocks and JG rank groups from rank k0 on, in the fragments' order: the 8 columns of MMA m of a block
+// are the features 8 (c / 2) + 2 m + c % 2, so that each thread ends with 8 neighbouring features of two rows.  Ranks
+// beyond the adapter's own count as zero.
+template <int JG, int NB, bool VEC>
+DEVI void load_b(const __nv_bfloat16* bt, int R, int n0, int ne, int k0, int rank, uint2 (&w)[NB][4][JG]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+#pragma unroll
+  for (int n = 0; n < NB; ++n)
+#pragma unroll
+    for (int m = 0; m < 4; ++m) {
+      const int nn = n0 + 32 * n + 8 * (g >> 1) + 2 * m + (g & 1);
+      const __nv_bfloat16* b = bt + (int64_t)nn * R + k0 + 4 * q4;
+#pragma unroll
+      for (int k = 0; k < JG; ++k) {
+        w[n][m][k] = make_uint2(0, 0);
+        const int left = rank - (k0 + 16 * k + 4 * q4);
+        if (nn < ne && left > 0) {
+          if (VEC) {                                       // R is a multiple of 4
+            w[n][m][k] = *reinterpret_cast<const uint2*>(b + 16 * k);
+          } else {
 #pragma unroll 1
-        for (int k0 = 0; k0 < t.rank; k0 += 16 * KBC) {
-          if (st == 0 || t.rank > 16 * KBC) {
-#pragma unroll
-            for (int k = 0; k < KBC; ++k)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (m0 + 8 * h + g < t.rows && k0 + 16 * k < t.rank)
-#pragma unroll 1
-                  for (int z = 0; z < p.splits; ++z) {
-                    const float4 w = *reinterpret_cast<const float4*>(
-                        p.v + (((int64_t)z * p.T + t.first + m0 + 8 * h + g) * p.S + s) * p.Rp + k0 + 16 * k + 4 * q4);
-                    f.x += w.x; f.y += w.y; f.z += w.z; f.w += w.w;
-                  }
-                const float u[4] = {f.x, f.y, f.z, f.w};
-                float d[4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  d[e] = u[e] - bf16_round(u[e]);
-                  if (!(fabsf(d[e]) <= 3.4e38f)) d[e] = 0.f;   // infinities and NaN stay in the first number
-                }
-                vh[k][h] = pack2(u[0], u[1]); vh[k][h + 2] = pack2(u[2], u[3]);
-                vl[k][h] = pack2(d[0], d[1]); vl[k][h + 2] = pack2(d[2], d[3]);
-              }
+            for (int e = 0; e < min(left, 4); ++e)
+              (e < 2 ? w[n][m][k].x : w[n][m][k].y) |= (uint32_t)__bfloat16_as_ushort(b[16 * k + e]) << 16 * (e & 1);
           }
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-              const int nn = n0 + 32 * n + 8 * (g >> 1) + 2 * m + (g & 1);
-              const __nv_bfloat16* b = p.b + ((int64_t)t.slot * p.N + nn) * p.R + k0 + 4 * q4;
-#pragma unroll
-              for (int k = 0; k < KBC; ++k) {
-                uint2 w = make_uint2(0, 0);
-                const int left = t.rank - (k0 + 16 * k + 4 * q4);    // ranks beyond the adapter's own are not read
-                if (nn < ne && left > 0) {
-                  if (VEC) {                                         // R is a multiple of 4
-                    w = *reinterpret_cast<const uint2*>(b + 16 * k);
-                    if (left < 4) {
-                      w.x &= left == 1 ? 0xffffu : ~0u;
-                      w.y &= left == 3 ? 0xffffu : 0u;
-                    }
-                  } else {
-#pragma unroll 1
-                    for (int e = 0; e < min(left, 4); ++e)
-                      (e < 2 ? w.x : w.y) |= (uint32_t)__bfloat16_as_ushort(b[16 * k + e]) << 16 * (e & 1);
-                  }
-                }
-                mma_16816(c[n][m], vl[k][0], vl[k][1], vl[k][2], vl[k][3], w.x, w.y);
-                mma_16816(c[n][m], vh[k][0], vh[k][1], vh[k][2], vh[k][3], w.x, w.y);
-              }
-            }
         }
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int at = n0 + 32 * n + 8 * q4;
-            if (yr[h] == nullptr || at >= ne) continue;
-            uint4 o = y[n][h];
-            if (t.slot >= 0) {
-              uint32_t* w = reinterpret_cast<uint32_t*>(&o);
-#pragma unroll
-              for (int m = 0; m < 4; ++m) {
-                const __nv_bfloat162 f = *reinterpret_cast<const __nv_bfloat162*>(&w[m]);
-                w[m] = pack2(__low2float(f) + c[n][m][2 * h], __high2float(f) + c[n][m][2 * h + 1]);
-              }
-            }
-            if (VEC && at + 8 <= ne) *reinterpret_cast<uint4*>(to[h] + at) = o;
-            else
-              for (int e = 0; e < 8; ++e)
-                if (at + e < ne) to[h][at + e] = reinterpret_cast<const __nv_bfloat16*>(&o)[e];
-          }
-        if (NS > 1) {
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) y[n][h] = yn[n][h];
+        if (VEC && left < 4) {
+          w[n][m][k].x &= left == 1 ? 0xffffu : ~0u;
+          w[n][m][k].y &= left == 3 ? 0xffffu : 0u;
         }
       }
     }
+}
+// the MMAs of load_b's block; v: shared memory [16][vs], from rank k0 on
+template <int JG, int NB>
+DEVI void second_product(const float* v, int vs, int left, int rows, const uint2 (&w)[NB][4][JG], float (&c)[NB][4][4]) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+#pragma unroll
+  for (int k = 0; k < JG; ++k) {
+    if (16 * k >= left) break;
+    uint32_t vh[4], vl[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      split_v(*reinterpret_cast<const float4*>(v + (8 * h + g) * vs + 16 * k + 4 * q4), 8 * h + g < rows, vh[h], vh[h + 2],
+              vl[h], vl[h + 2]);
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int m = 0; m < 4; ++m) {
+        mma_16816(c[n][m], vl[0], vl[1], vl[2], vl[3], w[n][m][k].x, w[n][m][k].y);
+        mma_16816(c[n][m], vh[0], vh[1], vh[2], vh[3], w[n][m][k].x, w[n][m][k].y);
+      }
   }
-  if (first) pdl_wait();
-  pdl_trigger();
 }
 
-template <int KBC>
-void launch_expand(const Args& p, bool tall, bool vec, unsigned tiles, cudaStream_t stream) {
-  const int ch = tall ? 256 : 512;
-  unsigned chunks = 0;
-  for (int s = 0; s < p.S; ++s) chunks += (p.off[s + 1] - p.off[s] + ch - 1) / ch;
-  auto k = tall ? (vec ? expand_kernel<KBC, 8, true> : expand_kernel<KBC, 8, false>)
-                : (vec ? expand_kernel<KBC, 1, true> : expand_kernel<KBC, 1, false>);
-  C10_CUDA_CHECK(launch_pdl(k, dim3(chunks, tiles), dim3(256), 0, stream, p));
+// Both products in one launch.  A cluster of 8 CTAs owns (16 rows of one adapter, up to 8 x 512 x steps features of one
+// slice): its CTAs and their warps share K, add up v through distributed shared memory in a fixed order, and each CTA
+// then expands its own features.  A's rows are read once per cluster (again from L2 where a slice takes several), B once.
+constexpr int CL = 8;
+
+template <int JG, bool FP8, bool VEC>
+__global__ void __launch_bounds__(256, 2) decode_kernel(const __grid_constant__ Args p) {
+  constexpr int NB = JG == 4 ? 1 : 2, STEP = 8 * 32 * NB;  // features of a CTA's step
+  extern __shared__ float sm[];
+  float* red = sm;                                         // [8 warps][16 tokens][RS]
+  float* part = red + 8 * 16 * RS<JG>;                     // [16][16 JG] this CTA's share of v
+  float* v = part + 16 * 16 * JG;                          // [16][Rp + 4]
+  const int vs = p.Rp + 4, i = blockIdx.y;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  const int cr = cluster_ctarank();
+  int s, ne;
+  const int nb = slice_of(p, blockIdx.x / CL, CL * STEP * p.steps, s, ne) + cr * STEP * p.steps + warp * 32 * NB;
+  const int per = ((p.K + 31) / 32 + CL * 8 - 1) / (CL * 8) * 32;
+  const int kb = (cr * 8 + warp) * per, ke = min(kb + per, p.K);
+  pdl_wait();
+  pdl_trigger();
+  Tile t;
+  if (!load_tile(p, i, t) || (t.slot < 0 && p.out == p.y)) return;         // uniform over the cluster
+  const __nv_bfloat16* yr[2];
+  __nv_bfloat16* to[2];
+  const uint8_t* x[2];
+  uint4 y[NB][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = row_of(p, i, 8 * h + g, t.rows);
+    x[h] = r >= 0 ? static_cast<const uint8_t*>(p.x) + r * p.x_ld * (FP8 ? 1 : 2) : nullptr;
+    yr[h] = r >= 0 ? p.y + r * p.y_ld : nullptr;
+    to[h] = p.out + r * p.out_ld;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) y[n][h] = load_y<VEC>(yr[h], nb + 32 * n + 8 * q4, ne);
+  }
+  const __nv_bfloat16* bt = p.b + (int64_t)max(t.slot, 0) * p.N * p.R;
+  uint2 w[NB][4][JG];                                      // B of the first step, on its way during the first product
+  load_b<JG, NB, VEC>(bt, p.R, nb, ne, 0, t.rank, w);
+  for (int j0 = 0; j0 < t.rank; j0 += 16 * JG) {
+    const __nv_bfloat16* a = p.a + ((int64_t)(t.slot * p.S + s) * p.R + j0) * p.K;
+    first_product<JG, FP8, VEC>(p, a, x, t.rows > 8, t.rank - j0, kb, ke, red);
+    if (j0) cluster_wait();                                // every share of the ranks before read
+    __syncthreads();
+#pragma unroll
+    for (int o = threadIdx.x; o < 256 * JG; o += 256) part[o] = red_sum<JG>(red, o);
+    cluster_sync();
+#pragma unroll
+    for (int o = threadIdx.x; o < 256 * JG; o += 256) {
+      float f[CL], sum = 0.f;
+#pragma unroll
+      for (int c = 0; c < CL; ++c)
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(f[c]) : "r"(mapa_shared(smem_u32(part + o), c)));
+#pragma unroll
+      for (int c = 0; c < CL; ++c) sum += f[c];
+      const int m = o / (16 * JG);
+      sum *= p.scale[t.slot];
+      if (FP8) {
+        const int r = row_of(p, i, m, t.rows);
+        sum *= r >= 0 ? p.xs[r] : 0.f;
+      }
+      if (j0 + o % (16 * JG) < p.Rp) v[m * vs + j0 + o % (16 * JG)] = sum;
+    }
+    cluster_arrive();
+  }
+  __syncthreads();
+#pragma unroll 1
+  for (int st = 0; st < p.steps; ++st) {
+    const int n0 = nb + STEP * st;
+    if (n0 >= ne) break;
+    uint4 yn[NB][2];
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        yn[n][h] = st + 1 < p.steps ? load_y<VEC>(yr[h], n0 + STEP + 32 * n + 8 * q4, ne) : make_uint4(0, 0, 0, 0);
+    float c[NB][4][4] = {};
+#pragma unroll 1
+    for (int k0 = 0; k0 < t.rank; k0 += 16 * JG) {
+      if (st || k0) load_b<JG, NB, VEC>(bt, p.R, n0, ne, k0, t.rank, w);
+      second_product<JG, NB>(v + k0, vs, t.rank - k0, t.rows, w, c);
+    }
+    store_step<NB, VEC>(to, yr, y, c, n0, ne, t.slot >= 0);
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) y[n][h] = yn[n][h];
+  }
+  if (t.rank > 0) cluster_wait();                          // the other CTAs have read this one's share
+}
+
+// v of 16-row tiles: one CTA per (tile, 16 JG rank rows of a slice, share of K).  The shares leave one partial v each, which
+// the expanding kernel adds up in order.
+template <int JG, bool FP8, bool VEC>
+__global__ void __launch_bounds__(256) shrink16_kernel(const __grid_constant__ Args p) {
+  __shared__ float red[8 * 16 * RS<JG>];
+  pdl_wait();
+  pdl_trigger();
+  const int i = blockIdx.x, groups = (p.Rp + 16 * JG - 1) / (16 * JG);
+  const int s = blockIdx.y / groups, j0 = blockIdx.y % groups * 16 * JG;
+  const int warp = threadIdx.x / 32, g = (threadIdx.x & 31) >> 2;
+  Tile t;
+  if (!load_tile(p, i, t) || j0 >= t.rank) return;         // uniform over the CTA
+  const uint8_t* x[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = row_of(p, i, 8 * h + g, t.rows);
+    x[h] = r >= 0 ? static_cast<const uint8_t*>(p.x) + r * p.x_ld * (FP8 ? 1 : 2) : nullptr;
+  }
+  const int per = ((p.K + 31) / 32 + p.splits * 8 - 1) / (p.splits * 8) * 32;
+  const int kb = (blockIdx.z * 8 + warp) * per;
+  first_product<JG, FP8, VEC>(p, p.a + ((int64_t)(t.slot * p.S + s) * p.R + j0) * p.K, x, t.rows > 8, t.rank - j0, kb,
+                              min(kb + per, p.K), red);
+  __syncthreads();
+#pragma unroll
+  for (int o = threadIdx.x; o < 256 * JG; o += 256) {
+    const int m = o / (16 * JG), j = j0 + o % (16 * JG);
+    if (m >= t.rows || j >= p.Rp) continue;
+    float f = p.scale[t.slot];
+    if (FP8) {
+      const int r = row_of(p, i, m, t.rows);
+      f *= r >= 0 ? p.xs[r] : 0.f;
+    }
+    p.v[(((int64_t)blockIdx.z * p.max_tiles + i) * 16 + m) * p.S * p.Rp + s * p.Rp + j] = red_sum<JG>(red, o) * f;
+  }
+}
+
+// out of 16-row tiles.  B and y, which do not depend on v, are read ahead of the wait for the shrinking kernel: that kernel
+// itself waited for whatever wrote them.
+template <int JG, bool VEC>
+__global__ void __launch_bounds__(256, 2) expand16_kernel(const __grid_constant__ Args p) {
+  constexpr int NB = JG == 4 ? 1 : 2, STEP = 8 * 32 * NB;
+  extern __shared__ float v[];                             // [16][Rp + 4]
+  const int vs = p.Rp + 4, i = blockIdx.y;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  int s, ne;
+  const int nb = slice_of(p, blockIdx.x, STEP, s, ne) + warp * 32 * NB;
+  Tile t;
+  if (!load_tile(p, i, t) || (t.slot < 0 && p.out == p.y)) {
+    pdl_wait();
+    return;
+  }
+  const __nv_bfloat16* yr[2];
+  __nv_bfloat16* to[2];
+  uint4 y[NB][2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = row_of(p, i, 8 * h + g, t.rows);
+    yr[h] = r >= 0 ? p.y + r * p.y_ld : nullptr;
+    to[h] = p.out + r * p.out_ld;
+#pragma unroll
+    for (int n = 0; n < NB; ++n) y[n][h] = load_y<VEC>(yr[h], nb + 32 * n + 8 * q4, ne);
+  }
+  const __nv_bfloat16* bt = p.b + (int64_t)max(t.slot, 0) * p.N * p.R;
+  uint2 w[NB][4][JG];
+  load_b<JG, NB, VEC>(bt, p.R, nb, ne, 0, t.rank, w);
+  pdl_wait();
+  pdl_trigger();
+  const int rk = (t.rank + 15) / 16 * 16;
+  for (int o = threadIdx.x; o < t.rows * rk; o += 256) {
+    const int m = o / rk, j = o % rk;
+    const float* q = p.v + (((int64_t)i * 16 + m) * p.S + s) * p.Rp + j;
+    float f[8], sum = 0.f;
+#pragma unroll
+    for (int z = 0; z < 8; ++z) f[z] = z < p.splits ? q[(int64_t)z * p.max_tiles * 16 * p.S * p.Rp] : 0.f;
+#pragma unroll
+    for (int z = 0; z < 8; ++z) sum += f[z];
+    v[m * vs + j] = sum;
+  }
+  __syncthreads();
+  if (nb >= ne) return;
+  float c[NB][4][4] = {};
+#pragma unroll 1
+  for (int k0 = 0; k0 < t.rank; k0 += 16 * JG) {
+    if (k0) load_b<JG, NB, VEC>(bt, p.R, nb, ne, k0, t.rank, w);
+    second_product<JG, NB>(v + k0, vs, t.rank - k0, t.rows, w, c);
+  }
+  store_step<NB, VEC>(to, yr, y, c, nb, ne, t.slot >= 0);
+}
+
+// ---------------------------------------------------------------------------------------------
+// 128-row tiles
+// ---------------------------------------------------------------------------------------------
+DEVI void cp_async16(uint32_t dst, const void* src, bool use) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(use ? 16 : 0) : "memory");
+}
+DEVI void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+DEVI void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+DEVI void st_shared16(uint32_t dst, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+DEVI uint4 ld_shared16(uint32_t src) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src) : "memory");
+  return v;
+}
+// 16-byte chunk `c` of row `r` in an operand tile of 128-byte rows, 128-byte swizzle (tiles 1024-byte aligned)
+DEVI uint32_t sw128(int r, int c) { return (uint32_t)(r * 128 + ((c ^ (r & 7)) << 4)); }
+// kind::f16 instruction descriptor: bf16 x bf16 -> fp32, both K-major, M = 128
+DEVI uint32_t idesc_bf16(int n) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
+}
+// TMEM -> registers: 16 lanes x 32 columns; a thread gets columns 8 m + 2 (lane % 4) + {0, 1} of rows lane / 4 (r[4 m],
+// r[4 m + 1]) and lane / 4 + 8 (r[4 m + 2], r[4 m + 3]), the order of the mma.sync accumulators
+DEVI void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+
+// v of 128-row tiles: D[128 x NC] = X[128 x K] A[NC x K]^T on tcgen05, NC <= 256 rank rows of all slices together, so that x
+// is read once.  The rows are gathered by cp.async into swizzled 64-k stages (e4m3 rows as they are, widened to bf16 in
+// shared memory); a cluster of `splits` CTAs shares K and adds up through distributed shared memory in a fixed order.
+// v leaves as the two bf16 numbers of each value that the expanding kernel multiplies with.
+constexpr int ST = 4;                                      // stages in flight
+
+template <bool FP8, bool VEC>
+__global__ void __launch_bounds__(256) shrink128_kernel(const __grid_constant__ Args p, int nc_max) {
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t bar[ST];
+  __shared__ uint32_t tmem_at;
+  const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, i = blockIdx.x;
+  const int sr0 = blockIdx.y * nc_max, nsr = min(nc_max, p.S * p.R - sr0), nc = (nsr + 15) / 16 * 16;
+  const uint32_t xbytes = 16384, abytes = (uint32_t)((nc_max + 15) / 16) * 2048, sbytes = xbytes + abytes;
+  const uint32_t fp8_at = base + ST * sbytes;              // e4m3 stages [ST][128 x 64]
+  const uint32_t cols = nc <= 32 ? 32 : nc <= 64 ? 64 : nc <= 128 ? 128 : 256;
+  pdl_wait();
+  pdl_trigger();
+  Tile t;
+  if (!load_tile(p, i, t) || t.rank == 0) return;          // uniform over the cluster
+  if (warp == 0) tmem_alloc(&tmem_at, cols);
+  if (tid < ST) mbar_init(&bar[tid], 1);
+  fence_mbar_init();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_at;
+
+  const int nk = (p.K + 63) / 64, per = (nk + p.splits - 1) / p.splits;
+  const int k0 = blockIdx.z * per, n = max(0, min(per, nk - k0));
+  // a thread moves chunk tid % 8 of rows tid / 8 + 32 q (e4m3: chunk tid % 4 of rows tid / 4 + 64 q)
+  const uint8_t* x[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int r = FP8 ? tid / 4 + 64 * q : tid / 8 + 32 * q, row = r < 128 ? row_of(p, i, r, t.rows) : -1;
+    x[q] = row >= 0 ? static_cast<const uint8_t*>(p.x) + row * p.x_ld * (FP8 ? 1 : 2) : nullptr;
+  }
+  const __nv_bfloat16* a = p.a + ((int64_t)t.slot * p.S * p.R + sr0) * p.K;
+  auto load = [&](int j) {                                 // 64-k block j of this CTA's share into its stage
+    const int k = (k0 + j) * 64;
+    const uint32_t xs = base + j % ST * sbytes, as = xs + xbytes;
+    if (FP8) {
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int r = tid / 4 + 64 * q, kk = k + tid % 4 * 16;
+        const uint32_t dst = fp8_at + j % ST * 8192 + r * 64 + tid % 4 * 16;
+        if (x[q] == nullptr) continue;
+        if (VEC && p.K % 16 == 0) cp_async16(dst, x[q] + min(kk, p.K - 16), kk < p.K);
+        else {
+          uint32_t w[4] = {};
+          for (int e = 0; e < 16; ++e)
+            if (kk + e < p.K) w[e / 4] |= (uint32_t)x[q][kk + e] << 8 * (e % 4);
+          st_shared16(dst, make_uint4(w[0], w[1], w[2], w[3]));
+        }
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int r = tid / 8 + 32 * q, kk = k + tid % 8 * 8;
+        if (x[q] == nullptr) continue;
+        if (VEC) cp_async16(xs + sw128(r, tid % 8), x[q] + 2 * min(kk, p.K - 8), kk < p.K);
+        else st_shared16(xs + sw128(r, tid % 8), load8<false, false>(x[q], kk, p.K));
+      }
+    }
+    const int kk = k + tid % 8 * 8;
+    for (int r = tid / 8; r < nsr; r += 32) {
+      if (VEC) cp_async16(as + sw128(r, tid % 8), a + (int64_t)r * p.K + min(kk, p.K - 8), kk < p.K);
+      else st_shared16(as + sw128(r, tid % 8), load8<false, false>(a + (int64_t)r * p.K, kk, p.K));
+    }
+  };
+#pragma unroll
+  for (int j = 0; j < ST - 1; ++j) {
+    if (j < n) load(j);
+    cp_async_commit();
+  }
+  bool ok = true;
+  for (int j = 0; j < n; ++j) {
+    cp_async_wait<ST - 2>();
+    const uint32_t xs = base + j % ST * sbytes, as = xs + xbytes;
+    if (FP8) {                                             // the chunks that this thread itself loaded
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int r = tid / 4 + 64 * q, c = tid % 4;
+        const uint4 f = ld_shared16(fp8_at + j % ST * 8192 + r * 64 + c * 16);
+        const uint2 e0 = e4m3x4_to_bf16(f.x), e1 = e4m3x4_to_bf16(f.y), e2 = e4m3x4_to_bf16(f.z), e3 = e4m3x4_to_bf16(f.w);
+        st_shared16(xs + sw128(r, 2 * c), make_uint4(e0.x, e0.y, e1.x, e1.y));
+        st_shared16(xs + sw128(r, 2 * c + 1), make_uint4(e2.x, e2.y, e3.x, e3.y));
+      }
+    }
+    fence_proxy_async();
+    if (__syncthreads_or(!ok)) { ok = false; break; }
+    if (tid == 0) {
+      tc_fence_after();
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        mma_f16(tmem, sdesc_sw128(xs + kk * 32), sdesc_sw128(as + kk * 32), idesc_bf16(nc), j > 0 || kk > 0);
+      mma_commit(&bar[j % ST]);
+    }
+    if (j >= 1) ok = mbar_wait(&bar[(j - 1) % ST], (j - 1) / ST & 1, p.status);    // its stage is free
+    if (ok && j + ST - 1 < n) load(j + ST - 1);
+    cp_async_commit();
+  }
+  cp_async_wait<0>();
+  if (n > 0 && ok) ok = mbar_wait(&bar[(n - 1) % ST], (n - 1) / ST & 1, p.status);
+  ok = !__syncthreads_or(!ok);
+  tc_fence_after();
+  // this CTA's sums, row by row, where the stages were: [128][nc + 4]
+  const int ld = nc + 4;
+  float* part = reinterpret_cast<float*>(raw + (base - smem_u32(raw)));
+  const int row = warp % 4 * 32 + lane;
+  for (int c = warp / 4 * 16; c < nc; c += 32) {
+    uint32_t r[16];
+    if (n > 0 && ok) {
+      tmem_ld_32x32b_x16(tmem + ((uint32_t)(warp % 4 * 32) << 16) + c, r);
+      tmem_ld_wait();
+    }
+#pragma unroll
+    for (int e = 0; e < 16; e += 4)
+      *reinterpret_cast<float4*>(part + row * ld + c + e) =
+          n > 0 && ok ? make_float4(__uint_as_float(r[e]), __uint_as_float(r[e + 1]), __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]))
+                      : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  tc_fence_before();
+  if (p.splits > 1) cluster_sync(); else __syncthreads();
+  if (warp == 0) {
+    tmem_relinquish();
+    tmem_dealloc(tmem, cols);
+  }
+  // the cluster's CTAs take rows in turn; a thread four neighbouring values of a row
+  const int rk = p.Rp / 4, total = t.rows * (nsr / p.R) * rk;
+  __nv_bfloat16* v = reinterpret_cast<__nv_bfloat16*>(p.v);
+  const float sc = p.scale[t.slot];
+  for (int o = tid + 256 * (p.splits > 1 ? blockIdx.z : 0); o < total; o += 256 * p.splits) {
+    const int m = o / (nsr / p.R * rk), ss = o / rk % (nsr / p.R), j = o % rk * 4;
+    float f = sc;
+    if (FP8) {
+      const int r = row_of(p, i, m, t.rows);
+      f *= r >= 0 ? p.xs[r] : 0.f;
+    }
+    float q[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float sum = 0.f;
+      if (j + e < t.rank) {
+        const float* at = part + m * ld + ss * p.R + j + e;
+        if (p.splits == 1) sum = *at;
+        else
+          for (int z = 0; z < p.splits; ++z) {
+            float w;
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w) : "r"(mapa_shared(smem_u32(at), z)));
+            sum += w;
+          }
+      }
+      q[e] = sum * f;
+    }
+    uint2 hi, lo;
+    split_v(make_float4(q[0], q[1], q[2], q[3]), true, hi.x, hi.y, lo.x, lo.y);
+    const int64_t at = (((int64_t)i * 128 + m) * p.S + sr0 / p.R + ss) * 2 * p.Rp + j;
+    *reinterpret_cast<uint2*>(v + at) = hi;
+    *reinterpret_cast<uint2*>(v + at + p.Rp) = lo;
+  }
+  if (p.splits > 1) cluster_sync();                        // nobody leaves while its sums are being read
+}
+
+// out of 128-row tiles: D[128 x 128] = V[128 x 2 r] [B; B][128 x 2 r]^T on tcgen05, feature tile by feature tile; the MMAs take
+// a fraction of the time that y and out need.  B's rows are staged in the order that gives each thread of the epilogue 8
+// neighbouring features of a row (the 16x256b TMEM load hands out column pairs), so y and out move in 16-byte vectors
+// between global memory and registers.  B of the next feature tile and y of this one are on their way during the MMAs.
+template <bool VECN, bool VECR>
+__global__ void __launch_bounds__(256, 2) expand128_kernel(const __grid_constant__ Args p) {
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t bar;
+  __shared__ uint32_t tmem_at;
+  const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, g = lane >> 2, q4 = lane & 3, i = blockIdx.y;
+  const int kc = (p.Rp + 63) / 64;                         // 64-rank operand tiles
+  const bool two = kc <= 3;                                // two stages of B, as far as shared memory goes
+  const uint32_t vb = base, bb = base + 2 * kc * 16384, bstage = two ? kc * 16384 : 0;
+  int s, ne;
+  const int nb = slice_of(p, blockIdx.x, 128 * p.steps, s, ne), nt = min(p.steps, (ne - nb + 127) / 128);
+  Tile t;
+  if (!load_tile(p, i, t) || (t.slot < 0 && p.out == p.y)) {
+    pdl_wait();
+    return;
+  }
+  if (warp == 0) tmem_alloc(&tmem_at, 128);
+  if (tid == 0) mbar_init(&bar, 1);
+  fence_mbar_init();
+  // rows of this thread: 32 (warp % 4) + 16 rh + 8 h + g; features 64 (warp / 4) + 32 cb + 8 q4 of a tile
+  int64_t yo[2][2], oo[2][2];
+#pragma unroll
+  for (int rh = 0; rh < 2; ++rh)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = row_of(p, i, warp % 4 * 32 + 16 * rh + 8 * h + g, t.rows);
+      yo[rh][h] = r >= 0 ? r * p.y_ld : -1;
+      oo[rh][h] = r * p.out_ld;
+    }
+  const bool rows_here = warp % 4 * 32 < t.rows;
+  const __nv_bfloat16* bt = p.b + (int64_t)max(t.slot, 0) * p.N * p.R;
+  const int rk16 = (t.rank + 15) / 16, chunks = rk16 * 2;  // MMA steps; 16-byte chunks of a rank row in use
+  auto load_b = [&](int j) {
+    const int n0 = nb + 128 * j;
+    for (int o = tid; o < 128 * chunks; o += 256) {
+      const int r = o / chunks, c = o % chunks;
+      const int nn = n0 + (r & ~31) + 8 * ((r & 7) >> 1) + 2 * (r >> 3 & 3) + (r & 1);
+      if (nn >= ne) continue;
+      const __nv_bfloat16* src = bt + (int64_t)nn * p.R + 8 * c;
+      const uint32_t dst = bb + (j & 1) * bstage + (c / 8) * 16384 + sw128(r, c % 8);
+      const int left = t.rank - 8 * c;
+      if (VECR && (left >= 8 || left <= 0)) cp_async16(dst, left > 0 ? src : bt, left > 0);
+      else {
+        uint32_t w[4] = {};
+        for (int e = 0; e < min(left, 8); ++e) w[e / 2] |= (uint32_t)__bfloat16_as_ushort(src[e]) << 16 * (e % 2);
+        st_shared16(dst, make_uint4(w[0], w[1], w[2], w[3]));
+      }
+    }
+  };
+  if (t.rank > 0) load_b(0);
+  cp_async_commit();
+  pdl_wait();
+  pdl_trigger();
+  if (t.rank > 0) {
+    const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(p.v);
+    for (int o = tid; o < t.rows * 2 * chunks; o += 256) {
+      const int r = o / (2 * chunks), hl = o / chunks % 2, c = o % chunks;
+      cp_async16(vb + (hl * kc + c / 8) * 16384 + sw128(r, c % 8),
+                 v + ((((int64_t)i * 128 + r) * p.S + s) * 2 + hl) * p.Rp + 8 * c, true);
+    }
+  }
+  cp_async_commit();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_at;
+  bool ok = true;
+  for (int j = 0; j < nt; ++j) {
+    const int n0 = nb + 128 * j;
+    uint4 y[2][2][2];
+#pragma unroll
+    for (int rh = 0; rh < 2; ++rh)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int cb = 0; cb < 2; ++cb)
+          y[rh][h][cb] = load_y<VECN>(yo[rh][h] >= 0 ? p.y + yo[rh][h] : nullptr, n0 + warp / 4 * 64 + 32 * cb + 8 * q4, ne);
+    if (t.rank > 0) {
+      if (two && j + 1 < nt) load_b(j + 1);
+      cp_async_commit();
+      cp_async_wait<1>();
+      fence_proxy_async();
+      tc_fence_before();
+      if (__syncthreads_or(!ok)) { ok = false; break; }
+      if (tid == 0) {
+        tc_fence_after();
+        const uint32_t bs = bb + (j & 1) * bstage;
+        for (int hl = 1; hl >= 0; --hl)
+          for (int kk = 0; kk < rk16; ++kk) {
+            const uint32_t o = (kk / 4) * 16384 + (kk % 4) * 32;
+            mma_f16(tmem, sdesc_sw128(vb + hl * kc * 16384 + o), sdesc_sw128(bs + o), idesc_bf16(128), hl == 0 || kk > 0);
+          }
+        mma_commit(&bar);
+      }
+      ok = __all_sync(0xffffffffu, mbar_wait(&bar, j & 1, p.status));
+      tc_fence_after();
+      if (!two && j + 1 < nt) {
+        load_b(j + 1);
+        cp_async_commit();
+      }
+    }
+    if (!rows_here || !ok) continue;
+#pragma unroll
+    for (int rh = 0; rh < 2; ++rh)
+#pragma unroll
+      for (int cb = 0; cb < 2; ++cb) {
+        uint32_t r[16];
+        if (t.rank > 0) {
+          tmem_ld_16x256b_x4(tmem + ((uint32_t)(warp % 4 * 32 + 16 * rh) << 16) + warp / 4 * 64 + 32 * cb, r);
+          tmem_ld_wait();
+        }
+        const int at = n0 + warp / 4 * 64 + 32 * cb + 8 * q4;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (yo[rh][h] < 0 || at >= ne) continue;
+          uint4 o = y[rh][h][cb];
+          if (t.rank > 0) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+              const __nv_bfloat162 f = *reinterpret_cast<const __nv_bfloat162*>(&w[m]);
+              w[m] = pack2(__low2float(f) + __uint_as_float(r[4 * m + 2 * h]),
+                           __high2float(f) + __uint_as_float(r[4 * m + 2 * h + 1]));
+            }
+          }
+          __nv_bfloat16* to = p.out + oo[rh][h] + at;
+          if (VECN && at + 8 <= ne) *reinterpret_cast<uint4*>(to) = o;
+          else
+            for (int e = 0; e < 8; ++e)
+              if (at + e < ne) to[e] = reinterpret_cast<const __nv_bfloat16*>(&o)[e];
+        }
+      }
+  }
+  cp_async_wait<0>();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) {
+    tmem_relinquish();
+    tmem_dealloc(tmem, 128);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------------------------
+template <typename... A>
+void launch(void (*kern)(A...), dim3 grid, int cx, int cz, size_t smem, cudaStream_t stream, A... args) {
+  if (smem > 48 * 1024)
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[2];
+  int n = 0;
+  if (pdl_enabled()) {
+    at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cx * cz > 1) {
+    at[n].id = cudaLaunchAttributeClusterDimension;
+    at[n].val.clusterDim.x = cx;
+    at[n].val.clusterDim.y = 1;
+    at[n++].val.clusterDim.z = cz;
+  }
+  cfg.attrs = at;
+  cfg.numAttrs = n;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, args...));
+}
+
+unsigned chunks(const Args& p, int span) {
+  unsigned n = 0;
+  for (int s = 0; s < p.S; ++s) n += (p.off[s + 1] - p.off[s] + span - 1) / span;
+  return n;
+}
+
+// 16-row tiles
+template <int JG>
+void launch16(Args& p, bool fp8, bool vec, const at::TensorOptions& opts, cudaStream_t st) {
+  constexpr int STEP = JG == 4 ? 256 : 512;
+  for (p.steps = 1; p.steps < 2 && (int64_t)chunks(p, CL * STEP * p.steps) * CL * p.max_tiles > 2 * 148;) p.steps *= 2;
+  const unsigned ch = chunks(p, CL * STEP * p.steps);
+  if ((int64_t)ch * CL * p.max_tiles <= 2 * 148) {
+    const size_t smem = (8 * 16 * RS<JG> + 256 * JG + 16 * (p.Rp + 4)) * sizeof(float);
+    auto k = fp8 ? (vec ? decode_kernel<JG, true, true> : decode_kernel<JG, true, false>)
+                 : (vec ? decode_kernel<JG, false, true> : decode_kernel<JG, false, false>);
+    launch(k, dim3(ch * CL, p.max_tiles), CL, 1, smem, st, p);
+    return;
+  }
+  const int groups = (p.Rp + 16 * JG - 1) / (16 * JG);
+  // shares of K of at least two 32-blocks a warp, for about four CTAs an SM
+  p.splits = std::max<int64_t>(1, std::min<int64_t>({8, 4 * 148 / ((int64_t)p.max_tiles * p.S * groups) + 1, p.K / 512}));
+  // v from the allocator, not a shared workspace: calls on several streams must not meet in it
+  torch::Tensor ws = torch::empty({(int64_t)p.splits * p.max_tiles * 16 * p.S * p.Rp}, opts);
+  p.v = ws.data_ptr<float>();
+  auto k = fp8 ? (vec ? shrink16_kernel<JG, true, true> : shrink16_kernel<JG, true, false>)
+               : (vec ? shrink16_kernel<JG, false, true> : shrink16_kernel<JG, false, false>);
+  launch(k, dim3(p.max_tiles, p.S * groups, p.splits), 1, 1, 0, st, p);
+  launch(vec ? expand16_kernel<JG, true> : expand16_kernel<JG, false>, dim3(chunks(p, STEP), p.max_tiles), 1, 1,
+         16 * (p.Rp + 4) * sizeof(float), st, p);
+}
+
+// 128-row tiles
+void launch128(Args& p, bool fp8, bool vec_k, bool vec_n, const at::TensorOptions& opts, cudaStream_t st) {
+  torch::Tensor ws = torch::empty({(int64_t)p.max_tiles * 128 * p.S * p.Rp}, opts);
+  p.v = ws.data_ptr<float>();
+  // rank rows of whole slices, at most 256 (the MMA's N)
+  const int nc = std::max(1, std::min(p.S, 256 / p.R)) * p.R, groups = (p.S * p.R + nc - 1) / nc, nc16 = (nc + 15) / 16 * 16;
+  const int64_t ctas = (int64_t)p.max_tiles * groups;
+  for (p.splits = 1; p.splits < 8 && ctas * p.splits * 2 <= 2 * 148 && p.K >= 64 * ST * p.splits * 2;) p.splits *= 2;
+  const size_t stages = ST * (16384 + (size_t)nc16 * 128 + (fp8 ? 8192 : 0)), sums = 128 * (nc16 + 4) * sizeof(float);
+  auto k = fp8 ? (vec_k ? shrink128_kernel<true, true> : shrink128_kernel<true, false>)
+               : (vec_k ? shrink128_kernel<false, true> : shrink128_kernel<false, false>);
+  launch(k, dim3(p.max_tiles, groups, p.splits), 1, p.splits, std::max(stages, sums) + 2048, st, p, nc);
+  // feature tiles of a CTA: v is staged once for all of them, as long as every SM has a few CTAs
+  for (p.steps = 1; p.steps < 16 && (int64_t)chunks(p, 128 * p.steps * 2) * p.max_tiles >= 4 * 148;) p.steps *= 2;
+  const int kc = (p.Rp + 63) / 64;
+  const size_t smem = (kc <= 3 ? 4 : 3) * kc * 16384 + 1024;
+  const bool vec_r = p.R % 8 == 0;
+  auto e = vec_n ? (vec_r ? expand128_kernel<true, true> : expand128_kernel<true, false>)
+                 : (vec_r ? expand128_kernel<false, true> : expand128_kernel<false, false>);
+  launch(e, dim3(chunks(p, 128 * p.steps), p.max_tiles), 1, 1, smem, st, p);
+}
+
+[[noreturn]] void refuse(const std::string& why) { throw pybind11::value_error("lora_add: " + why); }
+
+bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
+  const auto span = [](const torch::Tensor& t) {
+    return (t.size(0) - 1) * t.stride(0) * t.element_size() + t.size(1) * t.element_size();
+  };
+  const uint8_t *pa = (const uint8_t*)a.data_ptr(), *pb = (const uint8_t*)b.data_ptr();
+  return pa < pb + span(b) && pb < pa + span(a);
 }
 
 }  // namespace lora
 
-// x [T, K] bf16, or e4m3 with xs fp32 [T]; slices: S + 1 offsets from 0 to N; plan as described above with max_tiles
-// tile entries; out may be y.
-void lora_add(torch::Tensor y, torch::Tensor x, torch::Tensor xs, torch::Tensor a, torch::Tensor b,
-              torch::Tensor scale, torch::Tensor ranks, std::vector<int64_t> slices,
-              torch::Tensor plan, int64_t max_tiles, int64_t tile_rows, torch::Tensor out,
-              torch::Tensor status) {
-  const bool fp8 = x.scalar_type() == at::kFloat8_e4m3fn;
-  const int64_t T = x.size(0), K = x.size(1), L = a.size(0), S = a.size(1), R = a.size(2), N = b.size(1);
-  const at::cuda::CUDAGuard guard(x.device());
-  lora::Args p;
-  p.x = x.data_ptr(); p.xs = fp8 ? xs.data_ptr<float>() : nullptr; p.x_ld = x.stride(0);
-  p.a = (const __nv_bfloat16*)a.data_ptr(); p.b = (const __nv_bfloat16*)b.data_ptr();
-  p.scale = scale.data_ptr<float>(); p.rank = ranks.data_ptr<int>();
+// The stacked adapters of one projection; the tensors are checked by the caller (models/lora.AdapterBank).
+struct LoraBank {
+  torch::Tensor a, b, scale, ranks, status;
+  lora::Args args;
+  LoraBank(torch::Tensor a_, torch::Tensor b_, torch::Tensor scale_, torch::Tensor ranks_, std::vector<int64_t> slices,
+           torch::Tensor status_)
+      : a(a_), b(b_), scale(scale_), ranks(ranks_), status(status_) {
+    TORCH_CHECK(a.is_cuda() && (int64_t)slices.size() == a.size(1) + 1 && a.size(1) <= lora::MAX_S, "LoraBank");
+    args = {};
+    args.a = (const __nv_bfloat16*)a.data_ptr(); args.b = (const __nv_bfloat16*)b.data_ptr();
+    args.scale = scale.data_ptr<float>(); args.rank = ranks.data_ptr<int>(); args.status = status.data_ptr<int>();
+    args.L = a.size(0); args.S = a.size(1); args.R = a.size(2); args.K = a.size(3); args.N = b.size(1);
+    args.Rp = (args.R + 15) / 16 * 16;
+    for (size_t s = 0; s < slices.size(); ++s) args.off[s] = slices[s];
+  }
+};
+struct LoraPlan {
+  torch::Tensor buf;
+  int64_t rows, max_tiles, tile_rows, slots;
+  LoraPlan(torch::Tensor buf_, int64_t rows_, int64_t max_tiles_, int64_t tile_rows_, int64_t slots_)
+      : buf(buf_), rows(rows_), max_tiles(max_tiles_), tile_rows(tile_rows_), slots(slots_) {
+    TORCH_CHECK(buf.is_cuda() && buf.scalar_type() == at::kInt && buf.is_contiguous() && max_tiles >= 1 &&
+                    max_tiles <= 65535 && (tile_rows == 16 || tile_rows == 128) &&
+                    buf.numel() >= 4 + (4 + tile_rows) * max_tiles && (uintptr_t)buf.data_ptr() % 16 == 0,
+                "LoraPlan: int32 words on the device, 16-byte aligned");
+  }
+};
+
+torch::Tensor lora_add(const torch::Tensor& y, const torch::Tensor& x, const c10::optional<torch::Tensor>& xs,
+                       const LoraBank& bank, const LoraPlan& plan, const c10::optional<torch::Tensor>& out_) {
+  using lora::refuse;
+  lora::Args p = bank.args;
+  const bool fp8 = xs.has_value();
+  if (y.dim() != 2 || x.dim() != 2 || x.size(0) != y.size(0) || plan.rows != y.size(0)) refuse("rows of y, x and the plan");
+  if (x.size(1) != p.K || y.size(1) != p.N || plan.slots > p.L) refuse("features or slots of the adapters");
+  if (y.scalar_type() != at::kBFloat16 || x.scalar_type() != (fp8 ? at::kFloat8_e4m3fn : at::kBFloat16))
+    refuse("y bf16, x bf16 or (e4m3, scale)");
+  if (y.device() != bank.a.device() || x.device() != y.device() || plan.buf.device() != y.device())
+    refuse("operands on one device");
+  if (fp8 && (xs->device() != y.device() || xs->scalar_type() != at::kFloat || xs->dim() != 1 || xs->size(0) != x.size(0) ||
+              !xs->is_contiguous()))
+    refuse("x scales fp32 [T]");
+  const at::cuda::CUDAGuard guard(y.device());
+  const int64_t T = y.size(0);
+  if (out_.has_value() && (out_->sizes() != y.sizes() || out_->scalar_type() != y.scalar_type() || out_->device() != y.device()))
+    refuse("out as y");
+  torch::Tensor out = out_.has_value() ? *out_ : torch::empty({T, (int64_t)p.N}, y.options());
+  if (T == 0) return out;
+  if (T > (1 << 30)) refuse("rows");
+  if (x.stride(1) != 1 || y.stride(1) != 1 || out.stride(1) != 1) refuse("rows must be contiguous");
+  const bool same = out.data_ptr() == y.data_ptr() && out.stride(0) == y.stride(0);
+  if (out_.has_value() && ((!same && lora::overlap(out, y)) || lora::overlap(out, x) || (T > 1 && out.stride(0) < p.N)))
+    refuse("out overlaps y or x other than being y");
+  p.x = x.data_ptr(); p.xs = fp8 ? xs->data_ptr<float>() : nullptr; p.x_ld = x.stride(0);
   p.y = (const __nv_bfloat16*)y.data_ptr(); p.y_ld = y.stride(0);
   p.out = (__nv_bfloat16*)out.data_ptr(); p.out_ld = out.stride(0);
-  p.plan = plan.data_ptr<int>(); p.status = status.data_ptr<int>();
-  p.T = T; p.K = K; p.N = N; p.L = L; p.S = S; p.R = R; p.max_tiles = max_tiles;
-  p.Rp = (R + 15) / 16 * 16;
-  for (int s = 0; s <= S; ++s) p.off[s] = slices[s];
+  p.plan = plan.buf.data_ptr<int>(); p.T = T; p.max_tiles = plan.max_tiles; p.tile_rows = plan.tile_rows;
   auto stream = at::cuda::getCurrentCUDAStream();
-  const unsigned tiles = std::min<int64_t>(max_tiles, 4096);
-  // few tiles: shares of K over several CTAs, at least two 32-blocks a warp
-  const int64_t ctas = tiles * S * (p.Rp / 16);
-  p.splits = std::max<int64_t>(1, std::min<int64_t>({8, 148 / ctas, K / 512}));
-  // v from the allocator, not a shared workspace: calls on several streams must not meet in it
-  torch::Tensor ws = torch::empty({(int64_t)p.splits * T * S * p.Rp}, scale.options());
-  p.v = ws.data_ptr<float>();
-  const bool vec_k = K % 8 == 0 && p.x_ld % 8 == 0 && (uintptr_t)p.x % 16 == 0 && (uintptr_t)p.a % 16 == 0;
-  bool vec_n = R % 4 == 0 && p.y_ld % 8 == 0 && p.out_ld % 8 == 0 &&
-               ((uintptr_t)p.y | (uintptr_t)p.out | (uintptr_t)p.b) % 16 == 0;
-  for (int s = 0; s < S; ++s) vec_n = vec_n && slices[s] % 8 == 0;
-  auto shrink = fp8 ? (vec_k ? lora::shrink_kernel<true, true> : lora::shrink_kernel<true, false>)
-                    : (vec_k ? lora::shrink_kernel<false, true> : lora::shrink_kernel<false, false>);
-  C10_CUDA_CHECK(launch_pdl(shrink, dim3(tiles, S * p.Rp / 16, p.splits), dim3(256), 0, stream, p));
-  const bool tall = tile_rows > 16;
-  if (p.Rp <= 16) lora::launch_expand<1>(p, tall, vec_n, tiles, stream);
-  else if (p.Rp <= 32) lora::launch_expand<2>(p, tall, vec_n, tiles, stream);
-  else lora::launch_expand<4>(p, tall, vec_n, tiles, stream);
+  const bool vec_k = p.K % 8 == 0 && p.x_ld % 8 == 0 && (uintptr_t)p.x % 16 == 0 && (uintptr_t)p.a % 16 == 0 &&
+                     (!fp8 || p.tile_rows == 16 || p.x_ld % 16 == 0);
+  bool vec_n = p.y_ld % 8 == 0 && p.out_ld % 8 == 0 && ((uintptr_t)p.y | (uintptr_t)p.out) % 16 == 0 &&
+               (uintptr_t)p.b % 16 == 0;
+  for (int s = 0; s < p.S; ++s) vec_n = vec_n && p.off[s] % 8 == 0;
+  const auto opts = bank.scale.options();
+  if (p.tile_rows == 16) {
+    const bool vec = vec_k && vec_n && p.R % 4 == 0;
+    if (p.Rp <= 16) lora::launch16<1>(p, fp8, vec, opts, stream);
+    else if (p.Rp <= 32) lora::launch16<2>(p, fp8, vec, opts, stream);
+    else lora::launch16<4>(p, fp8, vec, opts, stream);
+  } else {
+    lora::launch128(p, fp8, vec_k, vec_n, opts, stream);
+  }
+  return out;
+}
+
+void lora_bind(pybind11::module_& m) {
+  pybind11::class_<LoraBank>(m, "LoraBank")
+      .def(pybind11::init<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor, std::vector<int64_t>, torch::Tensor>());
+  pybind11::class_<LoraPlan>(m, "LoraPlan").def(pybind11::init<torch::Tensor, int64_t, int64_t, int64_t, int64_t>());
+  m.def("lora_add", &lora_add, "projection output + the low-rank deltas of each row's adapter");
 }
 
 }  // namespace rad

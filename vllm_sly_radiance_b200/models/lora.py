@@ -37,11 +37,16 @@ class AdapterBank:
         self.a, self.b, self.scale, self.ranks, self.slices = a, b, scale, ranks, slices
         self.L, self.S, self.R, self.K, self.N = L, S, R, K, b.shape[1]
         self.device = a.device
+        self.handle = None
+        if a.is_cuda:
+            from ..ops._ext import ext
+            from ..ops.kernels import status_word
+            self.handle = ext().LoraBank(a, b, scale, ranks, slices, status_word(a.device))
 
 
 class AdapterPlan:
-    """The rows of one step sorted by adapter slot, cut into tiles of at most ``tile_rows`` rows of one adapter.
-    buf int32: [0] tiles in use, [4 + 4 i ...] (slot, first position, rows, 0), then the row of each position."""
+    """The rows of one step by adapter slot, in tiles of at most ``tile_rows`` rows of one adapter.  buf int32: [0] tiles
+    in use, from 4 on (slot, rows, 0, 0) per tile, then ``tile_rows`` row numbers per tile."""
 
     # rows per tile: decode batches (few rows per adapter), prompts
     TILE_DECODE, TILE_PROMPT = 16, 128
@@ -50,10 +55,14 @@ class AdapterPlan:
         self.buf, self.num_rows, self.max_tiles = buf, num_rows, max_tiles
         self.tile_rows, self.num_slots = tile_rows, num_slots
         self.slots = slots                       # host copy (CPU path)
+        self.handle = None
+        if buf.is_cuda:
+            from ..ops._ext import ext
+            self.handle = ext().LoraPlan(buf, num_rows, max_tiles, tile_rows, num_slots)
 
     @staticmethod
-    def words(num_rows: int, max_tiles: int) -> int:
-        return 4 + 4 * max_tiles + num_rows
+    def words(max_tiles: int, tile_rows: int) -> int:
+        return 4 + (4 + tile_rows) * max_tiles
 
     @staticmethod
     def pack(slots: np.ndarray, num_slots: int, out=None, max_tiles=None, tile_rows=None):
@@ -76,14 +85,14 @@ class AdapterPlan:
             raise ValueError(f"adapter plan: {n} tiles, room for {max_tiles}")
         grp = np.repeat(np.arange(len(starts)), per)
         j = np.arange(n) - np.repeat(np.cumsum(per) - per, per)
-        words = np.zeros(AdapterPlan.words(T, max_tiles), np.int32) if out is None else out
+        first = starts[grp] + j * tile_rows
+        rows = np.minimum(counts[grp] - j * tile_rows, tile_rows)
+        words = np.zeros(AdapterPlan.words(max_tiles, tile_rows), np.int32) if out is None else out
         words[:4] = (n, 0, 0, 0)
         tiles = words[4:4 + 4 * n].reshape(n, 4)
-        tiles[:, 0] = srt[starts[grp]]
-        tiles[:, 1] = starts[grp] + j * tile_rows
-        tiles[:, 2] = np.minimum(counts[grp] - j * tile_rows, tile_rows)
-        tiles[:, 3] = 0
-        words[4 + 4 * max_tiles:4 + 4 * max_tiles + T] = order
+        tiles[:, 0], tiles[:, 1] = srt[starts[grp]], rows
+        at = 4 + 4 * max_tiles + np.repeat(np.arange(n) * tile_rows - first, rows) + np.arange(T)
+        words[at] = order
         return words, max_tiles, tile_rows
 
     @staticmethod

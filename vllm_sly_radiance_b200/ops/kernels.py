@@ -363,6 +363,10 @@ def lora_add(y: torch.Tensor, x, bank, plan, out: Optional[torch.Tensor] = None)
     an adapter in ``bank`` (models/lora.AdapterBank), y[t] for the others.  x: bf16 [T, K] or the
     (e4m3, scale) pair the linear itself takes.  out may be y (in place); a new tensor by default."""
     xq, xs = x if isinstance(x, tuple) else (x, None)
+    if y.is_cuda:
+        if bank.handle is None or plan.handle is None:
+            raise ValueError("lora_add: operands on one device")
+        return ext().lora_add(y, xq, xs, bank.handle, plan.handle, out)    # checks them itself
     T = y.shape[0]
     if y.dim() != 2 or xq.dim() != 2 or xq.shape[0] != T or plan.num_rows != T:
         raise ValueError(f"lora_add: y {tuple(y.shape)}, x {tuple(xq.shape)} and a plan of "
@@ -375,8 +379,7 @@ def lora_add(y: torch.Tensor, x, bank, plan, out: Optional[torch.Tensor] = None)
         raise ValueError("lora_add: y bf16, x bf16 or (e4m3, scale)")
     if xs is not None and (xs.dtype != torch.float32 or xs.shape != (T,) or not xs.is_contiguous()):
         raise ValueError("lora_add: x scales fp32 [T]")
-    if y.device != bank.device or xq.device != y.device or plan.buf.device != y.device or \
-            (xs is not None and xs.device != y.device):
+    if any(t.device != y.device for t in (bank.a, xq, plan.buf)):
         raise ValueError("lora_add: operands on one device")
     if out is None:
         out = torch.empty(T, bank.N, dtype=torch.bfloat16, device=y.device)
@@ -386,13 +389,7 @@ def lora_add(y: torch.Tensor, x, bank, plan, out: Optional[torch.Tensor] = None)
         return out
     if xq.stride(1) != 1 or y.stride(1) != 1 or out.stride(1) != 1:
         raise ValueError("lora_add: rows must be contiguous")
-    if not y.is_cuda:
-        out.copy_(ref.lora_add(y, x, bank, plan.slots))
-        return out
-    dev = y.device
-    ext().lora_add(y, xq, xs if xs is not None else _empty(dev), bank.a, bank.b, bank.scale,
-                   bank.ranks, bank.slices, plan.buf, plan.max_tiles, plan.tile_rows, out,
-                   status_word(dev))
+    out.copy_(ref.lora_add(y, x, bank, plan.slots))
     return out
 
 
