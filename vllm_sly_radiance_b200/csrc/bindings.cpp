@@ -145,8 +145,7 @@ void allreduce_oneshot(std::vector<int64_t> peers, int64_t rank, torch::Tensor i
                        torch::Tensor weight, double eps, torch::Tensor res_out, torch::Tensor q,
                        torch::Tensor scale, int64_t num_blocks, torch::Tensor status);
 void lora_bind(pybind11::module_& m);
-void cache_move(torch::Tensor table, torch::Tensor pieces, torch::Tensor status, int64_t num_items,
-                torch::Tensor groups, torch::Tensor dst);
+void cache_moves_bind(pybind11::module_& m);
 }  // namespace rad
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -209,7 +208,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("push_allreduce_recv", &rad::push_allreduce_recv,
         "receiving half of the GEMM-fused all-reduce (+ add / RMSNorm / e4m3 quant)");
   rad::lora_bind(m);
-  m.def("cache_move", &rad::cache_move, "cache items (pages, states) -> other items of the same caches");
+  rad::cache_moves_bind(m);
   m.def("ipc_handle", &rad::ipc_handle, "CUDA IPC handle of a device buffer");
   m.def("ipc_open", &rad::ipc_open, "open a peer's IPC handle -> device pointer");
   m.def("ipc_close", &rad::ipc_close, "close an opened IPC mapping");

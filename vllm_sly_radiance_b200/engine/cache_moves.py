@@ -45,13 +45,17 @@ class _Items:
             else:
                 table.append([t.data_ptr(), t.stride(0) * es, 1, nbytes, 0, 0])
             pieces += [[i, j] for j in range((nbytes + PIECE_BYTES - 1) // PIECE_BYTES)]
+        self.handle = None
         if self.cuda:
+            from ..ops._ext import ext
+            from ..ops.kernels import status_word
             dev = tensors[0].device
-            self.table = torch.tensor(table, dtype=torch.int64, device=dev)
-            self.pieces = torch.tensor(pieces, dtype=torch.int32, device=dev)
+            self.handle = ext().CacheItems(name, torch.tensor(table, dtype=torch.int64, device=dev),
+                                           torch.tensor(pieces, dtype=torch.int32, device=dev).view(-1, 2),
+                                           status_word(dev), self.num, self.rows)
 
     def move(self, moves):
-        """moves: (src, dst) or, of pages, (src, dst, tokens) rows."""
+        """On the CPU: (src, dst) or, of pages, (src, dst, tokens) rows, with the checks of csrc/cache_moves.cu."""
         m = np.asarray(moves, dtype=np.int64)
         if m.ndim != 2 or m.shape[1] not in ((2, 3) if self.paged else (2,)):
             raise ValueError(f"cache moves: {self.name} as (src, dst{', tokens' if self.paged else ''}) rows")
@@ -61,62 +65,57 @@ class _Items:
             raise ValueError(f"cache moves: {self.name} outside 0 .. {self.num - 1}")
         if self.paged and (tokens.min() < 0 or tokens.max() > self.rows):
             raise ValueError(f"cache moves: 0 .. {self.rows} tokens of a page")
-        taken = np.zeros(self.num, np.int8)
-        taken[src] = 1
-        if taken[dst].any():
-            raise ValueError(f"cache moves: {self.name} both source and destination")
-        taken[dst] = 2
-        if np.count_nonzero(taken == 2) != len(dst):
-            raise ValueError(f"cache moves: {self.name} a destination twice")
-        if not self.cuda:
-            for s, d, n in zip(src, dst, tokens):
-                for t in self.tensors:
-                    if self.paged:
-                        t[d, :, :n] = t[s, :, :n]
-                    else:
-                        t[d] = t[s]
-            return
-        # the destinations of one (source, tokens) side by side: the source is read once
-        order = np.lexsort((tokens, src))
-        src, dst, tokens = src[order], dst[order], tokens[order]
-        new = np.r_[True, (src[1:] != src[:-1]) | (tokens[1:] != tokens[:-1])]
-        at = np.flatnonzero(new)
-        groups = np.stack([src[at], at, np.diff(np.r_[at, len(src)]), tokens[at]], 1)
-        if groups[:, 2].max() > 128:
-            raise ValueError(f"cache moves: at most 128 destinations of one source")
-        from ..ops._ext import ext
-        from ..ops.kernels import status_word
-        ext().cache_move(self.table, self.pieces, status_word(self.table.device), self.num,
-                         torch.from_numpy(groups.astype(np.int32)), torch.from_numpy(dst.astype(np.int32)))
+        if len(np.unique(dst)) != len(dst):
+            raise ValueError(f"cache moves: {self.name}: a destination twice")
+        if np.isin(src, dst).any():
+            raise ValueError(f"cache moves: {self.name}: both source and destination")
+        return src, dst, tokens
+
+    def apply(self, src, dst, tokens):
+        for s, d, n in zip(src, dst, tokens):
+            for t in self.tensors:
+                if self.paged:
+                    t[d, :, :n] = t[s, :, :n]
+                else:
+                    t[d] = t[s]
 
 
 class CacheMover:
-    """Copies inside ``caches`` (whose tensors must stay where they are).  All copies of a call read before any of
-    them writes: no item may be a source and a destination, or a destination twice.  Asynchronous on the current
+    """Copies inside ``caches`` (whose tensors must stay where they are).  No item of a call may be a source and a
+    destination, or a destination twice; everything is checked before anything moves.  Asynchronous on the current
     stream, without a host synchronisation."""
 
     def __init__(self, caches: ModelCaches):
         self.blocks = _Items("blocks", list(caches.k) + list(caches.v), True)
         self.slots = _Items("slots", list(caches.conv) + list(caches.ssm), False)
+        self.cuda = self.blocks.cuda or self.slots.cuda
 
     def copy(self, blocks=(), slots=()):
         """blocks: (src, dst) pages or (src, dst, tokens) for the first tokens of a page; slots: (src, dst)."""
-        if len(blocks):
-            self.blocks.move(blocks)
-        if len(slots):
-            self.slots.move(slots)
+        if self.cuda:
+            from ..ops._ext import ext
+            ext().cache_copy(self.blocks.handle, blocks, self.slots.handle, slots)
+            return
+        todo = [(k, k.move(m)) for k, m in ((self.blocks, blocks), (self.slots, slots)) if len(m)]
+        for k, m in todo:
+            k.apply(*m)
 
     def compact(self, tables: np.ndarray):
-        """tables: int [sequences, pages] block ids (<= 0: no page).  Moves the pages they name to blocks 1 .. n and
-        returns (the new tables, n)."""
-        tables = np.asarray(tables)
+        """tables: int32 or int64 [sequences, pages] block ids (<= 0: no page).  Moves the pages they name to blocks
+        1 .. n and returns (the new tables, n)."""
+        tables = np.ascontiguousarray(tables)
+        if tables.dtype not in (np.int32, np.int64):
+            raise ValueError(f"cache moves: tables of int32 or int64, got {tables.dtype}")
+        if self.blocks.cuda:
+            from ..ops._ext import ext
+            return ext().cache_compact(self.blocks.handle, tables)
         if tables.size and tables.max() >= self.blocks.num:
             raise ValueError(f"cache moves: blocks outside 0 .. {self.blocks.num - 1}")
         used = np.zeros(self.blocks.num, bool)
         used[tables[tables > 0]] = True
         src, dst, n = plan_compaction(used)
         if len(src):
-            self.blocks.move(np.stack([src, dst], 1))
+            self.copy(np.stack([src, dst], 1))
         to = np.arange(self.blocks.num, dtype=tables.dtype)
         to[src] = dst
         return np.where(tables > 0, to[np.maximum(tables, 0)], tables), n
