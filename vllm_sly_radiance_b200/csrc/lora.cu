@@ -7,7 +7,8 @@
 // bf16; s(n) is the part of a merged projection that output feature n belongs to.  The rows come sorted by adapter in
 // tiles of one adapter each (the plan): 16 rows a tile for decode batches, 128 for prompts.
 //
-// plan (int32): [0] tiles in use; from word 4 (slot, rows, 0, 0) per tile; then tile_rows row numbers per tile.
+// plan (int32): [0] tiles in use; from word 4 (slot, rows, 1 if the rows are consecutive, 0) per tile; then tile_rows row
+// numbers per tile.
 //
 // Three forms:
 //   decode_kernel           16-row tiles, all CTAs at once on the SMs: one launch, latency bound
@@ -22,6 +23,7 @@
 #include <torch/extension.h>
 
 #include "common.cuh"
+#include "tma_host.h"
 
 namespace rad {
 namespace lora {
@@ -50,14 +52,14 @@ struct Args {
   int off[MAX_S + 1];       // slice s = output features [off[s], off[s + 1])
 };
 
-struct Tile { int slot, rows, rank; };
+struct Tile { int slot, rows, rank, seq; };
 
 // Tile i < max_tiles.  False: not in use, or a plan of other rows or adapters (refused, status word).  The count and
 // the record are read together.
 DEVI bool load_tile(const Args& p, int i, Tile& t) {
   const int n = p.plan[0];
-  const int2 q = *reinterpret_cast<const int2*>(p.plan + 4 + 4 * (int64_t)i);
-  t.slot = q.x; t.rows = q.y; t.rank = 0;
+  const int4 q = *reinterpret_cast<const int4*>(p.plan + 4 + 4 * (int64_t)i);
+  t.slot = q.x; t.rows = q.y; t.rank = 0; t.seq = q.z;
   if (i >= n) return false;
   if (q.x >= p.L || q.y < 0 || q.y > p.tile_rows || n > p.max_tiles) {
     if (threadIdx.x == 0) atomicExch(p.status, (int)kErrBounds);
@@ -472,12 +474,6 @@ __global__ void __launch_bounds__(256, 2) expand16_kernel(const __grid_constant_
 // ---------------------------------------------------------------------------------------------
 // 128-row tiles
 // ---------------------------------------------------------------------------------------------
-DEVI void cp_async16(uint32_t dst, const void* src, bool use) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(use ? 16 : 0) : "memory");
-}
-DEVI void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-DEVI void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 DEVI void st_shared16(uint32_t dst, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -502,141 +498,83 @@ DEVI void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
       : "r"(taddr));
 }
 
-// v of 128-row tiles: D[128 x NC] = X[128 x K] A[NC x K]^T on tcgen05, NC <= 256 rank rows of all slices together, so that x
-// is read once.  The rows are gathered by cp.async into swizzled 64-k stages (e4m3 rows as they are, widened to bf16 in
-// shared memory); a cluster of `splits` CTAs shares K and adds up through distributed shared memory in a fixed order.
-// v leaves as the two bf16 numbers of each value that the expanding kernel multiplies with.
-constexpr int ST = 4;                                      // stages in flight
+// TMA, four rows of a 2-D map by number: 4 x box width, rows one after another
+DEVI void tma_gather4(uint32_t dst, const void* map, uint64_t* bar, int c, int4 r) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
+      "l"(map), "r"(smem_u32(bar)), "r"(c), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
+      : "memory");
+}
+DEVI void tma_2d(uint32_t dst, const void* map, uint64_t* bar, int c, int r) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(map), "r"(smem_u32(bar)), "r"(c), "r"(r)
+      : "memory");
+}
+DEVI void tma_5d(uint32_t dst, const void* map, uint64_t* bar, int c, int r) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %4, %4, %5}], [%2];" ::"r"(dst),
+      "l"(map), "r"(smem_u32(bar)), "r"(c), "r"(0), "r"(r)
+      : "memory");
+}
+// K-major operand tile with rows of `rb` = 32, 64 or 128 bytes, swizzled over its rows' width
+DEVI uint64_t sdesc_rows(uint32_t saddr, int rb) {
+  uint64_t d = 0;
+  d |= (uint64_t)((saddr & 0x3FFFF) >> 4);
+  d |= (uint64_t)1 << 16;                                  // LBO, not used by swizzled K-major tiles
+  d |= (uint64_t)((8 * rb) >> 4) << 32;                    // SBO: 8 rows
+  d |= (uint64_t)1 << 46;
+  d |= (uint64_t)(rb == 128 ? 2 : rb == 64 ? 4 : 6) << 61;
+  return d;
+}
+// byte offset of 16-byte chunk `c` of row `r` in such a tile
+DEVI uint32_t sw_rows(int r, int c, int rb) {
+  return (uint32_t)(r * rb + ((c ^ (rb == 128 ? r & 7 : rb == 64 ? r >> 1 & 3 : r >> 2 & 1)) << 4));
+}
+// Rows of a tile for TMA: consecutive rows in boxes of 16 (the last may reach into rows that nothing reads the results of),
+// others four by number (those beyond the tile repeat the first).  `lane` has one load of a 64-column tile; n: loads in use.
+struct TmaRows {
+  int n, each;                                             // loads, and rows of one
+  bool seq;
+  int4 r;
+};
+DEVI TmaRows tma_rows(const Args& p, int i, const Tile& t, int lane) {
+  TmaRows q;
+  const int* rows = p.plan + 4 + 4 * (int64_t)p.max_tiles + (int64_t)i * 128;
+  const int first = rows[0];
+  q.seq = t.seq && first >= 0 && first <= p.T - t.rows;
+  q.n = q.seq ? (t.rows + 15) / 16 : (t.rows + 3) / 4;
+  q.each = q.seq ? 16 : 4;
+  q.r = make_int4(first + 16 * lane, 0, 0, 0);
+  if (q.seq || lane >= q.n) return q;
+  q.r = *reinterpret_cast<const int4*>(rows + 4 * lane);
+  if (4 * lane + 1 >= t.rows) q.r.y = q.r.x;
+  if (4 * lane + 2 >= t.rows) q.r.z = q.r.x;
+  if (4 * lane + 3 >= t.rows) q.r.w = q.r.x;
+  if ((unsigned)q.r.x >= (unsigned)p.T || (unsigned)q.r.y >= (unsigned)p.T || (unsigned)q.r.z >= (unsigned)p.T ||
+      (unsigned)q.r.w >= (unsigned)p.T) {
+    atomicExch(p.status, (int)kErrBounds);
+    q.r = make_int4(0, 0, 0, 0);
+  }
+  return q;
+}
+DEVI void tma_load_rows(const TmaRows& q, uint32_t dst, const void* box, const void* gather, uint64_t* bar, int c, int lane,
+                        int row_bytes) {
+  if (lane >= q.n) return;
+  if (q.seq) tma_2d(dst + lane * 16 * row_bytes, box, bar, c, q.r.x);
+  else tma_gather4(dst + lane * 4 * row_bytes, gather, bar, c, q.r);
+}
 
-template <bool FP8, bool VEC>
-__global__ void __launch_bounds__(256) shrink128_kernel(const __grid_constant__ Args p, int nc_max) {
-  extern __shared__ uint8_t raw[];
-  __shared__ uint64_t bar[ST];
-  __shared__ uint32_t tmem_at;
-  const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, i = blockIdx.x;
-  const int sr0 = blockIdx.y * nc_max, nsr = min(nc_max, p.S * p.R - sr0), nc = (nsr + 15) / 16 * 16;
-  const uint32_t xbytes = 16384, abytes = (uint32_t)((nc_max + 15) / 16) * 2048, sbytes = xbytes + abytes;
-  const uint32_t fp8_at = base + ST * sbytes;              // e4m3 stages [ST][128 x 64]
-  const uint32_t cols = nc <= 32 ? 32 : nc <= 64 ? 64 : nc <= 128 ? 128 : 256;
-  pdl_wait();
-  pdl_trigger();
-  Tile t;
-  if (!load_tile(p, i, t) || t.rank == 0) return;          // uniform over the cluster
-  if (warp == 0) tmem_alloc(&tmem_at, cols);
-  if (tid < ST) mbar_init(&bar[tid], 1);
-  fence_mbar_init();
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = tmem_at;
-
-  const int nk = (p.K + 63) / 64, per = (nk + p.splits - 1) / p.splits;
-  const int k0 = blockIdx.z * per, n = max(0, min(per, nk - k0));
-  // a thread moves chunk tid % 8 of rows tid / 8 + 32 q (e4m3: chunk tid % 4 of rows tid / 4 + 64 q)
-  const uint8_t* x[4];
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int r = FP8 ? tid / 4 + 64 * q : tid / 8 + 32 * q, row = r < 128 ? row_of(p, i, r, t.rows) : -1;
-    x[q] = row >= 0 ? static_cast<const uint8_t*>(p.x) + row * p.x_ld * (FP8 ? 1 : 2) : nullptr;
-  }
-  const __nv_bfloat16* a = p.a + ((int64_t)t.slot * p.S * p.R + sr0) * p.K;
-  auto load = [&](int j) {                                 // 64-k block j of this CTA's share into its stage
-    const int k = (k0 + j) * 64;
-    const uint32_t xs = base + j % ST * sbytes, as = xs + xbytes;
-    if (FP8) {
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int r = tid / 4 + 64 * q, kk = k + tid % 4 * 16;
-        const uint32_t dst = fp8_at + j % ST * 8192 + r * 64 + tid % 4 * 16;
-        if (x[q] == nullptr) continue;
-        if (VEC && p.K % 16 == 0) cp_async16(dst, x[q] + min(kk, p.K - 16), kk < p.K);
-        else {
-          uint32_t w[4] = {};
-          for (int e = 0; e < 16; ++e)
-            if (kk + e < p.K) w[e / 4] |= (uint32_t)x[q][kk + e] << 8 * (e % 4);
-          st_shared16(dst, make_uint4(w[0], w[1], w[2], w[3]));
-        }
-      }
-    } else {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int r = tid / 8 + 32 * q, kk = k + tid % 8 * 8;
-        if (x[q] == nullptr) continue;
-        if (VEC) cp_async16(xs + sw128(r, tid % 8), x[q] + 2 * min(kk, p.K - 8), kk < p.K);
-        else st_shared16(xs + sw128(r, tid % 8), load8<false, false>(x[q], kk, p.K));
-      }
-    }
-    const int kk = k + tid % 8 * 8;
-    for (int r = tid / 8; r < nsr; r += 32) {
-      if (VEC) cp_async16(as + sw128(r, tid % 8), a + (int64_t)r * p.K + min(kk, p.K - 8), kk < p.K);
-      else st_shared16(as + sw128(r, tid % 8), load8<false, false>(a + (int64_t)r * p.K, kk, p.K));
-    }
-  };
-#pragma unroll
-  for (int j = 0; j < ST - 1; ++j) {
-    if (j < n) load(j);
-    cp_async_commit();
-  }
-  bool ok = true;
-  for (int j = 0; j < n; ++j) {
-    cp_async_wait<ST - 2>();
-    const uint32_t xs = base + j % ST * sbytes, as = xs + xbytes;
-    if (FP8) {                                             // the chunks that this thread itself loaded
-#pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        const int r = tid / 4 + 64 * q, c = tid % 4;
-        const uint4 f = ld_shared16(fp8_at + j % ST * 8192 + r * 64 + c * 16);
-        const uint2 e0 = e4m3x4_to_bf16(f.x), e1 = e4m3x4_to_bf16(f.y), e2 = e4m3x4_to_bf16(f.z), e3 = e4m3x4_to_bf16(f.w);
-        st_shared16(xs + sw128(r, 2 * c), make_uint4(e0.x, e0.y, e1.x, e1.y));
-        st_shared16(xs + sw128(r, 2 * c + 1), make_uint4(e2.x, e2.y, e3.x, e3.y));
-      }
-    }
-    fence_proxy_async();
-    if (__syncthreads_or(!ok)) { ok = false; break; }
-    if (tid == 0) {
-      tc_fence_after();
-#pragma unroll
-      for (int kk = 0; kk < 4; ++kk)
-        mma_f16(tmem, sdesc_sw128(xs + kk * 32), sdesc_sw128(as + kk * 32), idesc_bf16(nc), j > 0 || kk > 0);
-      mma_commit(&bar[j % ST]);
-    }
-    if (j >= 1) ok = mbar_wait(&bar[(j - 1) % ST], (j - 1) / ST & 1, p.status);    // its stage is free
-    if (ok && j + ST - 1 < n) load(j + ST - 1);
-    cp_async_commit();
-  }
-  cp_async_wait<0>();
-  if (n > 0 && ok) ok = mbar_wait(&bar[(n - 1) % ST], (n - 1) / ST & 1, p.status);
-  ok = !__syncthreads_or(!ok);
-  tc_fence_after();
-  // this CTA's sums, row by row, where the stages were: [128][nc + 4]
-  const int ld = nc + 4;
-  float* part = reinterpret_cast<float*>(raw + (base - smem_u32(raw)));
-  const int row = warp % 4 * 32 + lane;
-  for (int c = warp / 4 * 16; c < nc; c += 32) {
-    uint32_t r[16];
-    if (n > 0 && ok) {
-      tmem_ld_32x32b_x16(tmem + ((uint32_t)(warp % 4 * 32) << 16) + c, r);
-      tmem_ld_wait();
-    }
-#pragma unroll
-    for (int e = 0; e < 16; e += 4)
-      *reinterpret_cast<float4*>(part + row * ld + c + e) =
-          n > 0 && ok ? make_float4(__uint_as_float(r[e]), __uint_as_float(r[e + 1]), __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]))
-                      : make_float4(0.f, 0.f, 0.f, 0.f);
-  }
-  tc_fence_before();
-  if (p.splits > 1) cluster_sync(); else __syncthreads();
-  if (warp == 0) {
-    tmem_relinquish();
-    tmem_dealloc(tmem, cols);
-  }
-  // the cluster's CTAs take rows in turn; a thread four neighbouring values of a row
-  const int rk = p.Rp / 4, total = t.rows * (nsr / p.R) * rk;
+// The sums of the cluster's CTAs (part [128][ld], column ss * R + j) -> v, as two bf16 numbers each.  Thread `tid` of 256.
+template <bool FP8>
+DEVI void write_v(const Args& p, int i, const Tile& t, const float* part, int ld, int sr0, int nsr, int tid) {
+  const int ns = nsr / p.R, rk = p.Rp / 4, total = t.rows * ns * rk;
   __nv_bfloat16* v = reinterpret_cast<__nv_bfloat16*>(p.v);
   const float sc = p.scale[t.slot];
+  // the CTAs take the rows in turn; a thread four neighbouring values of a row
   for (int o = tid + 256 * (p.splits > 1 ? blockIdx.z : 0); o < total; o += 256 * p.splits) {
-    const int m = o / (nsr / p.R * rk), ss = o / rk % (nsr / p.R), j = o % rk * 4;
+    const int m = o / (ns * rk), ss = o / rk % ns, j = o % rk * 4;
     float f = sc;
     if (FP8) {
       const int r = row_of(p, i, m, t.rows);
@@ -650,7 +588,7 @@ __global__ void __launch_bounds__(256) shrink128_kernel(const __grid_constant__ 
         const float* at = part + m * ld + ss * p.R + j + e;
         if (p.splits == 1) sum = *at;
         else
-          for (int z = 0; z < p.splits; ++z) {
+          for (int z = 0; z < p.splits; ++z) {             // in the CTAs' order
             float w;
             asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w) : "r"(mapa_shared(smem_u32(at), z)));
             sum += w;
@@ -664,15 +602,402 @@ __global__ void __launch_bounds__(256) shrink128_kernel(const __grid_constant__ 
     *reinterpret_cast<uint2*>(v + at) = hi;
     *reinterpret_cast<uint2*>(v + at + p.Rp) = lo;
   }
+}
+
+// TMEM sums [128 x nc] -> part, by warp quadrant `wq` (32 rows) and column half `wh`
+DEVI void sums_to_smem(uint32_t tmem, bool have, int nc, float* part, int ld, int wq, int wh) {
+  const int row = wq * 32 + (threadIdx.x & 31);
+  for (int c = wh * 16; c < nc; c += 32) {
+    uint32_t r[16] = {};
+    if (have) {
+      tmem_ld_32x32b_x16(tmem + ((uint32_t)(wq * 32) << 16) + c, r);
+      tmem_ld_wait();
+    }
+#pragma unroll
+    for (int e = 0; e < 16; e += 4)
+      *reinterpret_cast<float4*>(part + row * ld + c + e) =
+          make_float4(__uint_as_float(r[e]), __uint_as_float(r[e + 1]), __uint_as_float(r[e + 2]), __uint_as_float(r[e + 3]));
+  }
+}
+DEVI uint32_t tmem_cols(int nc) { return nc <= 32 ? 32 : nc <= 64 ? 64 : nc <= 128 ? 128 : 256; }
+
+// v of 128-row tiles: D[128 x NC] = X[128 x K] A[NC x K]^T on tcgen05, NC <= 256 rank rows of all slices together, so that x
+// is read once.  Warp 0 fills a ring of 64-k stages by TMA, x row by row number; warp 1 issues the MMAs; e4m3 rows are
+// widened to bf16 in shared memory by the other eight warps, which also carry the sums out.  A cluster of `splits` CTAs
+// shares K and adds up through distributed shared memory in a fixed order.
+constexpr int TH = 320;
+
+template <bool FP8>
+__global__ void __launch_bounds__(TH) shrink128_kernel(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap xm,
+                                                       const __grid_constant__ CUtensorMap xg, const __grid_constant__ CUtensorMap am,
+                                                       int nc_max, int stages) {
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t full[8], empty[8], cfull[2], cempty[2], done;
+  __shared__ uint32_t tmem_at;
+  const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, i = blockIdx.x;
+  const int sr0 = blockIdx.y * nc_max, nsr = min(nc_max, p.S * p.R - sr0), nc = (nsr + 15) / 16 * 16;
+  const uint32_t abytes = (uint32_t)((nc_max + 15) / 16) * 2048, xbytes = FP8 ? 8192 : 16384;
+  // e4m3: two widened x tiles first, then stages of (e4m3 x, A); bf16: stages of (x, A)
+  const uint32_t ring = base + (FP8 ? 2 * 16384 : 0), sbytes = abytes + xbytes;      // A first: 1024-byte aligned
+  const uint32_t cols = tmem_cols(nc);
+  pdl_wait();
+  pdl_trigger();
+  Tile t;
+  if (!load_tile(p, i, t) || t.rank == 0) return;          // uniform over the cluster
+  if (warp == 1) tmem_alloc(&tmem_at, cols);
+  if (tid == 0) {
+    for (int q = 0; q < stages; ++q) {
+      mbar_init(&full[q], 1);
+      mbar_init(&empty[q], FP8 ? 9 : 1);
+    }
+    for (int q = 0; q < 2; ++q) {
+      mbar_init(&cfull[q], 8);
+      mbar_init(&cempty[q], 1);
+    }
+    mbar_init(&done, 1);
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_at;
+  const int nk = (p.K + 63) / 64, per = (nk + p.splits - 1) / p.splits;
+  const int k0 = blockIdx.z * per, n = max(0, min(per, nk - k0));
+  bool ok = true;
+  if (warp == 0) {                                         // loads
+    constexpr int RBYTES = FP8 ? 64 : 128;
+    const TmaRows rows = tma_rows(p, i, t, lane);
+    int j = 0;
+    for (; j < n; ++j) {
+      const int st = j % stages;
+      ok = __all_sync(~0u, j < stages || mbar_wait(&empty[st], (j / stages - 1) & 1, p.status));
+      if (!ok) break;
+      const uint32_t as = ring + st * sbytes, xs = as + abytes;
+      if (lane == 0) {
+        mbar_arrive_expect_tx(&full[st], abytes + rows.n * rows.each * RBYTES);
+        tma_2d(as, &am, &full[st], (k0 + j) * 64, t.slot * p.S * p.R + sr0);
+      }
+      __syncwarp();
+      tma_load_rows(rows, xs, &xm, &xg, &full[st], (k0 + j) * 64, lane, RBYTES);
+    }
+    for (int q = max(0, j - stages); q < j; ++q) mbar_wait(&full[q % stages], q / stages & 1, p.status);   // no copy in flight
+  } else if (warp == 1) {                                  // MMAs
+    for (int j = 0; j < n; ++j) {
+      const int st = j % stages;
+      ok = mbar_wait(&full[st], j / stages & 1, p.status) && (!FP8 || mbar_wait(&cfull[j & 1], j / 2 & 1, p.status));
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      if (lane == 0) {
+        tc_fence_after();
+        const uint32_t as = ring + st * sbytes, xs = FP8 ? base + (j & 1) * 16384 : as + abytes;
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk)
+          mma_f16(tmem, sdesc_sw128(xs + kk * 32), sdesc_sw128(as + kk * 32), idesc_bf16(nc), j > 0 || kk > 0);
+        mma_commit(&empty[st]);
+        if (FP8) mma_commit(&cempty[j & 1]);
+        if (j == n - 1) mma_commit(&done);
+      }
+      __syncwarp();
+    }
+  } else if (FP8) {                                        // e4m3 -> bf16
+    const int id = tid - 64, c = id % 4;
+    for (int j = 0; j < n; ++j) {
+      const int st = j % stages;
+      ok = mbar_wait(&full[st], j / stages & 1, p.status) && (j < 2 || mbar_wait(&cempty[j & 1], (j / 2 - 1) & 1, p.status));
+      if (!__all_sync(~0u, ok)) { ok = false; break; }
+      const uint32_t from = ring + st * sbytes + abytes, to = base + (j & 1) * 16384;
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        const int r = id / 4 + 64 * q;
+        if (r >= t.rows) continue;
+        const uint4 f = ld_shared16(from + r * 64 + c * 16);
+        const uint2 e0 = e4m3x4_to_bf16(f.x), e1 = e4m3x4_to_bf16(f.y), e2 = e4m3x4_to_bf16(f.z), e3 = e4m3x4_to_bf16(f.w);
+        st_shared16(to + sw128(r, 2 * c), make_uint4(e0.x, e0.y, e1.x, e1.y));
+        st_shared16(to + sw128(r, 2 * c + 1), make_uint4(e2.x, e2.y, e3.x, e3.y));
+      }
+      fence_proxy_async();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&cfull[j & 1]);
+        mbar_arrive(&empty[st]);
+      }
+    }
+  }
+  if (warp != 0 && n > 0 && ok) ok = mbar_wait(&done, 0, p.status);
+  ok = !__syncthreads_or(!ok);
+  tc_fence_after();
+  const int ld = nc + 4;
+  float* part = reinterpret_cast<float*>(raw + (base - smem_u32(raw)));    // where the stages were
+  if (warp >= 2) sums_to_smem(tmem, n > 0 && ok, nc, part, ld, warp % 4, (warp - 2) / 4);
+  tc_fence_before();
+  if (p.splits > 1) cluster_sync(); else __syncthreads();
+  if (warp == 1) {
+    tmem_relinquish();
+    tmem_dealloc(tmem, cols);
+  }
+  if (warp >= 2) write_v<FP8>(p, i, t, part, ld, sr0, nsr, tid - 64);
   if (p.splits > 1) cluster_sync();                        // nobody leaves while its sums are being read
 }
 
-// out of 128-row tiles: D[128 x 128] = V[128 x 2 r] [B; B][128 x 2 r]^T on tcgen05, feature tile by feature tile; the MMAs take
-// a fraction of the time that y and out need.  B's rows are staged in the order that gives each thread of the epilogue 8
-// neighbouring features of a row (the 16x256b TMEM load hands out column pairs), so y and out move in 16-byte vectors
-// between global memory and registers.  B of the next feature tile and y of this one are on their way during the MMAs.
-template <bool VECN, bool VECR>
-__global__ void __launch_bounds__(256, 2) expand128_kernel(const __grid_constant__ Args p) {
+// out of 128-row tiles: D[128 x 128] = V[128 x 2 r] [B; B][128 x 2 r]^T on tcgen05, feature tile by feature tile.  Warp 0 loads B
+// and y by TMA (rings of two tiles), warp 1 issues the MMAs into two TMEM buffers, eight warps add and store.  B's rows are
+// gathered in the order that gives each thread of the epilogue 8 neighbouring features of a row (the 16x256b TMEM load
+// hands out column pairs), so that out moves from registers in 16-byte vectors.
+__global__ void __launch_bounds__(TH) expand128_kernel(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap ym,
+                                                       const __grid_constant__ CUtensorMap yg, const __grid_constant__ CUtensorMap vm,
+                                                       const __grid_constant__ CUtensorMap bm, const __grid_constant__ CUtensorMap bg) {
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t bfull[2], bempty[2], yfull[2], yempty[2], dfull[2], dempty[2], vfull;
+  __shared__ uint32_t tmem_at;
+  const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, i = blockIdx.y;
+  const int rb = min(p.Rp, 64) <= 16 ? 32 : min(p.Rp, 64) <= 32 ? 64 : 128;    // bytes of an operand row
+  const int kc = (p.Rp + 63) / 64, ot = 128 * rb;          // operand tiles over the ranks, and their size
+  const int bst = kc <= 2 ? 2 : 1;                         // stages of B, as far as shared memory goes
+  const int yst = kc <= 3 ? 2 : 1;                         // and of y
+  const uint32_t yb = base, vb = yb + yst * 32768, bb = vb + 2 * kc * ot;
+  int s, ne;
+  const int nb = slice_of(p, blockIdx.x, 128 * p.steps, s, ne), nt = min(p.steps, (ne - nb + 127) / 128);
+  Tile t;
+  if (!load_tile(p, i, t) || (t.slot < 0 && p.out == p.y)) {
+    pdl_wait();
+    return;
+  }
+  if (warp == 1) tmem_alloc(&tmem_at, 256);
+  if (tid == 0) {
+    for (int q = 0; q < 2; ++q) {
+      mbar_init(&bfull[q], 1); mbar_init(&bempty[q], 1);
+      mbar_init(&yfull[q], 1); mbar_init(&yempty[q], 8);
+      mbar_init(&dfull[q], 1); mbar_init(&dempty[q], 8);
+    }
+    mbar_init(&vfull, 1);
+    fence_mbar_init();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_at;
+  const int rk16 = (t.rank + 15) / 16;                     // MMA steps
+  bool ok = true;
+  if (warp == 0) {                                         // loads
+    const int ks = (rk16 + 3) / 4;
+    const TmaRows rows = tma_rows(p, i, t, lane);
+    auto load = [&](int j) {
+      const int n0 = nb + 128 * j, halves = n0 + 64 < ne ? 2 : 1;
+      ok = __all_sync(~0u, j < yst || mbar_wait(&yempty[j % yst], (j / yst - 1) & 1, p.status));
+      if (!ok) return;
+      if (lane == 0) mbar_arrive_expect_tx(&yfull[j % yst], halves * rows.n * rows.each * 128);
+      __syncwarp();
+      for (int h = 0; h < halves; ++h)
+        tma_load_rows(rows, yb + j % yst * 32768 + h * 16384, &ym, &yg, &yfull[j % yst], n0 + 64 * h, lane, 128);
+      if (t.rank == 0) return;
+      const int st = j % bst;
+      ok = __all_sync(~0u, j < bst || mbar_wait(&bempty[st], (j / bst - 1) & 1, p.status));
+      if (!ok) return;
+      if (lane == 0) mbar_arrive_expect_tx(&bfull[st], ks * ot);
+      __syncwarp();
+      // 32 features in the epilogue's order: one box of a map that sees feature 8 a + 2 m + b as (b, a, m); at the end of the
+      // last adapter, where that box would leave the tensor, four rows at a time by number
+      const int64_t l0 = (int64_t)t.slot * p.N;
+      const int blk = lane >> 3, f = n0 + 32 * blk;
+      const bool box = l0 + f + 32 <= (int64_t)p.L * p.N && (l0 + f) % 8 == 0;
+      const int f4 = f + (lane & 1) * 16 + (lane >> 1 & 3) * 2;              // rows 4 lane .. + 3 of the tile
+      for (int k = 0; k < ks; ++k) {
+        if (box) {
+          if (lane % 8 == 0) tma_5d(bb + st * kc * ot + k * ot + blk * 32 * rb, &bm, &bfull[st], 64 * k, (int)((l0 + f) / 8));
+        } else {
+          tma_gather4(bb + st * kc * ot + k * ot + lane * 4 * rb, &bg, &bfull[st], 64 * k,
+                      make_int4((int)(l0 + min(f4, ne - 1)), (int)(l0 + min(f4 + 1, ne - 1)), (int)(l0 + min(f4 + 8, ne - 1)),
+                                (int)(l0 + min(f4 + 9, ne - 1))));
+        }
+      }
+    };
+    // y and B do not depend on v: the first tiles are on their way before the wait for the shrinking kernel, which itself
+    // waited for whatever wrote them
+    int j = 0;
+    load(j++);
+    pdl_wait();
+    if (ok && t.rank > 0 && lane == 0) {
+      mbar_arrive_expect_tx(&vfull, 2 * ks * ot);
+      for (int q = 0; q < 2 * ks; ++q)
+        tma_load_2d(raw + (vb - smem_u32(raw)) + (q / ks * kc + q % ks) * ot, &vm, &vfull,
+                    (s * 2 + q / ks) * p.Rp + 64 * (q % ks), i * 128);
+    }
+    __syncwarp();
+    for (; ok && j < nt; ++j) load(j);
+    for (int q = max(0, j - 2); q < j; ++q) {              // no copy stays in flight
+      if (q >= j - yst) mbar_wait(&yfull[q % yst], q / yst & 1, p.status);
+      if (t.rank > 0 && q >= j - bst) mbar_wait(&bfull[q % bst], q / bst & 1, p.status);
+    }
+    if (t.rank > 0) mbar_wait(&vfull, 0, p.status);
+  } else if (warp == 1) {                                  // MMAs
+    pdl_wait();                                            // a bounded wait covers no other kernel's time
+    for (int j = 0; t.rank > 0 && j < nt; ++j) {
+      const int st = j % bst;
+      ok = (j > 0 || mbar_wait(&vfull, 0, p.status)) && mbar_wait(&bfull[st], j / bst & 1, p.status) &&
+           (j < 2 || mbar_wait(&dempty[j & 1], (j / 2 - 1) & 1, p.status));
+      if (!__all_sync(~0u, ok)) { ok = false; break; }
+      const uint32_t bs = bb + st * kc * ot;
+      if (t.rank & 15) {                                   // what the slot holds beyond the adapter's rank counts as zero
+        for (int r = lane; r < 128; r += 32)
+          for (int k = t.rank; k < rk16 * 16; ++k)
+            asm volatile("st.shared.u16 [%0], %1;" ::"r"(bs + k / 64 * ot + sw_rows(r, k % 64 / 8, rb) + k % 8 * 2), "h"((uint16_t)0) : "memory");
+        fence_proxy_async();
+        __syncwarp();
+      }
+      if (lane == 0) {
+        tc_fence_after();
+        for (int hl = 1; hl >= 0; --hl)
+          for (int kk = 0; kk < rk16; ++kk) {
+            const uint32_t o = (kk / 4) * ot + (kk % 4) * 32;
+            mma_f16(tmem + (j & 1) * 128, sdesc_rows(vb + hl * kc * ot + o, rb), sdesc_rows(bs + o, rb), idesc_bf16(128),
+                    hl == 0 || kk > 0);
+          }
+        mma_commit(&bempty[st]);
+        mma_commit(&dfull[j & 1]);
+      }
+      __syncwarp();
+    }
+  } else {                                                 // out = y + D
+    const int wq = warp % 4, wh = (warp - 2) / 4, g = lane >> 2, q4 = lane & 3;
+    const bool rows_here = wq * 32 < t.rows;
+    __nv_bfloat16* to[2][2];
+#pragma unroll
+    for (int rh = 0; rh < 2; ++rh)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = row_of(p, i, wq * 32 + 16 * rh + 8 * h + g, t.rows);
+        to[rh][h] = r >= 0 ? p.out + r * p.out_ld + nb + wh * 64 + 8 * q4 : nullptr;
+      }
+    pdl_wait();
+    pdl_trigger();
+    for (int j = 0; j < nt; ++j) {
+      ok = mbar_wait(&yfull[j % yst], j / yst & 1, p.status) && (t.rank == 0 || mbar_wait(&dfull[j & 1], j / 2 & 1, p.status));
+      if (!__all_sync(~0u, ok)) { ok = false; break; }
+      tc_fence_after();
+      const int left = ne - nb - 128 * j - wh * 64 - 8 * q4;             // features from this thread's first on
+      if (rows_here) {
+#pragma unroll
+        for (int rh = 0; rh < 2; ++rh) {
+          uint32_t r[2][16];
+          if (t.rank > 0) {
+#pragma unroll
+            for (int cb = 0; cb < 2; ++cb)
+              tmem_ld_16x256b_x4(tmem + ((uint32_t)(wq * 32 + 16 * rh) << 16) + (j & 1) * 128 + wh * 64 + 32 * cb, r[cb]);
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (int cb = 0; cb < 2; ++cb)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (to[rh][h] == nullptr || 32 * cb >= left) continue;
+              uint4 o = ld_shared16(yb + j % yst * 32768 + wh * 16384 + sw128(wq * 32 + 16 * rh + 8 * h + g, 4 * cb + q4));
+              if (t.rank > 0) {
+                uint32_t* w = reinterpret_cast<uint32_t*>(&o);
+#pragma unroll
+                for (int m = 0; m < 4; ++m) {
+                  const __nv_bfloat162 f = *reinterpret_cast<const __nv_bfloat162*>(&w[m]);
+                  w[m] = pack2(__low2float(f) + __uint_as_float(r[cb][4 * m + 2 * h]),
+                               __high2float(f) + __uint_as_float(r[cb][4 * m + 2 * h + 1]));
+                }
+              }
+              __nv_bfloat16* at = to[rh][h] + 128 * j + 32 * cb;
+              if (left - 32 * cb >= 8) *reinterpret_cast<uint4*>(at) = o;
+              else {
+                const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  if (e < left - 32 * cb) at[e] = __ushort_as_bfloat16((uint16_t)(w[e / 2] >> 16 * (e % 2)));
+              }
+            }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&yempty[j % yst]);
+        if (t.rank > 0) mbar_arrive(&dempty[j & 1]);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tmem_relinquish();
+    tmem_dealloc(tmem, 256);
+  }
+}
+
+// 128-row tiles whose rows TMA cannot take (an odd K, N or row stride): the same products, operands moved by ordinary loads.
+// Eight warps fill the stage, one thread multiplies.
+template <bool FP8>
+__global__ void __launch_bounds__(256) shrink128_any_kernel(const __grid_constant__ Args p, int nc_max) {
+  extern __shared__ uint8_t raw[];
+  __shared__ uint64_t bar[2];
+  __shared__ uint32_t tmem_at;
+  const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
+  const int tid = threadIdx.x, warp = tid / 32, i = blockIdx.x;
+  const int sr0 = blockIdx.y * nc_max, nsr = min(nc_max, p.S * p.R - sr0), nc = (nsr + 15) / 16 * 16;
+  const uint32_t sbytes = 16384 + (uint32_t)((nc_max + 15) / 16) * 2048, cols = tmem_cols(nc);
+  pdl_wait();
+  pdl_trigger();
+  Tile t;
+  if (!load_tile(p, i, t) || t.rank == 0) return;          // uniform over the cluster
+  if (warp == 0) tmem_alloc(&tmem_at, cols);
+  if (tid < 2) mbar_init(&bar[tid], 1);
+  fence_mbar_init();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_at;
+  const int nk = (p.K + 63) / 64, per = (nk + p.splits - 1) / p.splits;
+  const int k0 = blockIdx.z * per, n = max(0, min(per, nk - k0));
+  const uint8_t* x[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int row = row_of(p, i, tid / 8 + 32 * q, t.rows);
+    x[q] = row >= 0 ? static_cast<const uint8_t*>(p.x) + row * p.x_ld * (FP8 ? 1 : 2) : nullptr;
+  }
+  const __nv_bfloat16* a = p.a + ((int64_t)t.slot * p.S * p.R + sr0) * p.K;
+  bool ok = true;
+  for (int j = 0; j < n; ++j) {
+    if (j >= 2) ok = mbar_wait(&bar[j & 1], (j / 2 - 1) & 1, p.status);     // its stage is free
+    const uint32_t xs = base + (j & 1) * sbytes, as = xs + 16384;
+    const int k = (k0 + j) * 64 + tid % 8 * 8;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (x[q]) st_shared16(xs + sw128(tid / 8 + 32 * q, tid % 8), load8<FP8, false>(x[q], k, p.K));
+    for (int r = tid / 8; r < nsr; r += 32)
+      st_shared16(as + sw128(r, tid % 8), load8<false, false>(a + (int64_t)r * p.K, k, p.K));
+    fence_proxy_async();
+    if (__syncthreads_or(!ok)) { ok = false; break; }
+    if (tid == 0) {
+      tc_fence_after();
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        mma_f16(tmem, sdesc_sw128(xs + kk * 32), sdesc_sw128(as + kk * 32), idesc_bf16(nc), j > 0 || kk > 0);
+      mma_commit(&bar[j & 1]);
+    }
+  }
+  if (n > 0 && ok) ok = mbar_wait(&bar[(n - 1) & 1], (n - 1) / 2 & 1, p.status);
+  ok = !__syncthreads_or(!ok);
+  tc_fence_after();
+  const int ld = nc + 4;
+  float* part = reinterpret_cast<float*>(raw + (base - smem_u32(raw)));    // where the stages were
+  sums_to_smem(tmem, n > 0 && ok, nc, part, ld, warp % 4, warp / 4);
+  tc_fence_before();
+  if (p.splits > 1) cluster_sync(); else __syncthreads();
+  if (warp == 0) {
+    tmem_relinquish();
+    tmem_dealloc(tmem, cols);
+  }
+  write_v<FP8>(p, i, t, part, ld, sr0, nsr, tid);
+  if (p.splits > 1) cluster_sync();                        // nobody leaves while its sums are being read
+}
+
+template <bool VECN>
+__global__ void __launch_bounds__(256, 2) expand128_any_kernel(const __grid_constant__ Args p) {
   extern __shared__ uint8_t raw[];
   __shared__ uint64_t bar;
   __shared__ uint32_t tmem_at;
@@ -710,30 +1035,23 @@ __global__ void __launch_bounds__(256, 2) expand128_kernel(const __grid_constant
       const int r = o / chunks, c = o % chunks;
       const int nn = n0 + (r & ~31) + 8 * ((r & 7) >> 1) + 2 * (r >> 3 & 3) + (r & 1);
       if (nn >= ne) continue;
-      const __nv_bfloat16* src = bt + (int64_t)nn * p.R + 8 * c;
-      const uint32_t dst = bb + (j & 1) * bstage + (c / 8) * 16384 + sw128(r, c % 8);
-      const int left = t.rank - 8 * c;
-      if (VECR && (left >= 8 || left <= 0)) cp_async16(dst, left > 0 ? src : bt, left > 0);
-      else {
-        uint32_t w[4] = {};
-        for (int e = 0; e < min(left, 8); ++e) w[e / 2] |= (uint32_t)__bfloat16_as_ushort(src[e]) << 16 * (e % 2);
-        st_shared16(dst, make_uint4(w[0], w[1], w[2], w[3]));
-      }
+      uint32_t w[4] = {};
+      for (int e = 0; e < min(t.rank - 8 * c, 8); ++e)     // ranks beyond the adapter's own count as zero
+        w[e / 2] |= (uint32_t)__bfloat16_as_ushort(bt[(int64_t)nn * p.R + 8 * c + e]) << 16 * (e % 2);
+      st_shared16(bb + (j & 1) * bstage + (c / 8) * 16384 + sw128(r, c % 8), make_uint4(w[0], w[1], w[2], w[3]));
     }
   };
   if (t.rank > 0) load_b(0);
-  cp_async_commit();
   pdl_wait();
   pdl_trigger();
   if (t.rank > 0) {
     const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(p.v);
     for (int o = tid; o < t.rows * 2 * chunks; o += 256) {
       const int r = o / (2 * chunks), hl = o / chunks % 2, c = o % chunks;
-      cp_async16(vb + (hl * kc + c / 8) * 16384 + sw128(r, c % 8),
-                 v + ((((int64_t)i * 128 + r) * p.S + s) * 2 + hl) * p.Rp + 8 * c, true);
+      st_shared16(vb + (hl * kc + c / 8) * 16384 + sw128(r, c % 8),
+                  *reinterpret_cast<const uint4*>(v + ((((int64_t)i * 128 + r) * p.S + s) * 2 + hl) * p.Rp + 8 * c));
     }
   }
-  cp_async_commit();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -750,9 +1068,6 @@ __global__ void __launch_bounds__(256, 2) expand128_kernel(const __grid_constant
         for (int cb = 0; cb < 2; ++cb)
           y[rh][h][cb] = load_y<VECN>(yo[rh][h] >= 0 ? p.y + yo[rh][h] : nullptr, n0 + warp / 4 * 64 + 32 * cb + 8 * q4, ne);
     if (t.rank > 0) {
-      if (two && j + 1 < nt) load_b(j + 1);
-      cp_async_commit();
-      cp_async_wait<1>();
       fence_proxy_async();
       tc_fence_before();
       if (__syncthreads_or(!ok)) { ok = false; break; }
@@ -766,12 +1081,10 @@ __global__ void __launch_bounds__(256, 2) expand128_kernel(const __grid_constant
           }
         mma_commit(&bar);
       }
+      if (two && j + 1 < nt) load_b(j + 1);
       ok = __all_sync(0xffffffffu, mbar_wait(&bar, j & 1, p.status));
       tc_fence_after();
-      if (!two && j + 1 < nt) {
-        load_b(j + 1);
-        cp_async_commit();
-      }
+      if (!two && j + 1 < nt) load_b(j + 1);
     }
     if (!rows_here || !ok) continue;
 #pragma unroll
@@ -805,7 +1118,6 @@ __global__ void __launch_bounds__(256, 2) expand128_kernel(const __grid_constant
         }
       }
   }
-  cp_async_wait<0>();
   tc_fence_before();
   __syncthreads();
   if (warp == 0) {
@@ -818,12 +1130,12 @@ __global__ void __launch_bounds__(256, 2) expand128_kernel(const __grid_constant
 // launches
 // ---------------------------------------------------------------------------------------------
 template <typename... A>
-void launch(void (*kern)(A...), dim3 grid, int cx, int cz, size_t smem, cudaStream_t stream, A... args) {
+void launch(void (*kern)(A...), dim3 grid, int threads, int cx, int cz, size_t smem, cudaStream_t stream, A... args) {
   if (smem > 48 * 1024)
     C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(256);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[2];
@@ -859,7 +1171,7 @@ void launch16(Args& p, bool fp8, bool vec, const at::TensorOptions& opts, cudaSt
     const size_t smem = (8 * 16 * RS<JG> + 256 * JG + 16 * (p.Rp + 4)) * sizeof(float);
     auto k = fp8 ? (vec ? decode_kernel<JG, true, true> : decode_kernel<JG, true, false>)
                  : (vec ? decode_kernel<JG, false, true> : decode_kernel<JG, false, false>);
-    launch(k, dim3(ch * CL, p.max_tiles), CL, 1, smem, st, p);
+    launch(k, dim3(ch * CL, p.max_tiles), 256, CL, 1, smem, st, p);
     return;
   }
   const int groups = (p.Rp + 16 * JG - 1) / (16 * JG);
@@ -870,31 +1182,53 @@ void launch16(Args& p, bool fp8, bool vec, const at::TensorOptions& opts, cudaSt
   p.v = ws.data_ptr<float>();
   auto k = fp8 ? (vec ? shrink16_kernel<JG, true, true> : shrink16_kernel<JG, true, false>)
                : (vec ? shrink16_kernel<JG, false, true> : shrink16_kernel<JG, false, false>);
-  launch(k, dim3(p.max_tiles, p.S * groups, p.splits), 1, 1, 0, st, p);
-  launch(vec ? expand16_kernel<JG, true> : expand16_kernel<JG, false>, dim3(chunks(p, STEP), p.max_tiles), 1, 1,
+  launch(k, dim3(p.max_tiles, p.S * groups, p.splits), 256, 1, 1, 0, st, p);
+  launch(vec ? expand16_kernel<JG, true> : expand16_kernel<JG, false>, dim3(chunks(p, STEP), p.max_tiles), 256, 1, 1,
          16 * (p.Rp + 4) * sizeof(float), st, p);
 }
 
 // 128-row tiles
-void launch128(Args& p, bool fp8, bool vec_k, bool vec_n, const at::TensorOptions& opts, cudaStream_t st) {
+int rank_rows(const Args& p) { return std::max(1, std::min(p.S, 256 / p.R)) * p.R; }   // of whole slices: the MMA's N
+
+void launch128(Args& p, const CUtensorMap& am, const CUtensorMap& bm, const CUtensorMap& bg, bool fp8, bool tma_k, bool tma_n, bool vec_n,
+               const at::TensorOptions& opts, cudaStream_t st) {
   torch::Tensor ws = torch::empty({(int64_t)p.max_tiles * 128 * p.S * p.Rp}, opts);
   p.v = ws.data_ptr<float>();
-  // rank rows of whole slices, at most 256 (the MMA's N)
-  const int nc = std::max(1, std::min(p.S, 256 / p.R)) * p.R, groups = (p.S * p.R + nc - 1) / nc, nc16 = (nc + 15) / 16 * 16;
+  const int nc = rank_rows(p), groups = (p.S * p.R + nc - 1) / nc, nc16 = (nc + 15) / 16 * 16;
   const int64_t ctas = (int64_t)p.max_tiles * groups;
-  for (p.splits = 1; p.splits < 8 && ctas * p.splits * 2 <= 2 * 148 && p.K >= 64 * ST * p.splits * 2;) p.splits *= 2;
-  const size_t stages = ST * (16384 + (size_t)nc16 * 128 + (fp8 ? 8192 : 0)), sums = 128 * (nc16 + 4) * sizeof(float);
-  auto k = fp8 ? (vec_k ? shrink128_kernel<true, true> : shrink128_kernel<true, false>)
-               : (vec_k ? shrink128_kernel<false, true> : shrink128_kernel<false, false>);
-  launch(k, dim3(p.max_tiles, groups, p.splits), 1, p.splits, std::max(stages, sums) + 2048, st, p, nc);
+  for (p.splits = 1; p.splits < 8 && ctas * p.splits * 2 <= 2 * 148 && p.K >= 256 * p.splits * 2;) p.splits *= 2;
+  const size_t sums = 128 * (nc16 + 4) * sizeof(float) + 1024;
+  const dim3 grid(p.max_tiles, groups, p.splits);
+  if (tma_k) {
+    const size_t fixed = 1024 + (fp8 ? 2 * 16384 : 0), stage = nc16 * 128 + (fp8 ? 8192 : 16384);
+    const int stages = std::min<size_t>(8, (113 * 1024 - fixed) / stage >= 3 ? (113 * 1024 - fixed) / stage : (225 * 1024 - fixed) / stage);
+    const auto map = [&](int box) {
+      return make_tma_2d(const_cast<void*>(p.x), fp8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.K, p.T,
+                         p.x_ld * (fp8 ? 1 : 2), 64, box, fp8 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    launch(fp8 ? shrink128_kernel<true> : shrink128_kernel<false>, grid, TH, 1, p.splits, std::max(fixed + stages * stage, sums),
+           st, p, map(16), map(1), am, nc, stages);
+  } else {
+    launch(fp8 ? shrink128_any_kernel<true> : shrink128_any_kernel<false>, grid, 256, 1, p.splits,
+           std::max((size_t)1024 + 2 * (16384 + nc16 * 128), sums), st, p, nc);
+  }
   // feature tiles of a CTA: v is staged once for all of them, as long as every SM has a few CTAs
   for (p.steps = 1; p.steps < 16 && (int64_t)chunks(p, 128 * p.steps * 2) * p.max_tiles >= 4 * 148;) p.steps *= 2;
-  const int kc = (p.Rp + 63) / 64;
-  const size_t smem = (kc <= 3 ? 4 : 3) * kc * 16384 + 1024;
-  const bool vec_r = p.R % 8 == 0;
-  auto e = vec_n ? (vec_r ? expand128_kernel<true, true> : expand128_kernel<true, false>)
-                 : (vec_r ? expand128_kernel<false, true> : expand128_kernel<false, false>);
-  launch(e, dim3(chunks(p, 128 * p.steps), p.max_tiles), 1, 1, smem, st, p);
+  const dim3 ge(chunks(p, 128 * p.steps), p.max_tiles);
+  const int kc = (p.Rp + 63) / 64, rb = p.Rp <= 16 ? 32 : p.Rp <= 32 ? 64 : 128;
+  if (tma_n) {
+    const auto map = [&](int box) {
+      return make_tma_2d((void*)p.y, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, p.N, p.T, p.y_ld * 2, 64, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    };
+    const CUtensorMap vm = make_tma_2d(p.v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (uint64_t)p.S * 2 * p.Rp, (uint64_t)p.max_tiles * 128,
+                                       (uint64_t)p.S * 4 * p.Rp, rb / 2, 128,
+                                       rb == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : rb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
+    launch(expand128_kernel, ge, TH, 1, 1, 1024 + (kc <= 3 ? 2 : 1) * 32768 + (size_t)(kc <= 2 ? 4 : 3) * kc * 128 * rb, st, p, map(16), map(1), vm,
+           bm, bg);
+  } else {
+    launch(vec_n ? expand128_any_kernel<true> : expand128_any_kernel<false>, ge, 256, 1, 1,
+           (size_t)(kc <= 3 ? 4 : 3) * kc * 16384 + 1024, st, p);
+  }
 }
 
 [[noreturn]] void refuse(const std::string& why) { throw pybind11::value_error("lora_add: " + why); }
@@ -913,6 +1247,8 @@ bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
 struct LoraBank {
   torch::Tensor a, b, scale, ranks, status;
   lora::Args args;
+  bool tma_k = false, tma_n = false;                       // rows of a / b that TMA can take
+  CUtensorMap am, bm, bg;
   LoraBank(torch::Tensor a_, torch::Tensor b_, torch::Tensor scale_, torch::Tensor ranks_, std::vector<int64_t> slices,
            torch::Tensor status_)
       : a(a_), b(b_), scale(scale_), ranks(ranks_), status(status_) {
@@ -923,6 +1259,24 @@ struct LoraBank {
     args.L = a.size(0); args.S = a.size(1); args.R = a.size(2); args.K = a.size(3); args.N = b.size(1);
     args.Rp = (args.R + 15) / 16 * 16;
     for (size_t s = 0; s < slices.size(); ++s) args.off[s] = slices[s];
+    const int64_t rows = (int64_t)args.L * args.S * args.R, brows = (int64_t)args.L * args.N;
+    if ((tma_k = args.K % 8 == 0 && (uintptr_t)args.a % 16 == 0 && rows < (1ll << 31)))
+      am = make_tma_2d(a.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, args.K, rows, args.K * 2ll, 64,
+                       (lora::rank_rows(args) + 15) / 16 * 16, CU_TENSOR_MAP_SWIZZLE_128B);
+    if ((tma_n = args.R % 8 == 0 && (uintptr_t)args.b % 16 == 0 && brows < (1ll << 31))) {
+      const int rb = args.Rp <= 16 ? 32 : args.Rp <= 32 ? 64 : 128;
+      const auto swz = rb == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : rb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+      bg = make_tma_2d(b.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, args.R, brows, args.R * 2ll, rb / 2, 1, swz);
+      // (rank, b, a, m, u): feature 8 (u + a) + 2 m + b; the last three u would reach beyond the tensor
+      const cuuint64_t row = args.R * 2ll, dims[5] = {(cuuint64_t)args.R, 2, 4, 4, (cuuint64_t)std::max<int64_t>(1, brows / 8 - 3)};
+      const cuuint64_t strides[4] = {row, 8 * row, 2 * row, 8 * row};
+      const cuuint32_t box[5] = {(cuuint32_t)rb / 2, 2, 4, 4, 1}, each[5] = {1, 1, 1, 1, 1};
+      tma_n = brows >= 32;
+      if (tma_n)
+        TORCH_CHECK(get_encode_tiled()(&bm, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, b.data_ptr(), dims, strides, box, each,
+                                       CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                       CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS, "LoraBank: tensor map of b");
+    }
   }
 };
 struct LoraPlan {
@@ -979,7 +1333,7 @@ torch::Tensor lora_add(const torch::Tensor& y, const torch::Tensor& x, const c10
     else if (p.Rp <= 32) lora::launch16<2>(p, fp8, vec, opts, stream);
     else lora::launch16<4>(p, fp8, vec, opts, stream);
   } else {
-    lora::launch128(p, fp8, vec_k, vec_n, opts, stream);
+    lora::launch128(p, bank.am, bank.bm, bank.bg, fp8, bank.tma_k && vec_k, bank.tma_n && vec_n, vec_n, opts, stream);
   }
   return out;
 }

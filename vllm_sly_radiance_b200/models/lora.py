@@ -46,7 +46,7 @@ class AdapterBank:
 
 class AdapterPlan:
     """The rows of one step by adapter slot, in tiles of at most ``tile_rows`` rows of one adapter.  buf int32: [0] tiles
-    in use, from 4 on (slot, rows, 0, 0) per tile, then ``tile_rows`` row numbers per tile."""
+    in use, from 4 on (slot, rows, 1 if the rows are consecutive, 0) per tile, then ``tile_rows`` row numbers per tile."""
 
     # rows per tile: decode batches (few rows per adapter), prompts
     TILE_DECODE, TILE_PROMPT = 16, 128
@@ -90,7 +90,8 @@ class AdapterPlan:
         words = np.zeros(AdapterPlan.words(max_tiles, tile_rows), np.int32) if out is None else out
         words[:4] = (n, 0, 0, 0)
         tiles = words[4:4 + 4 * n].reshape(n, 4)
-        tiles[:, 0], tiles[:, 1] = srt[starts[grp]], rows
+        tiles[:, 0], tiles[:, 1], tiles[:, 3] = srt[starts[grp]], rows, 0
+        tiles[:, 2] = order[first + rows - 1] - order[first] == rows - 1       # the order within a tile is ascending
         at = 4 + 4 * max_tiles + np.repeat(np.arange(n) * tile_rows - first, rows) + np.arange(T)
         words[at] = order
         return words, max_tiles, tile_rows
