@@ -15,19 +15,41 @@ def bank(L=3, S=2, R=8, Kd=32, N=24, sl=(0, 16, 24)):
 
 
 @pytest.mark.parametrize("T", [0, 1, 15, 16, 17, 100, 1000])
-@pytest.mark.parametrize("tile_rows", [None, 16, 128])
-def test_plan_covers_every_row_once(T, tile_rows):
+@pytest.mark.parametrize("tall_from", [None, 1, 128])
+@pytest.mark.parametrize("room", [None, 80])
+def test_plan_covers_every_row_once(T, tall_from, room):
     slots = np.random.default_rng(T).integers(-1, 7, T)
-    w, mt, tr = AdapterPlan.pack(slots, 7, tile_rows=tile_rows)
-    n = w[0]
-    assert w.size == AdapterPlan.words(mt, tr) and n <= mt
-    seen = []
-    for i, (s, rows, _, _) in enumerate(w[4:4 + 4 * n].reshape(n, 4)):
-        assert 0 < rows <= tr
-        r = w[4 + 4 * mt + i * tr:][:rows]
-        assert (slots[r] == s).all()
-        seen += r.tolist()
+    if T == 1000:
+        slots[300:700] = 2
+    w, t16, t128 = AdapterPlan.pack(slots, 7, tiles16=room, tiles128=room, tall_from=tall_from)
+    assert w.size == AdapterPlan.words(t16, t128)
+    seen, at = [], 0
+    for height, room_ in ((16, t16), (128, t128)):
+        n, none = w[at], w[at + 1]
+        tiles = w[at + 4:at + 4 + 4 * n].reshape(n, 4)
+        assert n <= room_ and (tiles[:none, 0] == -1).all() and (tiles[none:, 0] >= 0).all()
+        for i, (s, rows, seq, _) in enumerate(tiles):
+            assert 0 < rows <= height
+            r = w[at + 4 + 4 * room_ + i * height:][:rows]
+            assert (slots[r] == s).all() and seq == (np.diff(r) == 1).all()
+            seen += r.tolist()
+        at += 4 + (4 + height) * room_
     assert sorted(seen) == list(range(T))
+
+
+def test_plan_heights():
+    """Few rows of an adapter go into short tiles, unless there are tall tiles anyway and few such remainders."""
+    few = np.repeat(np.arange(3), 20)
+    assert AdapterPlan.pack(few, 3)[1:] == (6, 0)
+    assert AdapterPlan.pack(np.r_[few, np.full(60, 3)], 4)[1:] == (0, 4)
+    many = np.r_[np.zeros(200, int), np.arange(1, 41)]
+    assert AdapterPlan.pack(many, 41)[1:] == (40, 2)
+    assert AdapterPlan.pack(np.zeros(140, int), 1, tall_from=128)[1:] == (1, 1)
+
+
+def test_plan_of_short_tiles_only():
+    w, t16, t128 = AdapterPlan.pack(np.zeros(300, int), 1, tiles16=300, tiles128=0)
+    assert (t16, t128, w[0]) == (300, 0, 19)
 
 
 def test_plan_refusals():
@@ -36,7 +58,9 @@ def test_plan_refusals():
     with pytest.raises(ValueError):
         AdapterPlan.pack(np.array([-2]), 3)
     with pytest.raises(ValueError):
-        AdapterPlan.pack(np.arange(5), 5, max_tiles=4, tile_rows=16)
+        AdapterPlan.pack(np.arange(5), 5, tiles16=4)
+    with pytest.raises(ValueError):
+        AdapterPlan.pack(np.zeros(300, int), 5, tiles128=1)
 
 
 def test_cpu_form():

@@ -67,8 +67,9 @@ def run(y, x, a, b, sc, rk, sl, slots, inplace=False, tile_rows=None):
     if tile_rows is None:
         plan = AdapterPlan.build(np.asarray(slots), a.shape[0], DEV)
     else:
-        w, mt, tr = AdapterPlan.pack(np.asarray(slots), a.shape[0], tile_rows=tile_rows)
-        plan = AdapterPlan(torch.from_numpy(w).to(DEV), len(slots), mt, tr, a.shape[0])
+        w, t16, t128 = AdapterPlan.pack(np.asarray(slots), a.shape[0], tall_from=1 if tile_rows == 128 else None,
+                                        tiles128=0 if tile_rows == 16 else None)
+        plan = AdapterPlan(torch.from_numpy(w).to(DEV), len(slots), t16, t128, a.shape[0])
     yd = dev(y)
     got = K.lora_add(yd, dev(x), bank, plan, out=yd if inplace else None)
     torch.cuda.synchronize()
@@ -180,9 +181,9 @@ def test_lora_graph_replay_with_new_plan():
     T, L = 24, 6
     y, x, a, b, sc, rk, sl = make(T, 512, [192], 16, L, True, seed=3)
     bank = AdapterBank(a.to(DEV), b.to(DEV), sc.to(DEV), rk.to(DEV), sl)
-    words, mt, tr = AdapterPlan.pack(np.arange(T) % L, L, max_tiles=T, tile_rows=16)
+    words, t16, t128 = AdapterPlan.pack(np.arange(T) % L, L, tiles16=T, tiles128=0)
     buf = torch.from_numpy(words).to(DEV)
-    plan = AdapterPlan(buf, T, mt, tr, L)
+    plan = AdapterPlan(buf, T, t16, t128, L)
     yd, xd = y.to(DEV), dev(x)
     for _ in range(2):
         K.lora_add(yd, xd, bank, plan)
@@ -191,7 +192,7 @@ def test_lora_graph_replay_with_new_plan():
     with torch.cuda.graph(g):
         out = K.lora_add(yd, xd, bank, plan)
     for slots in (np.full(T, -1), np.full(T, 2), np.random.default_rng(0).integers(-1, L, T)):
-        w, _, _ = AdapterPlan.pack(slots, L, max_tiles=T, tile_rows=16)
+        w, _, _ = AdapterPlan.pack(slots, L, tiles16=T, tiles128=0)
         buf.copy_(torch.from_numpy(w))
         g.replay()
         torch.cuda.synchronize()
@@ -204,14 +205,14 @@ def test_lora_bad_plan_is_reported():
     """A plan buffer that names rows or slots that do not exist is refused on the device, with the status word set."""
     y, x, a, b, sc, rk, sl = make(4, 128, [64], 8, 2, False)
     bank = AdapterBank(a.to(DEV), b.to(DEV), sc.to(DEV), rk.to(DEV), sl)
-    for tile_rows, at, val in [(tr, *q) for tr in (16, 128) for q in ((0, 3), (4, 2), (5, 129), (5, -1), (12, 4), (12, -1))]:
-        w, mt, tr = AdapterPlan.pack(np.array([0, 0, 1, 1]), 2, tile_rows=tile_rows)
-        assert mt == 2
-        w[at] = val
-        plan = AdapterPlan(torch.from_numpy(w).to(DEV), 4, mt, tr, 2)
-        K.lora_add(y.to(DEV), x.to(DEV), bank, plan)
-        with pytest.raises(K.KernelFaultError):
-            K.check_status(torch.device(DEV, 0))
+    for tall in (0, 1):
+        for at, val in ((0, 3), (4, 2), (5, 129), (5, -1), (12, 4), (12, -1)):
+            w, t16, t128 = AdapterPlan.pack(np.array([0, 0, 1, 1]), 2, tall_from=1, tiles128=2 * tall)
+            w[at + 4 * tall] = val                      # an empty 16-row list is 4 words
+            plan = AdapterPlan(torch.from_numpy(w).to(DEV), 4, t16, t128, 2)
+            K.lora_add(y.to(DEV), x.to(DEV), bank, plan)
+            with pytest.raises(K.KernelFaultError):
+                K.check_status(torch.device(DEV, 0))
     K.check_status(torch.device(DEV, 0))
 
 

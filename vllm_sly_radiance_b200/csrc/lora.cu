@@ -7,8 +7,8 @@
 // bf16; s(n) is the part of a merged projection that output feature n belongs to.  The rows come sorted by adapter in
 // tiles of one adapter each (the plan): 16 rows a tile for decode batches, 128 for prompts.
 //
-// plan (int32): [0] tiles in use; from word 4 (slot, rows, 1 if the rows are consecutive, 0) per tile; then tile_rows row
-// numbers per tile.
+// plan (int32), one list of 16-row and one of 128-row tiles: [0] tiles in use, [1] those of rows without an adapter, which come
+// first; from word 4 (slot, rows, 1 if the rows are consecutive, 0) per tile; then the row numbers, 16 or 128 per tile.
 //
 // Three forms:
 //   decode_kernel           16-row tiles, all CTAs at once on the SMs: one launch, latency bound
@@ -21,6 +21,9 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
+
+#include <map>
+#include <mutex>
 
 #include "common.cuh"
 #include "tma_host.h"
@@ -68,9 +71,11 @@ DEVI bool load_tile(const Args& p, int i, Tile& t) {
   if (q.x >= 0) t.rank = min(max(p.rank[q.x], 0), p.R);
   return true;
 }
-// row number of row r of tile i (-1: beyond the tile, or refused)
-DEVI int row_of(const Args& p, int i, int r, int rows) {
-  const int v = p.plan[4 + 4 * (int64_t)p.max_tiles + (int64_t)i * p.tile_rows + r];
+// row number of row r of tile i (-1: beyond the tile, or refused); row_word: as stored, to be read ahead of the record
+DEVI int row_word(const Args& p, int i, int r) {
+  return p.plan[4 + 4 * (int64_t)p.max_tiles + (int64_t)i * p.tile_rows + r];
+}
+DEVI int check_row(const Args& p, int r, int rows, int v) {
   if (r >= rows) return -1;
   if (v < 0 || v >= p.T) {
     atomicExch(p.status, (int)kErrBounds);
@@ -78,6 +83,7 @@ DEVI int row_of(const Args& p, int i, int r, int rows) {
   }
   return v;
 }
+DEVI int row_of(const Args& p, int i, int r, int rows) { return check_row(p, r, rows, row_word(p, i, r)); }
 // slice of the CTA's `span` output features: -> first feature, end of the slice
 DEVI int slice_of(const Args& p, int ch, int span, int& s, int& ne) {
   s = 0;
@@ -291,14 +297,56 @@ DEVI void second_product(const float* v, int vs, int left, int rows, const uint2
   }
 }
 
-// Both products in one launch.  A cluster of 8 CTAs owns (16 rows of one adapter, up to 8 x 512 x steps features of one
+// features of a CTA's step: B of one step takes 16 registers (rank 64: 32), so that the next step's fits beside it
+template <int JG> constexpr int NBS = JG == 1 ? 2 : 1;
+template <int JG> constexpr int STEPF = 8 * 32 * NBS<JG>;
+
+// all steps of a warp's features from n0 on (STEPF apart); y and w hold the first step's
+template <int JG, bool VEC>
+DEVI void expand_steps(const Args& p, const Tile& t, const __nv_bfloat16* bt, const float* v, int vs, int n0, int ne, int steps,
+                       const __nv_bfloat16* const (&yr)[2], __nv_bfloat16* const (&to)[2], uint4 (&y)[NBS<JG>][2],
+                       uint2 (&w)[NBS<JG>][4][JG]) {
+  constexpr int NB = NBS<JG>;
+  const int q4 = threadIdx.x & 3;
+#pragma unroll 1
+  for (int st = 0; st < steps && n0 < ne; ++st, n0 += STEPF<JG>) {
+    uint4 yn[NB][2];
+    uint2 wn[NB][4][JG];
+    const bool more = st + 1 < steps;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        yn[n][h] = load_y<VEC>(more ? yr[h] : nullptr, n0 + STEPF<JG> + 32 * n + 8 * q4, ne);
+    load_b<JG, NB, VEC>(bt, p.R, n0 + STEPF<JG>, more ? ne : 0, 0, t.rank, wn);
+    float c[NB][4][4] = {};
+    second_product<JG, NB>(v, vs, t.rank, t.rows, w, c);
+#pragma unroll 1
+    for (int k0 = 16 * JG; k0 < t.rank; k0 += 16 * JG) {
+      load_b<JG, NB, VEC>(bt, p.R, n0, ne, k0, t.rank, w);
+      second_product<JG, NB>(v + k0, vs, t.rank - k0, t.rows, w, c);
+    }
+    store_step<NB, VEC>(to, yr, y, c, n0, ne, t.slot >= 0);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) y[n][h] = yn[n][h];
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int k = 0; k < JG; ++k) w[n][m][k] = wn[n][m][k];
+    }
+  }
+}
+
+// Both products in one launch.  A cluster of 8 CTAs owns (16 rows of one adapter, up to 8 x STEPF x steps features of one
 // slice): its CTAs and their warps share K, add up v through distributed shared memory in a fixed order, and each CTA
 // then expands its own features.  A's rows are read once per cluster (again from L2 where a slice takes several), B once.
 constexpr int CL = 8;
 
 template <int JG, bool FP8, bool VEC>
 __global__ void __launch_bounds__(256, 2) decode_kernel(const __grid_constant__ Args p) {
-  constexpr int NB = JG == 4 ? 1 : 2, STEP = 8 * 32 * NB;  // features of a CTA's step
+  constexpr int NB = NBS<JG>, STEP = STEPF<JG>;
   extern __shared__ float sm[];
   float* red = sm;                                         // [8 warps][16 tokens][RS]
   float* part = red + 8 * 16 * RS<JG>;                     // [16][16 JG] this CTA's share of v
@@ -312,6 +360,7 @@ __global__ void __launch_bounds__(256, 2) decode_kernel(const __grid_constant__ 
   const int kb = (cr * 8 + warp) * per, ke = min(kb + per, p.K);
   pdl_wait();
   pdl_trigger();
+  const int rw[2] = {row_word(p, i, g), row_word(p, i, 8 + g)};
   Tile t;
   if (!load_tile(p, i, t) || (t.slot < 0 && p.out == p.y)) return;         // uniform over the cluster
   const __nv_bfloat16* yr[2];
@@ -320,7 +369,7 @@ __global__ void __launch_bounds__(256, 2) decode_kernel(const __grid_constant__ 
   uint4 y[NB][2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int r = row_of(p, i, 8 * h + g, t.rows);
+    const int r = check_row(p, 8 * h + g, t.rows, rw[h]);
     x[h] = r >= 0 ? static_cast<const uint8_t*>(p.x) + r * p.x_ld * (FP8 ? 1 : 2) : nullptr;
     yr[h] = r >= 0 ? p.y + r * p.y_ld : nullptr;
     to[h] = p.out + r * p.out_ld;
@@ -357,28 +406,7 @@ __global__ void __launch_bounds__(256, 2) decode_kernel(const __grid_constant__ 
     cluster_arrive();
   }
   __syncthreads();
-#pragma unroll 1
-  for (int st = 0; st < p.steps; ++st) {
-    const int n0 = nb + STEP * st;
-    if (n0 >= ne) break;
-    uint4 yn[NB][2];
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        yn[n][h] = st + 1 < p.steps ? load_y<VEC>(yr[h], n0 + STEP + 32 * n + 8 * q4, ne) : make_uint4(0, 0, 0, 0);
-    float c[NB][4][4] = {};
-#pragma unroll 1
-    for (int k0 = 0; k0 < t.rank; k0 += 16 * JG) {
-      if (st || k0) load_b<JG, NB, VEC>(bt, p.R, n0, ne, k0, t.rank, w);
-      second_product<JG, NB>(v + k0, vs, t.rank - k0, t.rows, w, c);
-    }
-    store_step<NB, VEC>(to, yr, y, c, n0, ne, t.slot >= 0);
-#pragma unroll
-    for (int n = 0; n < NB; ++n)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) y[n][h] = yn[n][h];
-  }
+  expand_steps<JG, VEC>(p, t, bt, v, vs, nb, ne, p.steps, yr, to, y, w);
   if (t.rank > 0) cluster_wait();                          // the other CTAs have read this one's share
 }
 
@@ -392,12 +420,13 @@ __global__ void __launch_bounds__(256) shrink16_kernel(const __grid_constant__ A
   const int i = blockIdx.x, groups = (p.Rp + 16 * JG - 1) / (16 * JG);
   const int s = blockIdx.y / groups, j0 = blockIdx.y % groups * 16 * JG;
   const int warp = threadIdx.x / 32, g = (threadIdx.x & 31) >> 2;
+  const int rw[2] = {row_word(p, i, g), row_word(p, i, 8 + g)};
   Tile t;
   if (!load_tile(p, i, t) || j0 >= t.rank) return;         // uniform over the CTA
   const uint8_t* x[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int r = row_of(p, i, 8 * h + g, t.rows);
+    const int r = check_row(p, 8 * h + g, t.rows, rw[h]);
     x[h] = r >= 0 ? static_cast<const uint8_t*>(p.x) + r * p.x_ld * (FP8 ? 1 : 2) : nullptr;
   }
   const int per = ((p.K + 31) / 32 + p.splits * 8 - 1) / (p.splits * 8) * 32;
@@ -422,12 +451,13 @@ __global__ void __launch_bounds__(256) shrink16_kernel(const __grid_constant__ A
 // itself waited for whatever wrote them.
 template <int JG, bool VEC>
 __global__ void __launch_bounds__(256, 2) expand16_kernel(const __grid_constant__ Args p) {
-  constexpr int NB = JG == 4 ? 1 : 2, STEP = 8 * 32 * NB;
+  constexpr int NB = NBS<JG>;
   extern __shared__ float v[];                             // [16][Rp + 4]
   const int vs = p.Rp + 4, i = blockIdx.y;
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   int s, ne;
-  const int nb = slice_of(p, blockIdx.x, STEP, s, ne) + warp * 32 * NB;
+  const int nb = slice_of(p, blockIdx.x, STEPF<JG> * p.steps, s, ne) + warp * 32 * NB;
+  const int rw[2] = {row_word(p, i, g), row_word(p, i, 8 + g)};
   Tile t;
   if (!load_tile(p, i, t) || (t.slot < 0 && p.out == p.y)) {
     pdl_wait();
@@ -438,7 +468,7 @@ __global__ void __launch_bounds__(256, 2) expand16_kernel(const __grid_constant_
   uint4 y[NB][2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
-    const int r = row_of(p, i, 8 * h + g, t.rows);
+    const int r = check_row(p, 8 * h + g, t.rows, rw[h]);
     yr[h] = r >= 0 ? p.y + r * p.y_ld : nullptr;
     to[h] = p.out + r * p.out_ld;
 #pragma unroll
@@ -461,14 +491,7 @@ __global__ void __launch_bounds__(256, 2) expand16_kernel(const __grid_constant_
     v[m * vs + j] = sum;
   }
   __syncthreads();
-  if (nb >= ne) return;
-  float c[NB][4][4] = {};
-#pragma unroll 1
-  for (int k0 = 0; k0 < t.rank; k0 += 16 * JG) {
-    if (k0) load_b<JG, NB, VEC>(bt, p.R, nb, ne, k0, t.rank, w);
-    second_product<JG, NB>(v + k0, vs, t.rank - k0, t.rows, w, c);
-  }
-  store_step<NB, VEC>(to, yr, y, c, nb, ne, t.slot >= 0);
+  expand_steps<JG, VEC>(p, t, bt, v, vs, nb, ne, p.steps, yr, to, y, w);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -580,27 +603,33 @@ DEVI void write_v(const Args& p, int i, const Tile& t, const float* part, int ld
       const int r = row_of(p, i, m, t.rows);
       f *= r >= 0 ? p.xs[r] : 0.f;
     }
-    float q[4];
+    const float* at = part + m * ld + ss * p.R + j;
+    float q[4] = {};
+    if (p.R % 4 == 0) {                                    // (then j + 3 < R too)
+      float4 w[8];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float sum = 0.f;
-      if (j + e < t.rank) {
-        const float* at = part + m * ld + ss * p.R + j + e;
-        if (p.splits == 1) sum = *at;
-        else
-          for (int z = 0; z < p.splits; ++z) {             // in the CTAs' order
-            float w;
-            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w) : "r"(mapa_shared(smem_u32(at), z)));
-            sum += w;
-          }
-      }
-      q[e] = sum * f;
+      for (int z = 0; z < 8; ++z)                          // all CTAs' sums on their way together, added in order
+        if (z < p.splits && j < p.R)
+          w[z] = p.splits > 1 ? ld_dsmem_f4(mapa_shared(smem_u32(at), z)) : *reinterpret_cast<const float4*>(at);
+#pragma unroll
+      for (int z = 0; z < 8; ++z)
+        if (z < p.splits && j < p.R) q[0] += w[z].x, q[1] += w[z].y, q[2] += w[z].z, q[3] += w[z].w;
+    } else {
+      for (int z = 0; z < p.splits; ++z)
+        for (int e = 0; e < min(4, p.R - j); ++e) {
+          float w = at[e];
+          if (p.splits > 1)
+            asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(w) : "r"(mapa_shared(smem_u32(at + e), z)));
+          q[e] += w;
+        }
     }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) q[e] = j + e < t.rank ? q[e] * f : 0.f;
     uint2 hi, lo;
     split_v(make_float4(q[0], q[1], q[2], q[3]), true, hi.x, hi.y, lo.x, lo.y);
-    const int64_t at = (((int64_t)i * 128 + m) * p.S + sr0 / p.R + ss) * 2 * p.Rp + j;
-    *reinterpret_cast<uint2*>(v + at) = hi;
-    *reinterpret_cast<uint2*>(v + at + p.Rp) = lo;
+    __nv_bfloat16* to = v + (((int64_t)i * 128 + m) * p.S + sr0 / p.R + ss) * 2 * p.Rp + j;
+    *reinterpret_cast<uint2*>(to) = hi;
+    *reinterpret_cast<uint2*>(to + p.Rp) = lo;
   }
 }
 
@@ -645,7 +674,10 @@ __global__ void __launch_bounds__(TH) shrink128_kernel(const __grid_constant__ A
   pdl_trigger();
   Tile t;
   if (!load_tile(p, i, t) || t.rank == 0) return;          // uniform over the cluster
-  if (warp == 1) tmem_alloc(&tmem_at, cols);
+  if (warp == 1) {
+    tmem_alloc(&tmem_at, cols);
+    tmem_relinquish();                                   // until then the SM starts no other CTA that allocates
+  }
   if (tid == 0) {
     for (int q = 0; q < stages; ++q) {
       mbar_init(&full[q], 1);
@@ -732,201 +764,255 @@ __global__ void __launch_bounds__(TH) shrink128_kernel(const __grid_constant__ A
   if (warp >= 2) sums_to_smem(tmem, n > 0 && ok, nc, part, ld, warp % 4, (warp - 2) / 4);
   tc_fence_before();
   if (p.splits > 1) cluster_sync(); else __syncthreads();
-  if (warp == 1) {
-    tmem_relinquish();
-    tmem_dealloc(tmem, cols);
-  }
+  if (warp == 1) tmem_dealloc(tmem, cols);
   if (warp >= 2) write_v<FP8>(p, i, t, part, ld, sr0, nsr, tid - 64);
   if (p.splits > 1) cluster_sync();                        // nobody leaves while its sums are being read
 }
 
-// out of 128-row tiles: D[128 x 128] = V[128 x 2 r] [B; B][128 x 2 r]^T on tcgen05, feature tile by feature tile.  Warp 0 loads B
-// and y by TMA (rings of two tiles), warp 1 issues the MMAs into two TMEM buffers, eight warps add and store.  B's rows are
-// gathered in the order that gives each thread of the epilogue 8 neighbouring features of a row (the 16x256b TMEM load
-// hands out column pairs), so that out moves from registers in 16-byte vectors.
-__global__ void __launch_bounds__(TH) expand128_kernel(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap ym,
-                                                       const __grid_constant__ CUtensorMap yg, const __grid_constant__ CUtensorMap vm,
-                                                       const __grid_constant__ CUtensorMap bm, const __grid_constant__ CUtensorMap bg) {
+// out of 128-row tiles: D[128 x 64] = V[128 x 2 r] [B; B][64 x 2 r]^T on tcgen05, feature tile by feature tile.  Warp 0 loads B
+// and y by TMA (rings of two and three tiles), warp 1 issues the MMAs into two TMEM buffers, eight warps add and store; two
+// CTAs an SM, since a store warp's own chain of loads, adds and stores leaves an SM idle.  B's rows are gathered in the
+// order that gives each thread of the epilogue 8 neighbouring features of a row (the 16x256b TMEM load hands out column
+// pairs), so that out moves from registers in 16-byte vectors.  The CTAs divide the feature tiles of all row tiles evenly
+// and run them as segments of one row tile and slice each; the rings go on across segments.
+constexpr int FT = 64, YST = 4, BST = 4;
+// stages of y and B: two CTAs an SM up to rank 64 (113 KB each)
+__host__ __device__ inline int y_stages(int kc, int rb) { return kc == 1 ? (rb == 128 ? 3 : YST) : kc <= 3 ? YST : 2; }
+__host__ __device__ inline int b_stages(int kc, int rb) { return kc == 1 ? (rb == 128 ? 3 : BST) : 2; }
+
+struct Segment { int i, s, n0, ne, tiles; };               // row tile, slice, first feature, end of the slice, feature tiles
+// the segment that starts at unit u (row tile x feature tile), ending before u1
+DEVI Segment segment_at(const Args& p, int64_t u, int64_t u1, int per_row) {
+  Segment g;
+  g.i = (int)(u / per_row);
+  int f = (int)(u % per_row), n = 0;
+  for (g.s = 0;; ++g.s, f -= n) {
+    n = (p.off[g.s + 1] - p.off[g.s] + FT - 1) / FT;
+    if (f < n) break;
+  }
+  g.n0 = p.off[g.s] + FT * f;
+  g.ne = p.off[g.s + 1];
+  g.tiles = (int)min((int64_t)(n - f), u1 - u);
+  return g;
+}
+
+__global__ void __launch_bounds__(TH, 2) expand128_kernel(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap ym,
+                                                          const __grid_constant__ CUtensorMap yg, const __grid_constant__ CUtensorMap vm,
+                                                          const __grid_constant__ CUtensorMap bm, const __grid_constant__ CUtensorMap bg,
+                                                          int per_row) {
   extern __shared__ uint8_t raw[];
-  __shared__ uint64_t bfull[2], bempty[2], yfull[2], yempty[2], dfull[2], dempty[2], vfull;
+  __shared__ uint64_t bfull[BST], bempty[BST], yfull[YST], yempty[YST], dfull[BST], dempty[BST], vfull, vempty;
   __shared__ uint32_t tmem_at;
   const uint32_t base = (smem_u32(raw) + 1023) & ~1023u;
-  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31, i = blockIdx.y;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid & 31;
   const int rb = min(p.Rp, 64) <= 16 ? 32 : min(p.Rp, 64) <= 32 ? 64 : 128;    // bytes of an operand row
-  const int kc = (p.Rp + 63) / 64, ot = 128 * rb;          // operand tiles over the ranks, and their size
-  const int bst = kc <= 2 ? 2 : 1;                         // stages of B, as far as shared memory goes
-  const int yst = kc <= 3 ? 2 : 1;                         // and of y
-  const uint32_t yb = base, vb = yb + yst * 32768, bb = vb + 2 * kc * ot;
-  int s, ne;
-  const int nb = slice_of(p, blockIdx.x, 128 * p.steps, s, ne), nt = min(p.steps, (ne - nb + 127) / 128);
-  Tile t;
-  if (!load_tile(p, i, t) || (t.slot < 0 && p.out == p.y)) {
-    pdl_wait();
-    return;
+  const int kc = (p.Rp + 63) / 64, ot = 128 * rb;          // operand tiles over the ranks, and v's size of one
+  const int yst = y_stages(kc, rb), bst = b_stages(kc, rb);
+  const uint32_t yb = base, vb = yb + yst * 16384, bb = vb + 2 * kc * ot;
+  if (warp == 1) {
+    tmem_alloc(&tmem_at, BST * FT);
+    tmem_relinquish();                                   // until then the SM starts no other CTA that allocates
   }
-  if (warp == 1) tmem_alloc(&tmem_at, 256);
   if (tid == 0) {
-    for (int q = 0; q < 2; ++q) {
-      mbar_init(&bfull[q], 1); mbar_init(&bempty[q], 1);
-      mbar_init(&yfull[q], 1); mbar_init(&yempty[q], 8);
-      mbar_init(&dfull[q], 1); mbar_init(&dempty[q], 8);
+    for (int q = 0; q < YST; ++q) {
+      mbar_init(&yfull[q], 1);
+      mbar_init(&yempty[q], 8);
+    }
+    for (int q = 0; q < BST; ++q) {
+      mbar_init(&bfull[q], 1);
+      mbar_init(&bempty[q], 1);
+      mbar_init(&dfull[q], 1);
+      mbar_init(&dempty[q], 8);
     }
     mbar_init(&vfull, 1);
+    mbar_init(&vempty, 1);
     fence_mbar_init();
   }
+  // rows without an adapter come first in the plan: nothing to do for them where out is y
+  const int nt = min(p.plan[0], p.max_tiles), skip = p.out == p.y ? min(max(p.plan[1], 0), nt) : 0;
+  const int64_t units = (int64_t)(nt - skip) * per_row;
+  const int64_t u0 = (int64_t)skip * per_row + units * blockIdx.x / gridDim.x;
+  const int64_t u1 = (int64_t)skip * per_row + units * (blockIdx.x + 1) / gridDim.x;
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_at;
-  const int rk16 = (t.rank + 15) / 16;                     // MMA steps
   bool ok = true;
+  int yc = 0, bc = 0, vc = 0;                              // y tiles, B (and D) tiles, segments with an adapter so far
+  Tile t;
   if (warp == 0) {                                         // loads
-    const int ks = (rk16 + 3) / 4;
-    const TmaRows rows = tma_rows(p, i, t, lane);
-    auto load = [&](int j) {
-      const int n0 = nb + 128 * j, halves = n0 + 64 < ne ? 2 : 1;
-      ok = __all_sync(~0u, j < yst || mbar_wait(&yempty[j % yst], (j / yst - 1) & 1, p.status));
-      if (!ok) return;
-      if (lane == 0) mbar_arrive_expect_tx(&yfull[j % yst], halves * rows.n * rows.each * 128);
-      __syncwarp();
-      for (int h = 0; h < halves; ++h)
-        tma_load_rows(rows, yb + j % yst * 32768 + h * 16384, &ym, &yg, &yfull[j % yst], n0 + 64 * h, lane, 128);
-      if (t.rank == 0) return;
-      const int st = j % bst;
-      ok = __all_sync(~0u, j < bst || mbar_wait(&bempty[st], (j / bst - 1) & 1, p.status));
-      if (!ok) return;
-      if (lane == 0) mbar_arrive_expect_tx(&bfull[st], ks * ot);
-      __syncwarp();
+    bool waited = false;
+    for (int64_t u = u0; ok && u < u1;) {
+      const Segment g = segment_at(p, u, u1, per_row);
+      u += g.tiles;
+      if (!load_tile(p, g.i, t)) continue;
+      const int ks = ((t.rank + 15) / 16 + 3) / 4;
+      const TmaRows rows = tma_rows(p, g.i, t, lane);
       // 32 features in the epilogue's order: one box of a map that sees feature 8 a + 2 m + b as (b, a, m); at the end of the
-      // last adapter, where that box would leave the tensor, four rows at a time by number
+      // last adapter, where that box would leave the tensor, four rows at a time by number.  Lanes 0 .. 7 and 8 .. 15 have
+      // a block each.
       const int64_t l0 = (int64_t)t.slot * p.N;
-      const int blk = lane >> 3, f = n0 + 32 * blk;
-      const bool box = l0 + f + 32 <= (int64_t)p.L * p.N && (l0 + f) % 8 == 0;
-      const int f4 = f + (lane & 1) * 16 + (lane >> 1 & 3) * 2;              // rows 4 lane .. + 3 of the tile
-      for (int k = 0; k < ks; ++k) {
-        if (box) {
-          if (lane % 8 == 0) tma_5d(bb + st * kc * ot + k * ot + blk * 32 * rb, &bm, &bfull[st], 64 * k, (int)((l0 + f) / 8));
-        } else {
-          tma_gather4(bb + st * kc * ot + k * ot + lane * 4 * rb, &bg, &bfull[st], 64 * k,
-                      make_int4((int)(l0 + min(f4, ne - 1)), (int)(l0 + min(f4 + 1, ne - 1)), (int)(l0 + min(f4 + 8, ne - 1)),
-                                (int)(l0 + min(f4 + 9, ne - 1))));
+      const int fb = 32 * (lane >> 3), fg = fb + (lane & 1) * 16 + (lane >> 1 & 3) * 2;   // rows 4 lane .. + 3 of the tile
+      for (int j = 0; j < g.tiles; ++j, ++yc) {
+        const int n0 = g.n0 + FT * j, ys = yc % yst, st = bc % bst;
+        ok = __all_sync(~0u, yc < yst || mbar_wait(&yempty[ys], (yc / yst - 1) & 1, p.status));
+        if (!ok) break;
+        if (lane == 0) mbar_arrive_expect_tx(&yfull[ys], rows.n * rows.each * 128);
+        __syncwarp();
+        tma_load_rows(rows, yb + ys * 16384, &ym, &yg, &yfull[ys], n0, lane, 128);
+        if (t.rank == 0) continue;
+        ok = __all_sync(~0u, bc < bst || mbar_wait(&bempty[st], (bc / bst - 1) & 1, p.status));
+        if (!ok) { ++yc; break; }
+        if (lane == 0) mbar_arrive_expect_tx(&bfull[st], ks * FT * rb);
+        __syncwarp();
+        const int64_t f = l0 + n0 + fb;
+        const bool box = f + 32 <= (int64_t)p.L * p.N && f % 8 == 0;
+        for (int k = 0; k < ks && lane < 16; ++k) {
+          const uint32_t dst = bb + (st * kc + k) * FT * rb;
+          if (box) {
+            if (lane % 8 == 0) tma_5d(dst + fb * rb, &bm, &bfull[st], 64 * k, (int)(f / 8));
+          } else {
+            const int f4 = n0 + fg, last = g.ne - 1;
+            tma_gather4(dst + lane * 4 * rb, &bg, &bfull[st], 64 * k,
+                        make_int4((int)(l0 + min(f4, last)), (int)(l0 + min(f4 + 1, last)), (int)(l0 + min(f4 + 8, last)),
+                                  (int)(l0 + min(f4 + 9, last))));
+          }
         }
+        ++bc;
+        if (j > 0) continue;
+        // y and B do not depend on v: the first tile is on its way before the wait for the shrinking kernel, which itself
+        // waited for whatever wrote them
+        if (!waited) pdl_wait();
+        waited = true;
+        ok = __all_sync(~0u, vc == 0 || mbar_wait(&vempty, (vc - 1) & 1, p.status));
+        if (!ok) { ++yc; break; }
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&vfull, 2 * ks * ot);
+          for (int q = 0; q < 2 * ks; ++q)
+            tma_2d(vb + (q / ks * kc + q % ks) * ot, &vm, &vfull, (g.s * 2 + q / ks) * p.Rp + 64 * (q % ks), g.i * 128);
+        }
+        __syncwarp();
+        ++vc;
       }
-    };
-    // y and B do not depend on v: the first tiles are on their way before the wait for the shrinking kernel, which itself
-    // waited for whatever wrote them
-    int j = 0;
-    load(j++);
-    pdl_wait();
-    if (ok && t.rank > 0 && lane == 0) {
-      mbar_arrive_expect_tx(&vfull, 2 * ks * ot);
-      for (int q = 0; q < 2 * ks; ++q)
-        tma_load_2d(raw + (vb - smem_u32(raw)) + (q / ks * kc + q % ks) * ot, &vm, &vfull,
-                    (s * 2 + q / ks) * p.Rp + 64 * (q % ks), i * 128);
     }
-    __syncwarp();
-    for (; ok && j < nt; ++j) load(j);
-    for (int q = max(0, j - 2); q < j; ++q) {              // no copy stays in flight
-      if (q >= j - yst) mbar_wait(&yfull[q % yst], q / yst & 1, p.status);
-      if (t.rank > 0 && q >= j - bst) mbar_wait(&bfull[q % bst], q / bst & 1, p.status);
-    }
-    if (t.rank > 0) mbar_wait(&vfull, 0, p.status);
+    if (!waited) pdl_wait();
+    for (int q = max(0, yc - yst); q < yc; ++q) mbar_wait(&yfull[q % yst], q / yst & 1, p.status);   // no copy stays in flight
+    for (int q = max(0, bc - bst); q < bc; ++q) mbar_wait(&bfull[q % bst], q / bst & 1, p.status);
+    if (vc > 0) mbar_wait(&vfull, (vc - 1) & 1, p.status);
   } else if (warp == 1) {                                  // MMAs
     pdl_wait();                                            // a bounded wait covers no other kernel's time
-    for (int j = 0; t.rank > 0 && j < nt; ++j) {
-      const int st = j % bst;
-      ok = (j > 0 || mbar_wait(&vfull, 0, p.status)) && mbar_wait(&bfull[st], j / bst & 1, p.status) &&
-           (j < 2 || mbar_wait(&dempty[j & 1], (j / 2 - 1) & 1, p.status));
-      if (!__all_sync(~0u, ok)) { ok = false; break; }
-      const uint32_t bs = bb + st * kc * ot;
-      if (t.rank & 15) {                                   // what the slot holds beyond the adapter's rank counts as zero
-        for (int r = lane; r < 128; r += 32)
-          for (int k = t.rank; k < rk16 * 16; ++k)
-            asm volatile("st.shared.u16 [%0], %1;" ::"r"(bs + k / 64 * ot + sw_rows(r, k % 64 / 8, rb) + k % 8 * 2), "h"((uint16_t)0) : "memory");
-        fence_proxy_async();
+    for (int64_t u = u0; ok && u < u1;) {
+      const Segment g = segment_at(p, u, u1, per_row);
+      u += g.tiles;
+      if (!load_tile(p, g.i, t) || t.rank == 0) continue;
+      const int rk16 = (t.rank + 15) / 16;                 // MMA steps
+      for (int j = 0; j < g.tiles; ++j, ++bc) {
+        const int st = bc % bst, dt = bc % BST;
+        ok = (j > 0 || mbar_wait(&vfull, vc & 1, p.status)) && mbar_wait(&bfull[st], bc / bst & 1, p.status) &&
+             (bc < BST || mbar_wait(&dempty[dt], (bc / BST - 1) & 1, p.status));
+        if (!__all_sync(~0u, ok)) { ok = false; break; }
+        const uint32_t bs = bb + st * kc * FT * rb;
+        if (t.rank & 15) {                                 // what the slot holds beyond the adapter's rank counts as zero
+          for (int r = lane; r < FT; r += 32)
+            for (int k = t.rank; k < rk16 * 16; ++k)
+              asm volatile("st.shared.u16 [%0], %1;" ::"r"(bs + k / 64 * FT * rb + sw_rows(r, k % 64 / 8, rb) + k % 8 * 2),
+                           "h"((uint16_t)0) : "memory");
+          fence_proxy_async();
+          __syncwarp();
+        }
+        if (lane == 0) {
+          tc_fence_after();
+          for (int hl = 1; hl >= 0; --hl)
+            for (int kk = 0; kk < rk16; ++kk) {
+              const uint32_t o = (kk % 4) * 32;
+              mma_f16(tmem + dt * FT, sdesc_rows(vb + (hl * kc + kk / 4) * ot + o, rb), sdesc_rows(bs + kk / 4 * FT * rb + o, rb),
+                      idesc_bf16(FT), hl == 0 || kk > 0);
+            }
+          mma_commit(&bempty[st]);
+          mma_commit(&dfull[dt]);
+          if (j == g.tiles - 1) mma_commit(&vempty);
+        }
         __syncwarp();
       }
-      if (lane == 0) {
-        tc_fence_after();
-        for (int hl = 1; hl >= 0; --hl)
-          for (int kk = 0; kk < rk16; ++kk) {
-            const uint32_t o = (kk / 4) * ot + (kk % 4) * 32;
-            mma_f16(tmem + (j & 1) * 128, sdesc_rows(vb + hl * kc * ot + o, rb), sdesc_rows(bs + o, rb), idesc_bf16(128),
-                    hl == 0 || kk > 0);
-          }
-        mma_commit(&bempty[st]);
-        mma_commit(&dfull[j & 1]);
-      }
-      __syncwarp();
+      ++vc;
     }
   } else {                                                 // out = y + D
-    const int wq = warp % 4, wh = (warp - 2) / 4, g = lane >> 2, q4 = lane & 3;
-    const bool rows_here = wq * 32 < t.rows;
-    __nv_bfloat16* to[2][2];
-#pragma unroll
-    for (int rh = 0; rh < 2; ++rh)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = row_of(p, i, wq * 32 + 16 * rh + 8 * h + g, t.rows);
-        to[rh][h] = r >= 0 ? p.out + r * p.out_ld + nb + wh * 64 + 8 * q4 : nullptr;
-      }
+    const int wq = warp % 4, wh = (warp - 2) / 4, g8 = lane >> 2, q4 = lane & 3;
+    const uint32_t yat = yb + sw128(wq * 32 + g8, 4 * wh + q4);          // + 8 rows: the same swizzle
     pdl_wait();
     pdl_trigger();
-    for (int j = 0; j < nt; ++j) {
-      ok = mbar_wait(&yfull[j % yst], j / yst & 1, p.status) && (t.rank == 0 || mbar_wait(&dfull[j & 1], j / 2 & 1, p.status));
-      if (!__all_sync(~0u, ok)) { ok = false; break; }
-      tc_fence_after();
-      const int left = ne - nb - 128 * j - wh * 64 - 8 * q4;             // features from this thread's first on
-      if (rows_here) {
+    for (int64_t u = u0; ok && u < u1;) {
+      const Segment g = segment_at(p, u, u1, per_row);
+      u += g.tiles;
+      if (!load_tile(p, g.i, t)) continue;
+      const bool rows_here = wq * 32 < t.rows;
+      __nv_bfloat16* to[2][2];
 #pragma unroll
-        for (int rh = 0; rh < 2; ++rh) {
+      for (int rh = 0; rh < 2; ++rh)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = row_of(p, g.i, wq * 32 + 16 * rh + 8 * h + g8, t.rows);
+          to[rh][h] = r >= 0 ? p.out + r * p.out_ld + g.n0 + wh * 32 + 8 * q4 : nullptr;
+        }
+      for (int j = 0; j < g.tiles; ++j, ++yc) {
+        const int ys = yc % yst, st = bc % BST;
+        ok = mbar_wait(&yfull[ys], yc / yst & 1, p.status) && (t.rank == 0 || mbar_wait(&dfull[st], bc / BST & 1, p.status));
+        if (!__all_sync(~0u, ok)) { ok = false; break; }
+        tc_fence_after();
+        const int left = g.ne - g.n0 - FT * j - wh * 32 - 8 * q4;        // features from this thread's first on
+        if (rows_here) {
           uint32_t r[2][16];
           if (t.rank > 0) {
 #pragma unroll
-            for (int cb = 0; cb < 2; ++cb)
-              tmem_ld_16x256b_x4(tmem + ((uint32_t)(wq * 32 + 16 * rh) << 16) + (j & 1) * 128 + wh * 64 + 32 * cb, r[cb]);
+            for (int rh = 0; rh < 2; ++rh)
+              tmem_ld_16x256b_x4(tmem + ((uint32_t)(wq * 32 + 16 * rh) << 16) + st * FT + wh * 32, r[rh]);
+          }
+          uint4 o[2][2];
+#pragma unroll
+          for (int rh = 0; rh < 2; ++rh)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) o[rh][h] = ld_shared16(yat + ys * 16384 + (16 * rh + 8 * h) * 128);
+          if (t.rank > 0) {
             tmem_ld_wait();
+#pragma unroll
+            for (int rh = 0; rh < 2; ++rh)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                uint32_t* w = reinterpret_cast<uint32_t*>(&o[rh][h]);
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+                  w[m] = pack2(__uint_as_float(w[m] << 16) + __uint_as_float(r[rh][4 * m + 2 * h]),
+                               __uint_as_float(w[m] & 0xffff0000u) + __uint_as_float(r[rh][4 * m + 2 * h + 1]));
+              }
           }
 #pragma unroll
-          for (int cb = 0; cb < 2; ++cb)
+          for (int rh = 0; rh < 2; ++rh)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              if (to[rh][h] == nullptr || 32 * cb >= left) continue;
-              uint4 o = ld_shared16(yb + j % yst * 32768 + wh * 16384 + sw128(wq * 32 + 16 * rh + 8 * h + g, 4 * cb + q4));
-              if (t.rank > 0) {
-                uint32_t* w = reinterpret_cast<uint32_t*>(&o);
-#pragma unroll
-                for (int m = 0; m < 4; ++m) {
-                  const __nv_bfloat162 f = *reinterpret_cast<const __nv_bfloat162*>(&w[m]);
-                  w[m] = pack2(__low2float(f) + __uint_as_float(r[cb][4 * m + 2 * h]),
-                               __high2float(f) + __uint_as_float(r[cb][4 * m + 2 * h + 1]));
-                }
-              }
-              __nv_bfloat16* at = to[rh][h] + 128 * j + 32 * cb;
-              if (left - 32 * cb >= 8) *reinterpret_cast<uint4*>(at) = o;
+              if (to[rh][h] == nullptr || left <= 0) continue;
+              __nv_bfloat16* at = to[rh][h] + FT * j;
+              if (left >= 8) *reinterpret_cast<uint4*>(at) = o[rh][h];
               else {
-                const uint32_t w[4] = {o.x, o.y, o.z, o.w};
+                const uint32_t w[4] = {o[rh][h].x, o[rh][h].y, o[rh][h].z, o[rh][h].w};
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
-                  if (e < left - 32 * cb) at[e] = __ushort_as_bfloat16((uint16_t)(w[e / 2] >> 16 * (e % 2)));
+                  if (e < left) at[e] = __ushort_as_bfloat16((uint16_t)(w[e / 2] >> 16 * (e % 2)));
               }
             }
         }
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        mbar_arrive(&yempty[j % yst]);
-        if (t.rank > 0) mbar_arrive(&dempty[j & 1]);
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&yempty[ys]);
+          if (t.rank > 0) mbar_arrive(&dempty[st]);
+        }
+        if (t.rank > 0) ++bc;
       }
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 1) {
-    tmem_relinquish();
-    tmem_dealloc(tmem, 256);
-  }
+  if (warp == 1) tmem_dealloc(tmem, BST * FT);
 }
 
 // 128-row tiles whose rows TMA cannot take (an odd K, N or row stride): the same products, operands moved by ordinary loads.
@@ -944,7 +1030,10 @@ __global__ void __launch_bounds__(256) shrink128_any_kernel(const __grid_constan
   pdl_trigger();
   Tile t;
   if (!load_tile(p, i, t) || t.rank == 0) return;          // uniform over the cluster
-  if (warp == 0) tmem_alloc(&tmem_at, cols);
+  if (warp == 0) {
+    tmem_alloc(&tmem_at, cols);
+    tmem_relinquish();                                   // until then the SM starts no other CTA that allocates
+  }
   if (tid < 2) mbar_init(&bar[tid], 1);
   fence_mbar_init();
   tc_fence_before();
@@ -988,10 +1077,7 @@ __global__ void __launch_bounds__(256) shrink128_any_kernel(const __grid_constan
   sums_to_smem(tmem, n > 0 && ok, nc, part, ld, warp % 4, warp / 4);
   tc_fence_before();
   if (p.splits > 1) cluster_sync(); else __syncthreads();
-  if (warp == 0) {
-    tmem_relinquish();
-    tmem_dealloc(tmem, cols);
-  }
+  if (warp == 0) tmem_dealloc(tmem, cols);
   write_v<FP8>(p, i, t, part, ld, sr0, nsr, tid);
   if (p.splits > 1) cluster_sync();                        // nobody leaves while its sums are being read
 }
@@ -1013,7 +1099,10 @@ __global__ void __launch_bounds__(256, 2) expand128_any_kernel(const __grid_cons
     pdl_wait();
     return;
   }
-  if (warp == 0) tmem_alloc(&tmem_at, 128);
+  if (warp == 0) {
+    tmem_alloc(&tmem_at, 128);
+    tmem_relinquish();                                   // until then the SM starts no other CTA that allocates
+  }
   if (tid == 0) mbar_init(&bar, 1);
   fence_mbar_init();
   // rows of this thread: 32 (warp % 4) + 16 rh + 8 h + g; features 64 (warp / 4) + 32 cb + 8 q4 of a tile
@@ -1120,19 +1209,31 @@ __global__ void __launch_bounds__(256, 2) expand128_any_kernel(const __grid_cons
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 0) {
-    tmem_relinquish();
-    tmem_dealloc(tmem, 128);
-  }
+  if (warp == 0) tmem_dealloc(tmem, 128);
 }
 
 // ---------------------------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------------------------
+// Kernels with large stages: the size, and all of the SM's shared memory rather than what one CTA needs (without it the SM
+// runs one CTA where two fit).  Once per kernel, device and larger size.
+void allow_smem(const void* kern, size_t smem) {
+  if (smem <= 16 * 1024) return;
+  static std::mutex m;
+  static std::map<std::pair<const void*, int>, size_t> set;
+  int dev;
+  C10_CUDA_CHECK(cudaGetDevice(&dev));
+  const std::lock_guard<std::mutex> lock(m);
+  size_t& have = set[{kern, dev}];
+  if (smem <= have) return;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)std::max<size_t>(smem, 48 * 1024)));
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  have = smem;
+}
+
 template <typename... A>
 void launch(void (*kern)(A...), dim3 grid, int threads, int cx, int cz, size_t smem, cudaStream_t stream, A... args) {
-  if (smem > 48 * 1024)
-    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  allow_smem((const void*)kern, smem);
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(threads);
@@ -1164,10 +1265,12 @@ unsigned chunks(const Args& p, int span) {
 // 16-row tiles
 template <int JG>
 void launch16(Args& p, bool fp8, bool vec, const at::TensorOptions& opts, cudaStream_t st) {
-  constexpr int STEP = JG == 4 ? 256 : 512;
-  for (p.steps = 1; p.steps < 2 && (int64_t)chunks(p, CL * STEP * p.steps) * CL * p.max_tiles > 2 * 148;) p.steps *= 2;
+  constexpr int STEP = STEPF<JG>;
+  const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  // one launch while all its clusters run at once (two CTAs an SM); beyond, its chain of latencies counts once per wave
+  for (p.steps = 1; p.steps < 4 && (int64_t)chunks(p, CL * STEP * p.steps) * CL * p.max_tiles > 2 * sms;) p.steps *= 2;
   const unsigned ch = chunks(p, CL * STEP * p.steps);
-  if ((int64_t)ch * CL * p.max_tiles <= 2 * 148) {
+  if ((int64_t)ch * CL * p.max_tiles <= 2 * sms) {
     const size_t smem = (8 * 16 * RS<JG> + 256 * JG + 16 * (p.Rp + 4)) * sizeof(float);
     auto k = fp8 ? (vec ? decode_kernel<JG, true, true> : decode_kernel<JG, true, false>)
                  : (vec ? decode_kernel<JG, false, true> : decode_kernel<JG, false, false>);
@@ -1175,15 +1278,17 @@ void launch16(Args& p, bool fp8, bool vec, const at::TensorOptions& opts, cudaSt
     return;
   }
   const int groups = (p.Rp + 16 * JG - 1) / (16 * JG);
-  // shares of K of at least two 32-blocks a warp, for about four CTAs an SM
-  p.splits = std::max<int64_t>(1, std::min<int64_t>({8, 4 * 148 / ((int64_t)p.max_tiles * p.S * groups) + 1, p.K / 512}));
+  // shares of K of at least two 32-blocks a warp, as many as run at once (three CTAs an SM)
+  p.splits = std::max<int64_t>(1, std::min<int64_t>({8, 3 * sms / ((int64_t)p.max_tiles * p.S * groups), p.K / 512}));
   // v from the allocator, not a shared workspace: calls on several streams must not meet in it
   torch::Tensor ws = torch::empty({(int64_t)p.splits * p.max_tiles * 16 * p.S * p.Rp}, opts);
   p.v = ws.data_ptr<float>();
   auto k = fp8 ? (vec ? shrink16_kernel<JG, true, true> : shrink16_kernel<JG, true, false>)
                : (vec ? shrink16_kernel<JG, false, true> : shrink16_kernel<JG, false, false>);
   launch(k, dim3(p.max_tiles, p.S * groups, p.splits), 256, 1, 1, 0, st, p);
-  launch(vec ? expand16_kernel<JG, true> : expand16_kernel<JG, false>, dim3(chunks(p, STEP), p.max_tiles), 256, 1, 1,
+  // steps of a CTA: as many as leave two CTAs for every SM
+  for (p.steps = 1; p.steps < 16 && (int64_t)chunks(p, STEP * (p.steps + 1)) * p.max_tiles >= 2 * sms;) ++p.steps;
+  launch(vec ? expand16_kernel<JG, true> : expand16_kernel<JG, false>, dim3(chunks(p, STEP * p.steps), p.max_tiles), 256, 1, 1,
          16 * (p.Rp + 4) * sizeof(float), st, p);
 }
 
@@ -1212,9 +1317,6 @@ void launch128(Args& p, const CUtensorMap& am, const CUtensorMap& bm, const CUte
     launch(fp8 ? shrink128_any_kernel<true> : shrink128_any_kernel<false>, grid, 256, 1, p.splits,
            std::max((size_t)1024 + 2 * (16384 + nc16 * 128), sums), st, p, nc);
   }
-  // feature tiles of a CTA: v is staged once for all of them, as long as every SM has a few CTAs
-  for (p.steps = 1; p.steps < 16 && (int64_t)chunks(p, 128 * p.steps * 2) * p.max_tiles >= 4 * 148;) p.steps *= 2;
-  const dim3 ge(chunks(p, 128 * p.steps), p.max_tiles);
   const int kc = (p.Rp + 63) / 64, rb = p.Rp <= 16 ? 32 : p.Rp <= 32 ? 64 : 128;
   if (tma_n) {
     const auto map = [&](int box) {
@@ -1223,10 +1325,14 @@ void launch128(Args& p, const CUtensorMap& am, const CUtensorMap& bm, const CUte
     const CUtensorMap vm = make_tma_2d(p.v, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, (uint64_t)p.S * 2 * p.Rp, (uint64_t)p.max_tiles * 128,
                                        (uint64_t)p.S * 4 * p.Rp, rb / 2, 128,
                                        rb == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : rb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
-    launch(expand128_kernel, ge, TH, 1, 1, 1024 + (kc <= 3 ? 2 : 1) * 32768 + (size_t)(kc <= 2 ? 4 : 3) * kc * 128 * rb, st, p, map(16), map(1), vm,
-           bm, bg);
+    const size_t smem = 1024 + y_stages(kc, rb) * 16384 + (size_t)kc * rb * (2 * 128 + b_stages(kc, rb) * FT);
+    const int per_row = chunks(p, FT), sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+    const unsigned grid = std::min<int64_t>((int64_t)p.max_tiles * per_row, sms * (smem <= 113 * 1024 ? 2 : 1));
+    launch(expand128_kernel, dim3(grid), TH, 1, 1, smem, st, p, map(16), map(1), vm, bm, bg, per_row);
   } else {
-    launch(vec_n ? expand128_any_kernel<true> : expand128_any_kernel<false>, ge, 256, 1, 1,
+    // feature tiles of a CTA: v is staged once for all of them, as long as every SM has a few CTAs
+    for (p.steps = 1; p.steps < 16 && (int64_t)chunks(p, 128 * p.steps * 2) * p.max_tiles >= 4 * 148;) p.steps *= 2;
+    launch(vec_n ? expand128_any_kernel<true> : expand128_any_kernel<false>, dim3(chunks(p, 128 * p.steps), p.max_tiles), 256, 1, 1,
            (size_t)(kc <= 3 ? 4 : 3) * kc * 16384 + 1024, st, p);
   }
 }
@@ -1279,16 +1385,18 @@ struct LoraBank {
     }
   }
 };
+// The rows of a step: words of the 16-row list, then of the 128-row list (models/lora.AdapterPlan).
 struct LoraPlan {
   torch::Tensor buf;
-  int64_t rows, max_tiles, tile_rows, slots;
-  LoraPlan(torch::Tensor buf_, int64_t rows_, int64_t max_tiles_, int64_t tile_rows_, int64_t slots_)
-      : buf(buf_), rows(rows_), max_tiles(max_tiles_), tile_rows(tile_rows_), slots(slots_) {
-    TORCH_CHECK(buf.is_cuda() && buf.scalar_type() == at::kInt && buf.is_contiguous() && max_tiles >= 1 &&
-                    max_tiles <= 65535 && (tile_rows == 16 || tile_rows == 128) &&
-                    buf.numel() >= 4 + (4 + tile_rows) * max_tiles && (uintptr_t)buf.data_ptr() % 16 == 0,
+  int64_t rows, tiles16, tiles128, slots;
+  LoraPlan(torch::Tensor buf_, int64_t rows_, int64_t tiles16_, int64_t tiles128_, int64_t slots_)
+      : buf(buf_), rows(rows_), tiles16(tiles16_), tiles128(tiles128_), slots(slots_) {
+    TORCH_CHECK(buf.is_cuda() && buf.scalar_type() == at::kInt && buf.is_contiguous() && tiles16 >= 0 && tiles16 <= 65535 &&
+                    tiles128 >= 0 && tiles128 <= 65535 && buf.numel() >= words16() + 4 + 132 * tiles128 &&
+                    (uintptr_t)buf.data_ptr() % 16 == 0,
                 "LoraPlan: int32 words on the device, 16-byte aligned");
   }
+  int64_t words16() const { return 4 + 20 * tiles16; }
 };
 
 torch::Tensor lora_add(const torch::Tensor& y, const torch::Tensor& x, const c10::optional<torch::Tensor>& xs,
@@ -1319,21 +1427,24 @@ torch::Tensor lora_add(const torch::Tensor& y, const torch::Tensor& x, const c10
   p.x = x.data_ptr(); p.xs = fp8 ? xs->data_ptr<float>() : nullptr; p.x_ld = x.stride(0);
   p.y = (const __nv_bfloat16*)y.data_ptr(); p.y_ld = y.stride(0);
   p.out = (__nv_bfloat16*)out.data_ptr(); p.out_ld = out.stride(0);
-  p.plan = plan.buf.data_ptr<int>(); p.T = T; p.max_tiles = plan.max_tiles; p.tile_rows = plan.tile_rows;
+  p.T = T;
   auto stream = at::cuda::getCurrentCUDAStream();
-  const bool vec_k = p.K % 8 == 0 && p.x_ld % 8 == 0 && (uintptr_t)p.x % 16 == 0 && (uintptr_t)p.a % 16 == 0 &&
-                     (!fp8 || p.tile_rows == 16 || p.x_ld % 16 == 0);
+  const bool vec_k = p.K % 8 == 0 && p.x_ld % 8 == 0 && (uintptr_t)p.x % 16 == 0 && (uintptr_t)p.a % 16 == 0;
   bool vec_n = p.y_ld % 8 == 0 && p.out_ld % 8 == 0 && ((uintptr_t)p.y | (uintptr_t)p.out) % 16 == 0 &&
                (uintptr_t)p.b % 16 == 0;
   for (int s = 0; s < p.S; ++s) vec_n = vec_n && p.off[s] % 8 == 0;
   const auto opts = bank.scale.options();
-  if (p.tile_rows == 16) {
+  if (plan.tiles128) {
+    p.plan = plan.buf.data_ptr<int>() + plan.words16(); p.max_tiles = plan.tiles128; p.tile_rows = 128;
+    lora::launch128(p, bank.am, bank.bm, bank.bg, fp8, bank.tma_k && vec_k && (!fp8 || p.x_ld % 16 == 0), bank.tma_n && vec_n,
+                    vec_n, opts, stream);
+  }
+  if (plan.tiles16) {
+    p.plan = plan.buf.data_ptr<int>(); p.max_tiles = plan.tiles16; p.tile_rows = 16;
     const bool vec = vec_k && vec_n && p.R % 4 == 0;
     if (p.Rp <= 16) lora::launch16<1>(p, fp8, vec, opts, stream);
     else if (p.Rp <= 32) lora::launch16<2>(p, fp8, vec, opts, stream);
     else lora::launch16<4>(p, fp8, vec, opts, stream);
-  } else {
-    lora::launch128(p, bank.am, bank.bm, bank.bg, fp8, bank.tma_k && vec_k, bank.tma_n && vec_n, vec_n, opts, stream);
   }
   return out;
 }

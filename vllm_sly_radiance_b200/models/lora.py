@@ -45,28 +45,33 @@ class AdapterBank:
 
 
 class AdapterPlan:
-    """The rows of one step by adapter slot, in tiles of at most ``tile_rows`` rows of one adapter.  buf int32: [0] tiles
-    in use, from 4 on (slot, rows, 1 if the rows are consecutive, 0) per tile, then ``tile_rows`` row numbers per tile."""
+    """The rows of one step by adapter slot, in tiles of one adapter each: full tiles of 128 rows, what remains in one
+    more of them or, where it is short, in tiles of 16 (decode batches).  buf int32 holds the 16-row list, then the
+    128-row list: [0] tiles in use, [1] those of rows without an adapter, which come first; from 4 on (slot, rows, 1 if
+    the rows are consecutive, 0) per tile, then the row numbers, 16 or 128 per tile."""
 
-    # rows per tile: decode batches (few rows per adapter), prompts
-    TILE_DECODE, TILE_PROMPT = 16, 128
+    # rows of an adapter that are worth a 128-row tile: below, the 16-row kernels need less time
+    TALL_FROM = 49
+    # up to so many remainders go into 128-row tiles too, where there are such tiles: less time than two more launches
+    FEW = 24
 
-    def __init__(self, buf: torch.Tensor, num_rows: int, max_tiles: int, tile_rows: int, num_slots: int, slots=None):
-        self.buf, self.num_rows, self.max_tiles = buf, num_rows, max_tiles
-        self.tile_rows, self.num_slots = tile_rows, num_slots
+    def __init__(self, buf: torch.Tensor, num_rows: int, tiles16: int, tiles128: int, num_slots: int, slots=None):
+        self.buf, self.num_rows, self.tiles16, self.tiles128 = buf, num_rows, tiles16, tiles128
+        self.num_slots = num_slots
         self.slots = slots                       # host copy (CPU path)
         self.handle = None
         if buf.is_cuda:
             from ..ops._ext import ext
-            self.handle = ext().LoraPlan(buf, num_rows, max_tiles, tile_rows, num_slots)
+            self.handle = ext().LoraPlan(buf, num_rows, tiles16, tiles128, num_slots)
 
     @staticmethod
-    def words(max_tiles: int, tile_rows: int) -> int:
-        return 4 + (4 + tile_rows) * max_tiles
+    def words(tiles16: int, tiles128: int) -> int:
+        return 4 + (4 + 16) * tiles16 + 4 + (4 + 128) * tiles128
 
     @staticmethod
-    def pack(slots: np.ndarray, num_slots: int, out=None, max_tiles=None, tile_rows=None):
-        """-> (int32 words of the plan, max_tiles, tile_rows).  slots: adapter slot of each row, -1 = none."""
+    def pack(slots: np.ndarray, num_slots: int, out=None, tiles16=None, tiles128=None, tall_from=None):
+        """-> (int32 words of the plan, tiles16, tiles128).  slots: adapter slot of each row, -1 = none; tiles16 and
+        tiles128: room for so many tiles (default: as many as there are); tiles128 = 0 packs 16-row tiles only."""
         slots = np.asarray(slots)
         T = slots.shape[0]
         if slots.ndim != 1 or (T and (slots.min() < -1 or slots.max() >= num_slots)):
@@ -75,30 +80,40 @@ class AdapterPlan:
         srt = slots[order]
         starts = np.flatnonzero(np.r_[True, srt[1:] != srt[:-1]]) if T else np.zeros(0, np.int64)
         counts = np.diff(np.r_[starts, T])
-        if tile_rows is None:
-            tile_rows = AdapterPlan.TILE_PROMPT if T > 32 * max(1, len(starts)) else AdapterPlan.TILE_DECODE
-        per = (counts + tile_rows - 1) // tile_rows
-        n = int(per.sum())
-        if max_tiles is None:
-            max_tiles = max(1, n)
-        if n > max_tiles:
-            raise ValueError(f"adapter plan: {n} tiles, room for {max_tiles}")
-        grp = np.repeat(np.arange(len(starts)), per)
-        j = np.arange(n) - np.repeat(np.cumsum(per) - per, per)
-        first = starts[grp] + j * tile_rows
-        rows = np.minimum(counts[grp] - j * tile_rows, tile_rows)
-        words = np.zeros(AdapterPlan.words(max_tiles, tile_rows), np.int32) if out is None else out
-        words[:4] = (n, 0, 0, 0)
-        tiles = words[4:4 + 4 * n].reshape(n, 4)
-        tiles[:, 0], tiles[:, 1], tiles[:, 3] = srt[starts[grp]], rows, 0
-        tiles[:, 2] = order[first + rows - 1] - order[first] == rows - 1       # the order within a tile is ascending
-        at = 4 + 4 * max_tiles + np.repeat(np.arange(n) * tile_rows - first, rows) + np.arange(T)
-        words[at] = order
-        return words, max_tiles, tile_rows
+        if tall_from is None:
+            tall_from = AdapterPlan.TALL_FROM
+        full = counts // 128
+        tall = full + (counts % 128 >= tall_from) if tiles128 != 0 else 0 * counts
+        if tall.any() and np.count_nonzero(counts > tall * 128) <= AdapterPlan.FEW and tall_from < 128:
+            tall = (counts + 127) // 128
+        in_tall = np.minimum(tall * 128, counts)
+        short = (counts - in_tall + 15) // 16
+        n16, n128 = int(short.sum()), int(tall.sum())
+        tiles16 = n16 if tiles16 is None else tiles16
+        tiles128 = n128 if tiles128 is None else tiles128
+        if n16 > tiles16 or n128 > tiles128:
+            raise ValueError(f"adapter plan: {n16} and {n128} tiles, room for {tiles16} and {tiles128}")
+        words = np.zeros(AdapterPlan.words(tiles16, tiles128), np.int32) if out is None else out
+        at = 0
+        for height, per, first0, cnt, room in ((16, short, starts + in_tall, counts - in_tall, tiles16),
+                                               (128, tall, starts, in_tall, tiles128)):
+            n = int(per.sum())
+            grp = np.repeat(np.arange(len(starts)), per)
+            j = np.arange(n) - np.repeat(np.cumsum(per) - per, per)
+            first = first0[grp] + j * height
+            rows = np.minimum(cnt[grp] - j * height, height)
+            tile_slots = srt[first] if n else np.zeros(0, np.int64)
+            words[at:at + 4] = (n, np.count_nonzero(tile_slots < 0), 0, 0)
+            tiles = words[at + 4:at + 4 + 4 * n].reshape(n, 4)
+            tiles[:, 0], tiles[:, 1], tiles[:, 3] = tile_slots, rows, 0
+            tiles[:, 2] = order[first + rows - 1] - order[first] == rows - 1       # a tile's rows ascend
+            pos = np.arange(int(rows.sum())) - np.repeat(np.cumsum(rows) - rows, rows)   # of each row in its tile
+            words[at + 4 + 4 * room + np.repeat(np.arange(n) * height, rows) + pos] = order[np.repeat(first, rows) + pos]
+            at += 4 + (4 + height) * room
+        return words, tiles16, tiles128
 
     @staticmethod
     def build(slots, num_slots: int, device) -> "AdapterPlan":
         slots = slots.cpu().numpy() if isinstance(slots, torch.Tensor) else np.asarray(slots)
-        words, max_tiles, tile_rows = AdapterPlan.pack(slots, num_slots)
-        return AdapterPlan(torch.from_numpy(words).to(device), slots.shape[0], max_tiles, tile_rows, num_slots,
-                           slots=slots)
+        words, tiles16, tiles128 = AdapterPlan.pack(slots, num_slots)
+        return AdapterPlan(torch.from_numpy(words).to(device), slots.shape[0], tiles16, tiles128, num_slots, slots=slots)
