@@ -249,52 +249,68 @@ DEVI float red_sum(const float* red, int o) {
 template <int JG, int NB, bool VEC>
 DEVI void load_b(const __nv_bfloat16* bt, int R, int n0, int ne, int k0, int rank, uint2 (&w)[NB][4][JG]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
+  const int nf = n0 + 8 * (g >> 1) + (g & 1), left0 = rank - k0 - 4 * q4;
+  const __nv_bfloat16* b = bt + (int64_t)nf * R + k0 + 4 * q4;
+  if (VEC && n0 + 32 * NB <= ne && rank - k0 >= 16 * JG) {               // nothing to leave out
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int m = 0; m < 4; ++m)
+#pragma unroll
+        for (int k = 0; k < JG; ++k)
+          w[n][m][k] = *reinterpret_cast<const uint2*>(b + (uint32_t)((32 * n + 2 * m) * R) + 16 * k);
+    return;
+  }
 #pragma unroll
   for (int n = 0; n < NB; ++n)
 #pragma unroll
-    for (int m = 0; m < 4; ++m) {
-      const int nn = n0 + 32 * n + 8 * (g >> 1) + 2 * m + (g & 1);
-      const __nv_bfloat16* b = bt + (int64_t)nn * R + k0 + 4 * q4;
+    for (int m = 0; m < 4; ++m)
 #pragma unroll
       for (int k = 0; k < JG; ++k) {
-        w[n][m][k] = make_uint2(0, 0);
-        const int left = rank - (k0 + 16 * k + 4 * q4);
-        if (nn < ne && left > 0) {
+        const __nv_bfloat16* bk = b + (uint32_t)((32 * n + 2 * m) * R) + 16 * k;
+        const int left = left0 - 16 * k;
+        uint2 u = make_uint2(0, 0);
+        if (nf + 32 * n + 2 * m < ne && left > 0) {
           if (VEC) {                                       // R is a multiple of 4
-            w[n][m][k] = *reinterpret_cast<const uint2*>(b + 16 * k);
+            u = *reinterpret_cast<const uint2*>(bk);
           } else {
 #pragma unroll 1
             for (int e = 0; e < min(left, 4); ++e)
-              (e < 2 ? w[n][m][k].x : w[n][m][k].y) |= (uint32_t)__bfloat16_as_ushort(b[16 * k + e]) << 16 * (e & 1);
+              (e < 2 ? u.x : u.y) |= (uint32_t)__bfloat16_as_ushort(bk[e]) << 16 * (e & 1);
           }
         }
         if (VEC && left < 4) {
-          w[n][m][k].x &= left == 1 ? 0xffffu : ~0u;
-          w[n][m][k].y &= left == 3 ? 0xffffu : 0u;
+          u.x &= left == 1 ? 0xffffu : ~0u;
+          u.y &= left == 3 ? 0xffffu : 0u;
         }
+        w[n][m][k] = u;
       }
-    }
 }
-// the MMAs of load_b's block; v: shared memory [16][vs], from rank k0 on
-template <int JG, int NB>
-DEVI void second_product(const float* v, int vs, int left, int rows, const uint2 (&w)[NB][4][JG], float (&c)[NB][4][4]) {
+// v [16][vs] in shared memory, JG rank groups from k0 on, as the two bf16 operands of the MMA
+template <int JG>
+DEVI void load_v(const float* v, int vs, int k0, int rank, int rows, uint32_t (&vh)[JG][4], uint32_t (&vl)[JG][4]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
 #pragma unroll
-  for (int k = 0; k < JG; ++k) {
-    if (16 * k >= left) break;
-    uint32_t vh[4], vl[4];
+  for (int k = 0; k < JG; ++k)
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
-      split_v(*reinterpret_cast<const float4*>(v + (8 * h + g) * vs + 16 * k + 4 * q4), 8 * h + g < rows, vh[h], vh[h + 2],
-              vl[h], vl[h + 2]);
+    for (int h = 0; h < 2; ++h) {
+      const bool use = 8 * h + g < rows && k0 + 16 * k < rank;
+      const float4 f = use ? *reinterpret_cast<const float4*>(v + (8 * h + g) * vs + k0 + 16 * k + 4 * q4) : make_float4(0.f, 0.f, 0.f, 0.f);
+      split_v(f, use, vh[k][h], vh[k][h + 2], vl[k][h], vl[k][h + 2]);
+    }
+}
+// the MMAs of load_b's and load_v's operands
+template <int JG, int NB>
+DEVI void second_product(const uint32_t (&vh)[JG][4], const uint32_t (&vl)[JG][4], const uint2 (&w)[NB][4][JG], float (&c)[NB][4][4]) {
+#pragma unroll
+  for (int k = 0; k < JG; ++k)
 #pragma unroll
     for (int n = 0; n < NB; ++n)
 #pragma unroll
       for (int m = 0; m < 4; ++m) {
-        mma_16816(c[n][m], vl[0], vl[1], vl[2], vl[3], w[n][m][k].x, w[n][m][k].y);
-        mma_16816(c[n][m], vh[0], vh[1], vh[2], vh[3], w[n][m][k].x, w[n][m][k].y);
+        mma_16816(c[n][m], vl[k][0], vl[k][1], vl[k][2], vl[k][3], w[n][m][k].x, w[n][m][k].y);
+        mma_16816(c[n][m], vh[k][0], vh[k][1], vh[k][2], vh[k][3], w[n][m][k].x, w[n][m][k].y);
       }
-  }
 }
 
 // features of a CTA's step: B of one step takes 16 registers (rank 64: 32), so that the next step's fits beside it
@@ -308,23 +324,30 @@ DEVI void expand_steps(const Args& p, const Tile& t, const __nv_bfloat16* bt, co
                        uint2 (&w)[NBS<JG>][4][JG]) {
   constexpr int NB = NBS<JG>;
   const int q4 = threadIdx.x & 3;
+  uint32_t vh[JG][4], vl[JG][4];
+  load_v<JG>(v, vs, 0, t.rank, t.rows, vh, vl);
 #pragma unroll 1
   for (int st = 0; st < steps && n0 < ne; ++st, n0 += STEPF<JG>) {
     uint4 yn[NB][2];
     uint2 wn[NB][4][JG];
     const bool more = st + 1 < steps;
+    if (more) {
+      load_b<JG, NB, VEC>(bt, p.R, n0 + STEPF<JG>, ne, 0, t.rank, wn);
 #pragma unroll
-    for (int n = 0; n < NB; ++n)
+      for (int n = 0; n < NB; ++n)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        yn[n][h] = load_y<VEC>(more ? yr[h] : nullptr, n0 + STEPF<JG> + 32 * n + 8 * q4, ne);
-    load_b<JG, NB, VEC>(bt, p.R, n0 + STEPF<JG>, more ? ne : 0, 0, t.rank, wn);
+        for (int h = 0; h < 2; ++h) yn[n][h] = load_y<VEC>(yr[h], n0 + STEPF<JG> + 32 * n + 8 * q4, ne);
+    }
     float c[NB][4][4] = {};
-    second_product<JG, NB>(v, vs, t.rank, t.rows, w, c);
+    second_product<JG, NB>(vh, vl, w, c);
+    if (t.rank > 16 * JG) {
 #pragma unroll 1
-    for (int k0 = 16 * JG; k0 < t.rank; k0 += 16 * JG) {
-      load_b<JG, NB, VEC>(bt, p.R, n0, ne, k0, t.rank, w);
-      second_product<JG, NB>(v + k0, vs, t.rank - k0, t.rows, w, c);
+      for (int k0 = 16 * JG; k0 < t.rank; k0 += 16 * JG) {
+        uint32_t uh[JG][4], ul[JG][4];
+        load_b<JG, NB, VEC>(bt, p.R, n0, ne, k0, t.rank, w);
+        load_v<JG>(v, vs, k0, t.rank, t.rows, uh, ul);
+        second_product<JG, NB>(uh, ul, w, c);
+      }
     }
     store_step<NB, VEC>(to, yr, y, c, n0, ne, t.slot >= 0);
 #pragma unroll
