@@ -298,6 +298,10 @@ class EngineConfig:
     comm_backend: str = "fused"                 # fused (own NVLink kernels) | nccl (baseline)
     gemm_backend: str = "native"                # native (own tcgen05) | cublas (baseline fp8)
     device: str = "cuda"
+    # low-rank adapters beside the shared projections (models/lora.py)
+    max_loras: int = 0                  # adapter slots (0 = no adapters)
+    max_lora_rank: int = 16
+    lora_modules: Optional[str] = None  # loaded at start: "name=directory,name=directory"
 
     def __post_init__(self):
         for f in dataclasses.fields(self):

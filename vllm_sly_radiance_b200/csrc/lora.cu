@@ -1309,8 +1309,8 @@ void launch16(Args& p, bool fp8, bool vec, const at::TensorOptions& opts, cudaSt
   auto k = fp8 ? (vec ? shrink16_kernel<JG, true, true> : shrink16_kernel<JG, true, false>)
                : (vec ? shrink16_kernel<JG, false, true> : shrink16_kernel<JG, false, false>);
   launch(k, dim3(p.max_tiles, p.S * groups, p.splits), 256, 1, 1, 0, st, p);
-  // steps of a CTA: as many as leave two CTAs for every SM
-  for (p.steps = 1; p.steps < 16 && (int64_t)chunks(p, STEP * (p.steps + 1)) * p.max_tiles >= 2 * sms;) ++p.steps;
+  // steps of a CTA: as many as leave four CTAs for every SM
+  for (p.steps = 1; p.steps < 16 && (int64_t)chunks(p, STEP * (p.steps + 1)) * p.max_tiles >= 4 * sms;) ++p.steps;
   launch(vec ? expand16_kernel<JG, true> : expand16_kernel<JG, false>, dim3(chunks(p, STEP * p.steps), p.max_tiles), 256, 1, 1,
          16 * (p.Rp + 4) * sizeof(float), st, p);
 }

@@ -44,14 +44,15 @@ class _Items:
                               t.shape[3] * es, t.shape[2]])
             else:
                 table.append([t.data_ptr(), t.stride(0) * es, 1, nbytes, 0, 0])
-            pieces += [[i, j] for j in range((nbytes + PIECE_BYTES - 1) // PIECE_BYTES)]
+            n = (nbytes + PIECE_BYTES - 1) // PIECE_BYTES
+            pieces.append(np.stack([np.full(n, i, np.int32), np.arange(n, dtype=np.int32)], 1))
         self.handle = None
         if self.cuda:
             from ..ops._ext import ext
             from ..ops.kernels import status_word
             dev = tensors[0].device
             self.handle = ext().CacheItems(name, torch.tensor(table, dtype=torch.int64, device=dev),
-                                           torch.tensor(pieces, dtype=torch.int32, device=dev).view(-1, 2),
+                                           torch.from_numpy(np.concatenate(pieces)).to(dev),
                                            status_word(dev), self.num, self.rows)
 
     def move(self, moves):

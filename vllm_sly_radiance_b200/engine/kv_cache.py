@@ -18,6 +18,8 @@ import hashlib
 from collections import OrderedDict, deque
 from typing import Optional
 
+import numpy as np
+
 from .request import Request
 
 
@@ -149,9 +151,49 @@ class KVCacheManager:
             self.slots.release(req.state_slot)
             req.state_slot = None
 
+    # ---- forking and compacting (engine/cache_moves.CacheMover copies what these name) ----
+    def fork(self, parent: Request, child: Request):
+        """Give ``child`` the cache of ``parent``'s computed tokens: full blocks are shared, the partly filled one and
+        the state slot are new.  -> ([(src, dst, tokens)], [(src, dst)]) to copy, or None when out of blocks or slots
+        (nothing is taken then)."""
+        full, rest = divmod(parent.num_computed_tokens, self.block_size)
+        if (rest and self.blocks.num_free + len(self.lru) < 1) or self.slots.num_free < 1:
+            return None
+        child.state_slot = self.slots.alloc()
+        for b in parent.block_ids[:full]:
+            self.blocks.incref(b)
+        child.block_ids = list(parent.block_ids[:full])
+        copies = []
+        if rest:
+            child.block_ids.append(self._alloc_block())
+            copies.append((parent.block_ids[full], child.block_ids[full], rest))
+        child.num_computed_tokens = parent.num_computed_tokens
+        return copies, [(parent.state_slot, child.state_slot)]
+
+    def compact(self, requests):
+        """Renumber the blocks in use (by ``requests`` or by the prefix cache) to 1 .. n.  -> ((src, dst) arrays to
+        copy, n); every block behind n is free."""
+        from .cache_moves import plan_compaction
+        if self.offload is not None:
+            self.flush_offload()                  # evicted blocks are saved from where they are
+        used = np.array(self.blocks.ref) > 0
+        used[list(self.lru)] = True
+        src, dst, n = plan_compaction(used)
+        to = dict(zip(src.tolist(), dst.tolist()))
+        for r in requests:
+            r.block_ids = [to.get(b, b) for b in r.block_ids]
+        for s, d in to.items():
+            self.blocks.ref[d], self.blocks.ref[s] = self.blocks.ref[s], 0
+        self.cached = {h: to.get(b, b) for h, b in self.cached.items()}
+        self.block_hash = {to.get(b, b): h for b, h in self.block_hash.items()}
+        self.lru = OrderedDict((to.get(b, b), None) for b in self.lru)
+        self.blocks.free = deque(range(n + 1, self.blocks.num_blocks))
+        return (src, dst), n
+
     # ---- prefix caching ----
-    def _hashes(self, tokens: list[int]) -> list[str]:
-        out, prev = [], ""
+    def _hashes(self, tokens: list[int], salt: str = "") -> list[str]:
+        """salt: sets apart prefixes whose cache differs for the same tokens (another adapter)."""
+        out, prev = [], salt
         for i in range(0, len(tokens) - len(tokens) % self.block_size, self.block_size):
             h = hashlib.sha1((prev + ",".join(map(str, tokens[i:i + self.block_size]))).encode()).hexdigest()
             out.append(h)
@@ -167,7 +209,7 @@ class KVCacheManager:
         self.queries += 1
         if self.offload is not None:
             self.flush_offload()          # blocks evicted earlier this step become tier hits
-        hs = self._hashes(req.prompt_token_ids[:-1])
+        hs = self._hashes(req.prompt_token_ids[:-1], req.cache_salt)
         n = 0
         for h in hs:
             if h in self.cached:
@@ -234,7 +276,7 @@ class KVCacheManager:
         B = req.num_computed_tokens
         if not self.num_snapshots or not self.is_snapshot_point(req, B):
             return None
-        h = self._hashes(req.prompt_token_ids[:B])[-1]
+        h = self._hashes(req.prompt_token_ids[:B], req.cache_salt)[-1]
         if h in self.snap_by_hash:
             return None
         return self._reserve_snapshot(h)
@@ -277,7 +319,7 @@ class KVCacheManager:
         return sid
 
     def adopt_prefix(self, req: Request, num_tokens: int):
-        hs = self._hashes(req.prompt_token_ids[:num_tokens])
+        hs = self._hashes(req.prompt_token_ids[:num_tokens], req.cache_salt)
         # pin every GPU-resident block of the run first, so allocating the reloaded ones cannot
         # evict them
         got = {}
@@ -310,7 +352,7 @@ class KVCacheManager:
         if not self.enable_prefix_caching:
             return
         n_full = min(req.num_computed_tokens, req.num_prompt_tokens) // self.block_size
-        hs = self._hashes(req.prompt_token_ids[:n_full * self.block_size])
+        hs = self._hashes(req.prompt_token_ids[:n_full * self.block_size], req.cache_salt)
         for i, h in enumerate(hs):
             b = req.block_ids[i]
             if h not in self.cached and b not in self.block_hash:

@@ -12,10 +12,10 @@ class LLM:
     def __init__(self, model: str = "tiny_hybrid", tokenizer: Optional[str] = None, **kwargs):
         self.engine = LLMEngine(EngineConfig(model=model, **kwargs), tokenizer_path=tokenizer)
 
-    def generate(self, prompts: Union[str, list], sampling_params=None) -> list[RequestOutput]:
+    def generate(self, prompts: Union[str, list], sampling_params=None, adapters=None) -> list[RequestOutput]:
         if isinstance(prompts, str) or (prompts and isinstance(prompts[0], int)):
             prompts = [prompts]
-        return self.engine.generate(prompts, sampling_params)
+        return self.engine.generate(prompts, sampling_params, adapters)
 
     def chat(self, messages: list[dict], sampling_params=None, **template_kw) -> RequestOutput:
         text = self.engine.tokenizer.apply_chat_template(messages, add_generation_prompt=True,

@@ -1,7 +1,10 @@
 """LLMEngine: scheduler + KV/state cache manager + model runner (+ speculative decoding).
 
 API (vLLM-compatible subset): ``add_request``, ``abort_request``, ``step`` ->
-``list[RequestOutput]``, ``has_unfinished_requests``.  With tensor parallelism every rank runs
+``list[RequestOutput]``, ``has_unfinished_requests``; ``add_adapter`` / ``remove_adapter`` for the
+low-rank adapters that requests name, ``compact_cache``.  A request with ``SamplingParams.n`` > 1
+prefills its prompt once; before the prompt's last token its cache is forked (full pages shared,
+the partly filled page and the GDN state copied) and the samples run as requests of their own.  With tensor parallelism every rank runs
 the same engine on the same request stream (SPMD); rank 0 returns outputs.
 """
 from __future__ import annotations
@@ -10,6 +13,7 @@ import logging
 import time
 from typing import Optional, Union
 
+import numpy as np
 import torch
 
 from ..config import EngineConfig, ModelConfig
@@ -18,7 +22,7 @@ from ..ops import kernels as K
 from ..utils.metrics import EngineMetrics
 from .kv_cache import KVCacheManager
 from .model_runner import ModelRunner
-from .request import CompletionOutput, Request, RequestOutput, SamplingParams
+from .request import CompletionOutput, Request, RequestOutput, RequestStatus, SamplingParams
 from .scheduler import Scheduler
 from .tokenizer import IncrementalDetokenizer, get_tokenizer
 
@@ -100,6 +104,18 @@ class LLMEngine:
                                   max_model_len=config.max_model_len, device=self.device,
                                   enable_graphs=config.enable_cuda_graphs,
                                   graph_max_bs=config.cuda_graph_max_bs, num_spec_tokens=k)
+        from .cache_moves import CacheMover
+        self.mover = CacheMover(self.caches)
+        self.adapters = None
+        if config.max_loras:
+            from ..models.lora import ModelAdapters
+            self.adapters = model.adapters = ModelAdapters(model, config.max_loras, config.max_lora_rank)
+            self.runner.enable_adapters(config.max_loras)
+            for item in filter(None, (config.lora_modules or "").split(",")):
+                name, _, path = item.partition("=")
+                self.adapters.add(name.strip(), path.strip())
+        elif config.lora_modules:
+            raise ValueError("lora_modules needs max_loras")
         if config.capture_graphs_at_start and self.device.type == "cuda":
             t1 = time.time()
             self.runner.capture_all()
@@ -109,6 +125,9 @@ class LLMEngine:
             from ..spec_decode.proposer import build_proposer
             self.spec = build_proposer(config, self)
         self.requests: dict[str, Request] = {}
+        # n > 1: request id -> its samples' outputs; sample's own id -> (request id, index)
+        self.groups: dict[str, dict] = {}
+        self.member: dict[str, tuple] = {}
         self.detok: dict[str, IncrementalDetokenizer] = {}
         self.metrics = EngineMetrics()
         from ..utils.step_trace import StepTrace
@@ -120,17 +139,102 @@ class LLMEngine:
 
     # ------------------------------------------------------------------------------------------
     def add_request(self, prompt: Union[str, list[int]], params: Optional[SamplingParams] = None,
-                    request_id: Optional[str] = None) -> str:
+                    request_id: Optional[str] = None, adapter: Optional[str] = None) -> str:
+        """adapter: the name of a loaded adapter (add_adapter) that the request runs with."""
         params = params or SamplingParams()
         ids = self.tokenizer.encode(prompt) if isinstance(prompt, str) else list(prompt)
+        if adapter is not None and (self.adapters is None or adapter not in self.adapters.slots):
+            raise ValueError(f"adapter {adapter!r} is not loaded")
+        if params.n > 1 and self.spec is not None:
+            raise ValueError("n > 1 with speculative decoding is not supported")
         req = Request(ids, params, request_id, eos_token_id=self.eos_token_id)
+        reqs = [req]
+        for i in range(1, params.n):
+            r = Request(ids, params, f"{req.request_id}#{i}", eos_token_id=self.eos_token_id,
+                        arrival_time=req.arrival_time)
+            if params.seed is not None:
+                r.seed = params.seed + i
+            reqs.append(r)
+        for r in reqs:
+            if adapter is not None:
+                r.adapter, r.adapter_slot = adapter, self.adapters.slots[adapter]
+                r.cache_salt = self.adapters.salts[adapter]
         self.scheduler.add(req)
-        self.requests[req.request_id] = req
-        self.detok[req.request_id] = IncrementalDetokenizer(self.tokenizer, params.stop)
+        if params.n > 1:
+            rid = req.request_id
+            self.groups[rid] = dict(ids=[r.request_id for r in reqs], done=set(),
+                                    outs=[CompletionOutput(i, "", [], None) for i in range(params.n)])
+            self.member.update({r.request_id: (rid, i) for i, r in enumerate(reqs)})
+            if len(ids) == 1:                    # no cache to share
+                for r in reqs[1:]:
+                    self.scheduler.add(r)
+            else:
+                req.fork_children = reqs[1:]
+        for r in reqs:
+            self.requests[r.request_id] = r
+            self.detok[r.request_id] = IncrementalDetokenizer(self.tokenizer, params.stop)
         self.metrics.on_arrival()
         return req.request_id
 
+    # ---- adapters ----
+    def add_adapter(self, name: str, path: str):
+        """Load a low-rank adapter (PEFT directory) that requests can name."""
+        if self.adapters is None:
+            raise ValueError("the engine was started without adapter slots (max_loras)")
+        self.adapters.add(name, path)
+
+    def remove_adapter(self, name: str):
+        """Free an adapter's slot; refused while an open request uses it."""
+        if self.adapters is None:
+            raise ValueError("the engine was started without adapter slots (max_loras)")
+        if any(r.adapter == name for r in self.requests.values()):
+            raise ValueError(f"adapter {name!r} is in use")
+        self.adapters.remove(name)
+
+    # ---- cache ----
+    def compact_cache(self) -> int:
+        """Between steps: move the KV blocks in use to the front of the pool.  Returns their number;
+        every block behind them is free."""
+        if self.spec is not None and self.spec.drafter is not None:
+            raise ValueError("compacting with a drafter is not supported: its own cache follows the "
+                             "target's blocks")
+        live = {id(r): r for q in (self.scheduler.running, self.scheduler.waiting) for r in q}
+        (src, dst), n = self.kv.compact(live.values())
+        if len(src):
+            self.mover.copy(np.stack([src, dst], 1))
+        return n
+
+    def _copy_state(self, src: int, dst: int):
+        if self.mover.slots.num:
+            self.mover.copy(slots=[(src, dst)])
+
+    def _fork(self, parent: Request):
+        """The samples of a prompt start from its cache; one that finds no room waits and recomputes."""
+        children, parent.fork_children = parent.fork_children, []
+        blocks, slots = [], []
+        for c in children:
+            got = None
+            if len(self.scheduler.running) < self.scheduler.max_num_seqs:
+                got = self.kv.fork(parent, c)
+            if got is None:
+                self.scheduler.add(c)
+                continue
+            blocks += got[0]
+            slots += got[1]
+            c.status = RequestStatus.RUNNING
+            self.scheduler.running.append(c)
+        if self.kv.offload is not None:
+            self.kv.flush_offload()              # a block evicted for the copies is saved first
+        self.mover.copy(blocks, slots if self.mover.slots.num else [])
+
     def abort_request(self, request_id: str) -> bool:
+        group = self.groups.pop(request_id, None)
+        if group is not None:
+            ok = False
+            for rid in group["ids"]:
+                self.member.pop(rid, None)
+                ok = self.abort_request(rid) or ok
+            return ok
         ok = self.scheduler.abort(request_id)
         self.requests.pop(request_id, None)
         self.detok.pop(request_id, None)
@@ -151,8 +255,11 @@ class LLMEngine:
             return []
         for s in sched.seqs:         # prefix-cache hits resume from a GDN state snapshot
             if s.req.restore_snapshot is not None:
-                self.model.copy_state(self.caches, s.req.restore_snapshot, s.req.state_slot)
+                self._copy_state(s.req.restore_snapshot, s.req.state_slot)
                 self.kv.release_restore(s.req)     # the copy is on the stream: slot reusable
+        for s in sched.seqs:
+            if s.req.fork_children and s.req.num_computed_tokens == s.req.num_prompt_tokens - 1:
+                self._fork(s.req)
         try:
             if self.spec is not None:
                 result = self.spec.execute(sched)
@@ -176,10 +283,11 @@ class LLMEngine:
                 if not s.is_decode and s.req.state_slot is not None:
                     sid = self.kv.take_snapshot(s.req)
                     if sid is not None:
-                        self.model.copy_state(self.caches, s.req.state_slot, sid)
+                        self._copy_state(s.req.state_slot, sid)
         self.metrics.on_step(sched, result, time.perf_counter() - t0, self.kv.usage,
                              len(self.scheduler.running), len(self.scheduler.waiting))
         outs = []
+        progressed = {}
         fin_ids = {r.request_id for r in finished}
         for s in sched.seqs:
             req = s.req
@@ -191,22 +299,36 @@ class LLMEngine:
                 det.update(req.output_token_ids)
                 if det.stopped and not req.status.finished:
                     self.scheduler.abort(rid)
-                    from .request import RequestStatus
                     req.status = RequestStatus.FINISHED_STOPPED
                     fin_ids.add(rid)
             done = req.status.finished
             text = det.text if det else ""
-            outs.append(RequestOutput(
-                request_id=rid, prompt_token_ids=req.prompt_token_ids,
-                outputs=[CompletionOutput(0, text, list(req.output_token_ids),
-                                          req.status.value if done else None)],
-                finished=done,
-                metrics=dict(arrival=req.arrival_time, first_token=req.first_token_time,
-                             finish=req.finish_time, num_preemptions=req.num_preemptions)))
+            gid, index = self.member.get(rid, (None, 0))
+            comp = CompletionOutput(index, text, list(req.output_token_ids),
+                                    req.status.value if done else None)
+            met = dict(arrival=req.arrival_time, first_token=req.first_token_time,
+                       finish=req.finish_time, num_preemptions=req.num_preemptions)
+            if gid is None:
+                outs.append(RequestOutput(request_id=rid, prompt_token_ids=req.prompt_token_ids,
+                                          outputs=[comp], finished=done, metrics=met))
+            else:
+                self.groups[gid]["outs"][index] = comp
+                if done:
+                    self.groups[gid]["done"].add(index)
+                progressed[gid] = (req.prompt_token_ids, met)
             if done:
                 self.metrics.on_finish(req)
                 self.requests.pop(rid, None)
                 self.detok.pop(rid, None)
+        for gid, (prompt_ids, met) in progressed.items():      # n > 1: all samples in one output
+            g = self.groups[gid]
+            done = len(g["done"]) == len(g["ids"])
+            outs.append(RequestOutput(request_id=gid, prompt_token_ids=prompt_ids, outputs=list(g["outs"]),
+                                      finished=done, metrics=met))
+            if done:
+                self.groups.pop(gid)
+                for rid in g["ids"]:
+                    self.member.pop(rid, None)
         self.trace.end(tr, result.num_tokens)
         return outs
 
@@ -227,10 +349,13 @@ class LLMEngine:
             self.abort_request(rid)
         return len(ids)
 
-    def generate(self, prompts, params=None) -> list[RequestOutput]:
+    def generate(self, prompts, params=None, adapters=None) -> list[RequestOutput]:
+        """adapters: a loaded adapter's name for all prompts, or one name (or None) per prompt."""
         if isinstance(params, SamplingParams) or params is None:
             params = [params or SamplingParams()] * len(prompts)
-        order = [self.add_request(p, sp) for p, sp in zip(prompts, params)]
+        if adapters is None or isinstance(adapters, str):
+            adapters = [adapters] * len(prompts)
+        order = [self.add_request(p, sp, adapter=a) for p, sp, a in zip(prompts, params, adapters)]
         final = {}
         while self.has_unfinished_requests():
             for o in self.step():

@@ -89,6 +89,9 @@ class ModelRunner:
         self.last_timing = {}
         self._scratch: dict = {}
         self._h2d_event = None
+        # adapter plans: pinned staging and one device buffer, sized by the engine (enable_adapters)
+        self.h_lora = self.d_lora = None
+        self.lora_slots = 0
         self.last_io = (0, 0)      # (host->device, device->host) bytes copied by the last step
 
     # ------------------------------------------------------------------------------------------
@@ -125,11 +128,16 @@ class ModelRunner:
         s = min(s, max(1, (max_kv + (63 if decode else 255)) // (64 if decode else 256)))
         return s
 
-    def prepare(self, out: SchedulerOutput, pad_to: Optional[int] = None, nb_fixed: Optional[int] = None):
+    def prepare(self, out: SchedulerOutput, pad_to: Optional[int] = None, nb_fixed: Optional[int] = None,
+                adapters: Optional[bool] = None):
         """Pack host metadata for the scheduled seqs.  With pad_to, the batch is padded to a graph
         bucket of pure decode rows (1 token each).  Returns (meta, input_ids view, sample index,
-        per-seq sample counts)."""
+        per-seq sample counts).  adapters: whether the step has an adapter plan (default: when a
+        request of it has an adapter)."""
         L = self.L
+        if adapters is None:
+            adapters = any(s.req.adapter_slot >= 0 for s in out.seqs)
+        adapter_rows = []
         # the pinned staging buffers are reused: the previous asynchronous upload must have
         # finished reading them before they are overwritten
         if self._h2d_event is not None:
@@ -158,6 +166,7 @@ class ModelRunner:
                 else:
                     toks = req.all_token_ids[c0:c0 + s.num_new_tokens]
                 n = len(toks)
+                adapter_rows += [req.adapter_slot] * n
                 h[L.ids + tok_ptr:L.ids + tok_ptr + n] = toks
                 h[L.pos + tok_ptr:L.pos + tok_ptr + n] = np.arange(c0, c0 + n)
                 h[L.tseq + tok_ptr:L.tseq + tok_ptr + n] = b
@@ -187,6 +196,7 @@ class ModelRunner:
                     sample_cnt.append(0)
             else:   # padded decode row -> dummy slot / block 0
                 n = 1
+                adapter_rows.append(-1)
                 h[L.ids + tok_ptr] = 0
                 h[L.pos + tok_ptr] = 0
                 h[L.tseq + tok_ptr] = b
@@ -217,6 +227,7 @@ class ModelRunner:
         # H2D
         end = L.bt + B * nb
         self._h2d_bytes = end * 4 + T * 8
+        plan = self._adapter_plan(adapter_rows, pad_to) if adapters else None
         if self.device.type == "cuda":
             self.d_meta[:end].copy_(self.h_meta[:end], non_blocking=True)
             self.d_slots[:T].copy_(self.h_slots[:T], non_blocking=True)
@@ -226,6 +237,7 @@ class ModelRunner:
             self.d_meta[:end].copy_(self.h_meta[:end])
             self.d_slots[:T].copy_(self.h_slots[:T])
         meta = self._views(B, T, ntiles, nb)
+        meta.adapter_plan = plan
         # decode batches size the split count for the longest context, in graphs (replays keep
         # the captured count) and eagerly alike, so both paths compute identical numerics
         all_decode = all(s.is_decode for s in seqs)
@@ -234,6 +246,28 @@ class ModelRunner:
                                            else max_kv, decode=bool(decode_rows))
         ids = self.d_meta[L.ids:L.ids + T]
         return meta, ids, sample_idx, sample_cnt
+
+    def enable_adapters(self, slots: int):
+        """Room for the adapter plan of any step (models/lora.AdapterPlan) over `slots` adapters."""
+        from ..models.lora import AdapterPlan
+        self.lora_slots = slots
+        words = max(AdapterPlan.words(self.max_tokens // 16 + 9 * (slots + 1), self.max_tokens // 128 + slots + 1),
+                    AdapterPlan.words(self.max_seqs, 0))
+        self.h_lora = torch.zeros(words, dtype=torch.int32, pin_memory=self.device.type == "cuda")
+        self.d_lora = torch.zeros(words, dtype=torch.int32, device=self.device)
+
+    def _adapter_plan(self, rows: list, bucket: Optional[int]):
+        """The step's plan from the adapter slot of each row, uploaded with the step's metadata.  With bucket (a decode
+        graph) it has the fixed layout of that bucket: the graph reads whatever the next step puts there."""
+        from ..models.lora import AdapterPlan
+        slots = np.asarray(rows, dtype=np.int32)
+        room = dict(tiles16=bucket, tiles128=0) if bucket else {}
+        packed, t16, t128 = AdapterPlan.pack(slots, self.lora_slots, **room)
+        n = packed.size
+        self.h_lora.numpy()[:n] = packed
+        self.d_lora[:n].copy_(self.h_lora[:n], non_blocking=True)
+        self._h2d_bytes += 4 * n
+        return AdapterPlan(self.d_lora[:n], slots.size, t16, t128, self.lora_slots, slots=slots)
 
     # ------------------------------------------------------------------------------------------
     # execution
@@ -322,16 +356,18 @@ class ModelRunner:
     def _run_graph(self, out: SchedulerOutput, bucket: int):
         nb_fixed = self.max_blocks
         meta, ids, sample_idx, _ = self.prepare(out, pad_to=bucket, nb_fixed=nb_fixed)
+        adapters = meta.adapter_plan is not None
         reqs = [s.req for s in out.seqs]
         greedy = all(r.params.greedy for r in reqs)
         mode = "greedy" if greedy else ("full" if needs_full_vocab(reqs) else "window")
-        key = (bucket, mode)
+        key = (bucket, mode, "adapters") if adapters else (bucket, mode)
         g = self.graphs.get(key)
         if g is None:
             # warm up and capture on an all-padding batch (dummy state slot / KV block 0), so the
             # capture never advances the real sequences' GDN state; then restore the real batch
             from .scheduler import SchedulerOutput as _SO
-            dmeta, dids, _, _ = self.prepare(_SO([], 0, [], []), pad_to=bucket, nb_fixed=nb_fixed)
+            dmeta, dids, _, _ = self.prepare(_SO([], 0, [], []), pad_to=bucket, nb_fixed=nb_fixed,
+                                             adapters=adapters)
             g = self._capture(bucket, mode, dmeta, dids)
             self.graphs[key] = g
             meta, ids, sample_idx, _ = self.prepare(out, pad_to=bucket, nb_fixed=nb_fixed)

@@ -35,6 +35,8 @@ class SamplingParams:
             raise ValueError("top_p must be in (0, 1]")
         if self.max_tokens is not None and self.max_tokens < 1:
             raise ValueError("max_tokens must be >= 1")
+        if self.n < 1:
+            raise ValueError("n must be >= 1")
 
     @property
     def greedy(self) -> bool:
@@ -83,6 +85,12 @@ class Request:
         self.num_draft_tokens = 0
         self.num_accepted_tokens = 0
         self.spec_width = None
+        # adapter: slot in the model's banks (-1 = none), and what tells its cached prefixes apart
+        self.adapter: Optional[str] = None
+        self.adapter_slot = -1
+        self.cache_salt = ""
+        # samples of the same prompt that start from this request's cache (engine/llm_engine.py)
+        self.fork_children: list = []
 
     @property
     def all_token_ids(self) -> list[int]:

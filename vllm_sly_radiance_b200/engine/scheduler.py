@@ -161,9 +161,12 @@ class Scheduler:
 
     def _chunk(self, req: Request, n: int) -> int:
         """With GDN state snapshots on, a prefill chunk that would cross the request's snapshot
-        boundary ends exactly there, so the state at that boundary can be copied out."""
+        boundary ends exactly there, so the state at that boundary can be copied out.  A prompt that several samples
+        start from stops before its last token: its cache is forked there."""
         B = self.kv.snapshot_boundary(req)
         c = req.num_computed_tokens
+        if req.fork_children and c < req.num_prompt_tokens - 1 < c + n:
+            n = req.num_prompt_tokens - 1 - c
         if B > 0 and c < B < c + n:
             return B - c
         return n

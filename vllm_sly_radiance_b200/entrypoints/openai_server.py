@@ -41,11 +41,12 @@ class EngineLoop:
         self.thread = threading.Thread(target=self._loop, daemon=True)
         self.thread.start()
 
-    def submit(self, prompt, params: SamplingParams, request_id: str, loop) -> "asyncio.Queue":
+    def submit(self, prompt, params: SamplingParams, request_id: str, loop,
+               adapter: Optional[str] = None) -> "asyncio.Queue":
         q: asyncio.Queue = asyncio.Queue()
         with self.lock:
             self.outq[request_id] = (q, loop)
-        self.inbox.put(("add", prompt, params, request_id))
+        self.inbox.put(("add", prompt, params, request_id) + ((adapter,) if adapter else ()))
         return q
 
     def abort(self, request_id: str):
@@ -67,7 +68,7 @@ class EngineLoop:
             for c in cmds:
                 try:
                     if c[0] == "add":
-                        eng.add_request(c[1], c[2], c[3])
+                        eng.add_request(*c[1:])
                     elif c[0] == "abort":
                         eng.abort_request(c[1])
                         self._emit(c[1], None)
@@ -119,7 +120,8 @@ def _sampling_from_body(body: dict, default_max: int = 256) -> SamplingParams:
         presence_penalty=float(body.get("presence_penalty", 0.0)),
         frequency_penalty=float(body.get("frequency_penalty", 0.0)),
         repetition_penalty=float(body.get("repetition_penalty", 1.0)),
-        min_tokens=int(body.get("min_tokens", 0)))
+        min_tokens=int(body.get("min_tokens", 0)),
+        n=int(body.get("n") or 1))
 
 
 def build_app(engine, served_model_name: str = "model", reasoning_parser: Optional[str] = None,
@@ -131,6 +133,11 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
     loop_runner = EngineLoop(engine, broadcaster)
     names = [n.strip() for n in served_model_name.split(",") if n.strip()] or ["model"]
     app.state.engine_loop = loop_runner
+
+    def adapter_names():
+        """Loaded adapters are served as models of their own name."""
+        a = getattr(engine, "adapters", None)
+        return list(a.slots) if a is not None else []
 
     def err(msg, code=400):
         return JSONResponse({"error": {"message": msg, "type": "invalid_request_error", "code": code}},
@@ -153,14 +160,14 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
     async def models():
         return {"object": "list", "data": [{"id": n, "object": "model", "owned_by": "radiance",
                                             "max_model_len": engine.config.max_model_len}
-                                           for n in names]}
+                                           for n in names + adapter_names()]}
 
     @app.get("/metrics")
     async def metrics():
         return PlainTextResponse(engine.metrics.prometheus(names[0]))
 
-    async def _run(prompt, params, rid):
-        q = loop_runner.submit(prompt, params, rid, asyncio.get_running_loop())
+    async def _run(prompt, params, rid, adapter=None):
+        q = loop_runner.submit(prompt, params, rid, asyncio.get_running_loop(), adapter)
         while True:
             item = await q.get()
             if item is None:
@@ -172,8 +179,11 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
     @app.post("/v1/completions")
     async def completions(req: FReq):
         body = await req.json()
-        if body.get("model") and body["model"] not in names:
+        adapter = body.get("model") if body.get("model") in adapter_names() else None
+        if body.get("model") and body["model"] not in names and adapter is None:
             return err(f"model {body['model']!r} not found", 404)
+        if body.get("stream") and int(body.get("n") or 1) > 1:
+            return err("n > 1 with stream is not supported")
         prompt = body.get("prompt", "")
         if isinstance(prompt, list) and prompt and isinstance(prompt[0], str):
             prompt = prompt[0]
@@ -186,7 +196,7 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
         if body.get("stream"):
             async def gen():
                 sent = 0
-                async for o in _run(prompt, params, rid):
+                async for o in _run(prompt, params, rid, adapter):
                     if isinstance(o, dict):
                         yield f"data: {json.dumps({'error': o})}\n\n"
                         break
@@ -199,23 +209,26 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
                 yield "data: [DONE]\n\n"
             return StreamingResponse(gen(), media_type="text/event-stream")
         last = None
-        async for o in _run(prompt, params, rid):
+        async for o in _run(prompt, params, rid, adapter):
             last = o
         if last is None or isinstance(last, dict):
             return err(str(last), 500)
-        out = last.outputs[0]
         n_prompt = len(last.prompt_token_ids)
-        return {"id": rid, "object": "text_completion", "created": created, "model": names[0],
-                "choices": [{"index": 0, "text": out.text, "finish_reason": out.finish_reason,
-                             "token_ids": out.token_ids}],
-                "usage": {"prompt_tokens": n_prompt, "completion_tokens": len(out.token_ids),
-                          "total_tokens": n_prompt + len(out.token_ids)}}
+        n_out = sum(len(o.token_ids) for o in last.outputs)
+        return {"id": rid, "object": "text_completion", "created": created, "model": adapter or names[0],
+                "choices": [{"index": o.index, "text": o.text, "finish_reason": o.finish_reason,
+                             "token_ids": o.token_ids} for o in last.outputs],
+                "usage": {"prompt_tokens": n_prompt, "completion_tokens": n_out,
+                          "total_tokens": n_prompt + n_out}}
 
     @app.post("/v1/chat/completions")
     async def chat(req: FReq):
         body = await req.json()
-        if body.get("model") and body["model"] not in names:
+        adapter = body.get("model") if body.get("model") in adapter_names() else None
+        if body.get("model") and body["model"] not in names and adapter is None:
             return err(f"model {body['model']!r} not found", 404)
+        if body.get("stream") and int(body.get("n") or 1) > 1:
+            return err("n > 1 with stream is not supported")
         msgs = body.get("messages") or []
         kw = dict(body.get("chat_template_kwargs") or {})
         if body.get("tools"):
@@ -234,7 +247,7 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
             async def gen():
                 sent = 0
                 first = True
-                async for o in _run(prompt, params, rid):
+                async for o in _run(prompt, params, rid, adapter):
                     if isinstance(o, dict):
                         yield f"data: {json.dumps({'error': o})}\n\n"
                         break
@@ -263,28 +276,31 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
                 yield "data: [DONE]\n\n"
             return StreamingResponse(gen(), media_type="text/event-stream")
         last = None
-        async for o in _run(prompt, params, rid):
+        async for o in _run(prompt, params, rid, adapter):
             last = o
         if last is None or isinstance(last, dict):
             return err(str(last), 500)
-        out = last.outputs[0]
-        msg = {"role": "assistant", "content": out.text}
-        fr = out.finish_reason
-        if rp is not None:
-            reasoning, content = rp.split(out.text)
-            msg["content"] = content
-            if reasoning is not None:
-                msg["reasoning_content"] = reasoning
-        if tp is not None:
-            calls, rest = tp.parse(msg["content"] or "")
-            if calls:
-                msg["tool_calls"] = calls
-                msg["content"] = rest or None
-                fr = "tool_calls"
+        choices = []
+        for out in last.outputs:
+            msg = {"role": "assistant", "content": out.text}
+            fr = out.finish_reason
+            if rp is not None:
+                reasoning, content = rp.split(out.text)
+                msg["content"] = content
+                if reasoning is not None:
+                    msg["reasoning_content"] = reasoning
+            if tp is not None:
+                calls, rest = tp.parse(msg["content"] or "")
+                if calls:
+                    msg["tool_calls"] = calls
+                    msg["content"] = rest or None
+                    fr = "tool_calls"
+            choices.append({"index": out.index, "message": msg, "finish_reason": fr})
         n_prompt = len(last.prompt_token_ids)
-        return {"id": rid, "object": "chat.completion", "created": created, "model": names[0],
-                "choices": [{"index": 0, "message": msg, "finish_reason": fr}],
-                "usage": {"prompt_tokens": n_prompt, "completion_tokens": len(out.token_ids),
-                          "total_tokens": n_prompt + len(out.token_ids)}}
+        n_out = sum(len(o.token_ids) for o in last.outputs)
+        return {"id": rid, "object": "chat.completion", "created": created, "model": adapter or names[0],
+                "choices": choices,
+                "usage": {"prompt_tokens": n_prompt, "completion_tokens": n_out,
+                          "total_tokens": n_prompt + n_out}}
 
     return app

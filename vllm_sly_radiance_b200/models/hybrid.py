@@ -59,6 +59,7 @@ class StepMeta:
     num_splits: int = 1
     commit_len: Optional[torch.Tensor] = None   # spec-decode: tokens of each seq to commit to state
     gdn_write_out: bool = True
+    adapter_plan: Optional[object] = None       # models/lora.AdapterPlan; None: no row has an adapter
     _scratch: dict = field(default_factory=dict)
 
     def scratch_o(self, s, T, H, D):
@@ -483,9 +484,23 @@ class HybridModel:
             return self.tp.all_reduce(h)
         return h
 
+    adapters = None             # models/lora.ModelAdapters
+
     def forward(self, input_ids: torch.Tensor, meta: StepMeta, caches: ModelCaches,
                 aux_layers: Optional[list] = None, aux_out: Optional[list] = None,
                 gdn_save: Optional[list] = None) -> torch.Tensor:
+        """_forward with the step's adapters in effect."""
+        if self.adapters is None or meta.adapter_plan is None:
+            return self._forward(input_ids, meta, caches, aux_layers, aux_out, gdn_save)
+        self.adapters.step.plan = meta.adapter_plan
+        try:
+            return self._forward(input_ids, meta, caches, aux_layers, aux_out, gdn_save)
+        finally:
+            self.adapters.step.plan = None
+
+    def _forward(self, input_ids: torch.Tensor, meta: StepMeta, caches: ModelCaches,
+                 aux_layers: Optional[list] = None, aux_out: Optional[list] = None,
+                 gdn_save: Optional[list] = None) -> torch.Tensor:
         """Returns final-normed hidden states [T, H] bf16.  When `aux_layers` is given, the
         residual stream after each listed layer is appended to `aux_out` (drafter conditioning)."""
         cfg = self.cfg

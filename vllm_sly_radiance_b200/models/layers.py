@@ -107,7 +107,7 @@ class Linear:
         if isinstance(x, NormAct):
             M = x.h.shape[0]
             ok = (self.quant == "mxfp4" and x.h.is_cuda and M <= FUSE_MAX_ROWS and self.push is None
-                  and self.K <= FUSE_MAX_K)
+                  and not self._adapted() and self.K <= FUSE_MAX_K)
             if not ok:
                 q, s_, r = K.add_rms_quant(x.h, x.res, x.w, x.eps)
                 x.res_out.copy_(r)
@@ -118,7 +118,7 @@ class Linear:
             return out
         M = x.gu.shape[0]
         ok = (self.quant == "mxfp4" and x.gu.is_cuda and M <= FUSE_MAX_ROWS and self.push is None
-              and self.K <= FUSE_MAX_K)
+              and not self._adapted() and self.K <= FUSE_MAX_K)
         if not ok:
             act = K.silu_mul_quant(x.gu) if self.quant != "bf16" else K.silu_mul(x.gu)
             return self(act, out)
@@ -133,13 +133,19 @@ class Linear:
             return self.w.nbytes
         return self.w.numel() * self.w.element_size()
 
+    # adapters of this projection (models/lora.LinearAdapters) and their step's plan, when the model has any
+    lora = None
+
+    def _adapted(self) -> bool:
+        return self.lora is not None and self.lora.active
+
     # row-parallel linears of a TP>1 model get the NVLink communicator here: for decode-sized
     # batches their GEMM pushes its output tiles to every rank (fused GEMM -> all-reduce)
     push = None
 
     def can_finish(self, x) -> bool:
         """A decode-sized (e4m3, scale) input this MXFP4 linear can run with a fused finisher."""
-        return (FINISH_ON and self.quant == "mxfp4" and isinstance(x, tuple)
+        return (FINISH_ON and self.quant == "mxfp4" and isinstance(x, tuple) and not self._adapted()
                 and x[0].is_cuda and 0 < x[0].shape[0] <= K.GEMV_MAX_ROWS and self.push is None)
 
     def call_finish(self, x, mode: int, res=None, norm_w=None, eps: float = 0.0):
@@ -169,6 +175,12 @@ class Linear:
     def __call__(self, x: Act, out: Optional[torch.Tensor] = None) -> torch.Tensor:
         if isinstance(x, (NormAct, SiluAct)):
             return self._fused(x, out)
+        if self._adapted():
+            return self.lora.add(self._shared(x, out), x)
+        return self._shared(x, out)
+
+    def _shared(self, x: Act, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The projection that every row shares, without adapters."""
         if self.quant == "mxfp4":
             if isinstance(x, tuple):
                 q, s = x

@@ -1,8 +1,14 @@
 """Low-rank adapters beside the shared projections.
 
 ``AdapterBank`` stacks the adapters of one projection in fixed slots; ``AdapterPlan`` groups the rows of one step by
-adapter slot, once for all projections.  ``ops.kernels.lora_add`` adds the deltas to a projection's output."""
+adapter slot, once for all projections.  ``ops.kernels.lora_add`` adds the deltas to a projection's output.
+``ModelAdapters`` keeps the banks of a ``HybridModel`` and loads adapters in the PEFT layout (``adapter_config.json``,
+``adapter_model.safetensors``)."""
 from __future__ import annotations
+
+import json
+import os
+import re
 
 import numpy as np
 import torch
@@ -117,3 +123,148 @@ class AdapterPlan:
         slots = slots.cpu().numpy() if isinstance(slots, torch.Tensor) else np.asarray(slots)
         words, tiles16, tiles128 = AdapterPlan.pack(slots, num_slots)
         return AdapterPlan(torch.from_numpy(words).to(device), slots.shape[0], tiles16, tiles128, num_slots, slots=slots)
+
+
+class _Step:
+    """The plan of the forward in progress, shared by all adapted linears (None: no row has an adapter)."""
+    plan = None
+
+
+class LinearAdapters:
+    """The adapters of one ``Linear``: its bank and the model's current step."""
+
+    def __init__(self, bank: AdapterBank, step: _Step):
+        self.bank, self.step = bank, step
+
+    @property
+    def active(self) -> bool:
+        return self.step.plan is not None
+
+    def add(self, y, x):
+        from ..ops import kernels as K
+        return K.lora_add(y, x, self.bank, self.step.plan, out=y)
+
+
+# checkpoint module -> (linear of a layer, slice of its merged output)
+_MODULES = {
+    "self_attn.q_proj": ("qkv", 0), "self_attn.k_proj": ("qkv", 1), "self_attn.v_proj": ("qkv", 2),
+    "self_attn.o_proj": ("o_proj", 0), "linear_attn.in_proj_qkvz": ("in_proj", 0),
+    "linear_attn.in_proj_ba": ("in_proj", 1), "linear_attn.out_proj": ("out_proj", 0),
+    "mlp.gate_proj": ("gate_up", 0), "mlp.up_proj": ("gate_up", 1), "mlp.down_proj": ("down", 0),
+}
+
+
+class ModelAdapters:
+    """Banks for every projection of a model's layers (the mixers' and the dense MLP's), ``max_loras`` slots of up to
+    ``max_rank`` each.  Tensor parallelism and expert weights are not covered."""
+
+    def __init__(self, model, max_loras: int, max_rank: int):
+        if model.tp.size > 1:
+            raise ValueError("adapters with tensor parallelism are not supported")
+        if max_loras < 1 or not 1 <= max_rank <= MAX_RANK:
+            raise ValueError(f"adapters: at least one slot and a rank of 1 .. {MAX_RANK}")
+        self.model, self.max_loras, self.max_rank = model, max_loras, (max_rank + 7) // 8 * 8
+        self.step = _Step()
+        self.slots: dict = {}                    # name -> slot
+        self.salts: dict = {}                    # name -> what its cached prefixes are told apart by
+        self._loads = 0
+        cfg, dev = model.cfg, model.device
+        self.banks: list = []                    # per layer: linear name -> bank
+        for layer in model.layers:
+            lins = {}
+            m = layer.mixer
+            if layer.is_attn:
+                q = m.Hq * m.hd * (2 if m.gated else 1)
+                lins["qkv"] = (m.qkv, [0, q, q + m.Hkv * m.hd, q + 2 * m.Hkv * m.hd])
+                lins["o_proj"] = (m.o_proj, [0, m.o_proj.N])
+            else:
+                lins["in_proj"] = (m.in_proj, [0, m.conv_dim + m.value_dim, m.in_proj.N])
+                lins["out_proj"] = (m.out_proj, [0, m.out_proj.N])
+            if hasattr(layer.mlp, "gate_up"):
+                lins["gate_up"] = (layer.mlp.gate_up, [0, layer.mlp.gate_up.N // 2, layer.mlp.gate_up.N])
+                lins["down"] = (layer.mlp.down, [0, layer.mlp.down.N])
+            banks = {}
+            for name, (lin, sl) in lins.items():
+                S, R = len(sl) - 1, self.max_rank
+                banks[name] = AdapterBank(
+                    torch.zeros(max_loras, S, R, lin.K, dtype=torch.bfloat16, device=dev),
+                    torch.zeros(max_loras, lin.N, R, dtype=torch.bfloat16, device=dev),
+                    torch.zeros(max_loras, device=dev), torch.zeros(max_loras, dtype=torch.int32, device=dev), sl)
+                lin.lora = LinearAdapters(banks[name], self.step)
+            self.banks.append(banks)
+        self._perm = None
+        if any(not layer.is_attn for layer in model.layers):
+            from ..quant.loaders import gdn_in_proj_permutation
+            self._perm = gdn_in_proj_permutation(cfg)
+
+    @property
+    def nbytes(self) -> int:
+        return sum(2 * (b.a.numel() + b.b.numel()) for banks in self.banks for b in banks.values())
+
+    def add(self, name: str, path: str) -> int:
+        """Load the PEFT adapter in directory ``path`` under ``name``; returns its slot."""
+        from safetensors import safe_open
+        with open(os.path.join(path, "adapter_config.json")) as f:
+            cfg = json.load(f)
+        if cfg.get("use_dora") or cfg.get("bias", "none") != "none" or cfg.get("modules_to_save"):
+            raise ValueError(f"adapter {name!r}: only plain low-rank matrices are supported")
+        rank = int(cfg["r"])
+        alpha = float(cfg.get("lora_alpha", rank))
+        scale = alpha / rank ** 0.5 if cfg.get("use_rslora") else alpha / rank
+        with safe_open(os.path.join(path, "adapter_model.safetensors"), framework="pt", device="cpu") as f:
+            return self.add_tensors(name, {k: f.get_tensor(k) for k in f.keys()}, rank, scale)
+
+    def add_tensors(self, name: str, tensors: dict, rank: int, scale: float) -> int:
+        """tensors: ``...layers.<i>.<module>.lora_A.weight`` [rank, in] and ``lora_B.weight`` [out, rank]."""
+        if name in self.slots:
+            raise ValueError(f"adapter {name!r} is loaded already")
+        if not 1 <= rank <= self.max_rank:
+            raise ValueError(f"adapter {name!r}: rank {rank}, room for {self.max_rank}")
+        free = sorted(set(range(self.max_loras)) - set(self.slots.values()))
+        if not free:
+            raise ValueError(f"adapter {name!r}: all {self.max_loras} slots are taken")
+        slot = free[0]
+        parts: dict = {}
+        for key, t in tensors.items():
+            m = re.search(r"layers\.(\d+)\.(.+)\.lora_([AB])(?:\.default)?\.weight$", key)
+            if m is None or m.group(2) not in _MODULES or int(m.group(1)) >= len(self.banks) or \
+                    _MODULES[m.group(2)][0] not in self.banks[int(m.group(1))]:
+                raise ValueError(f"adapter {name!r}: no projection for {key}")
+            parts.setdefault((int(m.group(1)), m.group(2)), {})[m.group(3)] = t
+        for (i, module), p in parts.items():     # everything is checked before a slot is written
+            lin, s = _MODULES[module]
+            bank = self.banks[i][lin]
+            n = self._rows(module, bank, s)
+            if set(p) != {"A", "B"} or tuple(p["A"].shape) != (rank, bank.K) or tuple(p["B"].shape) != (n, rank):
+                raise ValueError(f"adapter {name!r}: layer {i} {module} does not fit [{rank}, {bank.K}] and [{n}, {rank}]")
+        for banks in self.banks:
+            for b in banks.values():
+                b.a[slot].zero_()
+                b.b[slot].zero_()
+                b.scale[slot] = scale
+                b.ranks[slot] = 0
+        for (i, module), p in parts.items():
+            lin, s = _MODULES[module]
+            bank = self.banks[i][lin]
+            w = p["B"]
+            if self._perm is not None and module.startswith("linear_attn.in_proj"):
+                w = w[self._perm[s]]             # the checkpoint groups these rows per key head
+            n0 = bank.slices[s]
+            bank.a[slot, s, :rank] = p["A"].to(bank.a)
+            bank.b[slot, n0:n0 + w.shape[0], :rank] = w.to(bank.b)
+            bank.ranks[slot] = rank
+        self._loads += 1
+        self.slots[name] = slot
+        self.salts[name] = f"{name}#{self._loads}"
+        return slot
+
+    def _rows(self, module: str, bank: AdapterBank, s: int) -> int:
+        if module == "linear_attn.in_proj_ba":   # the merged projection is padded to a multiple of 8
+            return len(self._perm[1])
+        return bank.slices[s + 1] - bank.slices[s]
+
+    def remove(self, name: str):
+        if name not in self.slots:
+            raise ValueError(f"adapter {name!r} is not loaded")
+        self.slots.pop(name)
+        self.salts.pop(name)
