@@ -10,10 +10,17 @@
 // plan (int32), one list of 16-row and one of 128-row tiles: [0] tiles in use, [1] those of rows without an adapter, which come
 // first; from word 4 (slot, rows, 1 if the rows are consecutive, 0) per tile; then the row numbers, 16 or 128 per tile.
 //
-// Three forms:
-//   decode_kernel           16-row tiles, all CTAs at once on the SMs: one launch, latency bound
-//   shrink16 + expand16     more 16-row tiles: two launches that overlap, bound by the adapters' bytes
-//   shrink128 + expand128   128-row tiles: tcgen05, bound by x, y and out
+// Three forms (times: 5120 -> 17408 features in two slices, B200):
+//   decode_kernel           16-row tiles whose clusters all run at once: one launch.  Bound by its chain of latencies (plan,
+//                           x and A, cluster, B): 6.2 us for one row of rank 16, 8.5 us for 8 rows of 8 adapters, where the
+//                           two launches below took 10.9 and 11.4 us.
+//   shrink16 + expand16     more 16-row tiles: two launches that overlap.  Bound by the same chain and, beyond some
+//                           30 adapters, by instructions: 25 us for 64 rows of 24 adapters up to rank 32 (one launch in
+//                           two waves: 43 us).
+//   shrink128 + expand128   128-row tiles: tcgen05.  Bound by memory: 8192 rows, rank 64, shrink 30 us (x at 4.7 TB/s), expand
+//                           115 us (y and out at 5.0 TB/s; a plain copy of tiles 64 features wide reaches 5.3 TB/s at best,
+//                           since its 128-byte rows open a DRAM page each, against 6.4 TB/s in address order).
+//                           On mma.sync the same products took 307 and 787 us.
 //
 // Rounding: products of bf16 (or e4m3) numbers are exact in the MMA and summed in 32 bits.  v enters the second product
 // as the sum of two bf16 numbers, so that its error is 2^-16 and not 2^-8: the second half doubles MMAs that wait on
@@ -313,7 +320,8 @@ DEVI void second_product(const uint32_t (&vh)[JG][4], const uint32_t (&vl)[JG][4
       }
 }
 
-// features of a CTA's step: B of one step takes 16 registers (rank 64: 32), so that the next step's fits beside it
+// features of a CTA's step: B of one step takes 16 registers, so that the next step's fits beside it (64 ranks at once spilled
+// and took 31 us where 32 at a time take 26: 8 tiles of rank 64)
 template <int JG> constexpr int NBS = JG == 1 ? 2 : 1;
 template <int JG> constexpr int STEPF = 8 * 32 * NBS<JG>;
 
@@ -1290,7 +1298,8 @@ template <int JG>
 void launch16(Args& p, bool fp8, bool vec, const at::TensorOptions& opts, cudaStream_t st) {
   constexpr int STEP = STEPF<JG>;
   const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  // one launch while all its clusters run at once (two CTAs an SM); beyond, its chain of latencies counts once per wave
+  // one launch while all its clusters run at once (two CTAs an SM); beyond, its chain of latencies counts once per wave:
+  // 64 rows of 24 adapters took 43 us so, and 20 to 25 us in two launches
   for (p.steps = 1; p.steps < 4 && (int64_t)chunks(p, CL * STEP * p.steps) * CL * p.max_tiles > 2 * sms;) p.steps *= 2;
   const unsigned ch = chunks(p, CL * STEP * p.steps);
   if ((int64_t)ch * CL * p.max_tiles <= 2 * sms) {
@@ -1466,8 +1475,7 @@ torch::Tensor lora_add(const torch::Tensor& y, const torch::Tensor& x, const c10
     p.plan = plan.buf.data_ptr<int>(); p.max_tiles = plan.tiles16; p.tile_rows = 16;
     const bool vec = vec_k && vec_n && p.R % 4 == 0;
     if (p.Rp <= 16) lora::launch16<1>(p, fp8, vec, opts, stream);
-    else if (p.Rp <= 32) lora::launch16<2>(p, fp8, vec, opts, stream);
-    else lora::launch16<4>(p, fp8, vec, opts, stream);
+    else lora::launch16<2>(p, fp8, vec, opts, stream);
   }
   return out;
 }

@@ -56,9 +56,12 @@ class AdapterPlan:
     128-row list: [0] tiles in use, [1] those of rows without an adapter, which come first; from 4 on (slot, rows, 1 if
     the rows are consecutive, 0) per tile, then the row numbers, 16 or 128 per tile."""
 
-    # rows of an adapter that are worth a 128-row tile: below, the 16-row kernels need less time
+    # Rows of an adapter that are worth a 128-row tile.  B200, 5120 -> 17408 features, 16-row against 128-row tiles: 48 rows
+    # of one adapter 7.6 / 15.6 us at rank 16 and 17.0 / 16.0 at rank 64; 48 rows each of 8 adapters 15.9 / 24.4 and
+    # 37.8 / 27.0; 64 rows each 20.1 / 24.9 and 49.9 / 27.9.
     TALL_FROM = 49
-    # up to so many remainders go into 128-row tiles too, where there are such tiles: less time than two more launches
+    # Where there are 128-row tiles, up to so many remainders go into such tiles too, rather than two more launches: beside
+    # 2048 rows, 16 remainders of 3 rows 58 / 63 us at rank 16 and 65 / 83 at rank 64, 24 of them 68 / 61 and 78 / 92.
     FEW = 24
 
     def __init__(self, buf: torch.Tensor, num_rows: int, tiles16: int, tiles128: int, num_slots: int, slots=None):
