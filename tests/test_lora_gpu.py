@@ -236,3 +236,31 @@ def test_lora_refusals():
             K.lora_add(args[0], args[1], bank, args[2], out=args[3] if len(args) > 3 else None)
     assert K.lora_add(y[:0], x[:0], bank, AdapterPlan.build([], 3, DEV)).shape == (0, 24)
     K.check_status(y.device)
+
+
+@pytest.mark.parametrize("tile_rows", [16, 128])
+@pytest.mark.parametrize("T", [1, 40])
+def test_lora_broadcast_and_unaligned_views(tile_rows, T):
+    """A broadcast x and y (row stride 0), and operands that start off any vector boundary."""
+    case = make(T, 128, [48, 16], 16, 2, False, seed=T)
+    y, x, a, b, sc, rk, sl = case
+    slots = np.arange(T) % 2
+    bank = AdapterBank(a.to(DEV), b.to(DEV), sc.to(DEV), rk.to(DEV), sl)
+    w, t16, t128 = AdapterPlan.pack(slots, 2, tall_from=1 if tile_rows == 128 else None, tiles128=0 if tile_rows == 16 else None)
+    plan = AdapterPlan(torch.from_numpy(w).to(DEV), T, t16, t128, 2)
+
+    def same(yd, xd, out=None):
+        want, tol = formula(yd.cpu(), xd.cpu(), a, b, sc, rk, sl, slots)
+        got = K.lora_add(yd, xd, bank, plan, out=out)
+        torch.cuda.synchronize()
+        K.check_status(got.device)
+        assert not (~((got.cpu().double() - want).abs() <= tol)).any()
+    same(y[:1].to(DEV).expand(T, 64), x.to(DEV))
+    same(y.to(DEV), x[:1].to(DEV).expand(T, 128))
+    same(y[:1].to(DEV).expand(T, 64), x[:1].to(DEV).expand(T, 128))
+
+    def shifted(t, off):
+        v = torch.empty(t.numel() + off, dtype=t.dtype, device=DEV)[off:].view(t.shape)
+        return v.copy_(t)
+    for off in (1, 4):
+        same(shifted(y, off), shifted(x, off), out=shifted(torch.zeros_like(y), 3 * off))

@@ -1456,9 +1456,11 @@ torch::Tensor lora_add(const torch::Tensor& y, const torch::Tensor& x, const c10
   const bool same = out.data_ptr() == y.data_ptr() && out.stride(0) == y.stride(0);
   if (out_.has_value() && ((!same && lora::overlap(out, y)) || lora::overlap(out, x) || (T > 1 && out.stride(0) < p.N)))
     refuse("out overlaps y or x other than being y");
-  p.x = x.data_ptr(); p.xs = fp8 ? xs->data_ptr<float>() : nullptr; p.x_ld = x.stride(0);
-  p.y = (const __nv_bfloat16*)y.data_ptr(); p.y_ld = y.stride(0);
-  p.out = (__nv_bfloat16*)out.data_ptr(); p.out_ld = out.stride(0);
+  // one row's stride says nothing: any that fits the widest loads
+  const auto ld = [T](const torch::Tensor& t) { return T == 1 ? (t.size(1) + 15) / 16 * 16 : t.stride(0); };
+  p.x = x.data_ptr(); p.xs = fp8 ? xs->data_ptr<float>() : nullptr; p.x_ld = ld(x);
+  p.y = (const __nv_bfloat16*)y.data_ptr(); p.y_ld = ld(y);
+  p.out = (__nv_bfloat16*)out.data_ptr(); p.out_ld = ld(out);
   p.T = T;
   auto stream = at::cuda::getCurrentCUDAStream();
   const bool vec_k = p.K % 8 == 0 && p.x_ld % 8 == 0 && (uintptr_t)p.x % 16 == 0 && (uintptr_t)p.a % 16 == 0;
@@ -1468,8 +1470,9 @@ torch::Tensor lora_add(const torch::Tensor& y, const torch::Tensor& x, const c10
   const auto opts = bank.scale.options();
   if (plan.tiles128) {
     p.plan = plan.buf.data_ptr<int>() + plan.words16(); p.max_tiles = plan.tiles128; p.tile_rows = 128;
-    lora::launch128(p, bank.am, bank.bm, bank.bg, fp8, bank.tma_k && vec_k && (!fp8 || p.x_ld % 16 == 0), bank.tma_n && vec_n,
-                    vec_n, opts, stream);
+    // TMA takes no rows on top of one another (a broadcast x or y)
+    lora::launch128(p, bank.am, bank.bm, bank.bg, fp8, bank.tma_k && vec_k && p.x_ld >= p.K && (!fp8 || p.x_ld % 16 == 0),
+                    bank.tma_n && vec_n && p.y_ld >= p.N, vec_n, opts, stream);
   }
   if (plan.tiles16) {
     p.plan = plan.buf.data_ptr<int>(); p.max_tiles = plan.tiles16; p.tile_rows = 16;

@@ -54,6 +54,16 @@ class LLMEngine:
         self.load_time = time.time() - t0
         self.tokenizer = tokenizer or get_tokenizer(tokenizer_path, mcfg.vocab_size)
         self.eos_token_id = getattr(self.tokenizer, "eos_token_id", None)
+        # ---- adapters (before the caches are sized by what memory is left) ----
+        self.adapters = None
+        if config.max_loras:
+            from ..models.lora import ModelAdapters
+            self.adapters = model.adapters = ModelAdapters(model, config.max_loras, config.max_lora_rank)
+            for item in filter(None, (config.lora_modules or "").split(",")):
+                name, _, path = item.partition("=")
+                self.adapters.add(name.strip(), path.strip())
+        elif config.lora_modules:
+            raise ValueError("lora_modules needs max_loras")
         # ---- cache sizing ----
         bs = config.block_size
         num_slots = config.max_num_seqs + 2
@@ -106,16 +116,8 @@ class LLMEngine:
                                   graph_max_bs=config.cuda_graph_max_bs, num_spec_tokens=k)
         from .cache_moves import CacheMover
         self.mover = CacheMover(self.caches)
-        self.adapters = None
-        if config.max_loras:
-            from ..models.lora import ModelAdapters
-            self.adapters = model.adapters = ModelAdapters(model, config.max_loras, config.max_lora_rank)
+        if self.adapters is not None:
             self.runner.enable_adapters(config.max_loras)
-            for item in filter(None, (config.lora_modules or "").split(",")):
-                name, _, path = item.partition("=")
-                self.adapters.add(name.strip(), path.strip())
-        elif config.lora_modules:
-            raise ValueError("lora_modules needs max_loras")
         if config.capture_graphs_at_start and self.device.type == "cuda":
             t1 = time.time()
             self.runner.capture_all()
