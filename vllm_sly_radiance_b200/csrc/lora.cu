@@ -212,7 +212,7 @@ DEVI void first_product(const Args& p, const __nv_bfloat16* a, const uint8_t* co
                         int ke, float* red) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   float c[JG][2][4] = {};
-#pragma unroll 2
+#pragma unroll (JG == 1 ? 4 : 2)
   for (int k = kb; k < ke; k += 32) {
     const uint4 z = make_uint4(0, 0, 0, 0);
     uint4 xa[2], aa[JG][2];
