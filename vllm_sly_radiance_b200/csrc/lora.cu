@@ -702,7 +702,6 @@ __global__ void __launch_bounds__(TH) shrink128_kernel(const __grid_constant__ A
   const uint32_t ring = base + (FP8 ? 2 * 16384 : 0), sbytes = abytes + xbytes;      // A first: 1024-byte aligned
   const uint32_t cols = tmem_cols(nc);
   pdl_wait();
-  pdl_trigger();
   Tile t;
   if (!load_tile(p, i, t) || t.rank == 0) return;          // uniform over the cluster
   if (warp == 1) {
@@ -725,6 +724,9 @@ __global__ void __launch_bounds__(TH) shrink128_kernel(const __grid_constant__ A
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_at;
+  // Only now may the expanding kernel start: its CTAs allocate TMEM at once and keep it until this kernel has finished, so
+  // that a CTA here that had yet to allocate could wait for one that waits for it.
+  pdl_trigger();
   const int nk = (p.K + 63) / 64, per = (nk + p.splits - 1) / p.splits;
   const int k0 = blockIdx.z * per, n = max(0, min(per, nk - k0));
   bool ok = true;
@@ -1058,7 +1060,6 @@ __global__ void __launch_bounds__(256) shrink128_any_kernel(const __grid_constan
   const int sr0 = blockIdx.y * nc_max, nsr = min(nc_max, p.S * p.R - sr0), nc = (nsr + 15) / 16 * 16;
   const uint32_t sbytes = 16384 + (uint32_t)((nc_max + 15) / 16) * 2048, cols = tmem_cols(nc);
   pdl_wait();
-  pdl_trigger();
   Tile t;
   if (!load_tile(p, i, t) || t.rank == 0) return;          // uniform over the cluster
   if (warp == 0) {
@@ -1071,6 +1072,7 @@ __global__ void __launch_bounds__(256) shrink128_any_kernel(const __grid_constan
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_at;
+  pdl_trigger();                                           // as in shrink128_kernel
   const int nk = (p.K + 63) / 64, per = (nk + p.splits - 1) / p.splits;
   const int k0 = blockIdx.z * per, n = max(0, min(per, nk - k0));
   const uint8_t* x[4];
@@ -1163,7 +1165,6 @@ __global__ void __launch_bounds__(256, 2) expand128_any_kernel(const __grid_cons
   };
   if (t.rank > 0) load_b(0);
   pdl_wait();
-  pdl_trigger();
   if (t.rank > 0) {
     const __nv_bfloat16* v = reinterpret_cast<const __nv_bfloat16*>(p.v);
     for (int o = tid; o < t.rows * 2 * chunks; o += 256) {
@@ -1176,6 +1177,7 @@ __global__ void __launch_bounds__(256, 2) expand128_any_kernel(const __grid_cons
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_at;
+  pdl_trigger();                                           // TMEM first: the next kernel's CTAs may allocate before they wait
   bool ok = true;
   for (int j = 0; j < nt; ++j) {
     const int n0 = nb + 128 * j;
