@@ -192,8 +192,9 @@ class KVCacheManager:
 
     # ---- prefix caching ----
     def _hashes(self, tokens: list[int], salt: str = "") -> list[str]:
-        """salt: sets apart prefixes whose cache differs for the same tokens (another adapter)."""
-        out, prev = [], salt
+        """salt: sets apart prefixes whose cache differs for the same tokens (another adapter).  It is hashed by itself:
+        in front of the first block's tokens as it is, "x#1" and "12,..." would read like "x#11" and "2,..."."""
+        out, prev = [], hashlib.sha1(salt.encode()).hexdigest() if salt else ""
         for i in range(0, len(tokens) - len(tokens) % self.block_size, self.block_size):
             h = hashlib.sha1((prev + ",".join(map(str, tokens[i:i + self.block_size]))).encode()).hexdigest()
             out.append(h)
