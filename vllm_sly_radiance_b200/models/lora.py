@@ -157,6 +157,11 @@ _MODULES = {
 }
 
 
+# settings of an adapter_config.json under which the delta is not alpha / r times B A of every matrix
+_UNSUPPORTED = ("use_dora", "bias", "lora_bias", "modules_to_save", "alpha_pattern", "rank_pattern", "layer_replication",
+                "trainable_token_indices", "alora_invocation_tokens")
+
+
 class ModelAdapters:
     """Banks for every projection of a model's layers (the mixers' and the dense MLP's), ``max_loras`` slots of up to
     ``max_rank`` each.  Tensor parallelism and expert weights are not covered."""
@@ -209,8 +214,11 @@ class ModelAdapters:
         from safetensors import safe_open
         with open(os.path.join(path, "adapter_config.json")) as f:
             cfg = json.load(f)
-        if cfg.get("use_dora") or cfg.get("bias", "none") != "none" or cfg.get("modules_to_save"):
-            raise ValueError(f"adapter {name!r}: only plain low-rank matrices are supported")
+        odd = [k for k in _UNSUPPORTED if cfg.get(k) not in (None, False, "none", [], {})]
+        odd += ["peft_type"] if cfg.get("peft_type", "LORA") != "LORA" else []
+        if odd:
+            raise ValueError(f"adapter {name!r}: only plain low-rank matrices with one rank and one alpha are supported, "
+                             f"not {', '.join(odd)}")
         rank = int(cfg["r"])
         alpha = float(cfg.get("lora_alpha", rank))
         scale = alpha / rank ** 0.5 if cfg.get("use_rslora") else alpha / rank
