@@ -432,7 +432,9 @@ __global__ void __launch_bounds__(256, 2) decode_kernel(const __grid_constant__ 
         const int r = row_of(p, i, m, t.rows);
         sum *= r >= 0 ? p.xs[r] : 0.f;
       }
-      if (j0 + o % (16 * JG) < p.Rp) v[m * vs + j0 + o % (16 * JG)] = sum;
+      // beyond the rank A counts as zero, and zero times an infinity of x is NaN
+      const int j = j0 + o % (16 * JG);
+      if (j < p.Rp) v[m * vs + j] = j < t.rank ? sum : 0.f;
     }
     cluster_arrive();
   }
@@ -474,7 +476,8 @@ __global__ void __launch_bounds__(256) shrink16_kernel(const __grid_constant__ A
       const int r = row_of(p, i, m, t.rows);
       f *= r >= 0 ? p.xs[r] : 0.f;
     }
-    p.v[(((int64_t)blockIdx.z * p.max_tiles + i) * 16 + m) * p.S * p.Rp + s * p.Rp + j] = red_sum<JG>(red, o) * f;
+    p.v[(((int64_t)blockIdx.z * p.max_tiles + i) * 16 + m) * p.S * p.Rp + s * p.Rp + j] =
+        j < t.rank ? red_sum<JG>(red, o) * f : 0.f;         // (zero times an infinity of x is NaN)
   }
 }
 
