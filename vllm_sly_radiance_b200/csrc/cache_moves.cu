@@ -201,9 +201,17 @@ void run(const CacheItems* const (&kinds)[2], std::vector<Group> (&g)[2], std::v
 
 using Moves = pybind11::array_t<int64_t, pybind11::array::c_style | pybind11::array::forcecast>;
 
+// whole numbers only: a cast would cut 1.5 to the item 1
+Moves whole(const pybind11::handle& rows) {
+  const pybind11::array a = pybind11::array::ensure(rows);
+  if (!a || (a.size() && a.dtype().kind() != 'i' && a.dtype().kind() != 'u')) refuse("moves as rows of whole numbers");
+  return Moves(a);
+}
+
 // both kinds in one launch; everything is checked before anything moves
-void copy(const CacheItems* blocks, const Moves& bm, const CacheItems* slots, const Moves& sm) {
+void copy(const CacheItems* blocks, const pybind11::handle& block_moves, const CacheItems* slots, const pybind11::handle& slot_moves) {
   const CacheItems* const kinds[2] = {blocks, slots};
+  const Moves bm = whole(block_moves), sm = whole(slot_moves);
   const Moves* m[2] = {&bm, &sm};
   std::vector<Group> g[2];
   std::vector<int> dst;

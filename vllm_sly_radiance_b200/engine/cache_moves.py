@@ -57,7 +57,13 @@ class _Items:
 
     def move(self, moves):
         """On the CPU: (src, dst) or, of pages, (src, dst, tokens) rows, with the checks of csrc/cache_moves.cu."""
-        m = np.asarray(moves, dtype=np.int64)
+        try:
+            m = np.asarray(moves)
+        except ValueError:                       # rows of several lengths
+            m = np.zeros(0)
+        if m.dtype.kind not in "iu":
+            raise ValueError(f"cache moves: {self.name} as rows of whole numbers")
+        m = m.astype(np.int64)
         if m.ndim != 2 or m.shape[1] not in ((2, 3) if self.paged else (2,)):
             raise ValueError(f"cache moves: {self.name} as (src, dst{', tokens' if self.paged else ''}) rows")
         src, dst = m[:, 0], m[:, 1]
