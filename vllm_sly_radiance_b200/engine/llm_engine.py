@@ -357,6 +357,8 @@ class LLMEngine:
             params = [params or SamplingParams()] * len(prompts)
         if adapters is None or isinstance(adapters, str):
             adapters = [adapters] * len(prompts)
+        if len(adapters) != len(prompts):
+            raise ValueError(f"{len(adapters)} adapters for {len(prompts)} prompts")
         order = [self.add_request(p, sp, adapter=a) for p, sp, a in zip(prompts, params, adapters)]
         final = {}
         while self.has_unfinished_requests():
