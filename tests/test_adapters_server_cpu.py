@@ -1,0 +1,41 @@
+"""Adapters and parallel samples through the OpenAI-compatible server (CPU)."""
+import pytest
+from fastapi.testclient import TestClient
+
+from test_adapters_cpu import engine, tensors
+from vllm_sly_radiance_b200.config import tiny_hybrid
+from vllm_sly_radiance_b200.entrypoints.openai_server import build_app
+
+BODY = {"prompt": "hello world", "max_tokens": 5, "temperature": 0, "ignore_eos": True}
+
+
+@pytest.fixture(scope="module")
+def served():
+    e = engine(max_loras=3, max_lora_rank=8)
+    e.adapters.add_tensors("x", tensors(tiny_hybrid(), 8, 2), 8, 2.0)
+    with TestClient(build_app(e, "tiny,alias")) as c:
+        yield e, c
+
+
+def post(c, path="/v1/completions", **body):
+    return c.post(path, json={**BODY, **body})
+
+
+def test_adapter_is_a_model_of_its_own(served):
+    e, c = served
+    assert [m["id"] for m in c.get("/v1/models").json()["data"]] == ["tiny", "alias", "x"]
+    base, x = post(c, model="tiny").json(), post(c, model="x").json()
+    assert (base["model"], x["model"]) == ("tiny", "x")
+    assert base["choices"][0]["token_ids"] != x["choices"][0]["token_ids"]
+    assert post(c, model="y").status_code == 404
+
+
+def test_an_adapter_cannot_take_the_base_models_name(served):
+    e, c = served
+    with pytest.raises(ValueError):
+        e.adapters.add_tensors("alias", tensors(tiny_hybrid(), 8, 2), 8, 2.0)
+    assert [m["id"] for m in c.get("/v1/models").json()["data"]] == ["tiny", "alias", "x"]
+    other = engine(max_loras=1, max_lora_rank=8)
+    other.adapters.add_tensors("tiny", tensors(tiny_hybrid(), 8, 2), 8, 2.0)
+    with pytest.raises(ValueError):
+        build_app(other, "tiny")

@@ -130,14 +130,19 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
     from fastapi.responses import JSONResponse, PlainTextResponse, StreamingResponse
 
     app = FastAPI()
-    loop_runner = EngineLoop(engine, broadcaster)
     names = [n.strip() for n in served_model_name.split(",") if n.strip()] or ["model"]
-    app.state.engine_loop = loop_runner
 
     def adapter_names():
         """Loaded adapters are served as models of their own name."""
         a = getattr(engine, "adapters", None)
         return list(a.slots) if a is not None else []
+
+    if set(names) & set(adapter_names()):
+        raise ValueError(f"an adapter and the model are both to be served as {set(names) & set(adapter_names())}")
+    if getattr(engine, "adapters", None) is not None:
+        engine.adapters.reserved = frozenset(names)
+    loop_runner = EngineLoop(engine, broadcaster)
+    app.state.engine_loop = loop_runner
 
     def err(msg, code=400):
         return JSONResponse({"error": {"message": msg, "type": "invalid_request_error", "code": code}},

@@ -174,6 +174,7 @@ class ModelAdapters:
         self.model, self.max_loras, self.max_rank = model, max_loras, (max_rank + 7) // 8 * 8
         self.step = _Step()
         self.slots: dict = {}                    # name -> slot
+        self.reserved: frozenset = frozenset()   # names that mean the model without an adapter (the server's)
         self.salts: dict = {}                    # name -> what its cached prefixes are told apart by
         self._loads = 0
         cfg, dev = model.cfg, model.device
@@ -229,6 +230,8 @@ class ModelAdapters:
         """tensors: ``...layers.<i>.<module>.lora_A.weight`` [rank, in] and ``lora_B.weight`` [out, rank]."""
         if name in self.slots:
             raise ValueError(f"adapter {name!r} is loaded already")
+        if name in self.reserved:
+            raise ValueError(f"adapter {name!r}: the model itself is served under this name")
         if not 1 <= rank <= self.max_rank:
             raise ValueError(f"adapter {name!r}: rank {rank}, room for {self.max_rank}")
         free = sorted(set(range(self.max_loras)) - set(self.slots.values()))
