@@ -325,3 +325,10 @@ class EngineConfig:
 
     def model_config(self) -> ModelConfig:
         return get_model_config(self.model)
+
+    def lora_items(self) -> list:
+        """(name, directory) of the adapters that are loaded at start."""
+        items = [i.partition("=") for i in (self.lora_modules or "").split(",") if i]
+        if items and not self.max_loras:
+            raise ValueError("lora_modules needs max_loras")
+        return [(name.strip(), path.strip()) for name, _, path in items]

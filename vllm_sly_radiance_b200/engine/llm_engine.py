@@ -56,14 +56,12 @@ class LLMEngine:
         self.eos_token_id = getattr(self.tokenizer, "eos_token_id", None)
         # ---- adapters (before the caches are sized by what memory is left) ----
         self.adapters = None
+        lora_items = config.lora_items()
         if config.max_loras:
             from ..models.lora import ModelAdapters
             self.adapters = model.adapters = ModelAdapters(model, config.max_loras, config.max_lora_rank)
-            for item in filter(None, (config.lora_modules or "").split(",")):
-                name, _, path = item.partition("=")
-                self.adapters.add(name.strip(), path.strip())
-        elif config.lora_modules:
-            raise ValueError("lora_modules needs max_loras")
+            for name, path in lora_items:
+                self.adapters.add(name, path)
         # ---- cache sizing ----
         bs = config.block_size
         num_slots = config.max_num_seqs + 2
@@ -145,7 +143,7 @@ class LLMEngine:
         """adapter: the name of a loaded adapter (add_adapter) that the request runs with."""
         params = params or SamplingParams()
         ids = self.tokenizer.encode(prompt) if isinstance(prompt, str) else list(prompt)
-        if adapter is not None and (self.adapters is None or adapter not in self.adapters.slots):
+        if adapter is not None and adapter not in self.adapter_names:
             raise ValueError(f"adapter {adapter!r} is not loaded")
         if params.n > 1 and self.spec is not None:
             raise ValueError("n > 1 with speculative decoding is not supported")
@@ -179,6 +177,11 @@ class LLMEngine:
         return req.request_id
 
     # ---- adapters ----
+    @property
+    def adapter_names(self) -> list:
+        """Names that requests can give as their adapter."""
+        return list(self.adapters.slots) if self.adapters is not None else []
+
     def add_adapter(self, name: str, path: str):
         """Load a low-rank adapter (PEFT directory) that requests can name."""
         if self.adapters is None:

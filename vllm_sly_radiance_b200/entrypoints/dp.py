@@ -3,7 +3,7 @@ engine-shaped front end.
 
 ``DataParallelEngine`` offers what the server's engine loop and ``LLMEngine.generate`` use --
 ``add_request``, ``abort_request``, ``has_unfinished_requests``, ``step``, ``config``,
-``metrics`` -- and routes each new request to the replica with the fewest requests in flight.
+``metrics``, ``adapter_names`` -- and routes each new request to the replica with the fewest requests in flight.
 A replica runs the full engine (scheduler, KV cache, CUDA graphs) on its own device and streams
 its ``RequestOutput`` objects back; the front end never touches a GPU.  Replicas may themselves be
 tensor-parallel groups only through the SPMD launcher (one process per rank); this module covers
@@ -50,7 +50,7 @@ def _replica_main(idx: int, cfg: EngineConfig, cmd_q, out_q):
                 running = False
             elif c[0] == "add":
                 try:
-                    eng.add_request(c[1], c[2], c[3])
+                    eng.add_request(c[1], c[2], c[3], **c[4])
                 except Exception as e:
                     out_q.put(("error", c[3], repr(e)))
             elif c[0] == "abort":
@@ -86,6 +86,8 @@ class DataParallelEngine:
             raise ValueError("data-parallel size must be >= 1")
         from ..engine.tokenizer import get_tokenizer
         self.config = config
+        # every replica loads the same adapters at start; there is no loading behind this front end later on
+        self.adapter_names = [name for name, _ in config.lora_items()]
         # the front end's own tokenizer (chat templates); the replicas detokenize their outputs
         self.tokenizer = get_tokenizer(tokenizer_path, config.model_config().vocab_size)
         self.n = num_replicas
@@ -124,12 +126,14 @@ class DataParallelEngine:
 
     # ---- engine-shaped API ----
     def add_request(self, prompt, params: Optional[SamplingParams] = None,
-                    request_id: Optional[str] = None) -> str:
+                    request_id: Optional[str] = None, adapter: Optional[str] = None) -> str:
+        if adapter is not None and adapter not in self.adapter_names:
+            raise ValueError(f"adapter {adapter!r} is not loaded")
         rid = request_id if request_id is not None else f"dp-{next(self._ids)}"
         r = min(range(self.n), key=lambda i: (self.inflight[i], i))
         self.owner[rid] = r
         self.inflight[r] += 1
-        self.cmd_qs[r].put(("add", prompt, params or SamplingParams(), rid))
+        self.cmd_qs[r].put(("add", prompt, params or SamplingParams(), rid, dict(adapter=adapter)))
         return rid
 
     def abort_request(self, request_id: str) -> None:
@@ -172,10 +176,14 @@ class DataParallelEngine:
                 raise RuntimeError(f"replica {idx} step failed: {info}")
         return outs
 
-    def generate(self, prompts, params=None) -> list[RequestOutput]:
+    def generate(self, prompts, params=None, adapters=None) -> list[RequestOutput]:
         if isinstance(params, SamplingParams) or params is None:
             params = [params or SamplingParams()] * len(prompts)
-        order = [self.add_request(p, sp) for p, sp in zip(prompts, params)]
+        if adapters is None or isinstance(adapters, str):
+            adapters = [adapters] * len(prompts)
+        if len(adapters) != len(prompts):
+            raise ValueError(f"{len(adapters)} adapters for {len(prompts)} prompts")
+        order = [self.add_request(p, sp, adapter=a) for p, sp, a in zip(prompts, params, adapters)]
         final = {}
         while self.has_unfinished_requests():
             for o in self.step(timeout=1.0):

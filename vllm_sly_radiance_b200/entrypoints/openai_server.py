@@ -134,8 +134,7 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
 
     def adapter_names():
         """Loaded adapters are served as models of their own name."""
-        a = getattr(engine, "adapters", None)
-        return list(a.slots) if a is not None else []
+        return list(getattr(engine, "adapter_names", []))
 
     if set(names) & set(adapter_names()):
         raise ValueError(f"an adapter and the model are both to be served as {set(names) & set(adapter_names())}")
