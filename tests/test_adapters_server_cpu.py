@@ -39,3 +39,25 @@ def test_an_adapter_cannot_take_the_base_models_name(served):
     other.adapters.add_tensors("tiny", tensors(tiny_hybrid(), 8, 2), 8, 2.0)
     with pytest.raises(ValueError):
         build_app(other, "tiny")
+
+
+CHAT = dict(path="/v1/chat/completions", prompt=None, messages=[{"role": "user", "content": "hi"}])
+
+
+@pytest.mark.parametrize("path", [{}, CHAT])
+def test_samples(served, path):
+    e, c = served
+    r = post(c, n=3, temperature=1.0, top_k=50, seed=4, **path).json()
+    assert [o["index"] for o in r["choices"]] == [0, 1, 2] and r["usage"]["completion_tokens"] == 15
+    assert post(c, n=1, **path).status_code == post(c, n=None, **path).status_code == 200
+    assert not e.requests and not e.groups
+
+
+@pytest.mark.parametrize("path", [{}, CHAT])
+@pytest.mark.parametrize("stream", [False, True])
+@pytest.mark.parametrize("n", [-1, 129, 10 ** 9, "many", [2], {"a": 1}, 1.5])
+def test_refused_numbers_of_samples(served, path, stream, n):
+    """The request is at fault (400), and nothing of it reaches the engine."""
+    e, c = served
+    assert post(c, n=n, stream=stream, **path).status_code == 400
+    assert not e.requests and not e.groups

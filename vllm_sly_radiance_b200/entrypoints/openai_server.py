@@ -102,6 +102,23 @@ class EngineLoop:
             loop.call_soon_threadsafe(q.put_nowait, item)
 
 
+# Samples of one request: each is a request of the engine and an entry of every output, made between two steps.
+MAX_SAMPLES = 128
+
+
+def _num_samples(body: dict) -> int:
+    n = body.get("n") or 1
+    try:
+        v = int(n)
+    except (TypeError, OverflowError):
+        raise ValueError("n must be a whole number") from None
+    if isinstance(n, float) and v != n:
+        raise ValueError("n must be a whole number")
+    if v > MAX_SAMPLES:
+        raise ValueError(f"n must be at most {MAX_SAMPLES}")
+    return v
+
+
 def _sampling_from_body(body: dict, default_max: int = 256) -> SamplingParams:
     stop = body.get("stop") or []
     if isinstance(stop, str):
@@ -121,7 +138,7 @@ def _sampling_from_body(body: dict, default_max: int = 256) -> SamplingParams:
         frequency_penalty=float(body.get("frequency_penalty", 0.0)),
         repetition_penalty=float(body.get("repetition_penalty", 1.0)),
         min_tokens=int(body.get("min_tokens", 0)),
-        n=int(body.get("n") or 1))
+        n=_num_samples(body))
 
 
 def build_app(engine, served_model_name: str = "model", reasoning_parser: Optional[str] = None,
@@ -186,8 +203,6 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
         adapter = body.get("model") if body.get("model") in adapter_names() else None
         if body.get("model") and body["model"] not in names and adapter is None:
             return err(f"model {body['model']!r} not found", 404)
-        if body.get("stream") and int(body.get("n") or 1) > 1:
-            return err("n > 1 with stream is not supported")
         prompt = body.get("prompt", "")
         if isinstance(prompt, list) and prompt and isinstance(prompt[0], str):
             prompt = prompt[0]
@@ -195,6 +210,8 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
             params = _sampling_from_body(body, 16)
         except ValueError as e:
             return err(str(e))
+        if body.get("stream") and params.n > 1:
+            return err("n > 1 with stream is not supported")
         rid = f"cmpl-{uuid.uuid4().hex}"
         created = int(time.time())
         if body.get("stream"):
@@ -231,8 +248,6 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
         adapter = body.get("model") if body.get("model") in adapter_names() else None
         if body.get("model") and body["model"] not in names and adapter is None:
             return err(f"model {body['model']!r} not found", 404)
-        if body.get("stream") and int(body.get("n") or 1) > 1:
-            return err("n > 1 with stream is not supported")
         msgs = body.get("messages") or []
         kw = dict(body.get("chat_template_kwargs") or {})
         if body.get("tools"):
@@ -242,6 +257,8 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
             params = _sampling_from_body(body, 256)
         except (ValueError, TypeError) as e:
             return err(str(e))
+        if body.get("stream") and params.n > 1:
+            return err("n > 1 with stream is not supported")
         rid = f"chatcmpl-{uuid.uuid4().hex}"
         created = int(time.time())
         rp = ReasoningParser(reasoning_parser, thinking=kw.get("enable_thinking", True)) \
