@@ -61,3 +61,15 @@ def test_refused_numbers_of_samples(served, path, stream, n):
     e, c = served
     assert post(c, n=n, stream=stream, **path).status_code == 400
     assert not e.requests and not e.groups
+
+
+def test_samples_from_a_server_with_speculative_decoding():
+    """A server that drafts answers n > 1 as one without does."""
+    e = engine(speculative_method="lookup", num_speculative_tokens=3)
+    with TestClient(build_app(e, "tiny")) as c:
+        one = post(c).json()["choices"][0]
+        r = post(c, n=2)
+        assert r.status_code == 200, r.text
+        assert [(o["index"], o["token_ids"]) for o in r.json()["choices"]] == [(i, one["token_ids"]) for i in range(2)]
+        assert post(c, CHAT["path"], prompt=None, messages=CHAT["messages"], n=3).status_code == 200
+    assert not e.requests and not e.groups

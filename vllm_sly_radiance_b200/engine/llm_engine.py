@@ -139,14 +139,17 @@ class LLMEngine:
 
     # ------------------------------------------------------------------------------------------
     def add_request(self, prompt: Union[str, list[int]], params: Optional[SamplingParams] = None,
-                    request_id: Optional[str] = None, adapter: Optional[str] = None) -> str:
-        """adapter: the name of a loaded adapter (add_adapter) that the request runs with."""
+                    request_id: Optional[str] = None, adapter: Optional[str] = None,
+                    share_prompt: bool = True) -> str:
+        """adapter: the name of a loaded adapter (add_adapter) that the request runs with.
+        share_prompt: the n samples of a request start from one prefill of their prompt; without it
+        each prefills the prompt itself, the only form that speculative decoding has."""
         params = params or SamplingParams()
         ids = self.tokenizer.encode(prompt) if isinstance(prompt, str) else list(prompt)
         if adapter is not None and adapter not in self.adapter_names:
             raise ValueError(f"adapter {adapter!r} is not loaded")
-        if params.n > 1 and self.spec is not None:
-            raise ValueError("n > 1 with speculative decoding is not supported")
+        if params.n > 1 and share_prompt and self.spec is not None:
+            raise ValueError("n > 1 from one prefill is not supported with speculative decoding")
         req = Request(ids, params, request_id, eos_token_id=self.eos_token_id)
         reqs = [req]
         for i in range(1, params.n):
@@ -165,7 +168,7 @@ class LLMEngine:
             self.groups[rid] = dict(ids=[r.request_id for r in reqs], done=set(),
                                     outs=[CompletionOutput(i, "", [], None) for i in range(params.n)])
             self.member.update({r.request_id: (rid, i) for i, r in enumerate(reqs)})
-            if len(ids) == 1:                    # no cache to share
+            if len(ids) == 1 or not share_prompt:          # no cache to share
                 for r in reqs[1:]:
                     self.scheduler.add(r)
             else:
@@ -362,7 +365,8 @@ class LLMEngine:
             adapters = [adapters] * len(prompts)
         if len(adapters) != len(prompts):
             raise ValueError(f"{len(adapters)} adapters for {len(prompts)} prompts")
-        order = [self.add_request(p, sp, adapter=a) for p, sp, a in zip(prompts, params, adapters)]
+        order = [self.add_request(p, sp, adapter=a, share_prompt=self.spec is None)
+                 for p, sp, a in zip(prompts, params, adapters)]
         final = {}
         while self.has_unfinished_requests():
             for o in self.step():

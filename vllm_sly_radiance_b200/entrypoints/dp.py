@@ -126,14 +126,16 @@ class DataParallelEngine:
 
     # ---- engine-shaped API ----
     def add_request(self, prompt, params: Optional[SamplingParams] = None,
-                    request_id: Optional[str] = None, adapter: Optional[str] = None) -> str:
+                    request_id: Optional[str] = None, adapter: Optional[str] = None,
+                    share_prompt: bool = True) -> str:
         if adapter is not None and adapter not in self.adapter_names:
             raise ValueError(f"adapter {adapter!r} is not loaded")
         rid = request_id if request_id is not None else f"dp-{next(self._ids)}"
         r = min(range(self.n), key=lambda i: (self.inflight[i], i))
         self.owner[rid] = r
         self.inflight[r] += 1
-        self.cmd_qs[r].put(("add", prompt, params or SamplingParams(), rid, dict(adapter=adapter)))
+        self.cmd_qs[r].put(("add", prompt, params or SamplingParams(), rid,
+                            dict(adapter=adapter, share_prompt=share_prompt)))
         return rid
 
     def abort_request(self, request_id: str) -> None:
@@ -183,7 +185,8 @@ class DataParallelEngine:
             adapters = [adapters] * len(prompts)
         if len(adapters) != len(prompts):
             raise ValueError(f"{len(adapters)} adapters for {len(prompts)} prompts")
-        order = [self.add_request(p, sp, adapter=a) for p, sp, a in zip(prompts, params, adapters)]
+        order = [self.add_request(p, sp, adapter=a, share_prompt=not self.config.speculative_method)
+                 for p, sp, a in zip(prompts, params, adapters)]
         final = {}
         while self.has_unfinished_requests():
             for o in self.step(timeout=1.0):

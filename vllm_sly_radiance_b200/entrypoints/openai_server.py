@@ -46,7 +46,10 @@ class EngineLoop:
         q: asyncio.Queue = asyncio.Queue()
         with self.lock:
             self.outq[request_id] = (q, loop)
-        self.inbox.put(("add", prompt, params, request_id) + ((adapter,) if adapter else ()))
+        opts = dict(adapter=adapter) if adapter else {}
+        if params.n > 1 and self.engine.config.speculative_method:
+            opts["share_prompt"] = False
+        self.inbox.put(("add", prompt, params, request_id, opts))
         return q
 
     def abort(self, request_id: str):
@@ -68,7 +71,7 @@ class EngineLoop:
             for c in cmds:
                 try:
                     if c[0] == "add":
-                        eng.add_request(*c[1:])
+                        eng.add_request(*c[1:4], **c[4])
                     elif c[0] == "abort":
                         eng.abort_request(c[1])
                         self._emit(c[1], None)

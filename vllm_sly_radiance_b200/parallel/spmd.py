@@ -28,7 +28,7 @@ def follower_loop(engine, broadcaster: RequestBroadcaster):
         stop = False
         for c in cmds:
             if c[0] == "add":
-                engine.add_request(c[1], c[2], c[3])
+                engine.add_request(*c[1:4], **c[4])
             elif c[0] == "abort":
                 engine.abort_request(c[1])
             elif c[0] == "shutdown":
