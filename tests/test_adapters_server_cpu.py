@@ -1,4 +1,6 @@
 """Adapters and parallel samples through the OpenAI-compatible server (CPU)."""
+import json
+
 import pytest
 from fastapi.testclient import TestClient
 
@@ -73,3 +75,47 @@ def test_samples_from_a_server_with_speculative_decoding():
         assert [(o["index"], o["token_ids"]) for o in r.json()["choices"]] == [(i, one["token_ids"]) for i in range(2)]
         assert post(c, CHAT["path"], prompt=None, messages=CHAT["messages"], n=3).status_code == 200
     assert not e.requests and not e.groups
+
+
+def stream(c, **body):
+    """-> (chunks, choices by index: text and finish reasons)."""
+    path = body.pop("path", "/v1/completions")
+    with c.stream("POST", path, json={**BODY, "stream": True, **body}) as r:
+        assert r.status_code == 200, r.read()
+        lines = [s[6:] for s in r.iter_lines() if s.startswith("data: ")]
+    assert lines[-1] == "[DONE]"
+    chunks = [json.loads(s) for s in lines[:-1]]
+    out = {}
+    for k in chunks:
+        (o,) = k["choices"]
+        text, ends, roles = out.setdefault(o["index"], ([], [], []))
+        assert not ends                          # nothing after a sample's end
+        text.append(o["text"] if "text" in o else o["delta"].get("content", ""))
+        roles += [o["delta"]["role"]] if "role" in o.get("delta", {}) else []
+        ends += [o["finish_reason"]] if o["finish_reason"] else []
+    return chunks, {i: ("".join(t), e, r) for i, (t, e, r) in out.items()}
+
+
+@pytest.mark.parametrize("path,content,roles", [({}, lambda o: o["text"], []), (CHAT, lambda o: o["message"]["content"], ["assistant"])])
+@pytest.mark.parametrize("n", [1, 3])
+def test_streamed_samples(served, path, content, roles, n):
+    """Every sample arrives under its index, as the whole answer has it."""
+    e, c = served
+    kw = dict(n=n, temperature=1.0, top_k=50, seed=4, max_tokens=12, **path)
+    want = post(c, **kw).json()["choices"]
+    _, got = stream(c, **kw)
+    assert got == {o["index"]: (content(o), [o["finish_reason"]], roles) for o in want} and len(got) == n
+    assert not e.requests and not e.groups
+
+
+def test_streamed_samples_with_parsers():
+    """Reasoning is split sample by sample."""
+    e = engine()
+    with TestClient(build_app(e, "tiny", reasoning_parser="qwen3")) as c:
+        kw = dict(n=2, temperature=1.0, top_k=50, seed=4, max_tokens=12, **CHAT)
+        want = post(c, **kw).json()["choices"]
+        chunks, got = stream(c, **kw)
+        for o in want:
+            r = "".join(k["choices"][0]["delta"].get("reasoning_content", "") for k in chunks
+                        if k["choices"][0]["index"] == o["index"])
+            assert (r, got[o["index"]][0]) == (o["message"]["reasoning_content"], o["message"]["content"])

@@ -144,6 +144,24 @@ def _sampling_from_body(body: dict, default_max: int = 256) -> SamplingParams:
         n=_num_samples(body))
 
 
+class _Tails:
+    """What a streamed request's outputs added since they were sent last, sample by sample."""
+
+    def __init__(self):
+        self.sent, self.done = {}, set()
+
+    def of(self, o):
+        """(output, new text) of the samples to send: every step of a single one, of several those that moved."""
+        for out in o.outputs:
+            delta = out.text[self.sent.get(out.index, 0):]
+            if len(o.outputs) > 1 and (out.index in self.done or not (delta or out.finish_reason)):
+                continue
+            self.sent[out.index] = len(out.text)
+            if out.finish_reason:
+                self.done.add(out.index)
+            yield out, delta
+
+
 def build_app(engine, served_model_name: str = "model", reasoning_parser: Optional[str] = None,
               tool_parser: Optional[str] = None, broadcaster=None):
     from fastapi import FastAPI
@@ -213,23 +231,20 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
             params = _sampling_from_body(body, 16)
         except ValueError as e:
             return err(str(e))
-        if body.get("stream") and params.n > 1:
-            return err("n > 1 with stream is not supported")
         rid = f"cmpl-{uuid.uuid4().hex}"
         created = int(time.time())
         if body.get("stream"):
             async def gen():
-                sent = 0
+                tails = _Tails()
                 async for o in _run(prompt, params, rid, adapter):
                     if isinstance(o, dict):
                         yield f"data: {json.dumps({'error': o})}\n\n"
                         break
-                    text = o.outputs[0].text
-                    delta, sent = text[sent:], len(text)
-                    chunk = {"id": rid, "object": "text_completion", "created": created,
-                             "model": names[0], "choices": [{"index": 0, "text": delta,
-                                                             "finish_reason": o.outputs[0].finish_reason}]}
-                    yield f"data: {json.dumps(chunk)}\n\n"
+                    for out, delta in tails.of(o):
+                        chunk = {"id": rid, "object": "text_completion", "created": created,
+                                 "model": names[0], "choices": [{"index": out.index, "text": delta,
+                                                                 "finish_reason": out.finish_reason}]}
+                        yield f"data: {json.dumps(chunk)}\n\n"
                 yield "data: [DONE]\n\n"
             return StreamingResponse(gen(), media_type="text/event-stream")
         last = None
@@ -260,43 +275,46 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
             params = _sampling_from_body(body, 256)
         except (ValueError, TypeError) as e:
             return err(str(e))
-        if body.get("stream") and params.n > 1:
-            return err("n > 1 with stream is not supported")
         rid = f"chatcmpl-{uuid.uuid4().hex}"
         created = int(time.time())
-        rp = ReasoningParser(reasoning_parser, thinking=kw.get("enable_thinking", True)) \
-            if reasoning_parser else None
+
+        def reasoning():
+            return ReasoningParser(reasoning_parser, thinking=kw.get("enable_thinking", True)) \
+                if reasoning_parser else None
+
         tp = ToolParser(tool_parser) if (tool_parser and body.get("tools")) else None
         if body.get("stream"):
             async def gen():
-                sent = 0
-                first = True
+                tails = _Tails()
+                parsers = {}                     # sample -> its reasoning parser, from its first chunk on
                 async for o in _run(prompt, params, rid, adapter):
                     if isinstance(o, dict):
                         yield f"data: {json.dumps({'error': o})}\n\n"
                         break
-                    text = o.outputs[0].text
-                    delta_text, sent = text[sent:], len(text)
-                    delta = {"role": "assistant"} if first else {}
-                    first = False
-                    if rp is not None:
-                        r, c = rp.stream(delta_text)
-                        if r:
-                            delta["reasoning_content"] = r
-                        if c:
-                            delta["content"] = c
-                    elif delta_text:
-                        delta["content"] = delta_text
-                    fr = o.outputs[0].finish_reason
-                    if fr and tp is not None:
-                        calls, _ = tp.parse(rp.content if rp else text)
-                        if calls:
-                            delta["tool_calls"] = [dict(c, index=i) for i, c in enumerate(calls)]
-                            fr = "tool_calls"
-                    chunk = {"id": rid, "object": "chat.completion.chunk", "created": created,
-                             "model": names[0], "choices": [{"index": 0, "delta": delta,
-                                                             "finish_reason": fr}]}
-                    yield f"data: {json.dumps(chunk)}\n\n"
+                    for out, delta_text in tails.of(o):
+                        delta = {}
+                        if out.index not in parsers:
+                            parsers[out.index] = reasoning()
+                            delta["role"] = "assistant"
+                        rp = parsers[out.index]
+                        if rp is not None:
+                            r, c = rp.stream(delta_text)
+                            if r:
+                                delta["reasoning_content"] = r
+                            if c:
+                                delta["content"] = c
+                        elif delta_text:
+                            delta["content"] = delta_text
+                        fr = out.finish_reason
+                        if fr and tp is not None:
+                            calls, _ = tp.parse(rp.content if rp else out.text)
+                            if calls:
+                                delta["tool_calls"] = [dict(c, index=i) for i, c in enumerate(calls)]
+                                fr = "tool_calls"
+                        chunk = {"id": rid, "object": "chat.completion.chunk", "created": created,
+                                 "model": names[0], "choices": [{"index": out.index, "delta": delta,
+                                                                 "finish_reason": fr}]}
+                        yield f"data: {json.dumps(chunk)}\n\n"
                 yield "data: [DONE]\n\n"
             return StreamingResponse(gen(), media_type="text/event-stream")
         last = None
@@ -304,7 +322,7 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
             last = o
         if last is None or isinstance(last, dict):
             return err(str(last), 500)
-        choices = []
+        choices, rp = [], reasoning()
         for out in last.outputs:
             msg = {"role": "assistant", "content": out.text}
             fr = out.finish_reason
