@@ -119,3 +119,10 @@ def test_streamed_samples_with_parsers():
             r = "".join(k["choices"][0]["delta"].get("reasoning_content", "") for k in chunks
                         if k["choices"][0]["index"] == o["index"])
             assert (r, got[o["index"]][0]) == (o["message"]["reasoning_content"], o["message"]["content"])
+
+
+@pytest.mark.parametrize("path", [{}, CHAT])
+def test_streams_name_the_adapter(served, path):
+    e, c = served
+    assert {k["model"] for k in stream(c, model="x", **path)[0]} == {"x"}
+    assert {k["model"] for k in stream(c, **path)[0]} == {"tiny"}

@@ -242,8 +242,8 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
                         break
                     for out, delta in tails.of(o):
                         chunk = {"id": rid, "object": "text_completion", "created": created,
-                                 "model": names[0], "choices": [{"index": out.index, "text": delta,
-                                                                 "finish_reason": out.finish_reason}]}
+                                 "model": adapter or names[0], "choices": [{"index": out.index, "text": delta,
+                                                                            "finish_reason": out.finish_reason}]}
                         yield f"data: {json.dumps(chunk)}\n\n"
                 yield "data: [DONE]\n\n"
             return StreamingResponse(gen(), media_type="text/event-stream")
@@ -312,8 +312,8 @@ def build_app(engine, served_model_name: str = "model", reasoning_parser: Option
                                 delta["tool_calls"] = [dict(c, index=i) for i, c in enumerate(calls)]
                                 fr = "tool_calls"
                         chunk = {"id": rid, "object": "chat.completion.chunk", "created": created,
-                                 "model": names[0], "choices": [{"index": out.index, "delta": delta,
-                                                                 "finish_reason": fr}]}
+                                 "model": adapter or names[0], "choices": [{"index": out.index, "delta": delta,
+                                                                            "finish_reason": fr}]}
                         yield f"data: {json.dumps(chunk)}\n\n"
                 yield "data: [DONE]\n\n"
             return StreamingResponse(gen(), media_type="text/event-stream")
