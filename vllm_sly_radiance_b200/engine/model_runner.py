@@ -9,6 +9,7 @@ Sampled token ids come back with one device->host copy.
 """
 from __future__ import annotations
 
+import itertools
 import math
 import time
 from dataclasses import dataclass
@@ -353,6 +354,11 @@ class ModelRunner:
         g = self.graphs.get(bucket)
         return g
 
+    @staticmethod
+    def _graph_key(bucket: int, mode: str, adapters: bool):
+        """Steps whose rows may have adapters run graphs of their own: the others keep their launches."""
+        return (bucket, mode, "adapters") if adapters else (bucket, mode)
+
     def _run_graph(self, out: SchedulerOutput, bucket: int):
         nb_fixed = self.max_blocks
         meta, ids, sample_idx, _ = self.prepare(out, pad_to=bucket, nb_fixed=nb_fixed)
@@ -360,7 +366,7 @@ class ModelRunner:
         reqs = [s.req for s in out.seqs]
         greedy = all(r.params.greedy for r in reqs)
         mode = "greedy" if greedy else ("full" if needs_full_vocab(reqs) else "window")
-        key = (bucket, mode, "adapters") if adapters else (bucket, mode)
+        key = self._graph_key(bucket, mode, adapters)
         g = self.graphs.get(key)
         if g is None:
             # warm up and capture on an all-padding batch (dummy state slot / KV block 0), so the
@@ -389,8 +395,9 @@ class ModelRunner:
         return self.h_out[:B].tolist()
 
     def capture_all(self):
-        """Capture the decode graphs of every bucket (greedy and sampled) up front, on dummy
-        all-padding batches, so no request pays a capture inside its step."""
+        """Capture the decode graphs of every bucket (greedy and sampled, and with adapter slots
+        those of steps with adapters too) up front, on dummy all-padding batches, so no request pays
+        a capture inside its step."""
         if not self.enable_graphs:
             return
         from .scheduler import SchedulerOutput as _SO
@@ -398,12 +405,14 @@ class ModelRunner:
             if bucket > self.graph_max_bs:
                 break
             # the full-vocabulary mode (top_k disabled) is captured when a batch first needs it
-            for mode in ("greedy", "window"):
-                if (bucket, mode) in self.graphs:
+            for mode, adapters in itertools.product(("greedy", "window"),
+                                                    (False, True) if self.lora_slots else (False,)):
+                key = self._graph_key(bucket, mode, adapters)
+                if key in self.graphs:
                     continue
                 dmeta, dids, _, _ = self.prepare(_SO([], 0, [], []), pad_to=bucket,
-                                                 nb_fixed=self.max_blocks)
-                self.graphs[(bucket, mode)] = self._capture(bucket, mode, dmeta, dids)
+                                                 nb_fixed=self.max_blocks, adapters=adapters)
+                self.graphs[key] = self._capture(bucket, mode, dmeta, dids)
         torch.cuda.synchronize(self.device)
 
     def _capture(self, bucket, mode, meta, ids):
