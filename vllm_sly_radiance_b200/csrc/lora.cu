@@ -1304,7 +1304,9 @@ void launch16(Args& p, bool fp8, bool vec, const at::TensorOptions& opts, cudaSt
   constexpr int STEP = STEPF<JG>;
   const int64_t sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   // one launch while all its clusters run at once (two CTAs an SM); beyond, its chain of latencies counts once per wave:
-  // 64 rows of 24 adapters took 43 us so, and 20 to 25 us in two launches
+  // 64 rows of 24 adapters took 43 us so, and 20 to 25 us in two launches.  Only the plan's room for tiles is known here: a
+  // decode graph's has room for a tile a row, and 64 rows of 4 adapters take 13.0 us so (rank 16, 5120 -> 17408), with a
+  // plan of their size 7.7
   for (p.steps = 1; p.steps < 4 && (int64_t)chunks(p, CL * STEP * p.steps) * CL * p.max_tiles > 2 * sms;) p.steps *= 2;
   const unsigned ch = chunks(p, CL * STEP * p.steps);
   if ((int64_t)ch * CL * p.max_tiles <= 2 * sms) {
@@ -1337,8 +1339,11 @@ void launch128(Args& p, const CUtensorMap& am, const CUtensorMap& bm, const CUte
   torch::Tensor ws = torch::empty({(int64_t)p.max_tiles * 128 * p.S * p.Rp}, opts);
   p.v = ws.data_ptr<float>();
   const int nc = rank_rows(p), groups = (p.S * p.R + nc - 1) / nc, nc16 = (nc + 15) / 16 * 16;
-  const int64_t ctas = (int64_t)p.max_tiles * groups;
-  for (p.splits = 1; p.splits < 8 && ctas * p.splits * 2 <= 2 * 148 && p.K >= 256 * p.splits * 2;) p.splits *= 2;
+  const int64_t ctas = (int64_t)p.max_tiles * groups, sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  // Shares of K: as many as give every SM two CTAs, each with four 64-k steps or more.  Both launches with 1, 2, 4, 8 shares:
+  // 5 tiles (rank 16, 5120 -> 16480) 71, 45, 32, 27 us; 12 (rank 64, 8704 -> 5120) 93, 55, 37, 28; 33 (rank 16, as the
+  // first) 113, 87, 75, 72; 64 (rank 64, 5120 -> 17408), where four fill the machine, 182, 162, 155, 165.
+  for (p.splits = 1; p.splits < 8 && ctas * p.splits * 2 <= 2 * sms && p.K >= 256 * p.splits * 2;) p.splits *= 2;
   const size_t sums = 128 * (nc16 + 4) * sizeof(float) + 1024;
   const dim3 grid(p.max_tiles, groups, p.splits);
   if (tma_k) {
@@ -1363,12 +1368,12 @@ void launch128(Args& p, const CUtensorMap& am, const CUtensorMap& bm, const CUte
                                        (uint64_t)p.S * 4 * p.Rp, rb / 2, 128,
                                        rb == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : rb == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
     const size_t smem = 1024 + y_stages(kc, rb) * 16384 + (size_t)kc * rb * (2 * 128 + b_stages(kc, rb) * FT);
-    const int per_row = chunks(p, FT), sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+    const int per_row = chunks(p, FT);
     const unsigned grid = std::min<int64_t>((int64_t)p.max_tiles * per_row, sms * (smem <= 113 * 1024 ? 2 : 1));
     launch(expand128_kernel, dim3(grid), TH, 1, 1, smem, st, p, map(16), map(1), vm, bm, bg, per_row);
   } else {
     // feature tiles of a CTA: v is staged once for all of them, as long as every SM has a few CTAs
-    for (p.steps = 1; p.steps < 16 && (int64_t)chunks(p, 128 * p.steps * 2) * p.max_tiles >= 4 * 148;) p.steps *= 2;
+    for (p.steps = 1; p.steps < 16 && (int64_t)chunks(p, 128 * p.steps * 2) * p.max_tiles >= 4 * sms;) p.steps *= 2;
     launch(vec_n ? expand128_any_kernel<true> : expand128_any_kernel<false>, dim3(chunks(p, 128 * p.steps), p.max_tiles), 256, 1, 1,
            (size_t)(kc <= 3 ? 4 : 3) * kc * 16384 + 1024, st, p);
   }

@@ -2,8 +2,10 @@
 
 A forked sequence shares its parent's full pages (reference counts, ``KVCacheManager.fork``); its partly filled page
 and the GDN layers' state, which both sequences will write, are copied.  Compacting moves the pages in use to the front
-of the pool, so that the pages behind them are free in one piece.  ``CacheMover`` runs either as one launch per item
-kind over all layers (``csrc/cache_moves.cu``)."""
+of the pool, so that the pages behind them are free in one piece.  ``CacheMover`` runs either as one launch over all
+layers, pages and states together (``csrc/cache_moves.cu``).  ``CacheMover.compact`` is for callers that keep block tables
+of their own; the engine's ``compact_cache`` plans from its reference counts (``KVCacheManager.compact``), moves the
+pages of its prefix cache too, and calls ``copy``."""
 from __future__ import annotations
 
 import numpy as np
