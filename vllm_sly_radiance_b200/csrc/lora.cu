@@ -212,6 +212,8 @@ DEVI void first_product(const Args& p, const __nv_bfloat16* a, const uint8_t* co
                         int ke, float* red) {
   const int warp = threadIdx.x / 32, lane = threadIdx.x & 31, g = lane >> 2, q4 = lane & 3;
   float c[JG][2][4] = {};
+  // Up to rank 16 four blocks of k in flight and not two: 1 row 5.95 / 6.13 us and the mixed step of 4096 rows 104.4 / 105.6
+  // with A from DRAM; with A in L2 61 single rows take 25.3 / 24.6.
 #pragma unroll (JG == 1 ? 4 : 2)
   for (int k = kb; k < ke; k += 32) {
     const uint4 z = make_uint4(0, 0, 0, 0);
