@@ -13,16 +13,18 @@ from vllm_sly_radiance_b200.entrypoints.openai_server import build_app
 def test_adapters_behind_two_replicas(tmp_path):
     path = save(tmp_path / "a", tiny_hybrid(), 8, 16, 1)
     kw = dict(max_loras=1, max_lora_rank=8, lora_modules=f"a={path}")
-    prompts, names = [list(range(5 + i, 40 + i)) for i in range(4)], ["a", None, "a", None]
+    prompts, names = [list(range(5 + i, 40 + i)) for i in range(4)], ["a", None, None, "a"]
     sp = SamplingParams(max_tokens=4, **GREEDY)
-    want = tokens(engine(**kw).generate(prompts, sp, names))
+    one = engine(**kw)                           # one request at a time: rows of a batch may differ by a rounding
+    want = [tokens(one.generate([p], sp, [n]))[0] for p, n in zip(prompts, names)]
     assert want[0] != tokens(engine().generate(prompts[:1], sp))[0]
     dp = DataParallelEngine(EngineConfig(model="tiny_hybrid", device="cpu", max_model_len=512, max_num_seqs=4, max_num_batched_tokens=96,
                                          num_kv_blocks=48, quantization="bf16", kv_cache_dtype="bf16", enable_cuda_graphs=False,
                                          block_size=16, **kw), 2)
     try:
         assert dp.adapter_names == ["a"]
-        assert tokens(dp.generate(prompts, sp, names)) == want
+        for i in (0, 2):                         # two requests at once, one on each replica
+            assert tokens(dp.generate(prompts[i:i + 2], sp, names[i:i + 2])) == want[i:i + 2]
         with pytest.raises(ValueError):
             dp.add_request(prompts[0], sp, adapter="b")
         with pytest.raises(ValueError):
