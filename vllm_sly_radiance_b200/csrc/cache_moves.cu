@@ -201,6 +201,11 @@ void run(const CacheItems* const (&kinds)[2], std::vector<Group> (&g)[2], std::v
 
 using Moves = pybind11::array_t<int64_t, pybind11::array::c_style | pybind11::array::forcecast>;
 
+bool none(const pybind11::handle& rows) {
+  const Py_ssize_t n = PySequence_Check(rows.ptr()) ? PySequence_Size(rows.ptr()) : -1;
+  if (n < 0) PyErr_Clear();
+  return n == 0;
+}
 // whole numbers only: a cast would cut 1.5 to the item 1
 Moves whole(const pybind11::handle& rows) {
   const pybind11::array a = pybind11::array::ensure(rows);
@@ -211,16 +216,17 @@ Moves whole(const pybind11::handle& rows) {
 // both kinds in one launch; everything is checked before anything moves
 void copy(const CacheItems* blocks, const pybind11::handle& block_moves, const CacheItems* slots, const pybind11::handle& slot_moves) {
   const CacheItems* const kinds[2] = {blocks, slots};
-  const Moves bm = whole(block_moves), sm = whole(slot_moves);
-  const Moves* m[2] = {&bm, &sm};
+  const pybind11::handle rows[2] = {block_moves, slot_moves};
   std::vector<Group> g[2];
   std::vector<int> dst;
-  for (int i = 0; i < 2; ++i)
-    if (m[i]->size()) {
-      if (m[i]->ndim() != 2) refuse("moves as rows");
-      if (!kinds[i]) refuse("the caches have no such items");
-      kinds[i]->group(m[i]->data(), m[i]->shape(0), m[i]->shape(1), g[i], dst);
-    }
+  for (int i = 0; i < 2; ++i) {
+    if (none(rows[i])) continue;
+    const Moves m = whole(rows[i]);
+    if (m.size() == 0) continue;
+    if (m.ndim() != 2) refuse("moves as rows");
+    if (!kinds[i]) refuse("the caches have no such items");
+    kinds[i]->group(m.data(), m.shape(0), m.shape(1), g[i], dst);
+  }
   if (!g[0].empty() || !g[1].empty()) run(kinds, g, dst);
 }
 
