@@ -146,6 +146,16 @@ void allreduce_oneshot(std::vector<int64_t> peers, int64_t rank, torch::Tensor i
                        torch::Tensor scale, int64_t num_blocks, torch::Tensor status);
 void lora_bind(pybind11::module_& m);
 void cache_moves_bind(pybind11::module_& m);
+void linear_fused_bind(pybind11::module_& m);
+std::vector<torch::Tensor> moe_route(const torch::Tensor& logits, int64_t k, bool sigmoid,
+                                     const c10::optional<torch::Tensor>& bias, int64_t groups, int64_t top_groups, bool renorm,
+                                     double scale);
+std::vector<torch::Tensor> moe_plan(const torch::Tensor& ids, int64_t E, int64_t first, int64_t tile);
+void moe_gather(const torch::Tensor& x, const c10::optional<torch::Tensor>& xs, const torch::Tensor& order, int64_t k,
+                const torch::Tensor& out, const c10::optional<torch::Tensor>& out_s, const torch::Tensor& status);
+void moe_combine(const torch::Tensor& rows, const torch::Tensor& pos, const torch::Tensor& w,
+                 const c10::optional<torch::Tensor>& shared, const c10::optional<torch::Tensor>& gate, const torch::Tensor& out,
+                 const torch::Tensor& status);
 }  // namespace rad
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -209,6 +219,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "receiving half of the GEMM-fused all-reduce (+ add / RMSNorm / e4m3 quant)");
   rad::lora_bind(m);
   rad::cache_moves_bind(m);
+  rad::linear_fused_bind(m);
+  m.def("moe_route", &rad::moe_route, "experts and weights of each token from the router's logits");
+  m.def("moe_plan", &rad::moe_plan, "(token, slot) pairs sorted by expert");
+  m.def("moe_gather", &rad::moe_gather, "activations of the plan's rows");
+  m.def("moe_combine", &rad::moe_combine, "weighted sum of each token's expert rows (+ gated shared rows)");
   m.def("ipc_handle", &rad::ipc_handle, "CUDA IPC handle of a device buffer");
   m.def("ipc_open", &rad::ipc_open, "open a peer's IPC handle -> device pointer");
   m.def("ipc_close", &rad::ipc_close, "close an opened IPC mapping");

@@ -1,0 +1,617 @@
+// Mixture of experts around the experts' products (linear_fused.cu): router, sorting plan, rows by expert, weighted sum.
+//
+//   route    s = softmax(l) or sigmoid(l);  c = s + bias;  group value = the two best c of a group added up (bias), or its
+//            best c;  the best `top_groups` groups;  in them the best k of c;  w = s (/ their sum) * scale
+//   plan     rows = the (token, slot) pairs of this rank's experts, those of one expert side by side, in the pairs' order
+//   gather   row r = the activations of its token
+//   combine  out[t] = sum_j w[t, j] rows[pos[t, j]] (+ sigmoid(gate[t]) shared[t])
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <cuda_fp16.h>
+#include <torch/extension.h>
+
+#include <atomic>
+
+#include "common.cuh"
+#include "refuse.h"
+
+namespace rad {
+namespace moe {
+
+constexpr int MAX_E = 1024;
+constexpr unsigned FULL = 0xffffffffu;
+
+DEVI float to_f(float x) { return x; }
+DEVI float to_f(__nv_bfloat16 x) { return __bfloat162float(x); }
+DEVI float to_f(__half x) { return __half2float(x); }
+
+// ---------------------------------------------------------------------------------------------
+// route: one warp a token.  The lanes of a group hold its experts in order, V neighbours each, so that a lane's own best two
+// and log2(lanes) exchanges give every group's value at once, and the lowest lane among equals has the lowest index.
+// Values become whole numbers of the same order (0: no candidate, 1: NaN, then -inf and up), whose warp maximum is one
+// instruction.  Without a bias the logits themselves are ranked, which is the scores' order.  With a bias the scores enter the
+// order: they are computed in 32 bits, and once more in 64 for the few tokens (about one in 200) where two candidates, or two
+// groups, lie so near that the rounding could have turned them.
+// ---------------------------------------------------------------------------------------------
+struct RouteArgs {
+  const void* logits;
+  const float* bias;
+  int64_t* ids;
+  float* w;
+  int64_t ld;
+  int T, E, k, groups, top_groups, gsize, lanes;           // lanes of a group
+  bool sigmoid, renorm, vec;
+  float scale;
+};
+
+DEVI uint32_t key_of(float c) {
+  if (c != c) return 1u;
+  const uint32_t b = __float_as_uint(c + 0.f);             // -0 as +0
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+DEVI uint64_t key_of(double c) {
+  if (c != c) return 1ull;
+  const uint64_t b = (uint64_t)__double_as_longlong(c + 0.0);
+  return b >> 63 ? ~b : b | (1ull << 63);
+}
+DEVI uint32_t warp_max_key(uint32_t v) { return __reduce_max_sync(FULL, v); }
+DEVI uint64_t warp_max_key(uint64_t v) {
+  const uint32_t hi = __reduce_max_sync(FULL, (uint32_t)(v >> 32));
+  const uint32_t lo = __reduce_max_sync(FULL, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
+  return (uint64_t)hi << 32 | lo;
+}
+template <typename F> struct KeyOf { using T = uint32_t; };
+template <> struct KeyOf<double> { using T = uint64_t; };
+
+DEVI float exp_of(float x) { return expf(x); }
+DEVI double exp_of(double x) { return exp(x); }
+
+// Lane j < k ends with the j-th expert and its score before renormalisation.  False: 32 bits could not tell the order.
+template <typename F, int V, bool BIAS>
+DEVI bool choose(const RouteArgs& p, const float (&l)[V], int e0, int n, float top, int lane, int& expert, F& score) {
+  using Key = typename KeyOf<F>::T;
+  // errors of a 32-bit score (below 2^-21 for scores up to 1) and of its sum with the bias, with a margin
+  const F tol = sizeof(F) == 8 ? F(0) : F(1.0 / (1 << 19));
+  F total = 0;                                             // of the softmax
+  if (!p.sigmoid && (BIAS || !p.renorm)) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < n) total += exp_of((F)l[i] - (F)top);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
+  }
+  auto score_of = [&](float x) -> F {
+    if (p.sigmoid) return F(1) / (F(1) + exp_of(-(F)x));
+    const F s = exp_of((F)x - (F)top);
+    return BIAS || !p.renorm ? (total > 0 ? s / total : total) : s;
+  };
+  bool clear = true;
+  F c[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    c[i] = 0;
+    if (i < n) c[i] = BIAS ? score_of(l[i]) + (F)p.bias[e0 + i] : (F)l[i];
+  }
+  if (p.groups > 1) {
+    // the group's value at each of its lanes
+    F b1 = -INFINITY, b2 = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < n) {
+        const F lo = c[i] < b1 ? c[i] : b1;
+        b1 = c[i] > b1 ? c[i] : b1;
+        b2 = lo > b2 ? lo : b2;
+      }
+    for (int o = p.lanes >> 1; o > 0; o >>= 1) {
+      const F o1 = __shfl_xor_sync(FULL, b1, o), o2 = __shfl_xor_sync(FULL, b2, o);
+      const F lo = o1 < b1 ? o1 : b1, hi2 = o2 > b2 ? o2 : b2;
+      b1 = o1 > b1 ? o1 : b1;
+      b2 = lo > hi2 ? lo : hi2;
+    }
+    const F value = BIAS ? b1 + b2 : b1;
+    const Key key = key_of(value);
+    const int mine = lane / p.lanes;
+    int rank = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const F other = __shfl_sync(FULL, value, g * p.lanes);
+      const Key ko = key_of(other);
+      rank += ko > key || (ko == key && g < mine);
+      if (BIAS && sizeof(F) == 4 && g != mine && mine < p.groups) {
+        const F d = value > other ? value - other : other - value;
+        clear &= d > tol * (F(2) + (value < 0 ? -value : value));
+      }
+    }
+    if (rank >= p.top_groups) n = 0;
+  }
+  Key best = 0;
+  int at = 0;
+  uint32_t taken = 0;
+  auto rescan = [&]() {
+    best = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const Key q = i < n && !(taken >> i & 1) ? key_of(c[i]) : Key(0);
+      if (q > best) best = q, at = i;
+    }
+  };
+  rescan();
+  F before = 0;
+  float chosen = 0.f;                                      // the logit
+  for (int j = 0; j < p.k + (BIAS && sizeof(F) == 4 ? 1 : 0); ++j) {
+    const Key m = warp_max_key(best);
+    if (m == 0) break;                                     // the candidate behind the last one does not exist
+    const int w = __ffs(__ballot_sync(FULL, best == m)) - 1;
+    float lw = l[0];
+    F cw = c[0];
+#pragma unroll
+    for (int i = 1; i < V; ++i)
+      if (i == at) lw = l[i], cw = c[i];
+    const int ew = __shfl_sync(FULL, e0 + at, w);
+    lw = __shfl_sync(FULL, lw, w);
+    if (BIAS && sizeof(F) == 4) {
+      cw = __shfl_sync(FULL, cw, w);
+      if (j > 0) clear &= before - cw > tol * (F(1) + (cw < 0 ? -cw : cw));
+      before = cw;
+    }
+    if (lane == j && j < p.k) expert = ew, chosen = lw;
+    if (lane == w) taken |= 1u << at, rescan();
+  }
+  score = lane < p.k ? score_of(chosen) : F(0);
+  return __all_sync(FULL, clear);
+}
+
+template <typename L, int V, bool BIAS>
+__global__ void __launch_bounds__(256) route_kernel(const __grid_constant__ RouteArgs p) {
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x % 32, t = blockIdx.x * 8 + threadIdx.x / 32;
+  if (t >= p.T) return;
+  const L* row = static_cast<const L*>(p.logits) + (int64_t)t * p.ld;
+  const int v = (p.gsize + p.lanes - 1) / p.lanes, group = lane / p.lanes, first = lane % p.lanes * v;
+  const int n = group < p.groups ? max(0, min(v, p.gsize - first)) : 0, e0 = group * p.gsize + first;
+  float l[V];
+  if (p.vec && V * sizeof(L) >= 16) {                      // a lane's experts are V and start on 16 bytes
+    if constexpr (V * sizeof(L) >= 16) {
+      constexpr int Q = 16 / sizeof(L);
+#pragma unroll
+      for (int i = 0; i < V; i += Q) {
+        uint4 q = make_uint4(0, 0, 0, 0);
+        if (i < n) q = *reinterpret_cast<const uint4*>(row + e0 + i);
+        const L* x = reinterpret_cast<const L*>(&q);
+#pragma unroll
+        for (int j = 0; j < Q; ++j) l[i + j] = to_f(x[j]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) l[i] = i < n ? to_f(row[e0 + i]) : 0.f;
+  }
+  float top = -INFINITY;
+  bool nan = false;
+#pragma unroll
+  for (int i = 0; i < V; ++i)
+    if (i < n) top = fmaxf(top, l[i]), nan |= l[i] != l[i];
+  top = warp_max(top);
+  nan = __any_sync(FULL, nan || (!p.sigmoid && top == INFINITY));
+  if (top == -INFINITY) top = 0.f;                         // every expert masked: scores of zero
+  int expert = 0;
+  float s = 0.f;
+  const bool clear = choose<float, V, BIAS>(p, l, e0, n, top, lane, expert, s);
+  if constexpr (BIAS) {
+    if (!clear) {
+      double d;
+      choose<double, V, BIAS>(p, l, e0, n, top, lane, expert, d);
+      s = (float)d;
+    }
+  }
+  if (p.renorm) {
+    const float sum = warp_sum(s);
+    s = sum > 0.f ? s / sum : 0.f;
+  }
+  if (lane < p.k) {
+    p.ids[(int64_t)t * p.k + lane] = expert;
+    p.w[(int64_t)t * p.k + lane] = nan ? NAN : s * p.scale;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------
+// plan: one cluster.  Every warp owns neighbouring pairs; it counts them by expert, the counts are added up over warps and
+// CTAs (distributed shared memory), and a second pass over the pairs hands out the rows.  Equal experts of 32 pairs find one
+// another by a warp match, so nothing is atomic and the rows come in the pairs' order.
+// ---------------------------------------------------------------------------------------------
+struct PlanArgs {
+  const void* ids;
+  int R, k, E, first, seg;                                 // pairs, experts of this rank, pairs of a warp
+  bool wide;                                               // ids of 64 bits
+  int* order;
+  int* pos;
+  int* counts;
+  int* starts;
+  int* items;                                              // (expert, first row, rows) per tile of `tile` rows
+  int tile, max_items;
+};
+constexpr int PLAN_WARPS = 32;
+
+DEVI int plan_expert(const PlanArgs& p, int f, int end) {
+  if (f >= end) return -1;
+  const int64_t e = (p.wide ? static_cast<const int64_t*>(p.ids)[f] : (int64_t) static_cast<const int*>(p.ids)[f]) - p.first;
+  return e >= 0 && e < p.E ? (int)e : -1;
+}
+
+// exclusive sums of v over the block's threads (1024); total: of all
+DEVI int block_scan(int v, int* warp_sums, int& total) {
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(FULL, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) warp_sums[warp] = x;
+  __syncthreads();
+  int s = warp_sums[lane], before = lane < warp ? s : 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(FULL, s, o);
+    before += __shfl_xor_sync(FULL, before, o);
+  }
+  total = s;
+  __syncthreads();
+  return x - v + before;
+}
+
+__global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ PlanArgs p) {
+  extern __shared__ int smem[];
+  int* cnt = smem;                                         // [warps][E]
+  int* tot = cnt + PLAN_WARPS * p.E;                       // [E] of this CTA
+  int* base = tot + p.E;                                   // [E] first row of this CTA's pairs
+  __shared__ int warp_sums[32];
+  const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  const uint32_t rank = cluster_ctarank();
+  const int ctas = gridDim.x;
+  pdl_trigger();
+  for (int i = threadIdx.x; i < PLAN_WARPS * p.E; i += blockDim.x) cnt[i] = 0;
+  __syncthreads();
+  pdl_wait();
+  int* mine = cnt + warp * p.E;
+  const int64_t f0 = ((int64_t)rank * PLAN_WARPS + warp) * p.seg;
+  const int lo = (int)min(f0, (int64_t)p.R), hi = (int)min(f0 + p.seg, (int64_t)p.R);
+  for (int f = lo + lane; f - lane < hi; f += 32) {
+    const int e = plan_expert(p, f, hi);
+    const unsigned same = __match_any_sync(FULL, e);
+    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  const int e = threadIdx.x;
+  int sum = 0;
+  if (e < p.E) {
+#pragma unroll 8
+    for (int w = 0; w < PLAN_WARPS; ++w) {
+      const int n = cnt[w * p.E + e];
+      cnt[w * p.E + e] = sum;
+      sum += n;
+    }
+    tot[e] = sum;
+  }
+  int all = sum, before = 0;
+  if (ctas > 1) {
+    cluster_sync();
+    if (e < p.E) {
+      all = 0;
+      const uint32_t at = smem_u32(tot + e);
+      for (int c = 0; c < ctas; ++c) {
+        int n;
+        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(n) : "r"(mapa_shared(at, c)));
+        if (c < (int)rank) before += n;
+        all += n;
+      }
+    }
+    cluster_arrive();                                      // the others may leave once this CTA has read their counts
+  }
+  int rows;
+  const int start = block_scan(all, warp_sums, rows);
+  if (e < p.E) {
+    base[e] = start + before;
+    if (rank == 0) p.counts[e] = all, p.starts[e] = start;
+  }
+  if (rank == 0 && threadIdx.x == 0) p.starts[p.E] = rows;
+  if (p.items && rank == 0) {
+    int tiles;
+    const int n = e < p.E ? (all + p.tile - 1) / p.tile : 0, i0 = block_scan(n, warp_sums, tiles);
+    for (int i = 0; i < n && i0 + i < p.max_items; ++i) {
+      int* q = p.items + 3 * (int64_t)(i0 + i);
+      q[0] = e;
+      q[1] = start + i * p.tile;
+      q[2] = min(p.tile, all - i * p.tile);
+    }
+    for (int i = tiles + threadIdx.x; i < p.max_items; i += blockDim.x)
+      p.items[3 * (int64_t)i] = p.items[3 * (int64_t)i + 1] = p.items[3 * (int64_t)i + 2] = 0;
+  }
+  __syncthreads();
+  for (int f = lo + lane; f - lane < hi; f += 32) {
+    const int x = plan_expert(p, f, hi);
+    const unsigned same = __match_any_sync(FULL, x);
+    int row = -1;
+    if (x >= 0) row = base[x] + mine[x] + __popc(same & ((1u << lane) - 1));
+    __syncwarp();
+    if (x >= 0 && lane == __ffs(same) - 1) mine[x] += __popc(same);
+    __syncwarp();
+    if (f < hi) {
+      p.pos[f] = row;
+      if (row >= 0) p.order[row] = f;
+    }
+  }
+  for (int r = rows + rank * blockDim.x + threadIdx.x; r < p.R; r += ctas * blockDim.x) p.order[r] = -1;
+  if (ctas > 1) cluster_wait();
+}
+
+// ---------------------------------------------------------------------------------------------
+// gather, combine: bound by memory, 16 bytes a thread
+// ---------------------------------------------------------------------------------------------
+// rows of `vecs` 16-byte pieces; x [T] -> out [R], a pair's row is its token's.  scale: fp32 beside each row, or null
+__global__ void __launch_bounds__(256) gather_kernel(const uint4* x, int64_t ld, const float* xs, const int* order, uint4* out,
+                                                     float* os, int R, int T, int k, unsigned vecs, int* status) {
+  pdl_trigger();
+  pdl_wait();
+  const unsigned i = blockIdx.x * 256 + threadIdx.x;
+  const int r = i / vecs, v = i % vecs;
+  if (r >= R) return;
+  const int f = order[r];
+  if (f < 0) return;
+  const int t = f / k;
+  if (t >= T) {
+    atomicExch(status, (int)kErrBounds);
+    return;
+  }
+  out[(int64_t)r * vecs + v] = x[t * ld + v];
+  if (os && v == 0) os[r] = xs[t];
+}
+
+struct CombineArgs {
+  const __nv_bfloat16* rows;
+  const int* pos;
+  const float* w;
+  const __nv_bfloat16* shared;
+  const float* gate;
+  __nv_bfloat16* out;
+  int64_t ld_rows, ld_shared, ld_gate, ld_out;
+  int T, k, H, R;
+  int* status;
+};
+
+// One thread: W neighbouring columns of a token.  The rows of K slots are asked for before the first is added.
+template <int W>
+__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ CombineArgs p) {
+  pdl_trigger();
+  pdl_wait();
+  constexpr int K = 8;
+  const unsigned vecs = (p.H + W - 1) / W;
+  const unsigned i = blockIdx.x * 256 + threadIdx.x;
+  const int t = i / vecs, c = i % vecs * W;
+  if (t >= p.T) return;
+  using Vec = typename std::conditional<W == 8, uint4, uint16_t>::type;
+  float acc[W];
+#pragma unroll
+  for (int q = 0; q < W; ++q) acc[q] = 0.f;
+  auto add = [&](const Vec& v, float w) {
+    const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(&v);
+#pragma unroll
+    for (int q = 0; q < W; ++q) acc[q] = fmaf(w, __bfloat162float(x[q]), acc[q]);
+  };
+  Vec sh;
+  float g = 0.f;
+  if (p.shared) {
+    sh = *reinterpret_cast<const Vec*>(p.shared + t * p.ld_shared + c);
+    g = p.gate ? 1.f / (1.f + __expf(-p.gate[t * p.ld_gate])) : 1.f;
+  }
+  for (int j0 = 0; j0 < p.k; j0 += K) {
+    Vec v[K];
+    float w[K];
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      int r = -1;
+      w[j] = 0.f;
+      if (j0 + j < p.k) {
+        r = p.pos[(int64_t)t * p.k + j0 + j];
+        w[j] = p.w[(int64_t)t * p.k + j0 + j];
+        if (r >= p.R) {
+          atomicExch(p.status, (int)kErrBounds);
+          r = -1;
+        }
+      }
+      v[j] = Vec{};
+      if (r >= 0) v[j] = *reinterpret_cast<const Vec*>(p.rows + r * p.ld_rows + c);
+      else w[j] = 0.f;                                     // another rank's expert, or none
+    }
+#pragma unroll
+    for (int j = 0; j < K; ++j) add(v[j], w[j]);
+  }
+  if (p.shared) add(sh, g);
+  Vec o;
+  __nv_bfloat16* x = reinterpret_cast<__nv_bfloat16*>(&o);
+#pragma unroll
+  for (int q = 0; q < W; ++q) x[q] = __float2bfloat16_rn(acc[q]);
+  *reinterpret_cast<Vec*>(p.out + t * p.ld_out + c) = o;
+}
+
+// ---------------------------------------------------------------------------------------------
+// launches
+// ---------------------------------------------------------------------------------------------
+template <typename L, int V>
+void launch_route(const RouteArgs& p, cudaStream_t stream) {
+  const dim3 grid((p.T + 7) / 8);
+  if (p.bias) C10_CUDA_CHECK(launch_pdl(route_kernel<L, V, true>, grid, dim3(256), 0, stream, p));
+  else C10_CUDA_CHECK(launch_pdl(route_kernel<L, V, false>, grid, dim3(256), 0, stream, p));
+}
+template <typename L>
+void launch_route(RouteArgs& p, cudaStream_t stream) {
+  const int v = (p.gsize + p.lanes - 1) / p.lanes;
+  const int V = v <= 2 ? 2 : v <= 4 ? 4 : v <= 8 ? 8 : v <= 16 ? 16 : 32;
+  // 16-byte loads where every lane's experts are whole pieces of 16 bytes
+  p.vec = v == V && p.gsize % v == 0 && V * sizeof(L) >= 16 && (uintptr_t)p.logits % 16 == 0 && p.ld * sizeof(L) % 16 == 0;
+  switch (V) {
+    case 2: launch_route<L, 2>(p, stream); break;
+    case 4: launch_route<L, 4>(p, stream); break;
+    case 8: launch_route<L, 8>(p, stream); break;
+    case 16: launch_route<L, 16>(p, stream); break;
+    default: launch_route<L, 32>(p, stream);
+  }
+}
+
+}  // namespace moe
+
+std::vector<torch::Tensor> moe_route(const torch::Tensor& logits, int64_t k, bool sigmoid,
+                                     const c10::optional<torch::Tensor>& bias, int64_t groups, int64_t top_groups, bool renorm,
+                                     double scale) {
+  const auto type = logits.scalar_type();
+  RAD_CHECK_VALUE(logits.is_cuda() && logits.dim() == 2 && (logits.size(0) <= 1 || logits.stride(0) >= logits.size(1)) &&
+                        (logits.size(1) <= 1 || logits.stride(1) == 1),
+                    "moe_route: logits [T, E], rows contiguous");
+  RAD_CHECK_VALUE(type == at::kFloat || type == at::kBFloat16 || type == at::kHalf, "moe_route: logits fp32, bf16 or fp16");
+  const int64_t T = logits.size(0), E = logits.size(1);
+  RAD_CHECK_VALUE(E >= 1 && E <= moe::MAX_E, "moe_route: 1 to ", moe::MAX_E, " experts, got ", E);
+  RAD_CHECK_VALUE(k >= 1 && k <= 32 && k <= E, "moe_route: top_k ", k, " of ", E, " experts (at most 32)");
+  RAD_CHECK_VALUE(groups >= 1 && groups <= 32 && E % groups == 0, "moe_route: ", groups, " groups of ", E, " experts");
+  RAD_CHECK_VALUE(top_groups >= 1 && top_groups <= groups && top_groups * (E / groups) >= k, "moe_route: ", k, " experts in ",
+                    top_groups, " of ", groups, " groups");
+  RAD_CHECK_VALUE(T < (1ll << 31) - 8, "moe_route: rows");
+  if (bias.has_value()) {
+    RAD_CHECK_VALUE(bias->device() == logits.device() && bias->scalar_type() == at::kFloat && bias->dim() == 1 &&
+                          bias->size(0) == E && bias->is_contiguous(),
+                      "moe_route: bias fp32 [E] on the logits' device");
+    RAD_CHECK_VALUE(groups == 1 || E / groups >= 2, "moe_route: a group's value is that of two experts");
+  }
+  moe::RouteArgs p = {};
+  int lanes = 32;
+  while (lanes * groups > 32) lanes /= 2;
+  RAD_CHECK_VALUE((E / groups + lanes - 1) / lanes <= 32, "moe_route: ", E, " experts in ", groups, " groups are too many");
+  const at::cuda::CUDAGuard guard(logits.device());
+  torch::Tensor ids = torch::empty({T, k}, logits.options().dtype(at::kLong));
+  torch::Tensor w = torch::empty({T, k}, logits.options().dtype(at::kFloat));
+  if (T == 0) return {ids, w};
+  p.logits = logits.data_ptr();
+  p.bias = bias.has_value() ? bias->data_ptr<float>() : nullptr;
+  p.ids = ids.data_ptr<int64_t>();
+  p.w = w.data_ptr<float>();
+  p.ld = T == 1 ? (E + 15) / 16 * 16 : logits.stride(0);
+  p.T = T; p.E = E; p.k = k; p.groups = groups; p.top_groups = top_groups; p.gsize = E / groups; p.lanes = lanes;
+  p.sigmoid = sigmoid; p.renorm = renorm; p.scale = (float)scale;
+  auto stream = at::cuda::getCurrentCUDAStream();
+  if (type == at::kFloat) moe::launch_route<float>(p, stream);
+  else if (type == at::kBFloat16) moe::launch_route<__nv_bfloat16>(p, stream);
+  else moe::launch_route<__half>(p, stream);
+  return {ids, w};
+}
+
+// -> order [T k], pos [T, k], counts [E], starts [E + 1], items [max_items, 3] (empty without a tile height)
+std::vector<torch::Tensor> moe_plan(const torch::Tensor& ids_, int64_t E, int64_t first, int64_t tile) {
+  const auto type = ids_.scalar_type();
+  RAD_CHECK_VALUE(ids_.is_cuda() && ids_.dim() == 2 && (type == at::kLong || type == at::kInt),
+                    "moe_plan: ids [T, k], int64 or int32");
+  RAD_CHECK_VALUE(E >= 1 && E <= moe::MAX_E, "moe_plan: 1 to ", moe::MAX_E, " experts, got ", E);
+  RAD_CHECK_VALUE(first >= 0 && first < (1ll << 30) && tile >= 0 && tile <= (1 << 20), "moe_plan: first expert, tile height");
+  const int64_t T = ids_.size(0), k = ids_.size(1), R = T * k;
+  RAD_CHECK_VALUE(k >= 1 && R < (1ll << 30), "moe_plan: 1 to 2^30 pairs");
+  const at::cuda::CUDAGuard guard(ids_.device());
+  const torch::Tensor ids = ids_.contiguous();
+  const auto opt = ids.options().dtype(at::kInt);
+  // order and pos, counts and starts come out of one allocation each: they live and die together
+  torch::Tensor both = torch::empty({2, R}, opt), few = torch::empty({2 * E + 1}, opt);
+  torch::Tensor order = both[0], pos = both[1].view({T, k}), counts = few.narrow(0, 0, E), starts = few.narrow(0, E, E + 1);
+  const int64_t max_items = tile ? (R + tile - 1) / tile + E : 0;
+  torch::Tensor items = torch::empty({max_items, 3}, opt);
+  moe::PlanArgs p = {};
+  p.ids = ids.data_ptr(); p.R = R; p.k = k; p.E = E; p.first = first; p.wide = type == at::kLong;
+  p.order = order.data_ptr<int>(); p.pos = pos.data_ptr<int>();
+  p.counts = counts.data_ptr<int>(); p.starts = starts.data_ptr<int>();
+  p.items = tile ? items.data_ptr<int>() : nullptr; p.tile = tile; p.max_items = max_items;
+  int ctas = 1;
+  while (ctas < 8 && R > 4096ll * ctas) ctas *= 2;
+  p.seg = ((R + 32 * ctas - 1) / (32 * ctas) + 31) / 32 * 32;
+  const size_t smem = (moe::PLAN_WARPS + 2) * E * sizeof(int);
+  static std::atomic<uint64_t> set{0};                     // devices whose kernel may take the shared memory of MAX_E experts
+  const int dev = ids.get_device();
+  if (smem > 48 * 1024 && (dev >= 64 || !(set.load() >> dev & 1))) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(moe::plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        (int)((moe::PLAN_WARPS + 2) * moe::MAX_E * sizeof(int))));
+    if (dev < 64) set.fetch_or(1ull << dev);
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(1024);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = at::cuda::getCurrentCUDAStream();
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim = {(unsigned)ctas, 1, 1};
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = pdl_enabled() ? 2 : 1;
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, moe::plan_kernel, p));
+  return {order, pos, counts, starts, items};
+}
+
+void moe_gather(const torch::Tensor& x, const c10::optional<torch::Tensor>& xs, const torch::Tensor& order, int64_t k,
+                const torch::Tensor& out, const c10::optional<torch::Tensor>& out_s, const torch::Tensor& status) {
+  const int64_t T = x.size(0), R = order.size(0), bytes = x.size(1) * x.element_size();
+  RAD_CHECK_VALUE(x.is_cuda() && x.dim() == 2 && x.stride(1) == 1 && bytes % 16 == 0 && (uintptr_t)x.data_ptr() % 16 == 0 &&
+                        (T <= 1 || x.stride(0) * x.element_size() % 16 == 0) && order.device() == x.device(),
+                    "moe_gather: rows of whole 16 bytes");
+  RAD_CHECK_VALUE(R == T * k && out.is_contiguous() && out.size(0) == R && out.size(1) == x.size(1), "moe_gather: rows");
+  RAD_CHECK_VALUE(!xs.has_value() || (xs->device() == x.device() && xs->scalar_type() == at::kFloat && xs->is_contiguous() &&
+                                        xs->numel() == T && out_s->numel() == R),
+                    "moe_gather: scales fp32 [T]");
+  if (R == 0 || bytes == 0) return;
+  const at::cuda::CUDAGuard guard(x.device());
+  const unsigned vecs = bytes / 16;
+  RAD_CHECK_VALUE(R * vecs < (1ll << 31), "moe_gather: rows");
+  C10_CUDA_CHECK(launch_pdl(moe::gather_kernel, dim3((R * vecs + 255) / 256), dim3(256), 0, at::cuda::getCurrentCUDAStream(),
+                            (const uint4*)x.data_ptr(), (int64_t)(x.stride(0) * x.element_size() / 16),
+                            xs.has_value() ? (const float*)xs->data_ptr<float>() : nullptr, (const int*)order.data_ptr<int>(),
+                            (uint4*)out.data_ptr(), xs.has_value() ? out_s->data_ptr<float>() : nullptr, (int)R, (int)T, (int)k,
+                            vecs, status.data_ptr<int>()));
+}
+
+void moe_combine(const torch::Tensor& rows, const torch::Tensor& pos, const torch::Tensor& w,
+                 const c10::optional<torch::Tensor>& shared, const c10::optional<torch::Tensor>& gate, const torch::Tensor& out,
+                 const torch::Tensor& status) {
+  const int64_t T = pos.size(0), k = pos.size(1), H = rows.size(1), R = rows.size(0);
+  const auto bf16_rows = [&](const torch::Tensor& t, int64_t n) {
+    return t.dim() == 2 && t.size(0) == n && t.size(1) == H && (H <= 1 || t.stride(1) == 1) && t.scalar_type() == at::kBFloat16 &&
+           t.device() == rows.device();
+  };
+  RAD_CHECK_VALUE(rows.is_cuda() && bf16_rows(rows, R) && R == T * k, "moe_combine: rows bf16 [T k, H]");
+  RAD_CHECK_VALUE(w.device() == rows.device() && w.scalar_type() == at::kFloat && w.is_contiguous() && w.dim() == 2 &&
+                        w.size(0) == T && w.size(1) == k,
+                    "moe_combine: weights fp32 [T, k]");
+  RAD_CHECK_VALUE(pos.device() == rows.device(), "moe_combine: operands on one device");
+  RAD_CHECK_VALUE(!shared.has_value() || bf16_rows(*shared, T), "moe_combine: shared bf16 [T, H]");
+  RAD_CHECK_VALUE(!gate.has_value() || (shared.has_value() && gate->device() == rows.device() &&
+                                          gate->scalar_type() == at::kFloat && gate->dim() == 1 && gate->size(0) == T),
+                    "moe_combine: gate fp32 [T], beside shared");
+  RAD_CHECK_VALUE(bf16_rows(out, T) && (T <= 1 || out.stride(0) >= H), "moe_combine: out bf16 [T, H]");
+  if (T == 0 || H == 0) return;
+  moe::CombineArgs p = {};
+  p.rows = (const __nv_bfloat16*)rows.data_ptr();
+  p.pos = pos.data_ptr<int>();
+  p.w = w.data_ptr<float>();
+  p.shared = shared.has_value() ? (const __nv_bfloat16*)shared->data_ptr() : nullptr;
+  p.gate = gate.has_value() ? gate->data_ptr<float>() : nullptr;
+  p.out = (__nv_bfloat16*)out.data_ptr();
+  p.ld_rows = rows.stride(0); p.ld_shared = shared.has_value() ? shared->stride(0) : 0;
+  p.ld_gate = gate.has_value() ? gate->stride(0) : 0; p.ld_out = out.stride(0);
+  p.T = T; p.k = k; p.H = H; p.R = R;
+  p.status = status.data_ptr<int>();
+  const at::cuda::CUDAGuard guard(rows.device());
+  const bool vec = H % 8 == 0 && (p.ld_rows | p.ld_shared | p.ld_out) % 8 == 0 &&
+                   ((uintptr_t)p.rows | (uintptr_t)p.shared | (uintptr_t)p.out) % 16 == 0;
+  const int64_t blocks = (T * (vec ? H / 8 : H) + 255) / 256;
+  RAD_CHECK_VALUE(blocks < (1ll << 23), "moe_combine: rows");
+  auto stream = at::cuda::getCurrentCUDAStream();
+  if (vec) C10_CUDA_CHECK(launch_pdl(moe::combine_kernel<8>, dim3(blocks), dim3(256), 0, stream, p));
+  else C10_CUDA_CHECK(launch_pdl(moe::combine_kernel<1>, dim3(blocks), dim3(256), 0, stream, p));
+}
+
+}  // namespace rad

@@ -230,3 +230,30 @@ class Linear:
             out.copy_(y)
             return out
         return y
+
+
+class LinearBank:
+    """bf16 weights of ``ops.kernels.linear_fused``: weight [N, K], or [E, N, K] of E experts (at most 1024), contiguous, with K a
+    multiple of 8; bias [N] / [E, N] bf16; act "none", or "swiglu" for rows [gate | up] (N even, output N / 2).  The weights
+    are used where they are, not copied."""
+
+    def __init__(self, weight: torch.Tensor, bias: Optional[torch.Tensor] = None, act: str = "none"):
+        if act not in ("none", "swiglu"):
+            raise ValueError(f"LinearBank: act none or swiglu, got {act!r}")
+        if weight.dim() == 2:
+            weight = weight[None]
+            bias = None if bias is None else bias[None]
+        if weight.dim() != 3 or weight.dtype != torch.bfloat16 or not weight.is_contiguous() or weight.numel() == 0:
+            raise ValueError("LinearBank: weight bf16 [N, K] or [E, N, K], contiguous")
+        self.E, self.N, self.K = weight.shape
+        if self.E > 1024 or self.K % 8 or (act == "swiglu" and self.N % 2):
+            raise ValueError("LinearBank: at most 1024 experts, K a multiple of 8, swiglu rows [gate | up]")
+        if bias is not None and (bias.shape != (self.E, self.N) or bias.dtype != torch.bfloat16
+                                 or bias.device != weight.device or not bias.is_contiguous()):
+            raise ValueError("LinearBank: bias bf16 [N] or [E, N], beside the weight")
+        self.weight, self.bias, self.act = weight, bias, act
+        self.width = self.N // 2 if act == "swiglu" else self.N
+        self.handle = None
+        if weight.is_cuda:
+            from ..ops._ext import ext
+            self.handle = ext().LinearBank(weight, bias, act == "swiglu", K.status_word(weight.device))

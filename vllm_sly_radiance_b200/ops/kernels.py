@@ -355,6 +355,138 @@ def moe_grouped_mlp(q, s, counts, w_gate_up, w_down, I: int, H: int) -> torch.Te
 
 
 # ---------------------------------------------------------------------------------------------
+# mixture of experts
+# ---------------------------------------------------------------------------------------------
+def moe_route(logits: torch.Tensor, top_k: int, score: str = "softmax", bias: Optional[torch.Tensor] = None,
+              groups: int = 1, top_groups: int = 1, renormalize: bool = True, scale: float = 1.0):
+    """Experts of each token from the router's logits [T, E] (fp32, bf16 or fp16) -> (ids [T, k] int64, best first,
+    weights [T, k] fp32).
+
+    Scores are the logits' softmax or sigmoid.  Experts are ranked by score + ``bias`` [E] (fp32, for balance), ties go to the
+    lowest index, and only experts of the ``top_groups`` best of ``groups`` equal groups count; a group's value is its best
+    expert's, with a bias that of its best two added up.  Weights are the chosen scores without the bias, divided by their sum
+    if ``renormalize``, times ``scale``.  A logit of -inf masks its expert: it is chosen only when no other is left, with
+    weight 0 (softmax) -- so do all weights of a row that is masked throughout.  A NaN among a row's logits (or +inf under a
+    softmax) makes its weights NaN; its ids stay distinct and in range."""
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(f"moe_route: score softmax or sigmoid, got {score!r}")
+    if logits.is_cuda:
+        return tuple(ext().moe_route(logits, top_k, score == "sigmoid", bias, groups, top_groups, renormalize, scale))
+    if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise ValueError("moe_route: logits [T, E], fp32, bf16 or fp16")
+    E = logits.shape[1]
+    if not 1 <= top_k <= min(32, E):
+        raise ValueError(f"moe_route: top_k {top_k} of {E} experts (at most 32)")
+    if groups < 1 or groups > 32 or E % groups or not 1 <= top_groups <= groups or top_groups * (E // groups) < top_k:
+        raise ValueError(f"moe_route: {top_k} experts in {top_groups} of {groups} groups of {E} experts")
+    if bias is not None and (bias.shape != (E,) or bias.dtype != torch.float32 or (groups > 1 and E // groups < 2)):
+        raise ValueError("moe_route: bias fp32 [E], groups of two experts or more")
+    return ref.moe_route(logits, top_k, score, bias, groups, top_groups, renormalize, scale)
+
+
+class MoEPlan:
+    """The (token, slot) pairs of a step's ``ids`` [T, k] sorted by expert: row r belongs to pair ``order[r]`` = t k + slot,
+    the pair's row is ``pos[t, slot]``; expert e has ``counts[e]`` rows from ``starts[e]`` on.  Pairs of other experts have
+    row -1, and the rows behind the last one are -1 in ``order``.  ``items``: (expert, first row, rows) per tile of ``tile``
+    rows, as the block-scaled grouped product takes them (empty tiles at the end)."""
+
+    def __init__(self, top_k, order, pos, counts, starts, items=None, tile=0):
+        self.top_k, self.order, self.pos, self.counts, self.starts = top_k, order, pos, counts, starts
+        self.items, self.tile = items, tile
+
+
+def moe_plan(ids: torch.Tensor, num_experts: int, first: int = 0, tile: int = 0) -> MoEPlan:
+    """Sort the pairs of ``ids`` [T, k] (int64 or int32) by expert, for the experts first .. first + num_experts - 1; rows of one
+    expert keep the pairs' order.  Other ids (another rank's, -1 for none) get no row.  tile > 0: work items too."""
+    if ids.is_cuda:
+        order, pos, counts, starts, items = ext().moe_plan(ids, num_experts, first, tile)
+        return MoEPlan(ids.shape[1], order, pos, counts, starts, items if tile else None, tile)
+    if ids.dim() != 2 or ids.dtype not in (torch.int64, torch.int32) or ids.shape[1] < 1:
+        raise ValueError("moe_plan: ids [T, k], int64 or int32")
+    if not 1 <= num_experts <= 1024 or first < 0 or tile < 0:
+        raise ValueError(f"moe_plan: 1 to 1024 experts from 0 on, got {num_experts} from {first}")
+    order, pos, counts, starts = ref.moe_plan(ids, num_experts, first)
+    items = None
+    if tile:
+        items = moe_work_items(counts.long(), tile, (ids.numel() + tile - 1) // tile + num_experts)
+    return MoEPlan(ids.shape[1], order, pos, counts, starts, items, tile)
+
+
+def moe_gather(x, plan: MoEPlan):
+    """Activations of the plan's rows: x [T, K] bf16 -> [T k, K], or an (e4m3, scale) pair -> a pair.  Rows behind the plan's
+    last one are left as the allocation has them."""
+    xq, xs = x if isinstance(x, tuple) else (x, None)
+    if xq.dim() != 2 or xq.shape[0] != plan.pos.shape[0]:
+        raise ValueError(f"moe_gather: x {tuple(xq.shape)} and a plan of {plan.pos.shape[0]} tokens")
+    if not xq.is_cuda:
+        t = plan.order.long().clamp(min=0) // plan.top_k
+        return (xq[t], xs[t]) if xs is not None else xq[t]
+    out = torch.empty(plan.order.numel(), xq.shape[1], dtype=xq.dtype, device=xq.device)
+    os_ = torch.empty(plan.order.numel(), dtype=torch.float32, device=xq.device) if xs is not None else None
+    ext().moe_gather(xq, xs, plan.order, plan.top_k, out, os_, status_word(xq.device))
+    return (out, os_) if xs is not None else out
+
+
+def moe_combine(rows: torch.Tensor, plan: MoEPlan, weights: torch.Tensor, shared: Optional[torch.Tensor] = None,
+                gate: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[t] = sum over slots of weights[t, j] * rows[pos[t, j]], slot by slot in 32 bits, rounded once to bf16; pairs without
+    a row add nothing.  rows [T k, H] bf16, weights [T, k] fp32.  shared [T, H] bf16 is added, times sigmoid(gate[t]) when
+    gate [T] fp32 is given."""
+    if rows.is_cuda:
+        out = torch.empty(plan.pos.shape[0], rows.shape[-1], dtype=torch.bfloat16, device=rows.device)
+        ext().moe_combine(rows, plan.pos, weights, shared, gate, out, status_word(rows.device))
+        return out
+    T, k = plan.pos.shape
+    if rows.dim() != 2 or rows.shape[0] != T * k or rows.dtype != torch.bfloat16:
+        raise ValueError("moe_combine: rows bf16 [T k, H]")
+    if weights.shape != (T, k) or weights.dtype != torch.float32:
+        raise ValueError("moe_combine: weights fp32 [T, k]")
+    if shared is not None and (shared.shape != (T, rows.shape[1]) or shared.dtype != torch.bfloat16):
+        raise ValueError("moe_combine: shared bf16 [T, H]")
+    if gate is not None and (shared is None or gate.shape != (T,) or gate.dtype != torch.float32):
+        raise ValueError("moe_combine: gate fp32 [T], beside shared")
+    return ref.moe_combine(rows, plan.pos, weights, shared, gate)
+
+
+def linear_fused(x: torch.Tensor, bank, plan: Optional[MoEPlan] = None, by_token: bool = False,
+                 scale: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[r] = residual[r] + scale[r] * act(x[row(r)] W^T + b) with W, b and act of ``bank`` (models/layers.LinearBank), summed
+    in 32 bits and rounded once to bf16.
+
+    Without a plan the bank has one weight and x [R, K] bf16 its rows.  With a plan (``moe_plan``) each row takes its expert's
+    weight; x holds the plan's rows in order or, ``by_token``, one row per token.  Rows of out [R, width] behind the plan's
+    last one are left as they were.  scale [R] fp32, residual [R, width] bf16; out may be residual (in place)."""
+    if x.is_cuda:
+        if bank.handle is None:
+            raise ValueError("linear_fused: operands on one device")
+        return ext().linear_fused(x, bank.handle, None if plan is None else plan.order, None if plan is None else plan.starts,
+                                  1 if plan is None else plan.top_k, by_token, scale, residual, out)
+    if x.dim() != 2 or x.shape[1] != bank.K or x.dtype != torch.bfloat16:
+        raise ValueError("linear_fused: x bf16 [rows, K]")
+    if plan is None and (bank.E != 1 or by_token):
+        raise ValueError("linear_fused: the weights of several experts, or rows by token, need a plan")
+    R = x.shape[0]
+    if plan is not None:
+        if plan.starts.numel() != bank.E + 1:
+            raise ValueError("linear_fused: a plan of as many experts as weights")
+        R = plan.order.numel()
+        if x.shape[0] != (R // plan.top_k if by_token else R):
+            raise ValueError("linear_fused: one row of x per token, or per row, of the plan")
+    if scale is not None and (scale.shape != (R,) or scale.dtype != torch.float32):
+        raise ValueError("linear_fused: scale fp32 [rows]")
+    for t in (residual, out):
+        if t is not None and (t.shape != (R, bank.width) or t.dtype != torch.bfloat16):
+            raise ValueError("linear_fused: residual and out bf16, of the output's shape")
+    y = ref.linear_fused(x, bank.weight, bank.bias, bank.act == "swiglu", plan, by_token, scale, residual)
+    if out is None:
+        return y
+    n = R if plan is None else int(plan.starts[-1])
+    out[:n] = y[:n]
+    return out
+
+
+# ---------------------------------------------------------------------------------------------
 # adapters
 # ---------------------------------------------------------------------------------------------
 def lora_add(y: torch.Tensor, x, bank, plan, out: Optional[torch.Tensor] = None) -> torch.Tensor:

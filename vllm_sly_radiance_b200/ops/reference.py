@@ -332,3 +332,82 @@ def lora_add(y, x, bank, slots) -> torch.Tensor:
             v = xf[rows] @ bank.a[l, s, :r].float().t()
             out[rows, n0:n1] += float(bank.scale[l]) * (v @ bank.b[l, n0:n1, :r].float().t())
     return out.to(torch.bfloat16)
+
+
+# ---------------------------------------------------------------------------------------------
+# mixture of experts
+# ---------------------------------------------------------------------------------------------
+def moe_route(logits, top_k, score, bias, groups, top_groups, renormalize, scale):
+    """Experts and weights of each token; the choice is made in 64 bits, ties go to the lowest index."""
+    l = logits.double()
+    top = l.amax(-1, keepdim=True)
+    if score == "softmax":
+        e = torch.exp(l - torch.where(top == -torch.inf, 0.0, top))
+        s = torch.where(e == 0, 0.0, e / e.sum(-1, keepdim=True))
+    else:
+        s = torch.sigmoid(l)
+    c = l if bias is None else s + bias.double()       # without a bias the logits rank as the scores do
+    c = torch.where(c.isnan(), -torch.inf, c)
+    if groups > 1:
+        g = c.unflatten(-1, (groups, -1))
+        value = g.amax(-1) if bias is None else g.topk(2, dim=-1).values.sum(-1)
+        best = torch.sort(value, dim=-1, descending=True, stable=True).indices[:, :top_groups]
+        keep = torch.zeros_like(value, dtype=torch.bool).scatter_(-1, best, True)
+        # other groups' experts rank behind a kept group's, whatever those hold
+        order = torch.sort(c, dim=-1, descending=True, stable=True).indices
+        kept = torch.gather(keep.repeat_interleave(g.shape[-1], -1), -1, order)
+        ids = torch.gather(order, -1, torch.sort(~kept, dim=-1, stable=True).indices[:, :top_k])
+    else:
+        ids = torch.sort(c, dim=-1, descending=True, stable=True).indices[:, :top_k]
+    w = torch.gather(s, -1, ids)
+    if renormalize:
+        w = torch.where(w == 0, 0.0, w / w.sum(-1, keepdim=True))
+    bad = l.isnan().any(-1, keepdim=True)
+    if score == "softmax":
+        bad = bad | (top == torch.inf)
+    return ids, torch.where(bad, torch.nan, w * scale).float()
+
+
+def moe_plan(ids, num_experts, first):
+    """-> order, pos, counts, starts (int32) of ops.kernels.MoEPlan."""
+    flat = ids.reshape(-1).long() - first
+    own = (flat >= 0) & (flat < num_experts)
+    key = torch.where(own, flat, num_experts)
+    order = torch.argsort(key, stable=True)
+    counts = torch.bincount(key, minlength=num_experts + 1)[:num_experts]
+    row = torch.empty_like(order)
+    row[order] = torch.arange(order.numel(), device=order.device)
+    starts = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
+    return (torch.where(own[order], order, -1).int(), torch.where(own, row, -1).view(ids.shape).int(), counts.int(),
+            starts.int())
+
+
+def linear_fused(x, weight, bias, swiglu, plan, by_token, scale, residual):
+    """act(x W^T + b) per expert, times scale, plus residual, in fp32, rounded once; rows of no expert are zero."""
+    xf = x.float()
+    R = plan.order.numel() if plan is not None else x.shape[0]
+    N = weight.shape[1]
+    out = torch.zeros(R, N // 2 if swiglu else N, device=x.device)
+    starts = plan.starts.tolist() if plan is not None else [0, R]
+    for e, (a, b) in enumerate(zip(starts, starts[1:])):
+        if a == b:
+            continue
+        y = (xf[plan.order[a:b].long() // plan.top_k] if by_token else xf[a:b]) @ weight[e].float().t()
+        if bias is not None:
+            y = y + bias[e].float()
+        out[a:b] = F.silu(y[:, :N // 2]) * y[:, N // 2:] if swiglu else y
+    if scale is not None:
+        out = out * scale[:, None]
+    if residual is not None:
+        out = out + residual.float()
+    return out.to(torch.bfloat16)
+
+
+def moe_combine(rows, pos, weights, shared, gate):
+    out = torch.zeros(pos.shape[0], rows.shape[1], device=rows.device)
+    for j in range(pos.shape[1]):
+        p = pos[:, j].long()
+        out += torch.where(p[:, None] >= 0, weights[:, j, None] * rows[p.clamp(min=0)].float(), 0.0)
+    if shared is not None:
+        out += shared.float() if gate is None else torch.sigmoid(gate.float())[:, None] * shared.float()
+    return out.to(torch.bfloat16)
