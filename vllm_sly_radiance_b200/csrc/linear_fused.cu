@@ -23,70 +23,117 @@
 namespace rad {
 namespace lf {
 
-constexpr int BM = 128, BK = 64, THREADS = 192;
+constexpr int BM = 128, BK = 64;
 constexpr int A_BYTES = BM * BK * 2;
-constexpr int OUT_COLS = 32;                               // rows of out that are staged at a time
-constexpr int OUT_LD = 144;                                // floats; the up half starts 16 banks behind the gate half
+constexpr int SUM_LD = 144;                                // floats of a staged row (SPLIT); the up half starts 16 banks behind the gate half
 constexpr int SMEM_MAX = 227 * 1024;
 constexpr int MAX_E = 1024;
+// warps: 0 loads weights (and rows in order), 1 issues MMAs, 8 carry sums out, 4 pick rows by token
+constexpr int EPI0 = 2, EPI_WARPS = 8, GATHER0 = EPI0 + EPI_WARPS, GATHER_WARPS = 4;
+constexpr int THREADS = 32 * (GATHER0 + GATHER_WARPS);
 
 struct Args {
   const int* starts;                                       // [E + 1] rows of the experts; null: one expert, R rows
   const int* order;                                        // [R] pair of a row, pair / k is its token; null: rows of x in order
+  const __nv_bfloat16* x;
   const __nv_bfloat16* bias;                               // [E, N]
   const __nv_bfloat16* res;
   const float* scale;
   __nv_bfloat16* out;
-  int64_t res_ld, out_ld;
+  int64_t x_ld, res_ld, out_ld;
   int R, T, k, E, N, W, K;                                 // W: width of out (N, or N / 2 with SwiGLU)
-  bool swiglu, vec;
+  bool vec;
   int* status;
 };
 
-template <int BN> struct Cfg {
-  static constexpr int B_BYTES = BN * BK * 2;
-  static constexpr int STAGE = A_BYTES + B_BYTES;
-  static constexpr int OUT = (BN < OUT_COLS ? BN : OUT_COLS) * OUT_LD * 4;
-  static constexpr int META = 2048 + 2 * (MAX_E + 1) * 4;
-  static constexpr int STAGES = (SMEM_MAX - 1024 - OUT - META) / STAGE;
-  static constexpr int SMEM = 1024 + STAGES * STAGE + OUT + META;
+// BN rows of a tile, of which a CTA of a pair stages half
+template <int BN, bool PAIR, bool SPLIT> struct Cfg {
+  static constexpr int B_ROWS = PAIR ? BN / 2 : BN;
+  static constexpr int STAGE = A_BYTES + B_ROWS * BK * 2;
+  static constexpr int SUMS = SPLIT ? BN * SUM_LD * 4 : 0;
+  static constexpr int META = 1024 + 2 * (MAX_E + 1) * 4;
+  static constexpr int STAGES = (SMEM_MAX - 1024 - SUMS - META) / STAGE < 12 ? (SMEM_MAX - 1024 - SUMS - META) / STAGE : 12;
+  static constexpr int SMEM = 1024 + STAGES * STAGE + SUMS + META;
   static constexpr int TMEM = 2 * BN < 32 ? 32 : 2 * BN;
 };
 
 struct Bars {
-  uint64_t full[16], empty[16], acc_full[2], acc_empty[2];
+  uint64_t full[12], picked[12], empty[12], acc_full[2], acc_empty[2];
   uint32_t tmem;
   int abort;
+};
+
+// x in boxes of 16, 32, 64 and 128 rows: a load instruction costs some 65 cycles whatever it brings, so that a stage of 128 rows
+// in boxes of 16 took 600 cycles of loads for 512 of MMAs (8192 rows, 5120 -> 17408: 1111 TFLOP/s)
+struct RowMaps {
+  CUtensorMap box[4];
 };
 
 struct Item {
   int e, n0, row0, rows;                                   // weight block (out's first feature), rows of out
 };
 
-DEVI uint32_t idesc_bf16(int n) {
-  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+DEVI uint32_t idesc_bf16(int m, int n) {
+  return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
-DEVI void tma_2d(uint32_t dst, const void* map, uint64_t* bar, int c, int r) {
+DEVI void tma_2d(uint32_t dst, const void* map, uint32_t bar, int c, int r) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
-      "l"(map), "r"(smem_u32(bar)), "r"(c), "r"(r)
+      "l"(map), "r"(bar), "r"(c), "r"(r)
       : "memory");
 }
-DEVI void tma_4d(uint32_t dst, const void* map, uint64_t* bar, int c0, int c1, int c2, int c3) {
+DEVI void tma_4d(uint32_t dst, const void* map, uint32_t bar, int c0, int c1, int c2, int c3) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-      "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
 }
-// four rows of a 2-D map by number, one after another
-DEVI void tma_gather4(uint32_t dst, const void* map, uint64_t* bar, int c, int4 r) {
+// the same on a CTA pair: into this CTA's memory, counted by the barrier at a cluster address
+DEVI void tma_2d_pair(uint32_t dst, const void* map, uint32_t bar, int c, int r) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
-      "l"(map), "r"(smem_u32(bar)), "r"(c), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w)
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(c), "r"(r)
       : "memory");
 }
-
+DEVI void tma_4d_pair(uint32_t dst, const void* map, uint32_t bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+      "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+DEVI void mma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// arrive on the barrier at a cluster address once the pair's MMAs so far are done
+DEVI void commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// arrive on the barrier at a cluster address.  What it announces (TMEM loads that were waited for, copies that have landed) is done
+// by then: a release of cluster scope took some 0.8 us (4096 rows by token on pairs: 541 us, 230 without)
+DEVI void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+DEVI void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
+      "%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]),
+        "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+        "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// 16 bytes global -> shared; none of them (zeros) unless `in`
+DEVI void cp_async16(uint32_t dst, const void* src, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+// arrive on this CTA's barrier once the thread's copies so far have landed
+DEVI void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 // Tiles before each expert -> tiles[0 .. E] from starts[0 .. E], by one warp: a lane adds up neighbours.
 DEVI void count_tiles(const Args& p, int bn, int* tiles, const int* starts, int lane) {
   const int each = (p.E + 31) / 32, e0 = min(p.E, lane * each), e1 = min(p.E, e0 + each);
@@ -123,106 +170,144 @@ DEVI Item item_of(const Args& p, int i, int blocks, int bn, int span, const int*
   return q;
 }
 
-// Staged sums st [columns][OUT_LD] (raw, position of a weight row in a column: out_pos) of `n` staged columns -> rows of out
-DEVI int out_pos(bool swiglu, int row) { return swiglu ? (row & 1) * 80 + row / 2 : row; }
-
-DEVI void store_rows(const Args& p, const Item& q, const float* st, int c0, int n, int tid) {
-  const int span = p.swiglu ? BM / 2 : BM, vecs = span / 8;
-  const int v = tid % vecs, f = q.n0 + v * 8;
-  if (f >= p.W) return;
-  const bool whole = p.vec && f + 8 <= p.W;
-  float b[8], bu[8];
-  if (p.bias) {
-    const __nv_bfloat16* bp = p.bias + (int64_t)q.e * p.N;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      b[i] = f + i < p.W ? __bfloat162float(bp[f + i]) : 0.f;
-      if (p.swiglu) bu[i] = f + i < p.W ? __bfloat162float(bp[p.W + f + i]) : 0.f;
-    }
+DEVI float silu(float g) { return __fdividef(g, 1.f + __expf(-g)); }
+DEVI uint32_t pack(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+// four neighbouring features f .. f + 3 of a row
+DEVI void store4(const Args& p, int64_t row, int f, uint32_t a, uint32_t b) {
+  __nv_bfloat16* out = p.out + row * p.out_ld + f;
+  if (p.vec && f + 4 <= p.W) {
+    *reinterpret_cast<uint2*>(out) = make_uint2(a, b);
+  } else {
+    uint16_t* o = reinterpret_cast<uint16_t*>(out);
+    if (f < p.W) o[0] = (uint16_t)a;
+    if (f + 1 < p.W) o[1] = (uint16_t)(a >> 16);
+    if (f + 2 < p.W) o[2] = (uint16_t)b;
+    if (f + 3 < p.W) o[3] = (uint16_t)(b >> 16);
   }
-  for (int c = tid / vecs; c < n; c += 128 / vecs) {
-    const int64_t r = q.row0 + c0 + c;
-    const float4* s = reinterpret_cast<const float4*>(st + c * OUT_LD + v * 8);
-    float y[8];
-    *reinterpret_cast<float4*>(y) = s[0];
-    *reinterpret_cast<float4*>(y + 4) = s[1];
-    if (p.bias) {
+}
+// scale and residual of one value
+DEVI float finish(const Args& p, float y, int64_t row, int f, bool in) {
+  if (p.scale) y *= in ? p.scale[row] : 0.f;
+  if (p.res) y += in ? __bfloat162float(p.res[row * p.res_ld + f]) : 0.f;
+  return y;
+}
+
+// 32 columns (rows of out from row0 on, n of them in use) of a warp's 32 weight rows -> out.  A lane holds one weight row; lanes
+// trade columns until each has four neighbouring features of one row, so that a store covers whole 32-byte sectors.
+template <bool SWIGLU>
+DEVI void store_columns(const Args& p, const float (&v)[32], int64_t row0, int n, int f0, int lane) {
+  const int l0 = lane & 1, l1 = lane >> 1 & 1, l2 = lane >> 2 & 1;
+  if constexpr (SWIGLU) {
+    // lane 2 j holds the gate and lane 2 j + 1 the up row of feature f0 + j
+    const int f = f0 + (lane >> 1);
+    float h[16];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] += b[i];
+    for (int j = 0; j < 16; ++j) {
+      const float o = __shfl_xor_sync(0xffffffffu, l0 ? v[2 * j] : v[2 * j + 1], 1);
+      const int c = 2 * j + l0;
+      h[j] = finish(p, l0 ? silu(o) * v[2 * j + 1] : silu(v[2 * j]) * o, row0 + c, f, c < n && f < p.W);
     }
-    if (p.swiglu) {
-      float u[8];
-      *reinterpret_cast<float4*>(u) = s[20];
-      *reinterpret_cast<float4*>(u + 4) = s[21];
+    uint32_t q[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        if (p.bias) u[i] += bu[i];
-        y[i] = __fdividef(y[i], 1.f + __expf(-y[i])) * u[i];
+    for (int j = 0; j < 8; ++j) {
+      const float o = __shfl_xor_sync(0xffffffffu, l1 ? h[2 * j] : h[2 * j + 1], 2);
+      q[j] = l1 ? pack(o, h[2 * j + 1]) : pack(h[2 * j], o);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t o = __shfl_xor_sync(0xffffffffu, l2 ? q[2 * j] : q[2 * j + 1], 4);
+      const int c = 8 * j + 4 * l2 + 2 * l1 + l0;
+      if (c < n) store4(p, row0 + c, f0 + (lane >> 1 & ~3), l2 ? o : q[2 * j], l2 ? q[2 * j + 1] : o);
+    }
+  } else {
+    const int f = f0 + lane;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float y[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) y[i] = finish(p, v[4 * j + i], row0 + 4 * j + i, f, 4 * j + i < n && f < p.W);
+      uint32_t q[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float o = __shfl_xor_sync(0xffffffffu, l0 ? y[2 * i] : y[2 * i + 1], 1);
+        q[i] = l0 ? pack(o, y[2 * i + 1]) : pack(y[2 * i], o);
       }
-    }
-    if (p.scale) {
-      const float a = p.scale[r];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] *= a;
-    }
-    __nv_bfloat16* out = p.out + r * p.out_ld + f;
-    const __nv_bfloat16* res = p.res + r * p.res_ld + f;
-    if (whole) {
-      uint4 o;
-      __nv_bfloat16* h = reinterpret_cast<__nv_bfloat16*>(&o);
-      if (p.res) {
-        const uint4 a = *reinterpret_cast<const uint4*>(res);
-        const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(&a);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] += __bfloat162float(x[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) h[i] = __float2bfloat16_rn(y[i]);
-      *reinterpret_cast<uint4*>(out) = o;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (f + i < p.W) out[i] = __float2bfloat16_rn(p.res ? y[i] + __bfloat162float(res[i]) : y[i]);
+      const uint32_t o = __shfl_xor_sync(0xffffffffu, l1 ? q[0] : q[1], 2);
+      const int c = 4 * j + 2 * l1 + l0;
+      if (c < n) store4(p, row0 + c, f0 + (lane & ~3), l1 ? o : q[0], l1 ? q[1] : o);
     }
   }
 }
 
-// SPLIT: a cluster shares one item's K; its CTAs' sums meet through distributed shared memory, each CTA adds up and stores some
-// of the rows.  Otherwise one CTA an SM runs every gridDim.x-th item.
-template <int BN, bool SPLIT>
-__global__ void __launch_bounds__(THREADS) kernel(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap wm,
-                                                  const __grid_constant__ CUtensorMap xm) {
-  using C = Cfg<BN>;
+// Staged sums of one row (position of a weight row: sum_pos) -> out, by 128 threads
+DEVI int sum_pos(bool swiglu, int row) { return swiglu ? (row & 1) * 80 + row / 2 : row; }
+
+template <bool SWIGLU>
+DEVI void store_row(const Args& p, const Item& q, const float* st, int c, int tid) {
+  const int f = q.n0 + tid;
+  if (tid >= (SWIGLU ? BM / 2 : BM) || f >= p.W) return;
+  const __nv_bfloat16* b = p.bias + (int64_t)q.e * p.N;
+  float y = st[tid];
+  if (p.bias) y += __bfloat162float(b[f]);
+  if (SWIGLU) {
+    float u = st[80 + tid];
+    if (p.bias) u += __bfloat162float(b[p.W + f]);
+    y = silu(y) * u;
+  }
+  const int64_t row = q.row0 + c;
+  p.out[row * p.out_ld + f] = __float2bfloat16_rn(finish(p, y, row, f, true));
+}
+
+// PAIR: two CTAs share a tile of 256 weight rows; each stages its 128 and its half of the tile's rows, and the first one issues
+// the MMAs of both.  SPLIT: a cluster shares one item's K; its CTAs' sums meet through distributed shared memory, each CTA adds
+// up and stores some of the rows.  Otherwise a CTA (or pair) an SM (or two) runs every n-th item.
+template <int BN, bool SWIGLU, bool PAIR, bool SPLIT>
+__global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap wm,
+                                                     const __grid_constant__ RowMaps xm) {
+  using C = Cfg<BN, PAIR, SPLIT>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* st = reinterpret_cast<float*>(smem + C::STAGES * C::STAGE);
-  Bars* bars = reinterpret_cast<Bars*>(smem + C::STAGES * C::STAGE + C::OUT);
-  int* tiles = reinterpret_cast<int*>(smem + C::STAGES * C::STAGE + C::OUT + 2048);
+  Bars* bars = reinterpret_cast<Bars*>(smem + C::STAGES * C::STAGE + C::SUMS);
+  int* tiles = reinterpret_cast<int*>(smem + C::STAGES * C::STAGE + C::SUMS + 1024);
   int* starts = tiles + MAX_E + 1;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int splits = SPLIT ? gridDim.y : 1;
-  const int rank = SPLIT ? blockIdx.y : 0;
-  const int span = p.swiglu ? BM / 2 : BM, blocks = (p.W + span - 1) / span;
+  const int splits = SPLIT ? gridDim.y : 1, share = SPLIT ? blockIdx.y : 0;
+  const int rank = PAIR ? cluster_ctarank() : 0;           // 0 issues the MMAs
+  const int unit = PAIR ? blockIdx.x >> 1 : blockIdx.x, units = PAIR ? gridDim.x >> 1 : gridDim.x;
+  constexpr int HALF = SWIGLU ? BM / 2 : BM;               // features of a CTA
+  constexpr int SPAN = PAIR ? 2 * HALF : HALF;
+  const int blocks = (p.W + SPAN - 1) / SPAN;
   const int all_k = (p.K + BK - 1) / BK;
-  const int k0 = (int)((int64_t)all_k * rank / splits), k1 = (int)((int64_t)all_k * (rank + 1) / splits);
+  const int k0 = (int)((int64_t)all_k * share / splits), k1 = (int)((int64_t)all_k * (share + 1) / splits);
+  const bool gather = p.order != nullptr;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(&bars->full[s], 1);
+      mbar_init(&bars->full[s], gather && PAIR ? 2 : 1);
+      mbar_init(&bars->picked[s], 32 * GATHER_WARPS);
       mbar_init(&bars->empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars->acc_full[b], 1);
-      mbar_init(&bars->acc_empty[b], 1);
+      mbar_init(&bars->acc_empty[b], EPI_WARPS * (PAIR ? 2 : 1));
     }
     bars->abort = 0;
     fence_mbar_init();
     tma_prefetch_desc(&wm);
-    tma_prefetch_desc(&xm);
   }
   if (warp == 1) {
-    tmem_alloc(&bars->tmem, C::TMEM);
-    tmem_relinquish();
+    if (PAIR) {
+      asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&bars->tmem)), "r"(C::TMEM)
+                   : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    } else {
+      tmem_alloc(&bars->tmem, C::TMEM);
+      tmem_relinquish();
+    }
   }
   pdl_wait();
   for (int e = threadIdx.x; e <= p.E; e += THREADS) starts[e] = p.starts ? p.starts[e] : e ? p.R : 0;
@@ -230,147 +315,242 @@ __global__ void __launch_bounds__(THREADS) kernel(const __grid_constant__ Args p
   if (warp == 2) count_tiles(p, BN, tiles, starts, lane);
   tc_fence_before();
   __syncthreads();
+  __syncwarp();
+  if (PAIR) cluster_sync();                                // both CTAs' barriers and tensor memory are there
   tc_fence_after();
   pdl_trigger();                                           // this block holds its tensor memory
   const uint32_t tmem = bars->tmem;
   const int items = tiles[p.E] * blocks;
   volatile int* abort = &bars->abort;
-  bool mine = (int)blockIdx.x < items;                     // SPLIT: this cluster has an item
+  const uint32_t abort_peer = PAIR ? mapa_shared(smem_u32(&bars->abort), rank ^ 1) : 0;
+  // a failed wait stops the CTA, and its partner
+  auto give_up = [&]() {
+    *abort = 1;
+    if (PAIR) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(abort_peer), "r"(1) : "memory");
+  };
+  auto in_order = [&](const Item& q) { return q.row0 >= 0 && q.rows > 0 && q.row0 + q.rows <= p.R; };
+  // rows of the MMA, and of them those that this CTA stages: [b0, b0 + bn)
+  auto mma_rows = [&](const Item& q) { return PAIR ? (q.rows + 31) / 32 * 32 : (q.rows + 15) / 16 * 16; };
 
   if (warp == 0) {
     uint32_t it = 0;
-    for (int i = blockIdx.x; i < items; i += gridDim.x) {
+    for (int i = unit; i < items; i += units) {
       if (__any_sync(0xffffffffu, *abort)) break;          // the same answer in all lanes
-      const Item q = item_of(p, i, blocks, BN, span, tiles, starts);
-      const bool ok = q.row0 >= 0 && q.rows > 0 && q.row0 + q.rows <= p.R;
-      // loads of the rows: four by number, or boxes of 16
-      const int each = p.order ? 4 : 16, loads = ok ? (q.rows + each - 1) / each : 0;
-      int4 rows[2];
-      if (p.order) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          int r[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int c = (lane + 32 * h) * 4 + j;
-            r[j] = ok && c < q.rows ? p.order[q.row0 + c] : 0;
-            if (r[j] < 0 || r[j] >= (int64_t)p.T * p.k) {
-              atomicExch(p.status, (int)kErrBounds);
-              r[j] = 0;
-            }
-            r[j] /= p.k;
-          }
-          rows[h] = make_int4(r[0], r[1], r[2], r[3]);
-        }
-      }
-      if (!ok) {
+      const Item q = item_of(p, i, blocks, BN, SPAN, tiles, starts);
+      if (!in_order(q)) {
         if (lane == 0) atomicExch(p.status, (int)kErrBounds);
-        *abort = 1;
+        give_up();
         break;
       }
+      // rows of the tile: the boxes that make up their number, one a lane, the largest first
+      const int bn = mma_rows(q) / (PAIR ? 2 : 1), box = min(lane, 3), above = bn >> (box + 5) << (box + 5);
+      const bool loads = !gather && lane < 4 && (bn >> (box + 4) & 1);
+      const uint32_t bbytes = gather ? 0 : bn * BK * 2;
+      const int row = q.row0 + rank * bn + above;
       for (int kb = k0; kb < k1; ++kb, ++it) {
         const int s = it % C::STAGES;
-        if (!mbar_wait(&bars->empty[s], ((it / C::STAGES) & 1) ^ 1, p.status)) *abort = 1;
+        if (!mbar_wait(&bars->empty[s], ((it / C::STAGES) & 1) ^ 1, p.status)) give_up();
         if (__any_sync(0xffffffffu, *abort)) break;
         const uint32_t a = smem_u32(smem + s * C::STAGE), b = a + A_BYTES;
+        uint32_t full = smem_u32(&bars->full[s]);
+        if (PAIR) full = mapa_shared(full, 0);
         if (lane == 0) {
-          mbar_arrive_expect_tx(&bars->full[s], A_BYTES + loads * each * BK * 2);
-          if (p.swiglu) tma_4d(a, &wm, &bars->full[s], kb * BK, 0, q.n0, q.e);
-          else tma_4d(a, &wm, &bars->full[s], kb * BK, q.n0, 0, q.e);
+          if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], (PAIR ? 2 : 1) * (A_BYTES + bbytes));
+          const int f = q.n0 + rank * HALF;
+          if (PAIR && SWIGLU) tma_4d_pair(a, &wm, full, kb * BK, 0, f, q.e);
+          else if (PAIR) tma_4d_pair(a, &wm, full, kb * BK, f, 0, q.e);
+          else if (SWIGLU) tma_4d(a, &wm, full, kb * BK, 0, f, q.e);
+          else tma_4d(a, &wm, full, kb * BK, f, 0, q.e);
         }
         __syncwarp();
-        if (p.order) {
-          if (lane < loads) tma_gather4(b + lane * 512, &xm, &bars->full[s], kb * BK, rows[0]);
-          if (lane + 32 < loads) tma_gather4(b + (lane + 32) * 512, &xm, &bars->full[s], kb * BK, rows[1]);
-        } else if (lane < loads) {
-          tma_2d(b + lane * 2048, &xm, &bars->full[s], kb * BK, q.row0 + lane * 16);
+        if (loads) {
+          if (PAIR) tma_2d_pair(b + above * 128, &xm.box[box], full, kb * BK, row);
+          else tma_2d(b + above * 128, &xm.box[box], full, kb * BK, row);
         }
       }
     }
     // given up: the loads in flight land before the block leaves
-    if (*abort)
+    if (*abort && rank == 0)
       for (uint32_t j = it > C::STAGES ? it - C::STAGES : 0; j < it; ++j)
         mbar_wait(&bars->full[j % C::STAGES], (j / C::STAGES) & 1, p.status);
   } else if (warp == 1) {
-    if (elect_one()) {
+    if (rank == 0 && elect_one()) {
+      const uint32_t empty1 = PAIR ? mapa_shared(smem_u32(&bars->empty[0]), 1) : 0;
+      const uint32_t acc_full1 = PAIR ? mapa_shared(smem_u32(&bars->acc_full[0]), 1) : 0;
       uint32_t it = 0, n = 0;
-      for (int i = blockIdx.x; i < items && !*abort; i += gridDim.x, ++n) {
-        const Item q = item_of(p, i, blocks, BN, span, tiles, starts);
+      for (int i = unit; i < items && !*abort; i += units, ++n) {
+        const Item q = item_of(p, i, blocks, BN, SPAN, tiles, starts);
         const int ab = n & 1;
-        if (!mbar_wait(&bars->acc_empty[ab], ((n >> 1) & 1) ^ 1, p.status)) { *abort = 1; break; }
+        if (!mbar_wait(&bars->acc_empty[ab], ((n >> 1) & 1) ^ 1, p.status)) { give_up(); break; }
         tc_fence_after();
-        const uint32_t idesc = idesc_bf16((q.rows + 15) / 16 * 16);
+        const uint32_t idesc = idesc_bf16(PAIR ? 2 * BM : BM, mma_rows(q));
         bool ok = true;
         for (int kb = k0; kb < k1; ++kb, ++it) {
           const int s = it % C::STAGES;
-          if (!mbar_wait(&bars->full[s], (it / C::STAGES) & 1, p.status)) { ok = false; break; }
+          const uint32_t ph = (it / C::STAGES) & 1;
+          if (!mbar_wait(&bars->full[s], ph, p.status)) { ok = false; break; }
+          if (gather) {
+            if (!mbar_wait(&bars->picked[s], ph, p.status)) { ok = false; break; }
+            fence_proxy_async();                           // the copies were ordinary writes
+          }
           tc_fence_after();
           const uint32_t a = smem_u32(smem + s * C::STAGE), b = a + A_BYTES;
 #pragma unroll
-          for (int j = 0; j < BK / 16; ++j)
-            mma_f16(tmem + ab * BN, sdesc_sw128(a + j * 32), sdesc_sw128(b + j * 32), idesc, kb > k0 || j > 0);
-          mma_commit(&bars->empty[s]);
+          for (int j = 0; j < BK / 16; ++j) {
+            if (PAIR) mma_pair(tmem + ab * BN, sdesc_sw128(a + j * 32), sdesc_sw128(b + j * 32), idesc, kb > k0 || j > 0);
+            else mma_f16(tmem + ab * BN, sdesc_sw128(a + j * 32), sdesc_sw128(b + j * 32), idesc, kb > k0 || j > 0);
+          }
+          if (PAIR) {
+            commit_pair(smem_u32(&bars->empty[s]));
+            commit_pair(empty1 + s * 8);
+          } else {
+            mma_commit(&bars->empty[s]);
+          }
         }
-        if (!ok) { *abort = 1; break; }
-        mma_commit(&bars->acc_full[ab]);
+        if (!ok) { give_up(); break; }
+        if (PAIR) {
+          commit_pair(smem_u32(&bars->acc_full[ab]));
+          commit_pair(acc_full1 + ab * 8);
+        } else {
+          mma_commit(&bars->acc_full[ab]);
+        }
       }
+    }
+    if (PAIR && gather && rank == 1 && elect_one()) {
+      // this CTA's picked rows, for the one that issues the MMAs
+      const uint32_t full0 = mapa_shared(smem_u32(&bars->full[0]), 0);
+      uint32_t it = 0;
+      for (int i = unit; i < items && !*abort; i += units)
+        for (int kb = k0; kb < k1; ++kb, ++it) {
+          const int s = it % C::STAGES;
+          if (!mbar_wait(&bars->picked[s], (it / C::STAGES) & 1, p.status)) { give_up(); break; }
+          fence_proxy_async();
+          arrive_at(full0 + s * 8);
+        }
     }
     __syncwarp();
-  } else {
-    const int quad = warp & 3, tid = threadIdx.x - 64, pos = out_pos(p.swiglu, quad * 32 + lane);
+  } else if (warp < GATHER0) {
+    const int quad = warp & 3, part = (warp - EPI0) / 4;   // 32 weight rows; columns 64 j + 32 part
+    uint32_t acc_empty = smem_u32(&bars->acc_empty[0]);
+    if (PAIR) acc_empty = mapa_shared(acc_empty, 0);
     uint32_t n = 0;
-    for (int i = blockIdx.x; i < items; i += gridDim.x, ++n) {
-      const Item q = item_of(p, i, blocks, BN, span, tiles, starts);
+    for (int i = unit; i < items; i += units, ++n) {
+      const Item q = item_of(p, i, blocks, BN, SPAN, tiles, starts);
       const int ab = n & 1;
-      const bool got = mbar_wait(&bars->acc_full[ab], (n >> 1) & 1, p.status);
-      if (!got) *abort = 1;
-      if (bar_sync_or(1, 128, *abort != 0)) break;
+      const int f0 = q.n0 + rank * HALF + quad * (HALF / 4);          // the warp's first feature
+      float bias = 0.f;
+      if (!SPLIT && p.bias) {
+        const int f = f0 + (SWIGLU ? lane >> 1 : lane);
+        if (f < p.W) bias = __bfloat162float(p.bias[(int64_t)q.e * p.N + f + (SWIGLU && (lane & 1) ? p.W : 0)]);
+      }
+      if (!mbar_wait(&bars->acc_full[ab], (n >> 1) & 1, p.status)) give_up();
+      if (__any_sync(0xffffffffu, *abort)) break;
       tc_fence_after();
       const uint32_t acc = tmem + ((uint32_t)(quad * 32) << 16) + ab * BN;
-      for (int c0 = 0; c0 < q.rows; c0 += OUT_COLS) {
-        const int cols = min(OUT_COLS, q.rows - c0);
-        for (int c = 0; c < cols; c += 16) {
-          uint32_t r[16];
-          tmem_ld_32x32b_x16(acc + c0 + c, r);
-          tmem_ld_wait();
+      if constexpr (SPLIT) {
+        if (part == 0) {
 #pragma unroll
-          for (int j = 0; j < 16; ++j) st[(c + j) * OUT_LD + pos] = __uint_as_float(r[j]);
+          for (int c = 0; c < BN; c += 16) {
+            uint32_t r[16];
+            tmem_ld_32x32b_x16(acc + c, r);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) st[(c + j) * SUM_LD + sum_pos(SWIGLU, quad * 32 + lane)] = __uint_as_float(r[j]);
+          }
         }
-        if (c0 + OUT_COLS >= q.rows) tc_fence_before();
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        if (c0 + OUT_COLS >= q.rows && tid == 0) mbar_arrive(&bars->acc_empty[ab]);
-        if (!SPLIT) {
-          store_rows(p, q, st, c0, cols, tid);
-          asm volatile("bar.sync 1, 128;" ::: "memory");
+      } else {
+        for (int c0 = 32 * part; c0 < q.rows; c0 += 64) {
+          uint32_t r[32];
+          if constexpr (BN == 16) {
+            uint32_t h[16];
+            tmem_ld_32x32b_x16(acc, h);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) r[j] = h[j], r[16 + j] = 0;
+          } else {
+            tmem_ld_x32(acc + c0, r);
+          }
+          tmem_ld_wait();
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) + bias;
+          if (c0 + 64 >= q.rows) {                         // this warp has read all that it needs
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) arrive_at(acc_empty + ab * 8);
+          }
+          store_columns<SWIGLU>(p, v, q.row0 + c0, min(32, q.rows - c0), f0, lane);
         }
+        if (32 * part >= q.rows && lane == 0) arrive_at(acc_empty + ab * 8);
       }
     }
+  } else if (gather) {
+    // rows by token: thread t brings 16-byte piece t % 8 of rows t / 8, t / 8 + 16, ... of every stage
+    const int tid = threadIdx.x - 32 * GATHER0, piece = tid % 8, r0 = tid / 8;
+    constexpr int EACH = C::B_ROWS / 16;
+    uint32_t it = 0;
+    for (int i = unit; i < items; i += units) {
+      if (__any_sync(0xffffffffu, *abort)) break;
+      const Item q = item_of(p, i, blocks, BN, SPAN, tiles, starts);
+      if (!in_order(q)) break;                             // warp 0 says so
+      const int bn = mma_rows(q) / (PAIR ? 2 : 1), first = rank * bn, mine = min(bn, q.rows - first);
+      const __nv_bfloat16* src[EACH];
+#pragma unroll
+      for (int h = 0; h < EACH; ++h) {
+        const int c = r0 + 16 * h;
+        src[h] = nullptr;
+        if (c < mine) {
+          int t = p.order[q.row0 + first + c];
+          if (t < 0 || t >= (int64_t)p.T * p.k) {
+            atomicExch(p.status, (int)kErrBounds);
+            t = 0;
+          }
+          src[h] = p.x + (int64_t)(t / p.k) * p.x_ld + piece * 8;
+        }
+      }
+      for (int kb = k0; kb < k1; ++kb, ++it) {
+        const int s = it % C::STAGES;
+        if (!mbar_wait(&bars->empty[s], ((it / C::STAGES) & 1) ^ 1, p.status)) give_up();
+        if (__any_sync(0xffffffffu, *abort)) break;
+        const uint32_t b = smem_u32(smem + s * C::STAGE) + A_BYTES + r0 * 128 + ((piece ^ (r0 & 7)) << 4);
+        const bool in = kb * BK + piece * 8 < p.K;
+#pragma unroll
+        for (int h = 0; h < EACH; ++h)
+          if (src[h]) cp_async16(b + h * 2048, in ? src[h] + kb * BK : src[h], in);
+        cp_async_arrive(&bars->picked[s]);
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
+  __syncwarp();
+  if (PAIR) cluster_sync();                                // the pair's MMAs and arrivals are done
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, C::TMEM);
+    if (PAIR)
+      asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(C::TMEM) : "memory");
+    else
+      tmem_dealloc(tmem, C::TMEM);
   }
   if constexpr (SPLIT) {
     cluster_sync();                                        // every CTA's sums are staged
-    if (mine && warp >= 2 && !*abort) {
-      const Item q = item_of(p, blockIdx.x, blocks, BN, span, tiles, starts);
-      const int tid = threadIdx.x - 64;
-      // rows rank, rank + splits, ... of the tile: add up the other CTAs' sums in their order
-      for (int c = rank; c < q.rows; c += splits) {
-        const uint32_t at = smem_u32(st + c * OUT_LD + out_pos(p.swiglu, tid));
+    if (unit < items && warp >= EPI0 && warp < EPI0 + 4 && !*abort) {
+      const Item q = item_of(p, unit, blocks, BN, SPAN, tiles, starts);
+      const int tid = threadIdx.x - 32 * EPI0;
+      float* sums = reinterpret_cast<float*>(smem);        // stage memory, which no load uses any more
+      // rows share, share + splits, ... of the tile: the CTAs' sums in their order
+      for (int c = share; c < q.rows; c += splits) {
+        const int at = c * SUM_LD + sum_pos(SWIGLU, tid);
         float sum = 0.f;
         for (int r = 0; r < splits; ++r) {
           float v;
-          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(at, r)));
+          asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(smem_u32(st + at), r)));
           sum += v;
         }
-        // into the stage memory, which no load uses any more
-        reinterpret_cast<float*>(smem)[c * OUT_LD + out_pos(p.swiglu, tid)] = sum;
+        sums[at] = sum;
       }
       asm volatile("bar.sync 1, 128;" ::: "memory");
-      for (int c = rank; c < q.rows; c += splits) store_rows(p, q, reinterpret_cast<float*>(smem) + c * OUT_LD, c, 1, tid);
+      for (int c = share; c < q.rows; c += splits) store_row<SWIGLU>(p, q, sums + c * SUM_LD, c, tid);
     }
     cluster_sync();                                        // the other CTAs have read this one's sums
   }
@@ -380,7 +560,7 @@ __global__ void __launch_bounds__(THREADS) kernel(const __grid_constant__ Args p
 // launches
 // ---------------------------------------------------------------------------------------------
 template <typename... A>
-void launch(void (*kern)(A...), dim3 grid, int cluster_y, size_t smem, cudaStream_t stream, A... args) {
+void launch(void (*kern)(A...), dim3 grid, dim3 cluster, size_t smem, cudaStream_t stream, A... args) {
   static std::mutex m;
   static std::map<std::pair<const void*, int>, bool> set;
   int dev;
@@ -402,9 +582,9 @@ void launch(void (*kern)(A...), dim3 grid, int cluster_y, size_t smem, cudaStrea
     at[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[n++].val.programmaticStreamSerializationAllowed = 1;
   }
-  if (cluster_y > 1) {
+  if (cluster.x * cluster.y > 1) {
     at[n].id = cudaLaunchAttributeClusterDimension;
-    at[n++].val.clusterDim = {1, (unsigned)cluster_y, 1};
+    at[n++].val.clusterDim = {cluster.x, cluster.y, 1};
   }
   cfg.attrs = at;
   cfg.numAttrs = n;
@@ -435,9 +615,10 @@ bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
   return x.first < y.second && y.first < x.second;
 }
 
-template <int BN>
-void run(const Args& p, const CUtensorMap& wm, const CUtensorMap& xm, int64_t items, int sms, cudaStream_t stream) {
-  launch(kernel<BN, false>, dim3((unsigned)std::min<int64_t>(items, sms)), 1, Cfg<BN>::SMEM, stream, p, wm, xm);
+template <int BN, bool PAIR, bool SPLIT>
+void run(const Args& p, bool swiglu, const CUtensorMap& wm, const RowMaps& xm, dim3 grid, dim3 cluster, cudaStream_t stream) {
+  launch(swiglu ? kernel<BN, true, PAIR, SPLIT> : kernel<BN, false, PAIR, SPLIT>, grid, cluster, Cfg<BN, PAIR, SPLIT>::SMEM, stream,
+         p, wm, xm);
 }
 
 }  // namespace lf
@@ -519,38 +700,39 @@ torch::Tensor linear_fused(const torch::Tensor& x, const LinearBank& bank, const
   p.out = (__nv_bfloat16*)out.data_ptr();
   p.res_ld = res.has_value() ? res->stride(0) : 0;
   p.out_ld = out.stride(0);
+  p.x = (const __nv_bfloat16*)x.data_ptr();
+  p.x_ld = x.stride(0);
   p.R = R; p.T = x.size(0); p.k = k; p.E = E; p.N = N; p.W = W; p.K = K;
-  p.swiglu = bank.swiglu;
-  // one row's stride says nothing
-  p.vec = ((uintptr_t)p.out | (uintptr_t)p.res) % 16 == 0 && (R == 1 || (p.out_ld | p.res_ld) % 8 == 0);
+  p.vec = (uintptr_t)p.out % 8 == 0 && (R == 1 || p.out_ld % 4 == 0);      // one row's stride says nothing
   p.status = bank.status.data_ptr<int>();
-  const CUtensorMap xm = make_tma_2d(x.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, K, x.size(0),
-                                     (x.size(0) == 1 ? K : x.stride(0)) * 2ll, lf::BK, by_token ? 1 : 16,
-                                     CU_TENSOR_MAP_SWIZZLE_128B);
+  lf::RowMaps xm = {};
+  if (!by_token)
+    for (int i = 0; i < 4; ++i)
+      xm.box[i] = make_tma_2d(x.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, K, x.size(0), (x.size(0) == 1 ? K : x.stride(0)) * 2ll,
+                              lf::BK, 16 << i, CU_TENSOR_MAP_SWIZZLE_128B);
   auto stream = at::cuda::getCurrentCUDAStream();
   const int sms = lf::sm_count(x.get_device());
-  // Tile height: about twice the rows that an expert has on average, so that few experts need a second pass over their weights
+  // Tile height: about twice the rows that an expert has on average, so that few experts need a second pass over their weights;
+  // above 64 rows CTA pairs, whose tiles are cut to 32 rows
   const int64_t avg = (R + E - 1) / E, want = E == 1 ? R : 2 * avg;
-  const int bn = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : want <= 128 ? 128 : 256;
-  const int span = bank.swiglu ? 64 : 128;
+  const int bn = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 256;
+  const int span = (bank.swiglu ? 64 : 128) * (bn == 256 ? 2 : 1);
   const int64_t blocks = (W + span - 1) / span, items = (std::min<int64_t>(E, R) + R / bn) * blocks;   // at most
-  if (items >= (1ll << 31)) refuse("rows");
+  if (items >= (1ll << 30)) refuse("rows");
+  const unsigned n = (unsigned)std::min<int64_t>(items, bn == 256 ? sms / 2 : sms);
   if (bn == 16) {
     // too few items for the SMs: clusters share the items' K, each CTA at least four 64-blocks
-    int splits = 1;
+    unsigned splits = 1;
     const int64_t kb = (K + 63) / 64;
     while (splits < 8 && items * splits * 2 <= sms && kb / (splits * 2) >= 4) splits *= 2;
-    if (splits > 1) {
-      lf::launch(lf::kernel<16, true>, dim3((unsigned)items, splits), splits, lf::Cfg<16>::SMEM, stream, p, bank.wm, xm);
-      return out;
-    }
-  }
-  switch (bn) {
-    case 16: lf::run<16>(p, bank.wm, xm, items, sms, stream); break;
-    case 32: lf::run<32>(p, bank.wm, xm, items, sms, stream); break;
-    case 64: lf::run<64>(p, bank.wm, xm, items, sms, stream); break;
-    case 128: lf::run<128>(p, bank.wm, xm, items, sms, stream); break;
-    default: lf::run<256>(p, bank.wm, xm, items, sms, stream);
+    if (splits > 1) lf::run<16, false, true>(p, bank.swiglu, bank.wm, xm, dim3((unsigned)items, splits), dim3(1, splits), stream);
+    else lf::run<16, false, false>(p, bank.swiglu, bank.wm, xm, dim3(n), dim3(1), stream);
+  } else if (bn == 32) {
+    lf::run<32, false, false>(p, bank.swiglu, bank.wm, xm, dim3(n), dim3(1), stream);
+  } else if (bn == 64) {
+    lf::run<64, false, false>(p, bank.swiglu, bank.wm, xm, dim3(n), dim3(1), stream);
+  } else {
+    lf::run<256, true, false>(p, bank.swiglu, bank.wm, xm, dim3(2 * n), dim3(2), stream);
   }
   return out;
 }
