@@ -42,6 +42,7 @@ struct Args {
   __nv_bfloat16* out;
   int64_t x_ld, res_ld, out_ld;
   int R, T, k, E, N, W, K;                                 // W: width of out (N, or N / 2 with SwiGLU)
+  int tile;                                                // rows of a tile, at most the kernel's BN
   bool vec;
   int* status;
 };
@@ -175,70 +176,107 @@ DEVI uint32_t pack(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-// four neighbouring features f .. f + 3 of a row
-DEVI void store4(const Args& p, int64_t row, int f, uint32_t a, uint32_t b) {
-  __nv_bfloat16* out = p.out + row * p.out_ld + f;
-  if (p.vec && f + 4 <= p.W) {
-    *reinterpret_cast<uint2*>(out) = make_uint2(a, b);
-  } else {
-    uint16_t* o = reinterpret_cast<uint16_t*>(out);
-    if (f < p.W) o[0] = (uint16_t)a;
-    if (f + 1 < p.W) o[1] = (uint16_t)(a >> 16);
-    if (f + 2 < p.W) o[2] = (uint16_t)b;
-    if (f + 3 < p.W) o[3] = (uint16_t)(b >> 16);
+
+// What four neighbouring features f .. f + 3 of a row need from memory
+struct Rest {
+  float scale;
+  uint2 res;
+};
+// column of a lane's j-th four features, and the first of them
+template <bool SWIGLU> DEVI int column_of(int j, int lane) { return SWIGLU ? 8 * j + (lane & 7) : 4 * j + (lane & 3); }
+template <bool SWIGLU> DEVI int feature_of(int lane) { return SWIGLU ? (lane >> 1) & ~3 : lane & ~3; }
+
+template <bool WHOLE, bool FULL> DEVI Rest load_rest(const Args& p, int64_t row, int f, bool in) {
+  Rest q = {1.f, make_uint2(0, 0)};
+  if (p.scale && (FULL || in)) q.scale = p.scale[row];
+  if (p.res && (FULL || in)) {
+    const __nv_bfloat16* r = p.res + row * p.res_ld + f;
+    if (WHOLE || (p.vec && f + 4 <= p.W)) {
+      q.res = *reinterpret_cast<const uint2*>(r);
+    } else {
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(r);
+      if (f < p.W) q.res.x = h[0];
+      if (f + 1 < p.W) q.res.x |= (uint32_t)h[1] << 16;
+      if (f + 2 < p.W) q.res.y = h[2];
+      if (f + 3 < p.W) q.res.y |= (uint32_t)h[3] << 16;
+    }
   }
+  return q;
 }
-// scale and residual of one value
-DEVI float finish(const Args& p, float y, int64_t row, int f, bool in) {
-  if (p.scale) y *= in ? p.scale[row] : 0.f;
-  if (p.res) y += in ? __bfloat162float(p.res[row * p.res_ld + f]) : 0.f;
-  return y;
+template <bool REST, bool WHOLE, bool FULL>
+DEVI void store4(const Args& p, __nv_bfloat16* out, int f, bool in, const Rest& q, float y0, float y1, float y2, float y3) {
+  if (REST) {
+    y0 *= q.scale, y1 *= q.scale, y2 *= q.scale, y3 *= q.scale;
+    if (p.res) {                                           // without one, -0 stays -0
+      y0 += __uint_as_float(q.res.x << 16), y1 += __uint_as_float(q.res.x & 0xffff0000u);
+      y2 += __uint_as_float(q.res.y << 16), y3 += __uint_as_float(q.res.y & 0xffff0000u);
+    }
+  }
+  const uint32_t a = pack(y0, y1), b = pack(y2, y3);
+  if (FULL || in) {
+    if (WHOLE || (p.vec && f + 4 <= p.W)) {
+      *reinterpret_cast<uint2*>(out) = make_uint2(a, b);
+    } else {
+      uint16_t* o = reinterpret_cast<uint16_t*>(out);
+      if (f < p.W) o[0] = (uint16_t)a;
+      if (f + 1 < p.W) o[1] = (uint16_t)(a >> 16);
+      if (f + 2 < p.W) o[2] = (uint16_t)b;
+      if (f + 3 < p.W) o[3] = (uint16_t)(b >> 16);
+    }
+  }
 }
 
 // 32 columns (rows of out from row0 on, n of them in use) of a warp's 32 weight rows -> out.  A lane holds one weight row; lanes
 // trade columns until each has four neighbouring features of one row, so that a store covers whole 32-byte sectors.
-template <bool SWIGLU>
+// WHOLE: the features are all in use and on 8 bytes; FULL: so are all columns, and nothing branches, so that the trades of all of
+// them overlap: 8192 rows by expert, 512 -> 2048: 174 us, 257 with a test at every store.
+template <bool SWIGLU, bool REST, bool WHOLE, bool FULL>
 DEVI void store_columns(const Args& p, const float (&v)[32], int64_t row0, int n, int f0, int lane) {
-  const int l0 = lane & 1, l1 = lane >> 1 & 1, l2 = lane >> 2 & 1;
-  if constexpr (SWIGLU) {
-    // lane 2 j holds the gate and lane 2 j + 1 the up row of feature f0 + j
-    const int f = f0 + (lane >> 1);
-    float h[16];
+  constexpr int J = SWIGLU ? 4 : 8, STEP = 32 / J;
+  const bool l0 = lane & 1, l1 = lane & 2, l2 = lane & 4;
+  const int f = f0 + feature_of<SWIGLU>(lane), c0 = column_of<SWIGLU>(0, lane);
+  // each pair of lanes trades one of two columns
+  auto trade = [&](float mine, float other, bool second, int lanes) {
+    return __shfl_xor_sync(0xffffffffu, second ? mine : other, lanes);
+  };
+  Rest rest[J];
+  if (REST)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) {
-      const float o = __shfl_xor_sync(0xffffffffu, l0 ? v[2 * j] : v[2 * j + 1], 1);
-      const int c = 2 * j + l0;
-      h[j] = finish(p, l0 ? silu(o) * v[2 * j + 1] : silu(v[2 * j]) * o, row0 + c, f, c < n && f < p.W);
-    }
-    uint32_t q[8];
+    for (int j = 0; j < J; ++j)
+      rest[j] = load_rest<WHOLE, FULL>(p, row0 + c0 + j * STEP, f, c0 + j * STEP < n && f < p.W);
+  __nv_bfloat16* out = p.out + (row0 + c0) * p.out_ld + f;
+  const int64_t step = STEP * p.out_ld;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float o = __shfl_xor_sync(0xffffffffu, l1 ? h[2 * j] : h[2 * j + 1], 2);
-      q[j] = l1 ? pack(o, h[2 * j + 1]) : pack(h[2 * j], o);
-    }
+  for (int j = 0; j < J; ++j, out += step) {
+    if (!FULL && j * STEP >= n) break;
+    float y[2][2];
+    if constexpr (SWIGLU) {
+      // lane 2 i holds the gate and lane 2 i + 1 the up row of feature f0 + i
+      float h[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t o = __shfl_xor_sync(0xffffffffu, l2 ? q[2 * j] : q[2 * j + 1], 4);
-      const int c = 8 * j + 4 * l2 + 2 * l1 + l0;
-      if (c < n) store4(p, row0 + c, f0 + (lane >> 1 & ~3), l2 ? o : q[2 * j], l2 ? q[2 * j + 1] : o);
-    }
-  } else {
-    const int f = f0 + lane;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float y[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) y[i] = finish(p, v[4 * j + i], row0 + 4 * j + i, f, 4 * j + i < n && f < p.W);
-      uint32_t q[2];
+      for (int i = 0; i < 4; ++i) {
+        const float a = v[8 * j + 2 * i], b = v[8 * j + 2 * i + 1], o = trade(a, b, l0, 1);
+        h[i] = silu(l0 ? o : a) * (l0 ? b : o);            // column 8 j + 2 i + l0
+      }
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const float o = __shfl_xor_sync(0xffffffffu, l0 ? y[2 * i] : y[2 * i + 1], 1);
-        q[i] = l0 ? pack(o, y[2 * i + 1]) : pack(y[2 * i], o);
+        const float o = trade(h[2 * i], h[2 * i + 1], l1, 2);
+        y[i][0] = l1 ? o : h[2 * i];
+        y[i][1] = l1 ? h[2 * i + 1] : o;
       }
-      const uint32_t o = __shfl_xor_sync(0xffffffffu, l1 ? q[0] : q[1], 2);
-      const int c = 4 * j + 2 * l1 + l0;
-      if (c < n) store4(p, row0 + c, f0 + (lane & ~3), l1 ? o : q[0], l1 ? q[1] : o);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const float a = v[4 * j + 2 * i], b = v[4 * j + 2 * i + 1], o = trade(a, b, l0, 1);
+        y[i][0] = l0 ? o : a;
+        y[i][1] = l0 ? b : o;
+      }
     }
+    const bool last = SWIGLU ? l2 : l1;
+    constexpr int LANES = SWIGLU ? 4 : 2;
+    const float o0 = trade(y[0][0], y[1][0], last, LANES), o1 = trade(y[0][1], y[1][1], last, LANES);
+    store4<REST, WHOLE, FULL>(p, out, f, c0 + j * STEP < n && f < p.W, rest[j], last ? o0 : y[0][0], last ? o1 : y[0][1],
+                        last ? y[1][0] : o0, last ? y[1][1] : o1);
   }
 }
 
@@ -258,7 +296,9 @@ DEVI void store_row(const Args& p, const Item& q, const float* st, int c, int ti
     y = silu(y) * u;
   }
   const int64_t row = q.row0 + c;
-  p.out[row * p.out_ld + f] = __float2bfloat16_rn(finish(p, y, row, f, true));
+  if (p.scale) y *= p.scale[row];
+  if (p.res) y += __bfloat162float(p.res[row * p.res_ld + f]);
+  p.out[row * p.out_ld + f] = __float2bfloat16_rn(y);
 }
 
 // PAIR: two CTAs share a tile of 256 weight rows; each stages its 128 and its half of the tile's rows, and the first one issues
@@ -312,7 +352,7 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Arg
   pdl_wait();
   for (int e = threadIdx.x; e <= p.E; e += THREADS) starts[e] = p.starts ? p.starts[e] : e ? p.R : 0;
   __syncthreads();
-  if (warp == 2) count_tiles(p, BN, tiles, starts, lane);
+  if (warp == 2) count_tiles(p, p.tile, tiles, starts, lane);
   tc_fence_before();
   __syncthreads();
   __syncwarp();
@@ -336,7 +376,7 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Arg
     uint32_t it = 0;
     for (int i = unit; i < items; i += units) {
       if (__any_sync(0xffffffffu, *abort)) break;          // the same answer in all lanes
-      const Item q = item_of(p, i, blocks, BN, SPAN, tiles, starts);
+      const Item q = item_of(p, i, blocks, p.tile, SPAN, tiles, starts);
       if (!in_order(q)) {
         if (lane == 0) atomicExch(p.status, (int)kErrBounds);
         give_up();
@@ -379,7 +419,7 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Arg
       const uint32_t acc_full1 = PAIR ? mapa_shared(smem_u32(&bars->acc_full[0]), 1) : 0;
       uint32_t it = 0, n = 0;
       for (int i = unit; i < items && !*abort; i += units, ++n) {
-        const Item q = item_of(p, i, blocks, BN, SPAN, tiles, starts);
+        const Item q = item_of(p, i, blocks, p.tile, SPAN, tiles, starts);
         const int ab = n & 1;
         if (!mbar_wait(&bars->acc_empty[ab], ((n >> 1) & 1) ^ 1, p.status)) { give_up(); break; }
         tc_fence_after();
@@ -431,11 +471,12 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Arg
     __syncwarp();
   } else if (warp < GATHER0) {
     const int quad = warp & 3, part = (warp - EPI0) / 4;   // 32 weight rows; columns 64 j + 32 part
+    const bool rest = p.scale || p.res;
     uint32_t acc_empty = smem_u32(&bars->acc_empty[0]);
     if (PAIR) acc_empty = mapa_shared(acc_empty, 0);
     uint32_t n = 0;
     for (int i = unit; i < items; i += units, ++n) {
-      const Item q = item_of(p, i, blocks, BN, SPAN, tiles, starts);
+      const Item q = item_of(p, i, blocks, p.tile, SPAN, tiles, starts);
       const int ab = n & 1;
       const int f0 = q.n0 + rank * HALF + quad * (HALF / 4);          // the warp's first feature
       float bias = 0.f;
@@ -478,7 +519,17 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Arg
             __syncwarp();
             if (lane == 0) arrive_at(acc_empty + ab * 8);
           }
-          store_columns<SWIGLU>(p, v, q.row0 + c0, min(32, q.rows - c0), f0, lane);
+          const int cols = min(32, q.rows - c0);
+          const bool whole = p.vec && f0 + HALF / 4 <= p.W;
+          if (whole && cols == 32) {
+            if (rest) store_columns<SWIGLU, true, true, true>(p, v, q.row0 + c0, cols, f0, lane);
+            else store_columns<SWIGLU, false, true, true>(p, v, q.row0 + c0, cols, f0, lane);
+          } else if (whole) {
+            if (rest) store_columns<SWIGLU, true, true, false>(p, v, q.row0 + c0, cols, f0, lane);
+            else store_columns<SWIGLU, false, true, false>(p, v, q.row0 + c0, cols, f0, lane);
+          } else {
+            store_columns<SWIGLU, true, false, false>(p, v, q.row0 + c0, cols, f0, lane);
+          }
         }
         if (32 * part >= q.rows && lane == 0) arrive_at(acc_empty + ab * 8);
       }
@@ -490,7 +541,7 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Arg
     uint32_t it = 0;
     for (int i = unit; i < items; i += units) {
       if (__any_sync(0xffffffffu, *abort)) break;
-      const Item q = item_of(p, i, blocks, BN, SPAN, tiles, starts);
+      const Item q = item_of(p, i, blocks, p.tile, SPAN, tiles, starts);
       if (!in_order(q)) break;                             // warp 0 says so
       const int bn = mma_rows(q) / (PAIR ? 2 : 1), first = rank * bn, mine = min(bn, q.rows - first);
       const __nv_bfloat16* src[EACH];
@@ -535,7 +586,7 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Arg
   if constexpr (SPLIT) {
     cluster_sync();                                        // every CTA's sums are staged
     if (unit < items && warp >= EPI0 && warp < EPI0 + 4 && !*abort) {
-      const Item q = item_of(p, unit, blocks, BN, SPAN, tiles, starts);
+      const Item q = item_of(p, unit, blocks, p.tile, SPAN, tiles, starts);
       const int tid = threadIdx.x - 32 * EPI0;
       float* sums = reinterpret_cast<float*>(smem);        // stage memory, which no load uses any more
       // rows share, share + splits, ... of the tile: the CTAs' sums in their order
@@ -703,7 +754,7 @@ torch::Tensor linear_fused(const torch::Tensor& x, const LinearBank& bank, const
   p.x = (const __nv_bfloat16*)x.data_ptr();
   p.x_ld = x.stride(0);
   p.R = R; p.T = x.size(0); p.k = k; p.E = E; p.N = N; p.W = W; p.K = K;
-  p.vec = (uintptr_t)p.out % 8 == 0 && (R == 1 || p.out_ld % 4 == 0);      // one row's stride says nothing
+  p.vec = ((uintptr_t)p.out | (uintptr_t)p.res) % 8 == 0 && (R == 1 || (p.out_ld | p.res_ld) % 4 == 0);   // one row's stride says nothing
   p.status = bank.status.data_ptr<int>();
   lf::RowMaps xm = {};
   if (!by_token)
@@ -712,27 +763,44 @@ torch::Tensor linear_fused(const torch::Tensor& x, const LinearBank& bank, const
                               lf::BK, 16 << i, CU_TENSOR_MAP_SWIZZLE_128B);
   auto stream = at::cuda::getCurrentCUDAStream();
   const int sms = lf::sm_count(x.get_device());
-  // Tile height: about twice the rows that an expert has on average, so that few experts need a second pass over their weights;
-  // above 64 rows CTA pairs, whose tiles are cut to 32 rows
-  const int64_t avg = (R + E - 1) / E, want = E == 1 ? R : 2 * avg;
-  const int bn = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 256;
-  const int span = (bank.swiglu ? 64 : 128) * (bn == 256 ? 2 : 1);
-  const int64_t blocks = (W + span - 1) / span, items = (std::min<int64_t>(E, R) + R / bn) * blocks;   // at most
+  const int64_t kb = (K + 63) / 64, half = bank.swiglu ? 64 : 128;
+  const auto blocks_of = [&](bool pair) { return (W + half * (pair ? 2 : 1) - 1) / (half * (pair ? 2 : 1)); };
+  const auto items_of = [&](bool pair, int64_t tile) { return (std::min<int64_t>(E, R) + R / tile) * blocks_of(pair); };   // at most
+  bool pair;
+  if (E > 1) {
+    // about twice the rows that an expert has on average, so that few experts need a second pass over their weights; above 64
+    // rows CTA pairs, whose MMAs are cut to 32 rows
+    const int64_t want = 2 * ((R + E - 1) / E);
+    p.tile = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 256;
+    pair = p.tile == 256;
+  } else {
+    // the height that takes the fewest cycles: waves of items x (k blocks x the longer of loads, at some 60 bytes a cycle and
+    // SM, and MMAs, 2 a row; start and end some 3000)
+    int64_t best = INT64_MAX;
+    p.tile = 16, pair = false;
+    for (int t = 16; t <= 256; t = t < 64 ? 2 * t : t + 32)
+      for (int two = t >= 64 && R > 32; two >= (t > 64); --two) {
+        const int64_t items = (R + t - 1) / t * blocks_of(two), units = two ? sms / 2 : sms;
+        const int64_t rows = std::min<int64_t>(t, R), stage = std::max<int64_t>((16384 + rows * 128 / (two ? 2 : 1)) / 60, 2 * rows);
+        const int64_t cost = (items + units - 1) / units * (kb * stage + 3000);
+        if (cost < best) best = cost, p.tile = t, pair = two;
+      }
+  }
+  const int64_t items = items_of(pair, p.tile);
   if (items >= (1ll << 30)) refuse("rows");
-  const unsigned n = (unsigned)std::min<int64_t>(items, bn == 256 ? sms / 2 : sms);
-  if (bn == 16) {
+  const unsigned n = (unsigned)std::min<int64_t>(items, pair ? sms / 2 : sms);
+  if (p.tile == 16) {
     // too few items for the SMs: clusters share the items' K, each CTA at least four 64-blocks
     unsigned splits = 1;
-    const int64_t kb = (K + 63) / 64;
     while (splits < 8 && items * splits * 2 <= sms && kb / (splits * 2) >= 4) splits *= 2;
     if (splits > 1) lf::run<16, false, true>(p, bank.swiglu, bank.wm, xm, dim3((unsigned)items, splits), dim3(1, splits), stream);
     else lf::run<16, false, false>(p, bank.swiglu, bank.wm, xm, dim3(n), dim3(1), stream);
-  } else if (bn == 32) {
-    lf::run<32, false, false>(p, bank.swiglu, bank.wm, xm, dim3(n), dim3(1), stream);
-  } else if (bn == 64) {
-    lf::run<64, false, false>(p, bank.swiglu, bank.wm, xm, dim3(n), dim3(1), stream);
-  } else {
+  } else if (pair) {
     lf::run<256, true, false>(p, bank.swiglu, bank.wm, xm, dim3(2 * n), dim3(2), stream);
+  } else if (p.tile == 32) {
+    lf::run<32, false, false>(p, bank.swiglu, bank.wm, xm, dim3(n), dim3(1), stream);
+  } else {
+    lf::run<64, false, false>(p, bank.swiglu, bank.wm, xm, dim3(n), dim3(1), stream);
   }
   return out;
 }
