@@ -48,6 +48,14 @@ class ModelConfig:
     num_experts_per_tok: int = 0
     moe_intermediate_size: int = 0
     shared_expert_intermediate_size: int = 0
+    # router: scores (softmax | sigmoid), a bias per expert for balance that only ranks, the best moe_top_groups of
+    # moe_num_groups groups of experts, weights divided by their sum, times a factor
+    moe_score: str = "softmax"
+    moe_router_bias: bool = False
+    moe_num_groups: int = 1
+    moe_top_groups: int = 1
+    moe_renormalize: bool = True
+    moe_routed_scale: float = 1.0
     # misc
     rms_norm_eps: float = 1e-6
     max_position_embeddings: int = 262144
@@ -239,6 +247,9 @@ def config_from_hf(d: dict) -> ModelConfig:
         num_experts=tc.get("num_experts", 0), num_experts_per_tok=tc.get("num_experts_per_tok", 0),
         moe_intermediate_size=tc.get("moe_intermediate_size", 0),
         shared_expert_intermediate_size=tc.get("shared_expert_intermediate_size", 0),
+        moe_score=tc.get("scoring_func") or "softmax", moe_router_bias=tc.get("topk_method") == "noaux_tc",
+        moe_num_groups=tc.get("n_group") or 1, moe_top_groups=tc.get("topk_group") or 1,
+        moe_renormalize=tc.get("norm_topk_prob") is not False, moe_routed_scale=tc.get("routed_scaling_factor") or 1.0,
         rms_norm_eps=tc.get("rms_norm_eps", 1e-6),
         tie_word_embeddings=tc.get("tie_word_embeddings", False))
 

@@ -1,11 +1,13 @@
-"""Mixture-of-experts block (256 routed experts, softmax top-8 with
-renormalised weights, one shared expert behind a sigmoid gate; Qwen3-Next MoE semantics, served
-TP-sharded by the reference through vLLM fused_moe, ``moe-configs/E=256,...``).
+"""Mixture-of-experts block (256 routed experts, softmax top-8 with renormalised weights, one shared
+expert behind a sigmoid gate; Qwen3-Next MoE semantics, served TP-sharded by the reference through
+vLLM fused_moe, ``moe-configs/E=256,...``; sigmoid scores, a balance bias and expert groups by
+configuration).
 
-Routed experts run as ONE grouped W4A8 launch per projection: tokens are dispatched into an
-expert-sorted buffer, a work table lists (expert, row tile) pairs, and the tcgen05 grouped GEMM
-(``mxfp4_grouped_gemm`` in ``csrc/mxfp4_gemm.cu``) reads each expert's MXFP4 weights from one
-stacked tensor.
+On the GPU: ``K.moe_route`` picks the experts, ``K.moe_plan`` sorts the (token, slot) pairs by expert,
+and routed experts run as ONE launch per projection -- the tcgen05 grouped W4A8 GEMM
+(``mxfp4_grouped_gemm`` in ``csrc/mxfp4_gemm.cu``) over rows gathered in that order, or the bf16
+product of ``csrc/linear_fused.cu``, which picks its rows by token and ends in SwiGLU.
+``K.moe_combine`` adds the rows up per token.
 
 Expert parallelism: the tensor-parallel ranks already hold every token of the step (attention is
 head-sharded), so each of the `size` ranks owns E/size experts and a 1/size slice of the shared
@@ -22,7 +24,7 @@ import torch
 from ..config import ModelConfig
 from ..ops import kernels as K
 from ..quant.mxfp4 import MXFP4Weight, cat_rows
-from .layers import Linear
+from .layers import Linear, LinearBank
 
 
 class MoEBlock:
@@ -68,6 +70,23 @@ class MoEBlock:
         s0, per = tp.shard(Is)
         self.shared_down = make_linear(slice_cols(wsd, s0, per), quant, "sh_down")
         self.shared_gate = W.tensor(prefix + "shared_gate", (1, H), "linear_bf16").to(torch.bfloat16)
+        # added to the scores when experts are ranked, not to the weights
+        self.router_bias = W.tensor(prefix + "router_bias", (E,), "router_bias").float() if cfg.moe_router_bias else None
+        self._prepare()
+
+    def _prepare(self):
+        """On the GPU: router and shared gate as one weight [rows in whole 8, H]; bf16 weights as ``K.linear_fused`` takes
+        them, in place -- the shared expert's two products (None in another format) and the routed experts'."""
+        self._gates = self._banks = None
+        if not self.router.is_cuda:
+            return
+        both = torch.cat([self.router, self.shared_gate])
+        self._gates = torch.cat([both, both.new_zeros(-both.shape[0] % 8, self.H)])
+        if self.dense_gu is not None and self.H % 8 == 0 and self.I % 8 == 0:
+            up, down = self.shared_gate_up, self.shared_down
+            bf16 = up.quant == "bf16" and down.K % 8 == 0
+            self._banks = (LinearBank(up.w, act="swiglu") if bf16 else None, LinearBank(down.w) if bf16 else None,
+                           LinearBank(self.dense_gu, act="swiglu"), LinearBank(self.dense_dn))
 
     def to(self, device):
         for k, v in list(vars(self).items()):
@@ -77,16 +96,26 @@ class MoEBlock:
                 setattr(self, k, v.to(device))
             elif isinstance(v, Linear):
                 v.to(device)
+        self._prepare()
         return self
 
     # ------------------------------------------------------------------------------------------
+    def _choose(self, logits: torch.Tensor):
+        cfg = self.cfg
+        return K.moe_route(logits, self.top_k, score=cfg.moe_score, bias=self.router_bias, groups=cfg.moe_num_groups,
+                           top_groups=cfg.moe_top_groups, renormalize=cfg.moe_renormalize, scale=cfg.moe_routed_scale)
+
     def route(self, x_bf16: torch.Tensor):
-        """softmax over all experts, top-k, renormalised weights -> (ids [T,k], weights [T,k])."""
-        logits = x_bf16.float() @ self.router.float().t()
-        p = torch.softmax(logits, -1)
-        w, ids = torch.topk(p, self.top_k, dim=-1)
-        w = w / w.sum(-1, keepdim=True)
-        return ids, w
+        """Scores over all experts, top-k, weights (``K.moe_route``) -> (ids [T,k], weights [T,k])."""
+        return self._choose(x_bf16.float() @ self.router.float().t())
+
+    def _route_and_gate(self, xb: torch.Tensor):
+        """-> (ids, weights, the shared expert's gate before its sigmoid [T]); on the GPU the router and the gate are one
+        product of bf16 numbers, summed in 32 bits."""
+        if not xb.is_cuda:
+            return *self.route(xb), (xb.float() @ self.shared_gate.float().t())[:, 0]
+        logits = torch.mm(xb, self._gates.t(), out_dtype=torch.float32)
+        return *self._choose(logits[:, :self.E]), logits[:, self.E]
 
     def forward(self, x):
         """x: (q, scale) from the fused producer or bf16 [T, H] -> bf16 [T, H]."""
@@ -96,13 +125,23 @@ class MoEBlock:
         else:
             xb = x
             q, s = K.quant_fp8(x) if self.quant == "mxfp4" else (None, None)
-        T = xb.shape[0]
-        ids, w = self.route(xb)
-        routed = self._experts(xb, (q, s), ids, w)
+        ids, w, gate = self._route_and_gate(xb)
+        if (xb.is_cuda and self._banks is not None and self._banks[0] is not None
+                and not (self.shared_gate_up._adapted() or self.shared_down._adapted())):
+            # bf16 weights: SwiGLU ends the shared expert's first product, gate and routed sum its second
+            up, down, _, _ = self._banks
+            routed = self._experts(xb, (q, s), ids, w)
+            return K.linear_fused(K.linear_fused(xb, up), down, scale=torch.sigmoid(gate), residual=routed, out=routed)
         sh = self.shared_down(K.silu_mul_quant(self.shared_gate_up((q, s) if q is not None else xb))
                               if self.quant == "mxfp4" else K.silu_mul(self.shared_gate_up(xb)))
-        gate = torch.sigmoid(xb.float() @ self.shared_gate.float().t())
-        return (routed.float() + gate * sh.float()).to(torch.bfloat16)
+        if self.ep is None and self._on_kernels(xb):
+            return self.local_experts(xb, (q, s), ids, w, shared=sh, gate=gate)
+        routed = self._experts(xb, (q, s), ids, w)
+        return (routed.float() + torch.sigmoid(gate)[:, None] * sh.float()).to(torch.bfloat16)
+
+    def _on_kernels(self, x: torch.Tensor) -> bool:
+        """The routed experts run as grouped products (bf16 rows have to be whole 16 bytes)."""
+        return x.is_cuda and (self.w_gate_up is not None or self._banks is not None)
 
     def _experts(self, xb, qs, ids, w):
         if self.ep is not None:
@@ -122,6 +161,11 @@ class MoEBlock:
         if self.w_gate_up is not None and le.is_cuda:
             y[order] = K.moe_grouped_mlp(q[order], s[order], counts, self.w_gate_up, self.w_down,
                                          self.I, self.H)
+            return y
+        if self._on_kernels(le):
+            _, _, up, down = self._banks
+            plan = K.moe_plan(le[:, None], self.e_local)
+            y[plan.order.long()] = K.linear_fused(K.linear_fused(xb, up, plan=plan, by_token=True), down, plan=plan)
             return y
         starts = torch.cumsum(counts, 0) - counts
         for e in range(self.e_local):
@@ -143,31 +187,28 @@ class MoEBlock:
                 y[idx] = (a @ self.dense_dn[e].float().t()).to(torch.bfloat16)
         return y
 
-    def local_experts(self, xb, qs, ids, w):
+    def local_experts(self, xb, qs, ids, w, shared=None, gate=None):
         """Experts [e0, e0+e_local) applied to every (token, slot) routed to them; the other
-        slots contribute zero (they belong to another rank's experts)."""
+        slots contribute zero (they belong to another rank's experts).  As grouped products,
+        shared rows times sigmoid(gate) join the sum."""
+        if self._on_kernels(xb):
+            # fixed shapes, no host sync (CUDA-graph safe)
+            if self.w_gate_up is None:
+                _, _, up, down = self._banks
+                plan = K.moe_plan(ids, self.e_local, first=self.e0)
+                rows = K.linear_fused(K.linear_fused(xb, up, plan=plan, by_token=True), down, plan=plan)
+            else:
+                plan = K.moe_plan(ids, self.e_local, first=self.e0,
+                                  tile=K.moe_tile(ids.numel(), self.e_local))
+                q, s = K.moe_gather(qs, plan)
+                rows = K.moe_grouped_mlp(q, s, plan, self.w_gate_up, self.w_down, self.I, self.H)
+            return K.moe_combine(rows, plan, w, shared=shared, gate=gate)
         T, k = ids.shape
         dev = xb.device
         flat_e = ids.reshape(-1) - self.e0
         flat_t = torch.arange(T, device=dev).repeat_interleave(k)
         flat_w = w.reshape(-1)
         own = (flat_e >= 0) & (flat_e < self.e_local)
-        if self.w_gate_up is not None and xb.is_cuda:
-            # fixed shapes, no host sync (CUDA-graph safe): foreign slots sort to the end and
-            # are not covered by any work item
-            key = torch.where(own, flat_e, torch.full_like(flat_e, self.e_local))
-            order = torch.argsort(key, stable=True)
-            st = flat_t[order]
-            sw = torch.where(own[order], flat_w[order], torch.zeros_like(flat_w))
-            # scatter-add, not bincount: bincount reads its maximum back to the host, which a
-            # CUDA-graph capture of the decode step cannot contain
-            counts = torch.zeros(self.e_local + 1, dtype=torch.long, device=dev).scatter_add_(
-                0, key, torch.ones_like(key))[:self.e_local]
-            q, s = qs
-            y = K.moe_grouped_mlp(q[st], s[st], counts, self.w_gate_up, self.w_down, self.I, self.H)
-            out = torch.zeros(T, self.H, dtype=torch.float32, device=dev)
-            out.index_add_(0, st, y.float() * sw[:, None])
-            return out.to(torch.bfloat16)
         out = torch.zeros(T, self.H, dtype=torch.float32, device=dev)
         flat_e, flat_t, flat_w = flat_e[own], flat_t[own], flat_w[own]
         if flat_e.numel() == 0:

@@ -9,7 +9,7 @@ The model asks for tensors by canonical name, always in this engine's layout (fu
   ATTN : qkv [Hq*2hd + 2Hkv*hd, H] as [q0,gate0,q1,gate1,...|k|v],  q_norm/k_norm [hd],
          o_proj [H, Hq*hd]
   MLP  : gate_up [2I, H] as [gate|up],  down [H, I]
-  MoE  : router [E, H],  experts.{e}.gate_up / down,  shared.gate_up / down,  shared_gate [1, H]
+  MoE  : router [E, H] (+ router_bias [E]),  experts.{e}.gate_up / down,  shared.gate_up / down,  shared_gate [1, H]
 
 Linear weights come back either as float tensors (quantized by the model at load) or as
 ``MXFP4Weight`` (pre-quantized checkpoints)."""
@@ -58,6 +58,8 @@ class RandomWeights:
         if kind == "A_log":
             return torch.log(torch.rand(*shape, generator=g, device=d) * 15 + 1).float()
         if kind == "dt_bias":
+            return (0.1 * torch.randn(*shape, generator=g, device=d)).float()
+        if kind == "router_bias":
             return (0.1 * torch.randn(*shape, generator=g, device=d)).float()
         if kind == "embed":
             return (torch.randn(*shape, generator=g, device=d) * self.cfg.init_std).to(torch.bfloat16)

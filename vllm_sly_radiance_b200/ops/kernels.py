@@ -334,12 +334,23 @@ def moe_work_items(counts: torch.Tensor, bn: int, max_items: int) -> torch.Tenso
     return torch.stack([e, starts[e] + j * bn, rows], 1).to(torch.int32).contiguous()
 
 
-def moe_grouped_gemm(q, s, w, n_per_group: int, counts: torch.Tensor) -> torch.Tensor:
-    """Expert-sorted rows (q, s) x stacked expert MXFP4 weights -> [R, n_per_group] bf16."""
+def moe_tile(rows: int, experts: int) -> int:
+    """Row tile of the block-scaled grouped product for `rows` rows of `experts` experts."""
+    avg = max(1, rows // max(1, experts))
+    return 16 if avg <= 16 else 32 if avg <= 32 else 64 if avg <= 64 else 128 if avg <= 128 else 256
+
+
+def moe_grouped_gemm(q, s, w, n_per_group: int, counts) -> torch.Tensor:
+    """Expert-sorted rows (q, s) x stacked expert MXFP4 weights -> [R, n_per_group] bf16.  counts: rows of each
+    expert, or a MoEPlan with work items, whose rows behind the last one are not written."""
     R = q.shape[0]
+    if isinstance(counts, MoEPlan):
+        out = torch.empty(R, n_per_group, dtype=torch.bfloat16, device=q.device)
+        ext().mxfp4_grouped_gemm(q, s, w.packed, w.sf, out, counts.items, counts.tile, n_per_group,
+                                 status_word(q.device))
+        return out
     E = counts.shape[0]
-    avg = max(1, R // max(1, counts.numel()))
-    bn = 16 if avg <= 16 else 32 if avg <= 32 else 64 if avg <= 64 else 128 if avg <= 128 else 256
+    bn = moe_tile(R, E)
     max_items = (R + bn - 1) // bn + E
     items = moe_work_items(counts, bn, max_items)
     out = torch.zeros(R, n_per_group, dtype=torch.bfloat16, device=q.device)   # uncovered rows = 0

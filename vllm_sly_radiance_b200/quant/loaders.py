@@ -291,12 +291,13 @@ class CheckpointWeights:
              "q_norm": "self_attn.q_norm.weight", "k_norm": "self_attn.k_norm.weight",
              "A_log": "linear_attn.A_log", "dt_bias": "linear_attn.dt_bias",
              "norm_w": "linear_attn.norm.weight", "router": "mlp.gate.weight",
+             "router_bias": "mlp.gate.e_score_correction_bias",
              "shared_gate": "mlp.shared_expert_gate.weight"}
         if leaf == "conv_w":
             w = self.raw(self._hf(L + "linear_attn.conv1d.weight"))
             return w.reshape(w.shape[0], -1).to(torch.bfloat16)
         t = self.raw(self._hf(L + m[leaf]))
-        if leaf in ("A_log", "dt_bias", "router", "shared_gate"):
+        if leaf in ("A_log", "dt_bias", "router", "router_bias", "shared_gate"):
             return t.float()
         return t.to(torch.bfloat16)
 
