@@ -147,15 +147,15 @@ void allreduce_oneshot(std::vector<int64_t> peers, int64_t rank, torch::Tensor i
 void lora_bind(pybind11::module_& m);
 void cache_moves_bind(pybind11::module_& m);
 void linear_fused_bind(pybind11::module_& m);
-std::vector<torch::Tensor> moe_route(const torch::Tensor& logits, int64_t k, bool sigmoid,
+std::tuple<torch::Tensor, torch::Tensor> moe_route(const torch::Tensor& logits, int64_t k, bool sigmoid,
                                      const c10::optional<torch::Tensor>& bias, int64_t groups, int64_t top_groups, bool renorm,
                                      double scale);
 std::vector<torch::Tensor> moe_plan(const torch::Tensor& ids, int64_t E, int64_t first, int64_t tile);
 void moe_gather(const torch::Tensor& x, const c10::optional<torch::Tensor>& xs, const torch::Tensor& order, int64_t k,
                 const torch::Tensor& out, const c10::optional<torch::Tensor>& out_s, const torch::Tensor& status);
-void moe_combine(const torch::Tensor& rows, const torch::Tensor& pos, const torch::Tensor& w,
-                 const c10::optional<torch::Tensor>& shared, const c10::optional<torch::Tensor>& gate, const torch::Tensor& out,
-                 const torch::Tensor& status);
+torch::Tensor moe_combine(const torch::Tensor& rows, const torch::Tensor& pos, const torch::Tensor& w,
+                          const c10::optional<torch::Tensor>& shared, const c10::optional<torch::Tensor>& gate,
+                          const torch::Tensor& status);
 }  // namespace rad
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {

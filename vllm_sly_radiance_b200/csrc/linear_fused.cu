@@ -9,6 +9,7 @@
 // Warp 0 fills the ring of 64-k stages, warp 1 issues the MMAs into one of two accumulators in tensor memory, four warps carry
 // the other one out through shared memory, so that rows leave in 16-byte pieces.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -735,7 +736,7 @@ torch::Tensor linear_fused(const torch::Tensor& x, const LinearBank& bank, const
   if (res.has_value() && !rows_of(*res)) refuse("residual bf16, of the output's shape");
   if (out_.has_value() && (!rows_of(*out_) || (R > 1 && out_->stride(0) < W))) refuse("out bf16, of the output's shape");
   const at::cuda::CUDAGuard guard(x.device());
-  torch::Tensor out = out_.has_value() ? *out_ : torch::empty({R, W}, x.options());
+  torch::Tensor out = out_.has_value() ? *out_ : (torch::Tensor)at::detail::empty_cuda({R, W}, at::kBFloat16, x.device(), c10::nullopt);
   if (R == 0) return out;
   if (out_.has_value()) {
     const bool same = res.has_value() && res->data_ptr() == out.data_ptr() && res->stride(0) == out.stride(0);

@@ -6,10 +6,12 @@
 //   gather   row r = the activations of its token
 //   combine  out[t] = sum_j w[t, j] rows[pos[t, j]] (+ sigmoid(gate[t]) shared[t])
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp16.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "common.cuh"
@@ -30,7 +32,7 @@ DEVI float to_f(__half x) { return __half2float(x); }
 // and log2(lanes) exchanges give every group's value at once, and the lowest lane among equals has the lowest index.
 // Values become whole numbers of the same order (0: no candidate, 1: NaN, then -inf and up), whose warp maximum is one
 // instruction.  Without a bias the logits themselves are ranked, which is the scores' order.  With a bias the scores enter the
-// order: they are computed in 32 bits, and once more in 64 for the few tokens (about one in 200) where two candidates, or two
+// order: they are computed in 32 bits, and once more in 64 for the few tokens (about one in 500) where two candidates, or two
 // groups, lie so near that the rounding could have turned them.
 // ---------------------------------------------------------------------------------------------
 struct RouteArgs {
@@ -60,108 +62,162 @@ DEVI uint64_t warp_max_key(uint64_t v) {
   const uint32_t lo = __reduce_max_sync(FULL, (uint32_t)(v >> 32) == hi ? (uint32_t)v : 0u);
   return (uint64_t)hi << 32 | lo;
 }
-template <typename F> struct KeyOf { using T = uint32_t; };
-template <> struct KeyOf<double> { using T = uint64_t; };
+DEVI float value_of(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7fffffffu : ~k); }       // of a key above 1
 
 DEVI float exp_of(float x) { return expf(x); }
 DEVI double exp_of(double x) { return exp(x); }
 
-// Lane j < k ends with the j-th expert and its score before renormalisation.  False: 32 bits could not tell the order.
-template <typename F, int V, bool BIAS>
-DEVI bool choose(const RouteArgs& p, const float (&l)[V], int e0, int n, float top, int lane, int& expert, F& score) {
-  using Key = typename KeyOf<F>::T;
-  // errors of a 32-bit score (below 2^-21 for scores up to 1) and of its sum with the bias, with a margin
-  const F tol = sizeof(F) == 8 ? F(0) : F(1.0 / (1 << 19));
-  F total = 0;                                             // of the softmax
-  if (!p.sigmoid && (BIAS || !p.renorm)) {
+// A score; without a bias and to be renormalised, a softmax's but for its sum, as only ratios matter
+template <typename F, bool BIAS> DEVI F score_of(const RouteArgs& p, float x, float top, F total) {
+  if (p.sigmoid) return F(1) / (F(1) + exp_of(-(F)x));
+  const F s = exp_of((F)x - (F)top);
+  return BIAS || !p.renorm ? (total > 0 ? s / total : total) : s;
+}
+
+// Best two of a lane's candidates -> of its group's
+template <typename F> DEVI void best_two(F& b1, F& b2, int lanes) {
+  for (int o = lanes >> 1; o > 0; o >>= 1) {
+    const F o1 = __shfl_xor_sync(FULL, b1, o), o2 = __shfl_xor_sync(FULL, b2, o);
+    const F lo = o1 < b1 ? o1 : b1, hi2 = o2 > b2 ? o2 : b2;
+    b1 = o1 > b1 ? o1 : b1;
+    b2 = lo > hi2 ? lo : hi2;
+  }
+}
+
+// The choice in 64 bits, with a bias -> the expert of lane j < k.  A call of its own, so that its registers do not cost the ordinary
+// path its warps.
+template <typename L, int V>
+__device__ __noinline__ int choose_wide(const RouteArgs& p, const L* row, int e0, int n, float top, int lane) {
+  double c[V], total = 1.0;
+  if (!p.sigmoid) {
+    total = 0.0;
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (i < n) total += exp_of((F)l[i] - (F)top);
+      if (i < n) total += exp((double)to_f(row[e0 + i]) - (double)top);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(FULL, total, o);
   }
-  auto score_of = [&](float x) -> F {
-    if (p.sigmoid) return F(1) / (F(1) + exp_of(-(F)x));
-    const F s = exp_of((F)x - (F)top);
-    return BIAS || !p.renorm ? (total > 0 ? s / total : total) : s;
-  };
-  bool clear = true;
-  F c[V];
+  double b1 = -INFINITY, b2 = -INFINITY;
+  // in step for all lanes: eight independent chains of double operations, where a loop waited for one after the other
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    c[i] = 0;
-    if (i < n) c[i] = BIAS ? score_of(l[i]) + (F)p.bias[e0 + i] : (F)l[i];
-  }
-  if (p.groups > 1) {
-    // the group's value at each of its lanes
-    F b1 = -INFINITY, b2 = -INFINITY;
+  for (int i = 0; i < V; ++i) c[i] = score_of<double, true>(p, i < n ? to_f(row[e0 + i]) : 0.f, top, total);
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (i < n) {
-        const F lo = c[i] < b1 ? c[i] : b1;
-        b1 = c[i] > b1 ? c[i] : b1;
-        b2 = lo > b2 ? lo : b2;
-      }
-    for (int o = p.lanes >> 1; o > 0; o >>= 1) {
-      const F o1 = __shfl_xor_sync(FULL, b1, o), o2 = __shfl_xor_sync(FULL, b2, o);
-      const F lo = o1 < b1 ? o1 : b1, hi2 = o2 > b2 ? o2 : b2;
-      b1 = o1 > b1 ? o1 : b1;
-      b2 = lo > hi2 ? lo : hi2;
+  for (int i = 0; i < V; ++i)
+    if (i < n) {
+      const double x = c[i] += (double)p.bias[e0 + i];
+      const double lo = x < b1 ? x : b1;
+      b1 = x > b1 ? x : b1;
+      b2 = lo > b2 ? lo : b2;
     }
-    const F value = BIAS ? b1 + b2 : b1;
-    const Key key = key_of(value);
+  if (p.groups > 1) {
+    best_two(b1, b2, p.lanes);
+    const double value = b1 + b2;
+    const uint64_t key = key_of(value);
     const int mine = lane / p.lanes;
     int rank = 0;
+#pragma unroll 1
     for (int g = 0; g < p.groups; ++g) {
-      const F other = __shfl_sync(FULL, value, g * p.lanes);
-      const Key ko = key_of(other);
-      rank += ko > key || (ko == key && g < mine);
-      if (BIAS && sizeof(F) == 4 && g != mine && mine < p.groups) {
-        const F d = value > other ? value - other : other - value;
-        clear &= d > tol * (F(2) + (value < 0 ? -value : value));
-      }
+      const uint64_t o = key_of(__shfl_sync(FULL, value, g * p.lanes));
+      rank += o > key || (o == key && g < mine);
     }
     if (rank >= p.top_groups) n = 0;
   }
-  Key best = 0;
-  int at = 0;
-  uint32_t taken = 0;
-  auto rescan = [&]() {
-    best = 0;
+  uint64_t keys[V];
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const Key q = i < n && !(taken >> i & 1) ? key_of(c[i]) : Key(0);
-      if (q > best) best = q, at = i;
+  for (int i = 0; i < V; ++i) keys[i] = i < n ? key_of(c[i]) : 0;
+  int expert = 0;
+#pragma unroll 1
+  for (int j = 0; j < p.k; ++j) {
+    uint64_t best = 0;
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (keys[i] > best) best = keys[i], at = i;
+    const uint64_t m = warp_max_key(best);
+    const int w = __ffs(__ballot_sync(FULL, best == m)) - 1, ew = __shfl_sync(FULL, e0 + at, w);
+    if (lane == j) expert = ew;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (lane == w && i == at) keys[i] = 0;
+  }
+  return expert;
+}
+
+// Lane j < k ends with the j-th expert.  False: 32 bits could not tell the order.  total: of the softmax, where it is needed
+template <int V, bool BIAS>
+DEVI bool choose(const RouteArgs& p, const float (&l)[V], int e0, int n, float top, int lane, int& expert, float& total) {
+  // Two candidates' error, relative to 1 + c: a sigmoid is off by at most 2^-22 (exp 2^-23, sum 2^-24, quotient 2^-24), a softmax
+  // by 2^-20 of it (its sum over 13 additions in a row), their sum with the bias by another 2^-24 of c; each with a margin
+  const float tol = p.sigmoid ? 1.f / (1 << 21) : 1.f / (1 << 19);
+  total = 0.f;
+  if (!p.sigmoid && (BIAS || !p.renorm)) {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < n) total += expf(l[i] - top);
+    total = warp_sum(total);
+  }
+  bool clear = true;
+  float c[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    c[i] = 0.f;
+    if (i < n) c[i] = BIAS ? score_of<float, BIAS>(p, l[i], top, total) + p.bias[e0 + i] : l[i];
+  }
+  if (p.groups > 1) {
+    float b1 = -INFINITY, b2 = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < n) {
+        const float lo = c[i] < b1 ? c[i] : b1;
+        b1 = c[i] > b1 ? c[i] : b1;
+        b2 = lo > b2 ? lo : b2;
+      }
+    best_two(b1, b2, p.lanes);
+    const float value = BIAS ? b1 + b2 : b1;
+    const uint32_t key = key_of(value);
+    const int mine = lane / p.lanes;
+    int rank = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const float other = __shfl_sync(FULL, value, g * p.lanes);
+      const uint32_t ko = key_of(other);
+      rank += ko > key || (ko == key && g < mine);
+      if (BIAS && g != mine && mine < p.groups) clear &= fabsf(value - other) > tol * (2.f + fabsf(value));
     }
-  };
-  rescan();
-  F before = 0;
-  float chosen = 0.f;                                      // the logit
-  for (int j = 0; j < p.k + (BIAS && sizeof(F) == 4 ? 1 : 0); ++j) {
-    const Key m = warp_max_key(best);
-    if (m == 0) break;                                     // the candidate behind the last one does not exist
-    const int w = __ffs(__ballot_sync(FULL, best == m)) - 1;
-    float lw = l[0];
-    F cw = c[0];
+    if (rank >= p.top_groups) n = 0;
+  }
+  uint32_t key[V], best = 0;
+  int at = 0;
 #pragma unroll
-    for (int i = 1; i < V; ++i)
-      if (i == at) lw = l[i], cw = c[i];
-    const int ew = __shfl_sync(FULL, e0 + at, w);
-    lw = __shfl_sync(FULL, lw, w);
-    if (BIAS && sizeof(F) == 4) {
-      cw = __shfl_sync(FULL, cw, w);
-      if (j > 0) clear &= before - cw > tol * (F(1) + (cw < 0 ? -cw : cw));
+  for (int i = 0; i < V; ++i) {
+    key[i] = i < n ? key_of(c[i]) : 0u;
+    if (key[i] > best) best = key[i], at = i;
+  }
+  float before = 0.f;
+  for (int j = 0; j < p.k + (BIAS ? 1 : 0); ++j) {
+    const uint32_t m = warp_max_key(best);
+    if (m == 0) break;                                     // the candidate behind the last one does not exist
+    const int w = __ffs(__ballot_sync(FULL, best == m)) - 1, ew = __shfl_sync(FULL, e0 + at, w);
+    if (BIAS) {
+      const float cw = m > 1 ? value_of(m) : NAN;
+      if (j > 0) clear &= before - cw > tol * (1.f + fabsf(cw));
       before = cw;
     }
-    if (lane == j && j < p.k) expert = ew, chosen = lw;
-    if (lane == w) taken |= 1u << at, rescan();
+    if (lane == j && j < p.k) expert = ew;
+    if (lane == w) {
+      best = 0;
+      const int gone = at;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        if (i == gone) key[i] = 0;
+        if (key[i] > best) best = key[i], at = i;
+      }
+    }
   }
-  score = lane < p.k ? score_of(chosen) : F(0);
   return __all_sync(FULL, clear);
 }
 
 template <typename L, int V, bool BIAS>
-__global__ void __launch_bounds__(256) route_kernel(const __grid_constant__ RouteArgs p) {
+__global__ void __launch_bounds__(256, V <= 8 ? 4 : 2) route_kernel(const __grid_constant__ RouteArgs p) {
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x % 32, t = blockIdx.x * 8 + threadIdx.x / 32;
@@ -195,15 +251,10 @@ __global__ void __launch_bounds__(256) route_kernel(const __grid_constant__ Rout
   nan = __any_sync(FULL, nan || (!p.sigmoid && top == INFINITY));
   if (top == -INFINITY) top = 0.f;                         // every expert masked: scores of zero
   int expert = 0;
-  float s = 0.f;
-  const bool clear = choose<float, V, BIAS>(p, l, e0, n, top, lane, expert, s);
-  if constexpr (BIAS) {
-    if (!clear) {
-      double d;
-      choose<double, V, BIAS>(p, l, e0, n, top, lane, expert, d);
-      s = (float)d;
-    }
-  }
+  float total, s = 0.f;
+  const bool clear = choose<V, BIAS>(p, l, e0, n, top, lane, expert, total);
+  if (BIAS && !clear) expert = choose_wide<L, V>(p, row, e0, n, top, lane);
+  if (lane < p.k) s = score_of<float, BIAS>(p, to_f(row[expert]), top, total);
   if (p.renorm) {
     const float sum = warp_sum(s);
     s = sum > 0.f ? s / sum : 0.f;
@@ -217,11 +268,12 @@ __global__ void __launch_bounds__(256) route_kernel(const __grid_constant__ Rout
 // ---------------------------------------------------------------------------------------------
 // plan: one cluster.  Every warp owns neighbouring pairs; it counts them by expert, the counts are added up over warps and
 // CTAs (distributed shared memory), and a second pass over the pairs hands out the rows.  Equal experts of 32 pairs find one
-// another by a warp match, so nothing is atomic and the rows come in the pairs' order.
+// another by a vote per bit of their number (a warp match instead took 12.2 us for 4096 pairs, this 8.7), so nothing is atomic
+// and the rows come in the pairs' order.
 // ---------------------------------------------------------------------------------------------
 struct PlanArgs {
   const void* ids;
-  int R, k, E, first, seg;                                 // pairs, experts of this rank, pairs of a warp
+  int R, k, E, first, seg, warps, bits;                    // pairs, experts of this rank, pairs of a warp, warps that have some
   bool wide;                                               // ids of 64 bits
   int* order;
   int* pos;
@@ -230,12 +282,22 @@ struct PlanArgs {
   int* items;                                              // (expert, first row, rows) per tile of `tile` rows
   int tile, max_items;
 };
-constexpr int PLAN_WARPS = 32;
+constexpr int PLAN_WARPS = 32, PLAN_CTAS = 16, PLAN_AHEAD = 8;
 
 DEVI int plan_expert(const PlanArgs& p, int f, int end) {
   if (f >= end) return -1;
   const int64_t e = (p.wide ? static_cast<const int64_t*>(p.ids)[f] : (int64_t) static_cast<const int*>(p.ids)[f]) - p.first;
   return e >= 0 && e < p.E ? (int)e : -1;
+}
+
+// lanes with the same expert; those without one (-1) are in nobody's set but their own
+DEVI unsigned same_expert(int e, int bits) {
+  unsigned same = __ballot_sync(FULL, e >= 0);
+  for (int b = 0; b < bits; ++b) {
+    const unsigned set = __ballot_sync(FULL, e >> b & 1);
+    same &= e >> b & 1 ? set : ~set;
+  }
+  return same;
 }
 
 // exclusive sums of v over the block's threads (1024); total: of all
@@ -263,31 +325,37 @@ DEVI int block_scan(int v, int* warp_sums, int& total) {
 __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ PlanArgs p) {
   extern __shared__ int smem[];
   int* cnt = smem;                                         // [warps][E]
-  int* tot = cnt + PLAN_WARPS * p.E;                       // [E] of this CTA
+  int* tot = cnt + p.warps * p.E;                          // [E] of this CTA
   int* base = tot + p.E;                                   // [E] first row of this CTA's pairs
   __shared__ int warp_sums[32];
   const int lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const uint32_t rank = cluster_ctarank();
   const int ctas = gridDim.x;
   pdl_trigger();
-  for (int i = threadIdx.x; i < PLAN_WARPS * p.E; i += blockDim.x) cnt[i] = 0;
+  for (int i = threadIdx.x; i < p.warps * p.E; i += blockDim.x) cnt[i] = 0;
   __syncthreads();
   pdl_wait();
   int* mine = cnt + warp * p.E;
-  const int64_t f0 = ((int64_t)rank * PLAN_WARPS + warp) * p.seg;
-  const int lo = (int)min(f0, (int64_t)p.R), hi = (int)min(f0 + p.seg, (int64_t)p.R);
-  for (int f = lo + lane; f - lane < hi; f += 32) {
-    const int e = plan_expert(p, f, hi);
-    const unsigned same = __match_any_sync(FULL, e);
-    if (e >= 0 && lane == __ffs(same) - 1) mine[e] += __popc(same);
-    __syncwarp();
+  const int64_t f0 = ((int64_t)rank * p.warps + warp) * p.seg;
+  const int lo = warp < p.warps ? (int)min(f0, (int64_t)p.R) : p.R, hi = warp < p.warps ? (int)min(f0 + p.seg, (int64_t)p.R) : p.R;
+  for (int f = lo; f < hi; f += 32 * PLAN_AHEAD) {
+    int x[PLAN_AHEAD];
+#pragma unroll
+    for (int u = 0; u < PLAN_AHEAD; ++u) x[u] = plan_expert(p, f + 32 * u + lane, hi);
+#pragma unroll
+    for (int u = 0; u < PLAN_AHEAD; ++u) {
+      if (f + 32 * u >= hi) break;
+      const unsigned same = same_expert(x[u], p.bits);
+      if (x[u] >= 0 && lane == __ffs(same) - 1) mine[x[u]] += __popc(same);
+      __syncwarp();
+    }
   }
   __syncthreads();
   const int e = threadIdx.x;
   int sum = 0;
   if (e < p.E) {
 #pragma unroll 8
-    for (int w = 0; w < PLAN_WARPS; ++w) {
+    for (int w = 0; w < p.warps; ++w) {
       const int n = cnt[w * p.E + e];
       cnt[w * p.E + e] = sum;
       sum += n;
@@ -329,17 +397,24 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
       p.items[3 * (int64_t)i] = p.items[3 * (int64_t)i + 1] = p.items[3 * (int64_t)i + 2] = 0;
   }
   __syncthreads();
-  for (int f = lo + lane; f - lane < hi; f += 32) {
-    const int x = plan_expert(p, f, hi);
-    const unsigned same = __match_any_sync(FULL, x);
-    int row = -1;
-    if (x >= 0) row = base[x] + mine[x] + __popc(same & ((1u << lane) - 1));
-    __syncwarp();
-    if (x >= 0 && lane == __ffs(same) - 1) mine[x] += __popc(same);
-    __syncwarp();
-    if (f < hi) {
-      p.pos[f] = row;
-      if (row >= 0) p.order[row] = f;
+  for (int f = lo; f < hi; f += 32 * PLAN_AHEAD) {
+    int x[PLAN_AHEAD];
+#pragma unroll
+    for (int u = 0; u < PLAN_AHEAD; ++u) x[u] = plan_expert(p, f + 32 * u + lane, hi);
+#pragma unroll
+    for (int u = 0; u < PLAN_AHEAD; ++u) {
+      if (f + 32 * u >= hi) break;
+      const unsigned same = same_expert(x[u], p.bits);
+      int row = -1;
+      if (x[u] >= 0) row = base[x[u]] + mine[x[u]] + __popc(same & ((1u << lane) - 1));
+      __syncwarp();
+      if (x[u] >= 0 && lane == __ffs(same) - 1) mine[x[u]] += __popc(same);
+      __syncwarp();
+      const int at = f + 32 * u + lane;
+      if (at < hi) {
+        p.pos[at] = row;
+        if (row >= 0) p.order[row] = at;
+      }
     }
   }
   for (int r = rows + rank * blockDim.x + threadIdx.x; r < p.R; r += ctas * blockDim.x) p.order[r] = -1;
@@ -380,64 +455,94 @@ struct CombineArgs {
   int* status;
 };
 
-// One thread: W neighbouring columns of a token.  The rows of K slots are asked for before the first is added.
+// rows are read once: past the L1
+DEVI uint4 load_once(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.L2::256B.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+DEVI uint16_t load_once(const uint16_t* p) { return *p; }
+
+// One thread: W neighbouring columns of a token at a time.  The rows of K slots are asked for before the first is added, and where
+// the next token's rows are before this one's have come.
 template <int W>
 __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ CombineArgs p) {
   pdl_trigger();
   pdl_wait();
   constexpr int K = 8;
-  const unsigned vecs = (p.H + W - 1) / W;
-  const unsigned i = blockIdx.x * 256 + threadIdx.x;
-  const int t = i / vecs, c = i % vecs * W;
-  if (t >= p.T) return;
+  const unsigned vecs = (p.H + W - 1) / W, total = vecs * (unsigned)p.T, step = gridDim.x * 256u;
   using Vec = typename std::conditional<W == 8, uint4, uint16_t>::type;
-  float acc[W];
-#pragma unroll
-  for (int q = 0; q < W; ++q) acc[q] = 0.f;
-  auto add = [&](const Vec& v, float w) {
-    const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(&v);
-#pragma unroll
-    for (int q = 0; q < W; ++q) acc[q] = fmaf(w, __bfloat162float(x[q]), acc[q]);
-  };
-  Vec sh;
-  float g = 0.f;
-  if (p.shared) {
-    sh = *reinterpret_cast<const Vec*>(p.shared + t * p.ld_shared + c);
-    g = p.gate ? 1.f / (1.f + __expf(-p.gate[t * p.ld_gate])) : 1.f;
-  }
-  for (int j0 = 0; j0 < p.k; j0 += K) {
-    Vec v[K];
-    float w[K];
+  int r[K];
+  float w[K];
+  auto places = [&](int t, int j0) {
 #pragma unroll
     for (int j = 0; j < K; ++j) {
-      int r = -1;
+      r[j] = -1;
       w[j] = 0.f;
       if (j0 + j < p.k) {
-        r = p.pos[(int64_t)t * p.k + j0 + j];
+        r[j] = p.pos[(int64_t)t * p.k + j0 + j];
         w[j] = p.w[(int64_t)t * p.k + j0 + j];
-        if (r >= p.R) {
-          atomicExch(p.status, (int)kErrBounds);
-          r = -1;
-        }
       }
-      v[j] = Vec{};
-      if (r >= 0) v[j] = *reinterpret_cast<const Vec*>(p.rows + r * p.ld_rows + c);
-      else w[j] = 0.f;                                     // another rank's expert, or none
     }
+  };
+  unsigned i = blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  places(i / vecs, 0);
+  while (true) {
+    const int t = i / vecs, c = i % vecs * W;
+    float acc[W];
 #pragma unroll
-    for (int j = 0; j < K; ++j) add(v[j], w[j]);
+    for (int q = 0; q < W; ++q) acc[q] = 0.f;
+    auto add = [&](const Vec& v, float a) {
+      const __nv_bfloat16* x = reinterpret_cast<const __nv_bfloat16*>(&v);
+#pragma unroll
+      for (int q = 0; q < W; ++q) acc[q] = fmaf(a, __bfloat162float(x[q]), acc[q]);
+    };
+    Vec sh;
+    float g = 1.f;
+    if (p.shared) {
+      sh = *reinterpret_cast<const Vec*>(p.shared + t * p.ld_shared + c);
+      if (p.gate) g = 1.f / (1.f + __expf(-p.gate[t * p.ld_gate]));
+    }
+    const unsigned next = i + step;
+    for (int j0 = 0; j0 < p.k; j0 += K) {
+      if (j0) places(t, j0);
+      Vec v[K];
+      float a[K];
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        if (r[j] >= p.R) {
+          atomicExch(p.status, (int)kErrBounds);
+          r[j] = -1;
+        }
+        v[j] = Vec{};
+        a[j] = r[j] >= 0 ? w[j] : 0.f;                     // another rank's expert, or none
+        if (r[j] >= 0) v[j] = load_once(reinterpret_cast<const Vec*>(p.rows + r[j] * p.ld_rows + c));
+      }
+      if (j0 + K >= p.k && next < total) places(next / vecs, 0);
+#pragma unroll
+      for (int j = 0; j < K; ++j) add(v[j], a[j]);
+    }
+    if (p.shared) add(sh, g);
+    Vec o;
+    __nv_bfloat16* x = reinterpret_cast<__nv_bfloat16*>(&o);
+#pragma unroll
+    for (int q = 0; q < W; ++q) x[q] = __float2bfloat16_rn(acc[q]);
+    *reinterpret_cast<Vec*>(p.out + t * p.ld_out + c) = o;
+    if (next >= total || next < i) break;
+    i = next;
   }
-  if (p.shared) add(sh, g);
-  Vec o;
-  __nv_bfloat16* x = reinterpret_cast<__nv_bfloat16*>(&o);
-#pragma unroll
-  for (int q = 0; q < W; ++q) x[q] = __float2bfloat16_rn(acc[q]);
-  *reinterpret_cast<Vec*>(p.out + t * p.ld_out + c) = o;
 }
 
 // ---------------------------------------------------------------------------------------------
 // launches
 // ---------------------------------------------------------------------------------------------
+torch::Tensor empty(at::IntArrayRef size, at::ScalarType type, const torch::Tensor& beside) {
+  return at::detail::empty_cuda(size, type, beside.device(), c10::nullopt);
+}
+
 template <typename L, int V>
 void launch_route(const RouteArgs& p, cudaStream_t stream) {
   const dim3 grid((p.T + 7) / 8);
@@ -461,7 +566,7 @@ void launch_route(RouteArgs& p, cudaStream_t stream) {
 
 }  // namespace moe
 
-std::vector<torch::Tensor> moe_route(const torch::Tensor& logits, int64_t k, bool sigmoid,
+std::tuple<torch::Tensor, torch::Tensor> moe_route(const torch::Tensor& logits, int64_t k, bool sigmoid,
                                      const c10::optional<torch::Tensor>& bias, int64_t groups, int64_t top_groups, bool renorm,
                                      double scale) {
   const auto type = logits.scalar_type();
@@ -487,8 +592,7 @@ std::vector<torch::Tensor> moe_route(const torch::Tensor& logits, int64_t k, boo
   while (lanes * groups > 32) lanes /= 2;
   RAD_CHECK_VALUE((E / groups + lanes - 1) / lanes <= 32, "moe_route: ", E, " experts in ", groups, " groups are too many");
   const at::cuda::CUDAGuard guard(logits.device());
-  torch::Tensor ids = torch::empty({T, k}, logits.options().dtype(at::kLong));
-  torch::Tensor w = torch::empty({T, k}, logits.options().dtype(at::kFloat));
+  torch::Tensor ids = moe::empty({T, k}, at::kLong, logits), w = moe::empty({T, k}, at::kFloat, logits);
   if (T == 0) return {ids, w};
   p.logits = logits.data_ptr();
   p.bias = bias.has_value() ? bias->data_ptr<float>() : nullptr;
@@ -515,24 +619,25 @@ std::vector<torch::Tensor> moe_plan(const torch::Tensor& ids_, int64_t E, int64_
   RAD_CHECK_VALUE(k >= 1 && R < (1ll << 30), "moe_plan: 1 to 2^30 pairs");
   const at::cuda::CUDAGuard guard(ids_.device());
   const torch::Tensor ids = ids_.contiguous();
-  const auto opt = ids.options().dtype(at::kInt);
-  // order and pos, counts and starts come out of one allocation each: they live and die together
-  torch::Tensor both = torch::empty({2, R}, opt), few = torch::empty({2 * E + 1}, opt);
-  torch::Tensor order = both[0], pos = both[1].view({T, k}), counts = few.narrow(0, 0, E), starts = few.narrow(0, E, E + 1);
+  torch::Tensor order = moe::empty({R}, at::kInt, ids), pos = moe::empty({T, k}, at::kInt, ids),
+                counts = moe::empty({E}, at::kInt, ids), starts = moe::empty({E + 1}, at::kInt, ids);
   const int64_t max_items = tile ? (R + tile - 1) / tile + E : 0;
-  torch::Tensor items = torch::empty({max_items, 3}, opt);
+  torch::Tensor items = tile ? moe::empty({max_items, 3}, at::kInt, ids) : counts;
   moe::PlanArgs p = {};
   p.ids = ids.data_ptr(); p.R = R; p.k = k; p.E = E; p.first = first; p.wide = type == at::kLong;
+  while (1ll << p.bits < E) ++p.bits;
   p.order = order.data_ptr<int>(); p.pos = pos.data_ptr<int>();
   p.counts = counts.data_ptr<int>(); p.starts = starts.data_ptr<int>();
   p.items = tile ? items.data_ptr<int>() : nullptr; p.tile = tile; p.max_items = max_items;
   int ctas = 1;
-  while (ctas < 8 && R > 4096ll * ctas) ctas *= 2;
-  p.seg = ((R + 32 * ctas - 1) / (32 * ctas) + 31) / 32 * 32;
+  while (ctas < moe::PLAN_CTAS && R > 4096ll * ctas) ctas *= 2;
+  p.seg = std::max<int64_t>(32, ((R + 32 * ctas - 1) / (32 * ctas) + 31) / 32 * 32);
+  p.warps = std::max<int64_t>(1, std::min<int64_t>(moe::PLAN_WARPS, (R + (int64_t)p.seg * ctas - 1) / ((int64_t)p.seg * ctas)));
   const size_t smem = (moe::PLAN_WARPS + 2) * E * sizeof(int);
-  static std::atomic<uint64_t> set{0};                     // devices whose kernel may take the shared memory of MAX_E experts
+  static std::atomic<uint64_t> set{0};                     // devices whose kernel may take clusters of 16 and the shared memory of MAX_E experts
   const int dev = ids.get_device();
-  if (smem > 48 * 1024 && (dev >= 64 || !(set.load() >> dev & 1))) {
+  if (dev >= 64 || !(set.load() >> dev & 1)) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(moe::plan_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     C10_CUDA_CHECK(cudaFuncSetAttribute(moe::plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                         (int)((moe::PLAN_WARPS + 2) * moe::MAX_E * sizeof(int))));
     if (dev < 64) set.fetch_or(1ull << dev);
@@ -574,9 +679,10 @@ void moe_gather(const torch::Tensor& x, const c10::optional<torch::Tensor>& xs, 
                             vecs, status.data_ptr<int>()));
 }
 
-void moe_combine(const torch::Tensor& rows, const torch::Tensor& pos, const torch::Tensor& w,
-                 const c10::optional<torch::Tensor>& shared, const c10::optional<torch::Tensor>& gate, const torch::Tensor& out,
-                 const torch::Tensor& status) {
+torch::Tensor moe_combine(const torch::Tensor& rows, const torch::Tensor& pos, const torch::Tensor& w,
+                          const c10::optional<torch::Tensor>& shared, const c10::optional<torch::Tensor>& gate,
+                          const torch::Tensor& status) {
+  RAD_CHECK_VALUE(rows.is_cuda() && rows.dim() == 2, "moe_combine: rows bf16 [T k, H]");
   const int64_t T = pos.size(0), k = pos.size(1), H = rows.size(1), R = rows.size(0);
   const auto bf16_rows = [&](const torch::Tensor& t, int64_t n) {
     return t.dim() == 2 && t.size(0) == n && t.size(1) == H && (H <= 1 || t.stride(1) == 1) && t.scalar_type() == at::kBFloat16 &&
@@ -591,8 +697,9 @@ void moe_combine(const torch::Tensor& rows, const torch::Tensor& pos, const torc
   RAD_CHECK_VALUE(!gate.has_value() || (shared.has_value() && gate->device() == rows.device() &&
                                           gate->scalar_type() == at::kFloat && gate->dim() == 1 && gate->size(0) == T),
                     "moe_combine: gate fp32 [T], beside shared");
-  RAD_CHECK_VALUE(bf16_rows(out, T) && (T <= 1 || out.stride(0) >= H), "moe_combine: out bf16 [T, H]");
-  if (T == 0 || H == 0) return;
+  const at::cuda::CUDAGuard guard(rows.device());
+  torch::Tensor out = moe::empty({T, H}, at::kBFloat16, rows);
+  if (T == 0 || H == 0) return out;
   moe::CombineArgs p = {};
   p.rows = (const __nv_bfloat16*)rows.data_ptr();
   p.pos = pos.data_ptr<int>();
@@ -604,14 +711,16 @@ void moe_combine(const torch::Tensor& rows, const torch::Tensor& pos, const torc
   p.ld_gate = gate.has_value() ? gate->stride(0) : 0; p.ld_out = out.stride(0);
   p.T = T; p.k = k; p.H = H; p.R = R;
   p.status = status.data_ptr<int>();
-  const at::cuda::CUDAGuard guard(rows.device());
   const bool vec = H % 8 == 0 && (p.ld_rows | p.ld_shared | p.ld_out) % 8 == 0 &&
                    ((uintptr_t)p.rows | (uintptr_t)p.shared | (uintptr_t)p.out) % 16 == 0;
   const int64_t blocks = (T * (vec ? H / 8 : H) + 255) / 256;
   RAD_CHECK_VALUE(blocks < (1ll << 23), "moe_combine: rows");
   auto stream = at::cuda::getCurrentCUDAStream();
-  if (vec) C10_CUDA_CHECK(launch_pdl(moe::combine_kernel<8>, dim3(blocks), dim3(256), 0, stream, p));
-  else C10_CUDA_CHECK(launch_pdl(moe::combine_kernel<1>, dim3(blocks), dim3(256), 0, stream, p));
+  // as many blocks as run at once, each over several tokens
+  const unsigned grid = (unsigned)std::min<int64_t>(blocks, 8ll * at::cuda::getDeviceProperties(rows.get_device())->multiProcessorCount);
+  if (vec) C10_CUDA_CHECK(launch_pdl(moe::combine_kernel<8>, dim3(grid), dim3(256), 0, stream, p));
+  else C10_CUDA_CHECK(launch_pdl(moe::combine_kernel<1>, dim3(grid), dim3(256), 0, stream, p));
+  return out;
 }
 
 }  // namespace rad

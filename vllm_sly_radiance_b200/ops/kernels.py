@@ -382,7 +382,7 @@ def moe_route(logits: torch.Tensor, top_k: int, score: str = "softmax", bias: Op
     if score not in ("softmax", "sigmoid"):
         raise ValueError(f"moe_route: score softmax or sigmoid, got {score!r}")
     if logits.is_cuda:
-        return tuple(ext().moe_route(logits, top_k, score == "sigmoid", bias, groups, top_groups, renormalize, scale))
+        return ext().moe_route(logits, top_k, score == "sigmoid", bias, groups, top_groups, renormalize, scale)
     if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise ValueError("moe_route: logits [T, E], fp32, bf16 or fp16")
     E = logits.shape[1]
@@ -444,9 +444,7 @@ def moe_combine(rows: torch.Tensor, plan: MoEPlan, weights: torch.Tensor, shared
     a row add nothing.  rows [T k, H] bf16, weights [T, k] fp32.  shared [T, H] bf16 is added, times sigmoid(gate[t]) when
     gate [T] fp32 is given."""
     if rows.is_cuda:
-        out = torch.empty(plan.pos.shape[0], rows.shape[-1], dtype=torch.bfloat16, device=rows.device)
-        ext().moe_combine(rows, plan.pos, weights, shared, gate, out, status_word(rows.device))
-        return out
+        return ext().moe_combine(rows, plan.pos, weights, shared, gate, status_word(rows.device))
     T, k = plan.pos.shape
     if rows.dim() != 2 or rows.shape[0] != T * k or rows.dtype != torch.bfloat16:
         raise ValueError("moe_combine: rows bf16 [T k, H]")
