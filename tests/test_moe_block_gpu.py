@@ -81,7 +81,7 @@ def test_rows_of_one_expert_each():
     assert torch.equal(y, K.moe_combine(K.linear_fused(K.linear_fused(x, up, plan=p, by_token=True), down, plan=p), p, w))
 
 
-@pytest.mark.parametrize("quant", ["bf16", "mxfp4"])
+@pytest.mark.parametrize("quant", ["bf16", "mxfp4", "int4"])
 def test_engine_with_decode_graphs(quant):
     """bf16 experts read counts on the host before: no decode graph could hold them."""
     prompts = [list(range(10, 60)), list(range(100, 131)), list(range(7, 27))]

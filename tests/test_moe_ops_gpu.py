@@ -372,3 +372,61 @@ def test_layer_in_a_graph_and_on_two_streams():
     torch.cuda.synchronize()
     assert all(torch.equal(a, want[i % 4]) for i, a in enumerate(got))
     assert K.check_status(DEV) == 0
+
+
+def test_two_graphs_of_one_layer():
+    """Captured calls share nothing: two graphs over the same weights replay in turn and on two streams."""
+    g = gen(12)
+    up, down, router = block(g, 16, 256, 128)
+    xs = [bf16(g, 40, 256), bf16(g, 3, 256)]
+    want = [layer(x, up, down, router, 4) for x in xs]
+    graphs = []
+    for x in xs:
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = layer(x, up, down, router, 4)
+        graphs.append((graph, out))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(10):
+        for (graph, out), st in zip(graphs, streams):
+            out.zero_()
+        torch.cuda.synchronize()
+        for (graph, out), st in zip(graphs, streams):
+            with torch.cuda.stream(st):
+                graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, y) for (_, out), y in zip(graphs, want))
+
+
+def test_bias_that_masks_and_same_expert_twice():
+    g = gen(13)
+    logits = randn(g, 30, 64)
+    bias = torch.zeros(64, device=DEV)
+    bias[::2] = -torch.inf                                  # half of the experts are never chosen
+    ids, w = K.moe_route(logits, 8, score="sigmoid", bias=bias)
+    want = torch.sort(logits[:, 1::2], dim=1, descending=True, stable=True).indices[:, :8] * 2 + 1
+    assert torch.equal(ids, want)
+    # a token that names one expert in several slots has a row for each
+    ids = torch.tensor([[3, 3, 1], [1, 3, 3]], device=DEV)
+    p = K.moe_plan(ids, 4)
+    assert p.order.tolist() == [2, 3, 0, 1, 4, 5] and p.pos.tolist() == [[2, 3, 0], [1, 4, 5]]
+    rows = bf16(g, 6, 16)
+    wt = torch.rand(2, 3, device=DEV, generator=g)
+    M.near(K.moe_combine(rows, p, wt), *M.combine(rows, p.pos, wt))
+
+
+@pytest.mark.parametrize("rows", [3, 40, 600])
+def test_linear_takes_any_magnitude(rows):
+    """Gates far to either side, zeros, the largest numbers: as the formula in 64 bits, rounded once."""
+    g = gen(rows)
+    x = bf16(g, rows, 64)
+    x[0] = 0
+    x[1] *= 2.0 ** 60
+    w = bf16(g, 96, 64)
+    i, z = torch.arange(rows, device=DEV), torch.zeros(rows, dtype=torch.long, device=DEV)
+    got = K.linear_fused(x, LinearBank(w, act="swiglu"))
+    want, bound = M.linear(x, w[None], None, "swiglu", i, z)
+    big = want.abs() > torch.finfo(torch.bfloat16).max      # beyond bf16: infinity of the same sign
+    assert torch.equal(got[big].double(), torch.sign(want[big]) * torch.inf)
+    M.near(got[~big], want[~big], bound[~big])

@@ -376,9 +376,10 @@ def moe_route(logits: torch.Tensor, top_k: int, score: str = "softmax", bias: Op
     Scores are the logits' softmax or sigmoid.  Experts are ranked by score + ``bias`` [E] (fp32, for balance), ties go to the
     lowest index, and only experts of the ``top_groups`` best of ``groups`` equal groups count; a group's value is its best
     expert's, with a bias that of its best two added up.  Weights are the chosen scores without the bias, divided by their sum
-    if ``renormalize``, times ``scale``.  A logit of -inf masks its expert: it is chosen only when no other is left, with
-    weight 0 (softmax) -- so do all weights of a row that is masked throughout.  A NaN among a row's logits (or +inf under a
-    softmax) makes its weights NaN; its ids stay distinct and in range."""
+    if ``renormalize``, times ``scale``.  A logit of -inf masks its expert, whose weight is 0: without a bias it is chosen
+    only when no other is left.  Chosen scores that add up to 0 (a row that is masked throughout) stay 0.  A NaN among a row's
+    logits (or +inf under a softmax) makes its weights NaN; its ids stay distinct and in range.  At most 1024 experts and 32 a
+    token."""
     if score not in ("softmax", "sigmoid"):
         raise ValueError(f"moe_route: score softmax or sigmoid, got {score!r}")
     if logits.is_cuda:
