@@ -764,11 +764,6 @@ torch::Tensor linear_fused(const torch::Tensor& x, const LinearBank& bank, const
   p.R = R; p.T = x.size(0); p.k = k; p.E = E; p.N = N; p.W = W; p.K = K;
   p.vec = ((uintptr_t)p.out | (uintptr_t)p.res) % 8 == 0 && (R == 1 || (p.out_ld | p.res_ld) % 4 == 0);   // one row's stride says nothing
   p.status = bank.status.data_ptr<int>();
-  lf::RowMaps xm = {};
-  if (!by_token)
-    for (int i = 0; i < 4; ++i)
-      xm.box[i] = make_tma_2d(x.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, K, x.size(0), (x.size(0) == 1 ? K : x.stride(0)) * 2ll,
-                              lf::BK, 16 << i, CU_TENSOR_MAP_SWIZZLE_128B);
   auto stream = at::cuda::getCurrentCUDAStream();
   const int sms = lf::sm_count(x.get_device());
   const int64_t kb = (K + 63) / 64, half = bank.swiglu ? 64 : 128;
@@ -797,6 +792,11 @@ torch::Tensor linear_fused(const torch::Tensor& x, const LinearBank& bank, const
   const int64_t items = items_of(pair, p.tile);
   if (items >= (1ll << 30)) refuse("rows");
   const unsigned n = (unsigned)std::min<int64_t>(items, pair ? sms / 2 : sms);
+  lf::RowMaps xm = {};
+  if (!by_token)                                           // the boxes that a CTA's rows may take
+    for (int i = 0; i < 4 && 16 << i <= (pair ? p.tile / 2 : p.tile); ++i)
+      xm.box[i] = make_tma_2d(x.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, K, x.size(0), (x.size(0) == 1 ? K : x.stride(0)) * 2ll,
+                              lf::BK, 16 << i, CU_TENSOR_MAP_SWIZZLE_128B);
   if (p.tile == 16) {
     // too few items for the SMs: clusters share the items' K, each CTA at least four 64-blocks
     unsigned splits = 1;

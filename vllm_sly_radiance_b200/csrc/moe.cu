@@ -426,7 +426,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
 
 // ---------------------------------------------------------------------------------------------
 // gather, combine: bound by memory, 16 bytes a thread.  combine reads rows of a few KB in as many places as a token has experts:
-// 8192 x 8 rows of 2048 and the shared rows take 74 us (4.5 TB/s), 64 with them in L2's reach.
+// 8192 x 8 rows of 2048 take 53 us (5.7 TB/s), with the shared rows 67 (74 while the gate's
+// sigmoid was taken before the rows were asked for).
 // ---------------------------------------------------------------------------------------------
 // rows of `vecs` 16-byte pieces; x [T] -> out [R], a pair's row is its token's.  scale: fp32 beside each row, or null
 __global__ void __launch_bounds__(256) gather_kernel(const uint4* x, int64_t ld, const float* xs, const int* order, uint4* out,
@@ -505,10 +506,10 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Co
       for (int q = 0; q < W; ++q) acc[q] = fmaf(a, __bfloat162float(x[q]), acc[q]);
     };
     Vec sh;
-    float g = 1.f;
+    float g = INFINITY;                                    // what its sigmoid is taken of, once the rows are asked for
     if (p.shared) {
-      sh = *reinterpret_cast<const Vec*>(p.shared + t * p.ld_shared + c);
-      if (p.gate) g = 1.f / (1.f + __expf(-p.gate[t * p.ld_gate]));
+      sh = load_once(reinterpret_cast<const Vec*>(p.shared + t * p.ld_shared + c));
+      if (p.gate) g = p.gate[t * p.ld_gate];
     }
     const unsigned next = i + step;
     for (int j0 = 0; j0 < p.k; j0 += K) {
@@ -529,7 +530,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ Co
 #pragma unroll
       for (int j = 0; j < K; ++j) add(v[j], a[j]);
     }
-    if (p.shared) add(sh, g);
+    if (p.shared) add(sh, 1.f / (1.f + __expf(-g)));
     Vec o;
     __nv_bfloat16* x = reinterpret_cast<__nv_bfloat16*>(&o);
 #pragma unroll
@@ -720,7 +721,8 @@ torch::Tensor moe_combine(const torch::Tensor& rows, const torch::Tensor& pos, c
   const int64_t blocks = (T * (vec ? H / 8 : H) + 255) / 256;
   RAD_CHECK_VALUE(blocks < (1ll << 23), "moe_combine: rows");
   auto stream = at::cuda::getCurrentCUDAStream();
-  // about as many blocks as run at once, each over several tokens (8192 x 8 rows of 2048: 74 us, 87 with a block for each token)
+  // about as many blocks as run at once, each over several tokens (8192 x 8 rows of 2048 and
+  // shared ones: 74 us, 87 with a block for each token)
   const unsigned grid = (unsigned)std::min<int64_t>(blocks, 4ll * at::cuda::getDeviceProperties(rows.get_device())->multiProcessorCount);
   if (vec) C10_CUDA_CHECK(launch_pdl(moe::combine_kernel<8>, dim3(grid), dim3(256), 0, stream, p));
   else C10_CUDA_CHECK(launch_pdl(moe::combine_kernel<1>, dim3(grid), dim3(256), 0, stream, p));
