@@ -769,25 +769,29 @@ torch::Tensor linear_fused(const torch::Tensor& x, const LinearBank& bank, const
   const int64_t kb = (K + 63) / 64, half = bank.swiglu ? 64 : 128;
   const auto blocks_of = [&](bool pair) { return (W + half * (pair ? 2 : 1) - 1) / (half * (pair ? 2 : 1)); };
   const auto items_of = [&](bool pair, int64_t tile) { return (std::min<int64_t>(E, R) + R / tile) * blocks_of(pair); };   // at most
-  bool pair;
-  if (E > 1) {
-    // about twice the rows that an expert has on average, so that few experts need a second pass over their weights; above 64
-    // rows CTA pairs, whose MMAs are cut to 32 rows
-    const int64_t want = 2 * ((R + E - 1) / E);
-    p.tile = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 256;
-    pair = p.tile == 256;
-  } else {
-    // the height that takes the fewest cycles: waves of items x (k blocks x the longer of loads, at some 60 bytes a cycle and
-    // SM, and MMAs, 2 a row; start and end some 3000)
+  bool pair = false;
+  // the height up to `most` that takes the fewest cycles: waves of items x (k blocks x the longer of loads, at some 60 bytes a
+  // cycle and SM, and MMAs, 2 a row; start and end some 3000)
+  const auto choose = [&](int most) {
     int64_t best = INT64_MAX;
-    p.tile = 16, pair = false;
-    for (int t = 16; t <= 256; t = t < 64 ? 2 * t : t + 32)
+    for (int t = 16; t <= most; t = t < 64 ? 2 * t : t + 32)
       for (int two = t >= 64 && R > 32; two >= (t > 64); --two) {
-        const int64_t items = (R + t - 1) / t * blocks_of(two), units = two ? sms / 2 : sms;
+        const int64_t items = E == 1 ? (R + t - 1) / t * blocks_of(two) : items_of(two, t), units = two ? sms / 2 : sms;
         const int64_t rows = std::min<int64_t>(t, R), stage = std::max<int64_t>((16384 + rows * 128 / (two ? 2 : 1)) / 60, 2 * rows);
         const int64_t cost = (items + units - 1) / units * (kb * stage + 3000);
         if (cost < best) best = cost, p.tile = t, pair = two;
       }
+  };
+  if (E > 1) {
+    // about twice the rows that an expert has on average, so that few experts need a second pass over their weights; above 64
+    // rows CTA pairs, whose MMAs are cut to 32 rows.  Where that leaves SMs without an item, lower tiles by their cost (500 tokens,
+    // 2 of 4 experts, 640 -> 700: 10.5 us, 15.8 on pairs)
+    const int64_t want = 2 * ((R + E - 1) / E);
+    p.tile = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 256;
+    pair = p.tile == 256;
+    if (p.tile > 16 && items_of(pair, p.tile) < (pair ? sms / 2 : sms)) choose(p.tile);
+  } else {
+    choose(256);
   }
   const int64_t items = items_of(pair, p.tile);
   if (items >= (1ll << 30)) refuse("rows");
