@@ -1,0 +1,43 @@
+"""The router's choice where 32 bits cannot tell candidates apart."""
+import math
+
+import pytest
+import torch
+
+from vllm_sly_radiance_b200.ops import kernels as K
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def gen(seed):
+    return torch.Generator(DEV).manual_seed(seed)
+
+
+@pytest.mark.parametrize("std", [2e-5, 1e-4])
+def test_groups_whose_best_two_cancel(std):
+    """Biases of +64 and -64: a group's value is about 1, its two terms are rounded to steps of 2^-17."""
+    logits = torch.randn(2000, 8, device=DEV, generator=gen(0)) * std
+    bias = torch.tensor([64.0, -64.0] * 4, device=DEV)
+    ids, _ = K.moe_route(logits, 2, score="sigmoid", bias=bias, groups=4, top_groups=1)
+    s = torch.sigmoid(logits.double())
+    best = (s[:, ::2] + s[:, 1::2]).argmax(1)              # values in 64 bits, the bias gone
+    assert torch.equal(ids, torch.stack([2 * best, 2 * best + 1], 1))
+
+
+def test_softmax_sum_that_loses_every_addition():
+    """1024 experts: expert 0 has e = 1, 36 others 0.98 * 2^-24 each, so that 32-bit additions one after the other leave 1.
+    With the bias, expert 0 is worth -35.3 * 2^-24 and expert 40 -33.5 * 2^-24; without the lost terms' 0 it would win."""
+    u = 2.0 ** -24
+    l = torch.full((1, 1024), -torch.inf)
+    l[0, 0] = 0.0
+    small = math.log(0.98 * u)
+    l[0, 1:32] = small
+    for lane in (1, 2, 4, 8, 16):
+        l[0, 32 * lane] = small
+    bias = torch.full((1024,), -8.0)
+    bias[0], bias[40] = -1.0, -33.5 * u
+    s = torch.softmax(l.double(), 1) + bias.double()
+    assert int(s.argmax()) == 40
+    ids, _ = K.moe_route(l.to(DEV), 1, bias=bias.to(DEV))
+    assert ids.tolist() == [[40]]

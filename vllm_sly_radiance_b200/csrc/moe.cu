@@ -148,9 +148,11 @@ __device__ __noinline__ int choose_wide(const RouteArgs& p, const L* row, int e0
 // Lane j < k ends with the j-th expert.  False: 32 bits could not tell the order.  total: of the softmax, where it is needed
 template <int V, bool BIAS>
 DEVI bool choose(const RouteArgs& p, const float (&l)[V], int e0, int n, float top, int lane, int& expert, float& total) {
-  // Two candidates' error, relative to 1 + c: a sigmoid is off by at most 2^-22 (exp 2^-23, sum 2^-24, quotient 2^-24), a softmax
-  // by 2^-20 of it (its sum over 13 additions in a row), their sum with the bias by another 2^-24 of c; each with a margin
-  const float tol = p.sigmoid ? 1.f / (1 << 21) : 1.f / (1 << 19);
+  // How far rounding can move two candidates' difference, u = 2^-24, relative to 1 + |c|.  A sigmoid is off by at most 2 u (exp 2 u
+  // of e, sum, quotient), two by 4 u.  A softmax's two are off by at most (V + 17) u of their sum, which is at most 1: exp 2 u and
+  // its argument 0.4 u each; the total V + 4 additions in a row, its terms' exp 2 u and their arguments ln E < 7 u; the quotient u.
+  // The bias adds u of each c.  Either with a margin.
+  const float tol = p.sigmoid ? 8.f / (1 << 24) : (V + 24.f) / (1 << 24);
   total = 0.f;
   if (!p.sigmoid && (BIAS || !p.renorm)) {
 #pragma unroll
@@ -183,7 +185,8 @@ DEVI bool choose(const RouteArgs& p, const float (&l)[V], int e0, int n, float t
       const float other = __shfl_sync(FULL, value, g * p.lanes);
       const uint32_t ko = key_of(other);
       rank += ko > key || (ko == key && g < mine);
-      if (BIAS && g != mine && mine < p.groups) clear &= fabsf(value - other) > tol * (2.f + fabsf(value));
+      // two scores more, and the rounding of each expert's c, which may cancel in the value; the other group asks this by its own
+      if (BIAS && g != mine && mine < p.groups) clear &= fabsf(value - other) > tol * (2.f + fabsf(b1) + fabsf(b2));
     }
     if (rank >= p.top_groups) n = 0;
   }
