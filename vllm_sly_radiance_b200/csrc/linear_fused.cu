@@ -680,6 +680,49 @@ void run(const Args& p, bool swiglu, const CUtensorMap& wm, const RowMaps& xm, d
          p, wm, xm);
 }
 
+// How a product of R rows is cut: rows of a tile, CTA pairs or single CTAs, CTAs that share an item's K, items at most
+struct Tiles {
+  int tile;
+  bool pair;
+  unsigned splits;
+  int64_t items;
+};
+
+Tiles tiles_of(int64_t R, int64_t E, int64_t W, int64_t K, bool swiglu, int sms) {
+  const int64_t kb = (K + 63) / 64, half = swiglu ? 64 : 128;
+  const auto blocks_of = [&](bool pair) { return (W + half * (pair ? 2 : 1) - 1) / (half * (pair ? 2 : 1)); };
+  const auto items_of = [&](bool pair, int64_t tile) { return (std::min<int64_t>(E, R) + R / tile) * blocks_of(pair); };   // at most
+  Tiles q = {16, false, 1, 0};
+  // the height up to `most` that takes the fewest cycles: waves of items x (k blocks x the longer of loads, at some 60 bytes a
+  // cycle and SM, and MMAs, 2 a row; start and end some 3000)
+  const auto choose = [&](int most) {
+    int64_t best = INT64_MAX;
+    for (int t = 16; t <= most; t = t < 64 ? 2 * t : t + 32)
+      for (int two = t >= 64 && R > 32; two >= (t > 64); --two) {
+        const int64_t items = E == 1 ? (R + t - 1) / t * blocks_of(two) : items_of(two, t), units = two ? sms / 2 : sms;
+        const int64_t rows = std::min<int64_t>(t, R), stage = std::max<int64_t>((16384 + rows * 128 / (two ? 2 : 1)) / 60, 2 * rows);
+        const int64_t cost = (items + units - 1) / units * (kb * stage + 3000);
+        if (cost < best) best = cost, q.tile = t, q.pair = two;
+      }
+  };
+  if (E > 1) {
+    // about twice the rows that an expert has on average, so that few experts need a second pass over their weights; above 64
+    // rows CTA pairs, whose MMAs are cut to 32 rows.  Where that leaves SMs without an item, lower tiles by their cost (500 tokens,
+    // 2 of 4 experts, 640 -> 700: 10.5 us, 15.8 on pairs)
+    const int64_t want = 2 * ((R + E - 1) / E);
+    q.tile = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 256;
+    q.pair = q.tile == 256;
+    if (q.tile > 16 && items_of(q.pair, q.tile) < (q.pair ? sms / 2 : sms)) choose(q.tile);
+  } else {
+    choose(256);
+  }
+  q.items = items_of(q.pair, q.tile);
+  // too few items for the SMs: clusters share the items' K, each CTA at least four 64-blocks
+  if (q.tile == 16)
+    while (q.splits < 8 && q.items * q.splits * 2 <= sms && kb / (q.splits * 2) >= 4) q.splits *= 2;
+  return q;
+}
+
 }  // namespace lf
 
 // The weights of a product [E, N, K] (models/layers.LinearBank checks them), with their tensor map
@@ -766,34 +809,10 @@ torch::Tensor linear_fused(const torch::Tensor& x, const LinearBank& bank, const
   p.status = bank.status.data_ptr<int>();
   auto stream = at::cuda::getCurrentCUDAStream();
   const int sms = lf::sm_count(x.get_device());
-  const int64_t kb = (K + 63) / 64, half = bank.swiglu ? 64 : 128;
-  const auto blocks_of = [&](bool pair) { return (W + half * (pair ? 2 : 1) - 1) / (half * (pair ? 2 : 1)); };
-  const auto items_of = [&](bool pair, int64_t tile) { return (std::min<int64_t>(E, R) + R / tile) * blocks_of(pair); };   // at most
-  bool pair = false;
-  // the height up to `most` that takes the fewest cycles: waves of items x (k blocks x the longer of loads, at some 60 bytes a
-  // cycle and SM, and MMAs, 2 a row; start and end some 3000)
-  const auto choose = [&](int most) {
-    int64_t best = INT64_MAX;
-    for (int t = 16; t <= most; t = t < 64 ? 2 * t : t + 32)
-      for (int two = t >= 64 && R > 32; two >= (t > 64); --two) {
-        const int64_t items = E == 1 ? (R + t - 1) / t * blocks_of(two) : items_of(two, t), units = two ? sms / 2 : sms;
-        const int64_t rows = std::min<int64_t>(t, R), stage = std::max<int64_t>((16384 + rows * 128 / (two ? 2 : 1)) / 60, 2 * rows);
-        const int64_t cost = (items + units - 1) / units * (kb * stage + 3000);
-        if (cost < best) best = cost, p.tile = t, pair = two;
-      }
-  };
-  if (E > 1) {
-    // about twice the rows that an expert has on average, so that few experts need a second pass over their weights; above 64
-    // rows CTA pairs, whose MMAs are cut to 32 rows.  Where that leaves SMs without an item, lower tiles by their cost (500 tokens,
-    // 2 of 4 experts, 640 -> 700: 10.5 us, 15.8 on pairs)
-    const int64_t want = 2 * ((R + E - 1) / E);
-    p.tile = want <= 16 ? 16 : want <= 32 ? 32 : want <= 64 ? 64 : 256;
-    pair = p.tile == 256;
-    if (p.tile > 16 && items_of(pair, p.tile) < (pair ? sms / 2 : sms)) choose(p.tile);
-  } else {
-    choose(256);
-  }
-  const int64_t items = items_of(pair, p.tile);
+  const lf::Tiles how = lf::tiles_of(R, E, W, K, bank.swiglu, sms);
+  const bool pair = how.pair;
+  const int64_t items = how.items;
+  p.tile = how.tile;
   if (items >= (1ll << 30)) refuse("rows");
   const unsigned n = (unsigned)std::min<int64_t>(items, pair ? sms / 2 : sms);
   lf::RowMaps xm = {};
@@ -802,10 +821,8 @@ torch::Tensor linear_fused(const torch::Tensor& x, const LinearBank& bank, const
       xm.box[i] = make_tma_2d(x.data_ptr(), CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, K, x.size(0), (x.size(0) == 1 ? K : x.stride(0)) * 2ll,
                               lf::BK, 16 << i, CU_TENSOR_MAP_SWIZZLE_128B);
   if (p.tile == 16) {
-    // too few items for the SMs: clusters share the items' K, each CTA at least four 64-blocks
-    unsigned splits = 1;
-    while (splits < 8 && items * splits * 2 <= sms && kb / (splits * 2) >= 4) splits *= 2;
-    if (splits > 1) lf::run<16, false, true>(p, bank.swiglu, bank.wm, xm, dim3((unsigned)items, splits), dim3(1, splits), stream);
+    if (how.splits > 1)
+      lf::run<16, false, true>(p, bank.swiglu, bank.wm, xm, dim3((unsigned)items, how.splits), dim3(1, how.splits), stream);
     else lf::run<16, false, false>(p, bank.swiglu, bank.wm, xm, dim3(n), dim3(1), stream);
   } else if (pair) {
     lf::run<256, true, false>(p, bank.swiglu, bank.wm, xm, dim3(2 * n), dim3(2), stream);
@@ -820,6 +837,11 @@ torch::Tensor linear_fused(const torch::Tensor& x, const LinearBank& bank, const
 void linear_fused_bind(pybind11::module_& m) {
   pybind11::class_<LinearBank>(m, "LinearBank")
       .def(pybind11::init<torch::Tensor, c10::optional<torch::Tensor>, bool, torch::Tensor>());
+  m.def("linear_fused_tiles", [](int64_t R, int64_t E, int64_t W, int64_t K, bool swiglu, int sms) {
+    RAD_CHECK_VALUE(R > 0 && E > 0 && W > 0 && K > 0 && sms > 1, "linear_fused_tiles: sizes above 0");
+    const lf::Tiles q = lf::tiles_of(R, E, W, K, swiglu, sms);
+    return std::make_tuple(q.tile, q.pair, q.splits);
+  }, "(rows of a tile, CTA pairs, CTAs that share K) of a product of R rows on `sms` SMs");
   m.def("linear_fused", &linear_fused, "bf16 product (one weight, or one per expert) with bias, SwiGLU, row scale and residual");
 }
 
