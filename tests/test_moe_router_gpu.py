@@ -1,9 +1,10 @@
-"""The router's choice where 32 bits cannot tell candidates apart."""
+"""The router's choice where 32 bits cannot tell candidates apart, and its weights where 32 bits cannot hold the scores."""
 import math
 
 import pytest
 import torch
 
+from test_moe_router_cpu import SMALL_SIGMOIDS, check_masked_rows, check_small_sigmoids, check_small_softmax
 from vllm_sly_radiance_b200.ops import kernels as K
 
 pytestmark = pytest.mark.gpu
@@ -41,3 +42,17 @@ def test_softmax_sum_that_loses_every_addition():
     assert int(s.argmax()) == 40
     ids, _ = K.moe_route(l.to(DEV), 1, bias=bias.to(DEV))
     assert ids.tolist() == [[40]]
+
+
+@pytest.mark.parametrize("logits", SMALL_SIGMOIDS)
+def test_sigmoid_scores_below_32_bits(logits):
+    check_small_sigmoids(logits, DEV)
+
+
+def test_softmax_scores_below_32_bits():
+    check_small_softmax(DEV)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_masked_rows_keep_weights_of_zero(score):
+    check_masked_rows(score, DEV)

@@ -69,11 +69,25 @@ DEVI float value_of(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7ffffff
 DEVI float exp_of(float x) { return expf(x); }
 DEVI double exp_of(double x) { return exp(x); }
 
-// A score; without a bias and to be renormalised, a softmax's but for its sum, as only ratios matter
-template <typename F, bool BIAS> DEVI F score_of(const RouteArgs& p, float x, float top, F total) {
+// A score
+template <typename F> DEVI F score_of(const RouteArgs& p, float x, float top, F total) {
   if (p.sigmoid) return F(1) / (F(1) + exp_of(-(F)x));
   const F s = exp_of((F)x - (F)top);
-  return BIAS || !p.renorm ? (total > 0 ? s / total : total) : s;
+  return total > 0 ? s / total : total;
+}
+
+// Lanes' chosen logits (-inf without one) -> their scores but for a common factor, of which no weight is left once they are divided by
+// their sum: relative to the largest where the scores themselves may be below what 32 bits hold
+DEVI float ratio_of(bool sigmoid, float x) {
+  if (sigmoid && !__any_sync(FULL, x < -80.f && x > -INFINITY)) return 1.f / (1.f + expf(-x));
+  const float a = sigmoid ? fminf(x, 0.f) : x;             // sigmoid(x) = e^min(x, 0) / (1 + e^-|x|)
+  float m = warp_max(a);
+  if (m == -INFINITY) m = 0.f;                             // masked throughout: scores of zero
+  const float d = a - m, e = expf(d);
+  if (!sigmoid) return e;
+  // what the difference rounded off, up to 2^-18 of e^d where the logits lie far apart
+  const float t = d - a, r = d > -128.f ? (a - (d - t)) - (m + t) : 0.f;
+  return fmaf(e, r, e) / (1.f + expf(-fabsf(x)));
 }
 
 // Best two of a lane's candidates -> of its group's
@@ -102,7 +116,7 @@ __device__ __noinline__ int choose_wide(const RouteArgs& p, const L* row, int e0
   double b1 = -INFINITY, b2 = -INFINITY;
   // in step for all lanes: eight independent chains of double operations, where a loop waited for one after the other
 #pragma unroll
-  for (int i = 0; i < V; ++i) c[i] = score_of<double, true>(p, i < n ? to_f(row[e0 + i]) : 0.f, top, total);
+  for (int i = 0; i < V; ++i) c[i] = score_of<double>(p, i < n ? to_f(row[e0 + i]) : 0.f, top, total);
 #pragma unroll
   for (int i = 0; i < V; ++i)
     if (i < n) {
@@ -165,7 +179,7 @@ DEVI bool choose(const RouteArgs& p, const float (&l)[V], int e0, int n, float t
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     c[i] = 0.f;
-    if (i < n) c[i] = BIAS ? score_of<float, BIAS>(p, l[i], top, total) + p.bias[e0 + i] : l[i];
+    if (i < n) c[i] = BIAS ? score_of<float>(p, l[i], top, total) + p.bias[e0 + i] : l[i];
   }
   if (p.groups > 1) {
     float b1 = -INFINITY, b2 = -INFINITY;
@@ -259,10 +273,12 @@ __global__ void __launch_bounds__(256, V <= 8 ? 4 : 2) route_kernel(const __grid
   float total, s = 0.f;
   const bool clear = choose<V, BIAS>(p, l, e0, n, top, lane, expert, total);
   if (BIAS && !clear) expert = choose_wide<L, V>(p, row, e0, n, top, lane);
-  if (lane < p.k) s = score_of<float, BIAS>(p, to_f(row[expert]), top, total);
   if (p.renorm) {
+    s = ratio_of(p.sigmoid, lane < p.k ? to_f(row[expert]) : -INFINITY);
     const float sum = warp_sum(s);
     s = sum > 0.f ? s / sum : 0.f;
+  } else if (lane < p.k) {
+    s = score_of<float>(p, to_f(row[expert]), top, total);
   }
   if (lane < p.k) {
     p.ids[(int64_t)t * p.k + lane] = expert;

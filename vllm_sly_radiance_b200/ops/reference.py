@@ -359,9 +359,17 @@ def moe_route(logits, top_k, score, bias, groups, top_groups, renormalize, scale
         ids = torch.gather(order, -1, torch.sort(~kept, dim=-1, stable=True).indices[:, :top_k])
     else:
         ids = torch.sort(c, dim=-1, descending=True, stable=True).indices[:, :top_k]
-    w = torch.gather(s, -1, ids)
     if renormalize:
+        # only ratios matter: relative to the largest, as the scores themselves may be below what 64 bits hold
+        x = torch.gather(l, -1, ids)
+        a = x if score == "softmax" else x.clamp(max=0)
+        m = a.amax(-1, keepdim=True)
+        w = torch.exp(a - torch.where(m == -torch.inf, 0.0, m))
+        if score == "sigmoid":
+            w = w / (1 + torch.exp(-x.abs()))
         w = torch.where(w == 0, 0.0, w / w.sum(-1, keepdim=True))
+    else:
+        w = torch.gather(s, -1, ids)
     bad = l.isnan().any(-1, keepdim=True)
     if score == "softmax":
         bad = bad | (top == torch.inf)
