@@ -44,6 +44,18 @@ def test_softmax_sum_that_loses_every_addition():
     assert ids.tolist() == [[40]]
 
 
+def test_bias_that_is_no_number():
+    """An expert whose bias is NaN ranks last, and adds nothing to its group's value."""
+    logits = torch.randn(50, 64, device=DEV, generator=gen(1))
+    bias = torch.randn(64, device=DEV, generator=gen(2)) * 0.1
+    bias[3], bias[17], bias[18], bias[40] = torch.nan, torch.nan, torch.nan, torch.nan
+    for kw in ({}, {"groups": 8, "top_groups": 3}):
+        got = K.moe_route(logits, 6, score="sigmoid", bias=bias, **kw)
+        want = K.moe_route(logits.cpu(), 6, score="sigmoid", bias=bias.cpu(), **kw)
+        assert torch.equal(got[0].cpu(), want[0])
+        assert (got[1].cpu() - want[1]).abs().max() < 2.0 ** -19
+
+
 @pytest.mark.parametrize("logits", SMALL_SIGMOIDS)
 def test_sigmoid_scores_below_32_bits(logits):
     check_small_sigmoids(logits, DEV)

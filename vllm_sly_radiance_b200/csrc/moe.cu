@@ -94,9 +94,9 @@ DEVI float ratio_of(bool sigmoid, float x) {
 template <typename F> DEVI void best_two(F& b1, F& b2, int lanes) {
   for (int o = lanes >> 1; o > 0; o >>= 1) {
     const F o1 = __shfl_xor_sync(FULL, b1, o), o2 = __shfl_xor_sync(FULL, b2, o);
-    const F lo = o1 < b1 ? o1 : b1, hi2 = o2 > b2 ? o2 : b2;
-    b1 = o1 > b1 ? o1 : b1;
-    b2 = lo > hi2 ? lo : hi2;
+    const F lo = min(o1, b1);
+    b1 = max(o1, b1);
+    b2 = max(lo, max(o2, b2));
   }
 }
 
@@ -120,10 +120,10 @@ __device__ __noinline__ int choose_wide(const RouteArgs& p, const L* row, int e0
 #pragma unroll
   for (int i = 0; i < V; ++i)
     if (i < n) {
-      const double x = c[i] += (double)p.bias[e0 + i];
-      const double lo = x < b1 ? x : b1;
-      b1 = x > b1 ? x : b1;
-      b2 = lo > b2 ? lo : b2;
+      c[i] += (double)p.bias[e0 + i];
+      const double x = fmax(c[i], -INFINITY), lo = fmin(x, b1);      // a NaN adds nothing to the group's value
+      b1 = fmax(x, b1);
+      b2 = fmax(lo, b2);
     }
   if (p.groups > 1) {
     best_two(b1, b2, p.lanes);
@@ -186,9 +186,9 @@ DEVI bool choose(const RouteArgs& p, const float (&l)[V], int e0, int n, float t
 #pragma unroll
     for (int i = 0; i < V; ++i)
       if (i < n) {
-        const float lo = c[i] < b1 ? c[i] : b1;
-        b1 = c[i] > b1 ? c[i] : b1;
-        b2 = lo > b2 ? lo : b2;
+        const float x = fmaxf(c[i], -INFINITY), lo = fminf(x, b1);   // a NaN adds nothing to the group's value
+        b1 = fmaxf(x, b1);
+        b2 = fmaxf(lo, b2);
       }
     best_two(b1, b2, p.lanes);
     const float value = BIAS ? b1 + b2 : b1;
