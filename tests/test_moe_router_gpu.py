@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-from test_moe_router_cpu import SMALL_SIGMOIDS, check_masked_rows, check_small_sigmoids, check_small_softmax
+from test_moe_router_cpu import SMALL_SIGMOIDS, check_masked_rows, check_small_sigmoids, check_small_softmax, close
 from vllm_sly_radiance_b200.ops import kernels as K
 
 pytestmark = pytest.mark.gpu
@@ -68,3 +68,17 @@ def test_softmax_scores_below_32_bits():
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_masked_rows_keep_weights_of_zero(score):
     check_masked_rows(score, DEV)
+
+
+@pytest.mark.parametrize("E,groups,tops,k", [(680, 17, 3, 8), (1023, 3, 2, 32), (1020, 5, 2, 7), (999, 9, 4, 16), (1023, 31, 5, 9)])
+@pytest.mark.parametrize("score,biased", [("softmax", False), ("sigmoid", True), ("softmax", True)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_groups_of_many_experts(E, groups, tops, k, score, biased, dtype):
+    """More than 32 experts for a lane: numbers of groups just above a power of two."""
+    logits = (torch.randn(21, E, device=DEV, generator=gen(E)) * 2).to(dtype)
+    bias = torch.randn(E, device=DEV, generator=gen(k)) * 0.1 if biased else None
+    kw = dict(score=score, groups=groups, top_groups=tops)
+    got = K.moe_route(logits, k, bias=bias, **kw)
+    want = K.moe_route(logits.cpu(), k, bias=None if bias is None else bias.cpu(), **kw)
+    assert torch.equal(got[0].cpu(), want[0])
+    close(got[1], want[1].double())
