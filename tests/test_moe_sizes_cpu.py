@@ -1,0 +1,34 @@
+"""MoE blocks of sizes beyond the kernels'."""
+import dataclasses
+
+import pytest
+import torch
+
+import moe_oracle as M
+from vllm_sly_radiance_b200.config import tiny_moe
+from vllm_sly_radiance_b200.models.hybrid import TPInfo
+from vllm_sly_radiance_b200.models.moe import MoEBlock
+from vllm_sly_radiance_b200.models.weights import RandomWeights
+
+
+def block(quant="bf16", device="cpu", **sizes):
+    cfg = dataclasses.replace(tiny_moe(), **sizes)
+    blk = MoEBlock(cfg, TPInfo(), quant, RandomWeights(cfg, 0, "cpu"), "layers.1.")
+    return blk.to(device) if device != "cpu" else blk
+
+
+def x_of(T):
+    return torch.randn(T, 256, generator=torch.Generator().manual_seed(T)).to(torch.bfloat16)
+
+
+MANY_A_TOKEN = dict(num_experts=64, num_experts_per_tok=40, moe_intermediate_size=32)
+MANY_EXPERTS = dict(num_experts=1100, num_experts_per_tok=4, moe_intermediate_size=32)
+
+
+@pytest.mark.parametrize("sizes", [MANY_A_TOKEN, MANY_EXPERTS])
+def test_block_of_any_size(sizes):
+    blk, x = block(**sizes), x_of(6)
+    ids, w = blk.route(x)
+    want_ids, want = M.route(x.float() @ blk.router.float().t(), sizes["num_experts_per_tok"])
+    assert torch.equal(ids, want_ids) and torch.allclose(w.double(), want, rtol=1e-6)
+    assert blk.forward(x).isfinite().all()

@@ -23,6 +23,7 @@ import torch
 
 from ..config import ModelConfig
 from ..ops import kernels as K
+from ..ops import reference as ref
 from ..quant.mxfp4 import MXFP4Weight, cat_rows
 from .layers import Linear, LinearBank
 
@@ -82,7 +83,7 @@ class MoEBlock:
             return
         both = torch.cat([self.router, self.shared_gate])
         self._gates = torch.cat([both, both.new_zeros(-both.shape[0] % 8, self.H)])
-        if self.dense_gu is not None and self.H % 8 == 0 and self.I % 8 == 0:
+        if (self.dense_gu is not None and self.H % 8 == 0 and self.I % 8 == 0 and self.e_local <= K.MOE_MAX_EXPERTS):
             up, down = self.shared_gate_up, self.shared_down
             bf16 = up.quant == "bf16" and down.K % 8 == 0
             self._banks = (LinearBank(up.w, act="swiglu") if bf16 else None, LinearBank(down.w) if bf16 else None,
@@ -100,10 +101,19 @@ class MoEBlock:
         return self
 
     # ------------------------------------------------------------------------------------------
+    # More experts, or more a token, than the router's and the plan's kernels take: plain torch operations, without a stop for the host
     def _choose(self, logits: torch.Tensor):
         cfg = self.cfg
-        return K.moe_route(logits, self.top_k, score=cfg.moe_score, bias=self.router_bias, groups=cfg.moe_num_groups,
-                           top_groups=cfg.moe_top_groups, renormalize=cfg.moe_renormalize, scale=cfg.moe_routed_scale)
+        route = K.moe_route if self.E <= K.MOE_MAX_EXPERTS and self.top_k <= K.MOE_MAX_TOP_K else ref.moe_route
+        return route(logits, self.top_k, score=cfg.moe_score, bias=self.router_bias, groups=cfg.moe_num_groups,
+                     top_groups=cfg.moe_top_groups, renormalize=cfg.moe_renormalize, scale=cfg.moe_routed_scale)
+
+    def _plan(self, ids: torch.Tensor, tile: int = 0) -> K.MoEPlan:
+        if self.e_local <= K.MOE_MAX_EXPERTS:
+            return K.moe_plan(ids, self.e_local, first=self.e0, tile=tile)
+        order, pos, counts, starts = ref.moe_plan(ids, self.e_local, self.e0)
+        items = K.moe_work_items(counts.long(), tile, (ids.numel() + tile - 1) // tile + self.e_local) if tile else None
+        return K.MoEPlan(ids.shape[1], order, pos, counts, starts, items, tile)
 
     def route(self, x_bf16: torch.Tensor):
         """Scores over all experts, top-k, weights (``K.moe_route``) -> (ids [T,k], weights [T,k])."""
@@ -195,11 +205,10 @@ class MoEBlock:
             # fixed shapes, no host sync (CUDA-graph safe)
             if self.w_gate_up is None:
                 _, _, up, down = self._banks
-                plan = K.moe_plan(ids, self.e_local, first=self.e0)
+                plan = self._plan(ids)
                 rows = K.linear_fused(K.linear_fused(xb, up, plan=plan, by_token=True), down, plan=plan)
             else:
-                plan = K.moe_plan(ids, self.e_local, first=self.e0,
-                                  tile=K.moe_tile(ids.numel(), self.e_local))
+                plan = self._plan(ids, tile=K.moe_tile(ids.numel(), self.e_local))
                 q, s = K.moe_gather(qs, plan)
                 rows = K.moe_grouped_mlp(q, s, plan, self.w_gate_up, self.w_down, self.I, self.H)
             return K.moe_combine(rows, plan, w, shared=shared, gate=gate)

@@ -368,6 +368,9 @@ def moe_grouped_mlp(q, s, counts, w_gate_up, w_down, I: int, H: int) -> torch.Te
 # ---------------------------------------------------------------------------------------------
 # mixture of experts
 # ---------------------------------------------------------------------------------------------
+MOE_MAX_EXPERTS, MOE_MAX_TOP_K = 1024, 32        # of the router's and the plan's kernels
+
+
 def moe_route(logits: torch.Tensor, top_k: int, score: str = "softmax", bias: Optional[torch.Tensor] = None,
               groups: int = 1, top_groups: int = 1, renormalize: bool = True, scale: float = 1.0):
     """Experts of each token from the router's logits [T, E] (fp32, bf16 or fp16) -> (ids [T, k] int64, best first,
@@ -387,7 +390,9 @@ def moe_route(logits: torch.Tensor, top_k: int, score: str = "softmax", bias: Op
     if logits.dim() != 2 or logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
         raise ValueError("moe_route: logits [T, E], fp32, bf16 or fp16")
     E = logits.shape[1]
-    if not 1 <= top_k <= min(32, E):
+    if not 1 <= E <= MOE_MAX_EXPERTS:
+        raise ValueError(f"moe_route: 1 to {MOE_MAX_EXPERTS} experts, got {E}")
+    if not 1 <= top_k <= min(MOE_MAX_TOP_K, E):
         raise ValueError(f"moe_route: top_k {top_k} of {E} experts (at most 32)")
     if groups < 1 or groups > 32 or E % groups or not 1 <= top_groups <= groups or top_groups * (E // groups) < top_k:
         raise ValueError(f"moe_route: {top_k} experts in {top_groups} of {groups} groups of {E} experts")
@@ -415,7 +420,7 @@ def moe_plan(ids: torch.Tensor, num_experts: int, first: int = 0, tile: int = 0)
         return MoEPlan(ids.shape[1], order, pos, counts, starts, items if tile else None, tile)
     if ids.dim() != 2 or ids.dtype not in (torch.int64, torch.int32) or ids.shape[1] < 1:
         raise ValueError("moe_plan: ids [T, k], int64 or int32")
-    if not 1 <= num_experts <= 1024 or first < 0 or tile < 0:
+    if not 1 <= num_experts <= MOE_MAX_EXPERTS or first < 0 or tile < 0:
         raise ValueError(f"moe_plan: 1 to 1024 experts from 0 on, got {num_experts} from {first}")
     order, pos, counts, starts = ref.moe_plan(ids, num_experts, first)
     items = None

@@ -382,7 +382,8 @@ def moe_plan(ids, num_experts, first):
     own = (flat >= 0) & (flat < num_experts)
     key = torch.where(own, flat, num_experts)
     order = torch.argsort(key, stable=True)
-    counts = torch.bincount(key, minlength=num_experts + 1)[:num_experts]
+    # scatter-add, not bincount: that reads its maximum back to the host, which no CUDA graph can hold
+    counts = key.new_zeros(num_experts + 1).scatter_add_(0, key, torch.ones_like(key))[:num_experts]
     row = torch.empty_like(order)
     row[order] = torch.arange(order.numel(), device=order.device)
     starts = torch.cat([counts.new_zeros(1), counts.cumsum(0)])
