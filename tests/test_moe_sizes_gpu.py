@@ -1,4 +1,4 @@
-"""MoE blocks of sizes beyond the kernels' on the GPU."""
+"""MoE blocks of sizes beyond the kernels' on the GPU, and without a shared expert."""
 import pytest
 import torch
 
@@ -46,3 +46,9 @@ def test_block_scaled_block_of_any_size_in_a_graph(sizes):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+def test_block_without_shared_expert():
+    c, g = (block(device=d, shared_expert_intermediate_size=0) for d in ("cpu", DEV))
+    near(g.forward(x_of(20).to(DEV)), c.forward(x_of(20)))
+    assert K.check_status(DEV) == 0

@@ -85,7 +85,7 @@ class MoEBlock:
         self._gates = torch.cat([both, both.new_zeros(-both.shape[0] % 8, self.H)])
         if (self.dense_gu is not None and self.H % 8 == 0 and self.I % 8 == 0 and self.e_local <= K.MOE_MAX_EXPERTS):
             up, down = self.shared_gate_up, self.shared_down
-            bf16 = up.quant == "bf16" and down.K % 8 == 0
+            bf16 = up.quant == "bf16" and down.K % 8 == 0 and down.K > 0          # K is 0 without a shared expert
             self._banks = (LinearBank(up.w, act="swiglu") if bf16 else None, LinearBank(down.w) if bf16 else None,
                            LinearBank(self.dense_gu, act="swiglu"), LinearBank(self.dense_dn))
 
