@@ -1,4 +1,4 @@
-"""MoE blocks of sizes beyond the kernels'."""
+"""MoE blocks of sizes beyond the kernels', and routers that no block can have."""
 import dataclasses
 
 import pytest
@@ -32,3 +32,13 @@ def test_block_of_any_size(sizes):
     want_ids, want = M.route(x.float() @ blk.router.float().t(), sizes["num_experts_per_tok"])
     assert torch.equal(ids, want_ids) and torch.allclose(w.double(), want, rtol=1e-6)
     assert blk.forward(x).isfinite().all()
+
+
+@pytest.mark.parametrize("router", [dict(moe_score="tanh"), dict(moe_num_groups=3), dict(moe_num_groups=4, moe_top_groups=5),
+                                    dict(moe_num_groups=8, moe_top_groups=1), dict(moe_num_groups=0),
+                                    dict(moe_num_groups=16, moe_top_groups=8, moe_router_bias=True),
+                                    dict(num_experts_per_tok=17), dict(num_experts_per_tok=0)])
+def test_router_that_cannot_be_is_refused_at_load(router):
+    """Not by the first forward pass."""
+    with pytest.raises(ValueError, match="MoE"):
+        block(**router)

@@ -37,6 +37,15 @@ class MoEBlock:
         self.E, self.H, self.I = E, H, I
         self.top_k = cfg.num_experts_per_tok
         self.quant = quant
+        groups, tops = cfg.moe_num_groups, cfg.moe_top_groups
+        if cfg.moe_score not in ("softmax", "sigmoid"):
+            raise ValueError(f"MoE router: scores softmax or sigmoid, got {cfg.moe_score!r}")
+        if not 1 <= self.top_k <= E:
+            raise ValueError(f"MoE router: {self.top_k} experts a token of {E}")
+        if not 1 <= groups <= 32 or E % groups or not 1 <= tops <= groups or tops * (E // groups) < self.top_k:
+            raise ValueError(f"MoE router: {self.top_k} experts in {tops} of {groups} groups of {E} experts")
+        if cfg.moe_router_bias and groups > 1 and E // groups < 2:
+            raise ValueError("MoE router: with a bias a group's value is that of two experts")
         # experts owned by this rank: expert parallel over the tensor-parallel group (tokens
         # replicated, partial sums all-reduced), or over a data-parallel group `ep` (tokens
         # local to each rank, rows exchanged by the EP transport's dispatch / combine)
