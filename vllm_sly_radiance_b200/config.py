@@ -248,7 +248,9 @@ def config_from_hf(d: dict) -> ModelConfig:
         moe_intermediate_size=tc.get("moe_intermediate_size", 0),
         shared_expert_intermediate_size=tc.get("shared_expert_intermediate_size", 0),
         moe_score=tc.get("scoring_func") or "softmax", moe_router_bias=tc.get("topk_method") == "noaux_tc",
-        moe_num_groups=tc.get("n_group") or 1, moe_top_groups=tc.get("topk_group") or 1,
+        # a plain greedy choice knows no groups, whatever the file says of them
+        moe_num_groups=1 if tc.get("topk_method") == "greedy" else tc.get("n_group") or 1,
+        moe_top_groups=1 if tc.get("topk_method") == "greedy" else tc.get("topk_group") or 1,
         moe_renormalize=tc.get("norm_topk_prob") is not False, moe_routed_scale=tc.get("routed_scaling_factor") or 1.0,
         rms_norm_eps=tc.get("rms_norm_eps", 1e-6),
         tie_word_embeddings=tc.get("tie_word_embeddings", False))
