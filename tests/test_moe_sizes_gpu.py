@@ -1,4 +1,4 @@
-"""MoE blocks of sizes beyond the kernels' on the GPU, and without a shared expert."""
+"""MoE blocks of sizes beyond the kernels' on the GPU, without a shared expert, and routed rows without a stop for the host."""
 import pytest
 import torch
 
@@ -52,3 +52,15 @@ def test_block_without_shared_expert():
     c, g = (block(device=d, shared_expert_intermediate_size=0) for d in ("cpu", DEV))
     near(g.forward(x_of(20).to(DEV)), c.forward(x_of(20)))
     assert K.check_status(DEV) == 0
+
+
+def test_rows_by_expert_do_not_stop_for_the_host():
+    g = block(device=DEV)
+    x, le = x_of(50).to(DEV), torch.randint(0, 16, (50,), generator=torch.Generator().manual_seed(0)).to(DEV)
+    want = g.expert_rows(None, None, x, le)
+    torch.cuda.set_sync_debug_mode("error")
+    try:
+        got = g.expert_rows(None, None, x, le)
+    finally:
+        torch.cuda.set_sync_debug_mode("default")
+    assert torch.equal(got, want)

@@ -174,17 +174,17 @@ class MoEBlock:
         dev = le.device
         if n == 0:
             return torch.zeros(0, self.H, dtype=torch.bfloat16, device=dev)
-        order = torch.argsort(le, stable=True)
-        counts = torch.bincount(le, minlength=self.e_local)
         y = torch.empty(n, self.H, dtype=torch.bfloat16, device=dev)
-        if self.w_gate_up is not None and le.is_cuda:
-            y[order] = K.moe_grouped_mlp(q[order], s[order], counts, self.w_gate_up, self.w_down,
-                                         self.I, self.H)
-            return y
-        if self._on_kernels(le):
+        if self.w_gate_up is None and self._on_kernels(le):
             _, _, up, down = self._banks
             plan = K.moe_plan(le[:, None], self.e_local)
             y[plan.order.long()] = K.linear_fused(K.linear_fused(xb, up, plan=plan, by_token=True), down, plan=plan)
+            return y
+        order = torch.argsort(le, stable=True)
+        counts = torch.bincount(le, minlength=self.e_local)
+        if self.w_gate_up is not None and le.is_cuda:
+            y[order] = K.moe_grouped_mlp(q[order], s[order], counts, self.w_gate_up, self.w_down,
+                                         self.I, self.H)
             return y
         starts = torch.cumsum(counts, 0) - counts
         for e in range(self.e_local):
