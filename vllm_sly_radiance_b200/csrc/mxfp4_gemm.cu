@@ -883,8 +883,8 @@ static WFmt weight_fmt(int64_t row_bytes, int K) {
   if (row_bytes * 2 == Kp) return {0, (int)Kp};
   if (row_bytes * 4 == Kp * 3) return {1, (int)Kp};
   if (row_bytes == Kp) return {2, (int)Kp};
-  TORCH_CHECK(false, "MX weight: a row of ", row_bytes, " bytes is not K = ", Kp,
-              " (activation K rounded up to 128) as e2m1, e2m3 or e4m3");
+  TORCH_CHECK(false, text_all("MX weight: a row of ", row_bytes, " bytes is not K = ", Kp,
+                              " (activation K rounded up to 128) as e2m1, e2m3 or e4m3"));
   return {0, 0};
 }
 

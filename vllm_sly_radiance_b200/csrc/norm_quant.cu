@@ -15,6 +15,7 @@
 #include <torch/extension.h>
 
 #include "common.cuh"
+#include "refuse.h"
 
 namespace rad {
 namespace nq {
@@ -299,7 +300,7 @@ static inline void check_vec(const torch::Tensor& t, const char* what, int align
   const int64_t es = t.element_size();
   TORCH_CHECK(t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % align == 0 &&
                   (t.dim() < 2 || (t.stride(0) * es) % align == 0),
-              what, ": vector access needs a ", align, "-byte aligned base and row stride");
+              text_all(what, ": vector access needs a ", align, "-byte aligned base and row stride"));
 }
 
 }  // namespace nq

@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <torch/extension.h>
 
+#include "refuse.h"
+
 namespace rad {
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
@@ -39,9 +41,9 @@ inline CUtensorMap make_tma_2d(void* base, CUtensorMapDataType dtype, uint64_t i
   CUresult r = get_encode_tiled()(&m, dtype, 2, base, dims, strides, box, estr,
                                   CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promo,
                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with code ", (int)r,
+  TORCH_CHECK(r == CUDA_SUCCESS, text_all("cuTensorMapEncodeTiled failed with code ", (int)r,
               " (inner=", inner, " rows=", rows, " stride=", row_stride_bytes, " box=", box_inner,
-              "x", box_rows, ")");
+              "x", box_rows, ")"));
   return m;
 }
 
@@ -58,7 +60,7 @@ inline CUtensorMap make_tma_3d(void* base, CUtensorMapDataType dtype, uint64_t d
                                   CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled (3d) failed with code ", (int)r);
+  TORCH_CHECK(r == CUDA_SUCCESS, text_all("cuTensorMapEncodeTiled (3d) failed with code ", (int)r));
   return m;
 }
 
