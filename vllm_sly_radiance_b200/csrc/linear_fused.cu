@@ -36,9 +36,10 @@ constexpr int A_BYTES = BM * BK * 2;
 constexpr int SUM_LD = 144;                                // floats of a staged row (SPLIT); the up half starts 16 banks behind the gate half
 constexpr int SMEM_MAX = 227 * 1024;
 constexpr int MAX_E = 1024;
-// warps: 0 loads weights (and rows in order), 1 issues MMAs, 8 carry sums out, 4 pick rows by token
-constexpr int EPI0 = 2, EPI_WARPS = 8, GATHER0 = EPI0 + EPI_WARPS, GATHER_WARPS = 4;
-constexpr int THREADS = 32 * (GATHER0 + GATHER_WARPS);
+// warps: 0 loads weights (and rows in order), 1 issues MMAs, 8 carry sums out, 4 pick rows by token; on a pair one more, which tells the
+// first CTA that the second one's sums are out
+constexpr int EPI0 = 2, EPI_WARPS = 8, GATHER0 = EPI0 + EPI_WARPS, GATHER_WARPS = 4, RELAY = GATHER0 + GATHER_WARPS;
+constexpr int threads(bool pair) { return 32 * (RELAY + (pair ? 1 : 0)); }
 
 struct Args {
   const int* starts;                                       // [E + 1] rows of the experts; null: one expert, R rows
@@ -67,7 +68,8 @@ template <int BN, bool PAIR, bool SPLIT> struct Cfg {
 };
 
 struct Bars {
-  uint64_t full[12], picked[12], empty[12], acc_full[2], acc_empty[2];
+  uint4 token;                                             // what send_token copies
+  uint64_t full[12], picked[12], empty[12], acc_full[2], acc_empty[2], drained[2];
   uint32_t tmem;
   int abort;
 };
@@ -122,9 +124,43 @@ DEVI void mma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t i
 DEVI void commit_pair(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-// arrive on the barrier at a cluster address.  What it announces (TMEM loads that were waited for, copies that have landed) is done
-// by then: a release of cluster scope took some 0.8 us (4096 rows by token on pairs: 541 us, 230 without)
-DEVI void arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// Arrive on the other CTA's barrier, after all that this thread has seen: a release of cluster scope.  It takes some 0.8 us, so that a
+// thread does it which nobody waits for (the warp RELAY, once an item; 512 -> 2048, 4096 tokens of 256 experts: 124 us, 123 with no release)
+DEVI void arrive_at(uint32_t bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// Tell the other CTA's barrier of what this thread has seen, for the tensor cores to read: a copy of 16 bytes in the proxy of
+// the MMAs, whose arrival counts there as bytes of the stage do.  The thread does not wait, as it would for a release of cluster scope at
+// some 0.8 us a stage (4096 tokens of 256 experts, 2048 -> 512 SwiGLU: 559 us, this 228, and 226 with an arrival that orders nothing)
+DEVI void send_token(uint32_t dst, uint32_t src, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], 16, [%2];" ::"r"(dst), "r"(src),
+               "r"(bar)
+               : "memory");
+}
+// mbar_wait for arrivals of the other CTA
+DEVI bool wait_cluster(uint64_t* bar, uint32_t phase, int* err) {
+  const auto done = [&]() {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, P;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(phase)
+        : "memory");
+    return ok != 0;
+  };
+  if (done()) return true;
+  const uint64_t t0 = globaltimer_ns(), limit = wait_limit_ns(err, 2, kWaitNs);
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i)
+      if (done()) return true;
+    if (globaltimer_ns() - t0 > limit) break;
+  }
+  if (err) atomicExch(err, (int)kErrMbarTimeout);
+  return false;
+}
 DEVI void tmem_ld_x32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
       "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,"
@@ -313,7 +349,7 @@ DEVI void store_row(const Args& p, const Item& q, const float* st, int c, int ti
 // the MMAs of both.  SPLIT: a cluster shares one item's K; its CTAs' sums meet through distributed shared memory, each CTA adds
 // up and stores some of the rows.  Otherwise a CTA (or pair) an SM (or two) runs every n-th item.
 template <int BN, bool SWIGLU, bool PAIR, bool SPLIT>
-__global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap wm,
+__global__ void __launch_bounds__(threads(PAIR), 1) kernel(const __grid_constant__ Args p, const __grid_constant__ CUtensorMap wm,
                                                      const __grid_constant__ RowMaps xm) {
   using C = Cfg<BN, PAIR, SPLIT>;
   extern __shared__ uint8_t smem_raw[];
@@ -335,15 +371,17 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Arg
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(&bars->full[s], gather && PAIR ? 2 : 1);
+      mbar_init(&bars->full[s], 1);
       mbar_init(&bars->picked[s], 32 * GATHER_WARPS);
       mbar_init(&bars->empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&bars->acc_full[b], 1);
-      mbar_init(&bars->acc_empty[b], EPI_WARPS * (PAIR ? 2 : 1));
+      mbar_init(&bars->acc_empty[b], EPI_WARPS + (PAIR ? 1 : 0));
+      mbar_init(&bars->drained[b], EPI_WARPS);
     }
     bars->abort = 0;
+    bars->token = make_uint4(0, 0, 0, 0);
     fence_mbar_init();
     tma_prefetch_desc(&wm);
   }
@@ -358,7 +396,7 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Arg
     }
   }
   pdl_wait();
-  for (int e = threadIdx.x; e <= p.E; e += THREADS) starts[e] = p.starts ? p.starts[e] : e ? p.R : 0;
+  for (int e = threadIdx.x; e <= p.E; e += threads(PAIR)) starts[e] = p.starts ? p.starts[e] : e ? p.R : 0;
   __syncthreads();
   if (warp == 2) count_tiles(p, p.tile, tiles, starts, lane);
   tc_fence_before();
@@ -403,7 +441,8 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Arg
         uint32_t full = smem_u32(&bars->full[s]);
         if (PAIR) full = mapa_shared(full, 0);
         if (lane == 0) {
-          if (rank == 0) mbar_arrive_expect_tx(&bars->full[s], (PAIR ? 2 : 1) * (A_BYTES + bbytes));
+          if (rank == 0)
+            mbar_arrive_expect_tx(&bars->full[s], (PAIR ? 2 : 1) * (A_BYTES + bbytes) + (PAIR && gather ? sizeof(bars->token) : 0));
           const int f = q.n0 + rank * HALF;
           if (PAIR && SWIGLU) tma_4d_pair(a, &wm, full, kb * BK, 0, f, q.e);
           else if (PAIR) tma_4d_pair(a, &wm, full, kb * BK, f, 0, q.e);
@@ -429,7 +468,11 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Arg
       for (int i = unit; i < items && !*abort; i += units, ++n) {
         const Item q = item_of(p, i, blocks, p.tile, SPAN, tiles, starts);
         const int ab = n & 1;
-        if (!mbar_wait(&bars->acc_empty[ab], ((n >> 1) & 1) ^ 1, p.status)) { give_up(); break; }
+        const uint32_t aph = ((n >> 1) & 1) ^ 1;
+        if (!(PAIR ? wait_cluster(&bars->acc_empty[ab], aph, p.status) : mbar_wait(&bars->acc_empty[ab], aph, p.status))) {
+          give_up();
+          break;
+        }
         tc_fence_after();
         const uint32_t idesc = idesc_bf16(PAIR ? 2 * BM : BM, mma_rows(q));
         bool ok = true;
@@ -466,22 +509,21 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Arg
     }
     if (PAIR && gather && rank == 1 && elect_one()) {
       // this CTA's picked rows, for the one that issues the MMAs
-      const uint32_t full0 = mapa_shared(smem_u32(&bars->full[0]), 0);
+      const uint32_t full0 = mapa_shared(smem_u32(&bars->full[0]), 0), token0 = mapa_shared(smem_u32(&bars->token), 0);
       uint32_t it = 0;
       for (int i = unit; i < items && !*abort; i += units)
         for (int kb = k0; kb < k1; ++kb, ++it) {
           const int s = it % C::STAGES;
           if (!mbar_wait(&bars->picked[s], (it / C::STAGES) & 1, p.status)) { give_up(); break; }
           fence_proxy_async();
-          arrive_at(full0 + s * 8);
+          send_token(token0, smem_u32(&bars->token), full0 + s * 8);
         }
     }
     __syncwarp();
   } else if (warp < GATHER0) {
     const int quad = warp & 3, part = (warp - EPI0) / 4;   // 32 weight rows; columns 64 j + 32 part
     const bool rest = p.scale || p.res;
-    uint32_t acc_empty = smem_u32(&bars->acc_empty[0]);
-    if (PAIR) acc_empty = mapa_shared(acc_empty, 0);
+    uint64_t* out_of = PAIR && rank ? bars->drained : bars->acc_empty;
     uint32_t n = 0;
     for (int i = unit; i < items; i += units, ++n) {
       const Item q = item_of(p, i, blocks, p.tile, SPAN, tiles, starts);
@@ -525,7 +567,7 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Arg
           if (c0 + 64 >= q.rows) {                         // this warp has read all that it needs
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) arrive_at(acc_empty + ab * 8);
+            if (lane == 0) mbar_arrive(&out_of[ab]);
           }
           const int cols = min(32, q.rows - c0);
           const bool whole = p.vec && f0 + HALF / 4 <= p.W;
@@ -539,9 +581,21 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Arg
             store_columns<SWIGLU, true, false, false>(p, v, q.row0 + c0, cols, f0, lane);
           }
         }
-        if (32 * part >= q.rows && lane == 0) arrive_at(acc_empty + ab * 8);
+        if (32 * part >= q.rows && lane == 0) mbar_arrive(&out_of[ab]);
       }
     }
+  } else if (PAIR && warp == RELAY) {
+    if (rank == 1 && elect_one()) {
+      const uint32_t acc_empty0 = mapa_shared(smem_u32(&bars->acc_empty[0]), 0);
+      uint32_t n = 0;
+      for (int i = unit; i < items && !*abort; i += units, ++n) {
+        if (!mbar_wait(&bars->drained[n & 1], (n >> 1) & 1, p.status)) { give_up(); break; }
+        tc_fence_after();
+        tc_fence_before();
+        arrive_at(acc_empty0 + (n & 1) * 8);
+      }
+    }
+    __syncwarp();
   } else if (gather) {
     // rows by token: thread t brings 16-byte piece t % 8 of rows t / 8, t / 8 + 16, ... of every stage
     const int tid = threadIdx.x - 32 * GATHER0, piece = tid % 8, r0 = tid / 8;
@@ -619,7 +673,7 @@ __global__ void __launch_bounds__(THREADS, 1) kernel(const __grid_constant__ Arg
 // launches
 // ---------------------------------------------------------------------------------------------
 template <typename... A>
-void launch(void (*kern)(A...), dim3 grid, dim3 cluster, size_t smem, cudaStream_t stream, A... args) {
+void launch(void (*kern)(A...), dim3 grid, int threads, dim3 cluster, size_t smem, cudaStream_t stream, A... args) {
   static std::mutex m;
   static std::map<std::pair<const void*, int>, bool> set;
   int dev;
@@ -632,7 +686,7 @@ void launch(void (*kern)(A...), dim3 grid, dim3 cluster, size_t smem, cudaStream
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(THREADS);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[2];
@@ -676,8 +730,8 @@ bool overlap(const torch::Tensor& a, const torch::Tensor& b) {
 
 template <int BN, bool PAIR, bool SPLIT>
 void run(const Args& p, bool swiglu, const CUtensorMap& wm, const RowMaps& xm, dim3 grid, dim3 cluster, cudaStream_t stream) {
-  launch(swiglu ? kernel<BN, true, PAIR, SPLIT> : kernel<BN, false, PAIR, SPLIT>, grid, cluster, Cfg<BN, PAIR, SPLIT>::SMEM, stream,
-         p, wm, xm);
+  launch(swiglu ? kernel<BN, true, PAIR, SPLIT> : kernel<BN, false, PAIR, SPLIT>, grid, threads(PAIR), cluster,
+         Cfg<BN, PAIR, SPLIT>::SMEM, stream, p, wm, xm);
 }
 
 // How a product of R rows is cut: rows of a tile, CTA pairs or single CTAs, CTAs that share an item's K, items at most
