@@ -10,11 +10,12 @@
 // picked by token come by asynchronous 16-byte copies of four more warps: TMA takes four rows by number a load and some 65 cycles
 // for each, which a tile of more than 32 rows waits for (512 tokens, 256 experts: 264 us, this 166).
 //
-// Up to 32 rows an expert it is bound by memory, the weights (256 experts, top-8, 2048 -> 512 SwiGLU and 512 -> 2048, B200):
-// 64 tokens 124 and 63 us (6.5 TB/s), 1024 tokens 173 and 95 us (6.3 and 6.1 TB/s), one token 12 us, of which 5 are the bytes
-// and the rest one chain of latencies (plan, first tiles, the cluster's sum).  With more rows tiles wait for what L2 hands out,
-// weights and rows together some 10 TB/s: 8192 tokens 338 and 187 us.  One weight, 5120 -> 8704 SwiGLU, 4096 rows: 481 us,
-// 1519 TFLOP/s, MMAs.
+// Up to 32 rows an expert it is bound by memory, the weights (256 experts, top-8, 2048 -> 512 SwiGLU and 512 -> 2048, B200, best of
+// 7 graphs of 10 calls): 64 tokens, which use 197 of the experts, 126 and 65 us (6.5 and 6.4 TB/s), 1024 tokens 172 and 94 us (6.3
+// and 6.1 TB/s), one token 10 us, of which 5 are the bytes and the rest one chain of latencies (plan, first tiles, the cluster's sum).
+// With more rows tiles wait for what L2 hands out, weights and rows together some 10 TB/s: 4096 tokens 228 and 124 us, 8192 tokens
+// 342 and 192 us (call after call for longer, when clocks fall, 400).  One weight, 5120 -> 8704 SwiGLU, 4096 rows: 451 us, 1619
+// TFLOP/s, MMAs.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -273,7 +274,7 @@ DEVI void store4(const Args& p, __nv_bfloat16* out, int f, bool in, const Rest& 
 // 32 columns (rows of out from row0 on, n of them in use) of a warp's 32 weight rows -> out.  A lane holds one weight row; lanes
 // trade columns until each has four neighbouring features of one row, so that a store covers whole 32-byte sectors.
 // WHOLE: the features are all in use and on 8 bytes; FULL: so are all columns, and nothing branches, so that the trades of all of
-// them overlap: 8192 rows by expert, 512 -> 2048: 174 us, 257 with a test at every store.
+// them overlap: 8192 tokens of 256 experts, 512 -> 2048, took half as long again (257 us) with a test at every store.
 template <bool SWIGLU, bool REST, bool WHOLE, bool FULL>
 DEVI void store_columns(const Args& p, const float (&v)[32], int64_t row0, int n, int f0, int lane) {
   constexpr int J = SWIGLU ? 4 : 8, STEP = 32 / J;

@@ -35,8 +35,8 @@ DEVI float to_f(__half x) { return __half2float(x); }
 // order: they are computed in 32 bits, and once more in 64 for the few tokens (about one in 500) where two candidates, or two
 // groups, lie so near that the rounding could have turned them.
 // ---------------------------------------------------------------------------------------------
-// Bound by one warp's chain of instructions: 3.1 us for one token, 11 us for 8192 of 256 experts, 19 us with groups and a bias
-// (their bytes take 1.4 us).
+// Bound by one warp's chain of instructions (device times, graphs of 10 calls): 3.2 us for one token, 11 us for 8192 of 256 experts,
+// 22 us with sigmoid scores, groups and a bias (their bytes take 1.4 us).
 struct RouteArgs {
   const void* logits;
   const float* bias;
@@ -292,7 +292,8 @@ __global__ void __launch_bounds__(256, V <= 8 ? 4 : V <= 32 ? 2 : 1) route_kerne
 // another by a vote per bit of their number (a warp match instead took 12.2 us for 4096 pairs, this 8.7), so nothing is atomic
 // and the rows come in the pairs' order.
 // ---------------------------------------------------------------------------------------------
-// Bound by the same kind of chain: 3.4 us for 512 pairs (one CTA), 16 us for 131072 (16 CTAs, votes and shared memory).
+// Bound by the same kind of chain: 3.5 us for 512 pairs (one CTA), 18 us for 131072 (16 CTAs, votes and shared memory; 16 where half
+// of the experts are another rank's).
 struct PlanArgs {
   const void* ids;
   int R, k, E, first, seg, warps, bits;                    // pairs, experts of this rank, pairs of a warp, warps that have some
@@ -445,8 +446,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Plan
 
 // ---------------------------------------------------------------------------------------------
 // gather, combine: bound by memory, 16 bytes a thread.  combine reads rows of a few KB in as many places as a token has experts:
-// 8192 x 8 rows of 2048 take 53 us (5.7 TB/s), with the shared rows 67 (74 while the gate's
-// sigmoid was taken before the rows were asked for).
+// 8192 x 8 rows of 2048 take 53 us (5.7 TB/s), with the shared rows 66 (5.1 TB/s; 74 while the gate's
+// sigmoid was taken before the rows were asked for).  gather: the same rows in e4m3 43 us (their bytes take 23).
 // ---------------------------------------------------------------------------------------------
 // rows of `vecs` 16-byte pieces; x [T] -> out [R], a pair's row is its token's.  scale: fp32 beside each row, or null
 __global__ void __launch_bounds__(256) gather_kernel(const uint4* x, int64_t ld, const float* xs, const int* order, uint4* out,
@@ -742,8 +743,8 @@ torch::Tensor moe_combine(const torch::Tensor& rows, const torch::Tensor& pos, c
   const int64_t blocks = (T * (vec ? H / 8 : H) + 255) / 256;
   RAD_CHECK_VALUE(blocks < (1ll << 23), "moe_combine: rows");
   auto stream = at::cuda::getCurrentCUDAStream();
-  // about as many blocks as run at once, each over several tokens (8192 x 8 rows of 2048 and
-  // shared ones: 74 us, 87 with a block for each token)
+  // four blocks an SM, of which two run at once (116 registers), each over several tokens (8192 x 8 rows of 2048 and shared ones:
+  // 66 us, 83 with three, which leave half of the places empty at the end, 76 with a block for every 256 pieces)
   const unsigned grid = (unsigned)std::min<int64_t>(blocks, 4ll * at::cuda::getDeviceProperties(rows.get_device())->multiProcessorCount);
   if (vec) C10_CUDA_CHECK(launch_pdl(moe::combine_kernel<8>, dim3(grid), dim3(256), 0, stream, p));
   else C10_CUDA_CHECK(launch_pdl(moe::combine_kernel<1>, dim3(grid), dim3(256), 0, stream, p));

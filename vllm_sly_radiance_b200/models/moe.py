@@ -209,7 +209,12 @@ class MoEBlock:
     def local_experts(self, xb, qs, ids, w, shared=None, gate=None):
         """Experts [e0, e0+e_local) applied to every (token, slot) routed to them; the other
         slots contribute zero (they belong to another rank's experts).  As grouped products,
-        shared rows times sigmoid(gate) join the sum."""
+        shared rows times sigmoid(gate) join the sum.
+
+        Each expert's row is rounded to bf16 between the down product and the weighted sum, which halves what the sum
+        reads; the loop over bf16 experts below keeps it in 32 bits, but rounds gate, up and their product where the
+        grouped products round the product alone.  Against 64 bits (K 512 and 256, top-8) the block's result is off by
+        2.9e-3 with the grouped products, 3.6e-3 with the loop, in the 2-norm."""
         if self._on_kernels(xb):
             # fixed shapes, no host sync (CUDA-graph safe)
             if self.w_gate_up is None:

@@ -380,9 +380,10 @@ def moe_route(logits: torch.Tensor, top_k: int, score: str = "softmax", bias: Op
     lowest index, and only experts of the ``top_groups`` best of ``groups`` equal groups count; a group's value is its best
     expert's, with a bias that of its best two added up.  Weights are the chosen scores without the bias, divided by their sum
     if ``renormalize``, times ``scale``.  A logit of -inf masks its expert, whose weight is 0: without a bias it is chosen
-    only when no other is left.  Chosen scores that add up to 0 (a row that is masked throughout) stay 0.  A NaN among a row's
-    logits (or +inf under a softmax) makes its weights NaN; its ids stay distinct and in range.  At most 1024 experts and 32 a
-    token."""
+    only when no other is left.  Chosen scores that add up to 0 (a row that is masked throughout) stay 0; renormalised ones may be
+    smaller than any number.  A NaN among a row's logits (or +inf under a softmax) makes its weights NaN; its ids stay distinct and
+    in range.  An expert whose bias is NaN ranks last.  At most 1024 experts, 32 groups and 32 experts a token; on the GPU each
+    row of the logits is contiguous and no row overlaps another."""
     if score not in ("softmax", "sigmoid"):
         raise ValueError(f"moe_route: score softmax or sigmoid, got {score!r}")
     if logits.is_cuda:
@@ -431,7 +432,7 @@ def moe_plan(ids: torch.Tensor, num_experts: int, first: int = 0, tile: int = 0)
 
 def moe_gather(x, plan: MoEPlan):
     """Activations of the plan's rows: x [T, K] bf16 -> [T k, K], or an (e4m3, scale) pair -> a pair.  Rows behind the plan's
-    last one are left as the allocation has them."""
+    last one are left as the allocation has them.  On the GPU rows of x are whole 16 bytes, on 16 bytes."""
     xq, xs = x if isinstance(x, tuple) else (x, None)
     if xq.dim() != 2 or xq.shape[0] != plan.pos.shape[0]:
         raise ValueError(f"moe_gather: x {tuple(xq.shape)} and a plan of {plan.pos.shape[0]} tokens")
@@ -471,7 +472,8 @@ def linear_fused(x: torch.Tensor, bank, plan: Optional[MoEPlan] = None, by_token
 
     Without a plan the bank has one weight and x [R, K] bf16 its rows.  With a plan (``moe_plan``) each row takes its expert's
     weight; x holds the plan's rows in order or, ``by_token``, one row per token.  Rows of out [R, width] behind the plan's
-    last one are left as they were.  scale [R] fp32, residual [R, width] bf16; out may be residual (in place)."""
+    last one are left as they were.  scale [R] fp32, residual [R, width] bf16; out may be residual (in place), else it
+    overlaps neither that nor x.  On the GPU rows of x start on 16 bytes and do not overlap."""
     if x.is_cuda:
         if bank.handle is None:
             raise ValueError("linear_fused: operands on one device")
